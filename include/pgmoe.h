@@ -305,6 +305,101 @@ int pgmoe_linear_forward_packed(const pgmoe_weights* W, int32_t member_rows, con
 int pgmoe_dequant_rows(const pgmoe_weights* W, const int32_t* rows, int32_t n, void* out, int32_t out_dtype,
                        void* stream);
 
+/* ---- operators of the decoder layer around the FFN: rotary + paged KV append, attention, sampling ---- */
+
+/* The K and V pages of one attention layer (device pointers, 16-byte aligned): element d of row r of head h
+ * of page p is at p * page_stride + h * head_stride + r * row_stride + d, in k and in v alike (strides in
+ * elements, multiples of 8). */
+typedef struct pgmoe_kv_cache {
+    void* k;
+    void* v;
+    int64_t page_stride, head_stride, row_stride;
+    int32_t n_pages;
+    int32_t page_size;  /* rows of a page: 16, 32, 64, 128 or 256 */
+    int32_t n_kv_heads;
+    int32_t head_dim;   /* 64, 128 or 256 */
+    int32_t dtype;      /* PGMOE_DT_F16 or PGMOE_DT_BF16 */
+} pgmoe_kv_cache;
+
+/* What one call holds of each sequence.  Sequence b's tokens are the rows q_start[b] .. q_start[b + 1] - 1
+ * of the call's q / k / v (non-decreasing, starting at 0; NULL: token b is sequence b's only one); they are
+ * the last of its lens[b] own keys, so token i of n has own index lens[b] - n + i.  Own key j lies in row
+ * j % page_size of page page_table[b * table_stride + j / page_size].  prefix_len keys before them (in the
+ * pages prefix_pages, which need not be full) are shared by every sequence.  The positions of the own keys
+ * follow the prefix: prefix_len + j.  All arrays are int32 on the device and are read when the kernels run:
+ * a captured graph replays on their present contents.  Nothing is read or written through a page id
+ * outside [0, n_pages) or past max_pages pages of a table row. */
+typedef struct pgmoe_kv_batch {
+    const int32_t* page_table;   /* [n_seqs][max_pages], rows table_stride apart */
+    const int32_t* lens;         /* [n_seqs]; negative counts as 0 */
+    const int32_t* q_start;      /* [n_seqs + 1] or NULL */
+    const int32_t* prefix_pages; /* [ceil(prefix_len / page_size)]; NULL when prefix_len is 0 */
+    int64_t table_stride;
+    int32_t n_seqs;              /* 1 .. 4096 */
+    int32_t max_pages;
+    int32_t prefix_len;
+} pgmoe_kv_batch;
+
+/* Appends n_tokens new keys and values to the cache, with the rotary positions (and, with norm weights, the
+ * per-head RMSNorm of q and k before them) applied on the way, and writes the rotated queries to q_out
+ * [n_tokens, n_q_heads, head_dim] in the cache's type.  q [n_tokens, n_q_heads, head_dim], k and v
+ * [n_tokens, n_kv_heads, head_dim]: PGMOE_DT_* src_dtype, head_dim contiguous, token and head strides in
+ * elements (16-byte multiples), e.g. the parts of one fused projection's output.
+ * The first rot_dim elements of a head turn in pairs (i, i + rot_dim / 2), or (2i, 2i + 1) with interleaved
+ * != 0, by position * turns[i] full turns (turns: float64 [rot_dim / 2], radians per position over 2 pi),
+ * reduced in float64; cosine and sine are scaled by attn_factor.  rot_dim: 0 (turns may be NULL) or a
+ * multiple of 16 up to head_dim.  q_norm / k_norm: fp32 [head_dim] or NULL; x * (1 / sqrt(mean(x^2) + eps)) * w
+ * in fp32.  Every value is rounded once, to the cache's type.  A token with a negative own index, or whose
+ * page does not exist, gets its query and no cache row; rows of q_out behind the last sequence are left
+ * alone.  Two tokens must not fall on one cache row. */
+int pgmoe_rope_append(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, const void* q, int64_t q_token_stride,
+                      int64_t q_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                      const void* v, int64_t v_token_stride, int64_t v_head_stride, int32_t src_dtype,
+                      int32_t n_tokens, int32_t n_q_heads, const double* turns, int32_t rot_dim, int32_t interleaved,
+                      float attn_factor, const float* q_norm, const float* k_norm, float eps, void* q_out,
+                      void* stream);
+
+/* Attention of n_tokens queries over the cache: query i of n of sequence b sees the prefix_len shared keys
+ * and its own keys 0 .. lens[b] - n + i:
+ *   out = softmax(scale * q . K^T) . V,   lse = log(sum(exp(scale * q . K^T)))
+ * scores, statistics and sums in fp32, probabilities rounded to the cache's type for the product with V.
+ * n_q_heads: a multiple of n_kv_heads; query head h reads KV head h / (n_q_heads / n_kv_heads).  q, out
+ * [n_tokens, n_q_heads, head_dim] in the cache's type (q with strides as above; out contiguous, not
+ * overlapping q); lse fp32 [n_tokens, n_q_heads] or NULL.  A query that sees no key gets zeros and an lse
+ * of -inf; one that sees a key on a page that does not exist gets NaN; what masked keys and unused rows of
+ * pages hold is never seen, not even a NaN.  Rows behind the last sequence are left alone. */
+size_t pgmoe_attend_workspace_bytes(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, int32_t n_tokens,
+                                    int32_t n_q_heads);
+int pgmoe_attend(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, const void* q, int64_t q_token_stride,
+                 int64_t q_head_stride, int32_t n_tokens, int32_t n_q_heads, float scale, void* out, float* lse,
+                 void* ws, size_t ws_bytes, void* stream);
+
+/* Sampling parameters: a device array of one value a row, or NULL for the scalar beside it. */
+typedef struct pgmoe_sampling {
+    const float* temperatures;
+    const int32_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    double temperature; /* <= 0: the largest logit (the lowest index among equals) */
+    double top_p;       /* >= 1: off */
+    double min_p;       /* <= 0: off */
+    int32_t top_k;      /* <= 0: off */
+} pgmoe_sampling;
+
+/* One token a row of logits [rows, vocab] (PGMOE_DT_*, rows row_stride elements apart), drawn with the
+ * given uniform numbers u [rows] (fp32, [0, 1)):
+ *   w_i = exp((x_i - max x) / temperature); tokens ordered by logit, equal ones by index;
+ *   kept: the shortest of three prefixes of that order, one token at least: the first top_k; those before
+ *   which the sum of w is below top_p times the sum of all; those with w >= min_p;
+ *   token (int64 [rows]): the first in index order at which the sum of the kept w exceeds u times their
+ *   total; logprob (fp32 [rows] or NULL): log(w_token / total).
+ * Weights are summed in 64-bit fixed point, so no order of sums shows in the result.  NaN and -inf logits
+ * have no weight; with +inf ones only those have.  A row without any logit above -inf gives token -1 and
+ * logprob -inf.  vocab: 1 .. 2^20. */
+size_t pgmoe_sample_workspace_bytes(int32_t rows, int32_t vocab);
+int pgmoe_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab, const float* u,
+                 const pgmoe_sampling* S, int64_t* token, float* logprob, void* ws, size_t ws_bytes, void* stream);
+
 /* pgmoe_moe_forward with per-kernel timing.  No counterpart in the reference: it is for
  * benchmarks and profilers that want each kernel's duration from the caller's own stream.
  * The i-th kernel the call launches (i < n_events) records start_events[i] when it begins

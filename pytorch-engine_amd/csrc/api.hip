@@ -6,7 +6,9 @@
 #include <mutex>
 
 #include "common.h"
+#include "kv.h"
 #include "launch.h"
+#include "sample.h"
 
 namespace pgmoe {
 
@@ -35,6 +37,45 @@ int fail(int code, const char* fmt, ...) {
 int check_launch(const char* what) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(PGMOE_E_HIP, "%s launch failed: %s", what, hipGetErrorString(e));
+    return PGMOE_OK;
+}
+
+static int check_kv(const char* what, const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, int T, int hq, KvCache* c,
+                    KvBatch* b) {
+    if (!C || !B) return fail(PGMOE_E_INVALID, "%s: NULL cache or batch", what);
+    if (C->dtype != PGMOE_DT_F16 && C->dtype != PGMOE_DT_BF16)
+        return fail(PGMOE_E_UNSUPPORTED, "%s: cache dtype %d (fp16 or bf16)", what, C->dtype);
+    if (C->head_dim != 64 && C->head_dim != 128 && C->head_dim != 256)
+        return fail(PGMOE_E_UNSUPPORTED, "%s: head_dim %d (64, 128 or 256)", what, C->head_dim);
+    const int ps = C->page_size;
+    if (ps != 16 && ps != 32 && ps != 64 && ps != 128 && ps != 256)
+        return fail(PGMOE_E_UNSUPPORTED, "%s: page_size %d (16, 32, 64, 128 or 256)", what, ps);
+    if (C->n_pages < 1 || C->n_kv_heads < 1 || C->n_kv_heads > 1024)
+        return fail(PGMOE_E_INVALID, "%s: %d pages of %d KV heads", what, C->n_pages, C->n_kv_heads);
+    if (!C->k || !C->v || (((uintptr_t)C->k | (uintptr_t)C->v) & 15))
+        return fail(PGMOE_E_INVALID, "%s: k and v pages must be 16-byte aligned device pointers", what);
+    if (C->page_stride < 0 || C->head_stride < 0 || C->row_stride < C->head_dim || C->page_stride % 8 ||
+        C->head_stride % 8 || C->row_stride % 8 || C->row_stride > (1 << 22))
+        return fail(PGMOE_E_INVALID, "%s: cache strides must be multiples of 8 elements, rows not overlapping", what);
+    if (T < 0 || T > (1 << 24)) return fail(PGMOE_E_INVALID, "%s: %d tokens", what, T);
+    if (hq < 1 || hq % C->n_kv_heads || hq > 65535)
+        return fail(PGMOE_E_INVALID, "%s: %d query heads on %d KV heads", what, hq, C->n_kv_heads);
+    if (B->n_seqs < 1 || B->n_seqs > kMaxSeqs)
+        return fail(PGMOE_E_UNSUPPORTED, "%s: %d sequences (1 .. %d)", what, B->n_seqs, kMaxSeqs);
+    if (B->max_pages < 1 || (int64_t)B->max_pages * ps > (1 << 30) || B->prefix_len < 0 || B->prefix_len > (1 << 30))
+        return fail(PGMOE_E_INVALID, "%s: page table of %d pages, prefix of %d", what, B->max_pages, B->prefix_len);
+    if (!B->page_table || !B->lens || (B->prefix_len && !B->prefix_pages))
+        return fail(PGMOE_E_INVALID, "%s: NULL page table, lens or prefix pages", what);
+    if (B->n_seqs > 1 && B->table_stride < B->max_pages)
+        return fail(PGMOE_E_INVALID, "%s: page table rows overlap", what);
+    if (!B->q_start && T > B->n_seqs)
+        return fail(PGMOE_E_INVALID, "%s: %d tokens of %d sequences without q_start", what, T, B->n_seqs);
+    int shift = 4;
+    while ((1 << shift) < ps) ++shift;
+    *c = KvCache{(uint16_t*)C->k, (uint16_t*)C->v, C->page_stride, C->head_stride, C->row_stride, C->n_pages, shift,
+                 C->n_kv_heads, C->head_dim, C->dtype == PGMOE_DT_BF16};
+    *b = KvBatch{B->page_table, B->lens, B->q_start, B->prefix_pages, B->table_stride, B->n_seqs, B->max_pages,
+                 B->prefix_len};
     return PGMOE_OK;
 }
 
@@ -707,6 +748,93 @@ int pgmoe_moe_status(const pgmoe_layer* L, void* ws, size_t ws_bytes, int32_t* s
     }
     *status = v;
     return PGMOE_OK;
+}
+
+int pgmoe_rope_append(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, const void* q, int64_t q_token_stride,
+                      int64_t q_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                      const void* v, int64_t v_token_stride, int64_t v_head_stride, int32_t src_dtype,
+                      int32_t n_tokens, int32_t n_q_heads, const double* turns, int32_t rot_dim, int32_t interleaved,
+                      float attn_factor, const float* q_norm, const float* k_norm, float eps, void* q_out,
+                      void* stream) {
+    KvCache kc;
+    KvBatch kb;
+    int rc = check_kv("rope_append", C, B, n_tokens, n_q_heads, &kc, &kb);
+    if (rc) return rc;
+    if (src_dtype != PGMOE_DT_F32 && src_dtype != PGMOE_DT_F16 && src_dtype != PGMOE_DT_BF16)
+        return fail(PGMOE_E_UNSUPPORTED, "rope_append: input dtype %d", src_dtype);
+    if (rot_dim < 0 || rot_dim > kc.dim || rot_dim % 16)
+        return fail(PGMOE_E_INVALID, "rope_append: rot_dim %d (0 or a multiple of 16 up to head_dim %d)", rot_dim, kc.dim);
+    if (!(eps >= 0.0f)) return fail(PGMOE_E_INVALID, "rope_append: negative eps");
+    if (n_tokens == 0) return PGMOE_OK;
+    if (!q || !k || !v || !q_out || (rot_dim && !turns)) return fail(PGMOE_E_INVALID, "rope_append: NULL pointer");
+    const int64_t unit = src_dtype == PGMOE_DT_F32 ? 4 : 8;  // elements of 16 bytes
+    const void* const src[3] = {q, k, v};
+    const int64_t tok[3] = {q_token_stride, k_token_stride, v_token_stride};
+    const int64_t head[3] = {q_head_stride, k_head_stride, v_head_stride};
+    for (int i = 0; i < 3; ++i)
+        if (((uintptr_t)src[i] & 15) || tok[i] % unit || head[i] % unit)
+            return fail(PGMOE_E_INVALID, "rope_append: %c must be 16-byte aligned with strides of whole 16 bytes", "qkv"[i]);
+    if (((uintptr_t)q_out | (uintptr_t)q_norm | (uintptr_t)k_norm) & 15)
+        return fail(PGMOE_E_INVALID, "rope_append: q_out and norm weights must be 16-byte aligned");
+    return launch_rope_append(kc, kb, src, tok, head, src_dtype, n_tokens, n_q_heads, turns, rot_dim, interleaved != 0,
+                              attn_factor, q_norm, k_norm, eps, (uint16_t*)q_out, as_stream(stream));
+}
+
+size_t pgmoe_attend_workspace_bytes(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, int32_t n_tokens,
+                                    int32_t n_q_heads) {
+    KvCache kc;
+    KvBatch kb;
+    if (check_kv("attend", C, B, n_tokens, n_q_heads, &kc, &kb) || n_tokens == 0) return 0;
+    return attend_ws_bytes(kc, kb, n_tokens, n_q_heads);
+}
+
+int pgmoe_attend(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, const void* q, int64_t q_token_stride,
+                 int64_t q_head_stride, int32_t n_tokens, int32_t n_q_heads, float scale, void* out, float* lse,
+                 void* ws, size_t ws_bytes, void* stream) {
+    KvCache kc;
+    KvBatch kb;
+    int rc = check_kv("attend", C, B, n_tokens, n_q_heads, &kc, &kb);
+    if (rc) return rc;
+    if (!(scale > 0.0f) || scale > 3e38f) return fail(PGMOE_E_INVALID, "attend: scale must be positive and finite");
+    if (n_tokens == 0) return PGMOE_OK;
+    if (!q || !out) return fail(PGMOE_E_INVALID, "attend: NULL pointer");
+    if (((uintptr_t)q & 15) || q_token_stride % 8 || q_head_stride % 8)
+        return fail(PGMOE_E_INVALID, "attend: q must be 16-byte aligned with strides of whole 16 bytes");
+    if ((uintptr_t)out & 15) return fail(PGMOE_E_INVALID, "attend: out must be 16-byte aligned");
+    if ((uintptr_t)ws & 255) return fail(PGMOE_E_INVALID, "workspace must be 256-byte aligned");
+    const size_t need = attend_ws_bytes(kc, kb, n_tokens, n_q_heads);
+    if (ws_bytes < need || (need && !ws))
+        return fail(PGMOE_E_WORKSPACE, "workspace %zu bytes, need %zu", ws_bytes, need);
+    return launch_attend(kc, kb, (const uint16_t*)q, q_token_stride, q_head_stride, n_tokens, n_q_heads, scale,
+                         (uint16_t*)out, lse, ws, as_stream(stream));
+}
+
+size_t pgmoe_sample_workspace_bytes(int32_t rows, int32_t vocab) {
+    return rows <= 0 || vocab <= 0 || vocab > kMaxVocab ? 0 : sample_ws_bytes(rows, vocab);
+}
+
+int pgmoe_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab, const float* u,
+                 const pgmoe_sampling* S, int64_t* token, float* logprob, void* ws, size_t ws_bytes, void* stream) {
+    if (rows < 0) return fail(PGMOE_E_INVALID, "sample: negative row count");
+    if (vocab < 1 || vocab > kMaxVocab) return fail(PGMOE_E_UNSUPPORTED, "sample: vocab %d (1 .. %d)", vocab, kMaxVocab);
+    if (dtype != PGMOE_DT_F32 && dtype != PGMOE_DT_F16 && dtype != PGMOE_DT_BF16)
+        return fail(PGMOE_E_UNSUPPORTED, "sample: logits dtype %d", dtype);
+    if (!S) return fail(PGMOE_E_INVALID, "sample: NULL parameters");
+    if (!(S->temperature >= 0.0) || S->temperature > 1e300 || !(S->top_p >= 0.0) || !(S->min_p >= 0.0))
+        return fail(PGMOE_E_INVALID, "sample: temperature, top_p and min_p must be finite and not negative");
+    if (rows == 0) return PGMOE_OK;
+    if (!logits || !u || !token) return fail(PGMOE_E_INVALID, "sample: NULL pointer");
+    if (rows > 1 && row_stride < vocab) return fail(PGMOE_E_INVALID, "sample: rows overlap");
+    if (((uintptr_t)logits & (dtype == PGMOE_DT_F32 ? 3 : 1)) || ((uintptr_t)token & 7))
+        return fail(PGMOE_E_INVALID, "sample: misaligned pointer");
+    if ((uintptr_t)ws & 255) return fail(PGMOE_E_INVALID, "workspace must be 256-byte aligned");
+    const size_t need = sample_ws_bytes(rows, vocab);
+    if (ws_bytes < need || (need && !ws))
+        return fail(PGMOE_E_WORKSPACE, "workspace %zu bytes, need %zu", ws_bytes, need);
+    int bits = 0;
+    while ((1 << bits) < vocab) ++bits;
+    const SampleArgs A{logits, dtype, row_stride, rows, vocab, u, *S, token, logprob, 62 - bits, ws};
+    return launch_sample(A, as_stream(stream));
 }
 
 int pgmoe_moe_forward_timed(const pgmoe_layer* L, const uint16_t* x, int32_t M, float* out, void* ws,

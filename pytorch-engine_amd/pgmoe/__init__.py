@@ -5,11 +5,13 @@
 (model.py:778-846) on the same kernels; ``pgmoe.ops`` exposes the C-ABI stages.
 """
 
+from .attention import HipPagedKVCache, HipRotary, KVBatch
 from .gguf import GGMLType, GGUFFile, GGUFWriter, InMemoryGGUF, MoEConfig
 from .dense import HipDenseMLP
 from .linear import FusedLinearPack, GGUFQuantLinear, HipQuantLinear
 from .moe import HipSparseMoEMLP
 from .norm import GGUFRMSNorm, HipRMSNorm, exec_fused_add_rmsnorm, exec_fused_rmsnorm
+from .sampling import sample_tokens
 
 # The reference's class names, so `from pgmoe import GGUFSparseMoEMLP` swaps the block in.
 GGUFSparseMoEMLP = HipSparseMoEMLP
@@ -18,4 +20,4 @@ GGUFDenseMLP = HipDenseMLP
 __all__ = ["GGMLType", "GGUFFile", "GGUFWriter", "InMemoryGGUF", "MoEConfig", "HipSparseMoEMLP",
            "GGUFSparseMoEMLP", "HipDenseMLP", "GGUFDenseMLP", "GGUFRMSNorm", "HipRMSNorm",
            "exec_fused_add_rmsnorm", "exec_fused_rmsnorm", "GGUFQuantLinear", "HipQuantLinear",
-           "FusedLinearPack"]
+           "FusedLinearPack", "HipPagedKVCache", "HipRotary", "KVBatch", "sample_tokens"]

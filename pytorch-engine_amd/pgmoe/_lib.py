@@ -74,6 +74,47 @@ class Dense(ctypes.Structure):
     ]
 
 
+class KVCache(ctypes.Structure):
+    _fields_ = [
+        ("k", _P),
+        ("v", _P),
+        ("page_stride", _I64),
+        ("head_stride", _I64),
+        ("row_stride", _I64),
+        ("n_pages", _I32),
+        ("page_size", _I32),
+        ("n_kv_heads", _I32),
+        ("head_dim", _I32),
+        ("dtype", _I32),
+    ]
+
+
+class KVBatch(ctypes.Structure):
+    _fields_ = [
+        ("page_table", _P),
+        ("lens", _P),
+        ("q_start", _P),
+        ("prefix_pages", _P),
+        ("table_stride", _I64),
+        ("n_seqs", _I32),
+        ("max_pages", _I32),
+        ("prefix_len", _I32),
+    ]
+
+
+class Sampling(ctypes.Structure):
+    _fields_ = [
+        ("temperatures", _P),
+        ("top_ks", _P),
+        ("top_ps", _P),
+        ("min_ps", _P),
+        ("temperature", ctypes.c_double),
+        ("top_p", ctypes.c_double),
+        ("min_p", ctypes.c_double),
+        ("top_k", _I32),
+    ]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -129,13 +170,22 @@ def lib() -> ctypes.CDLL:
     L.pgmoe_expert_down.argtypes = [ctypes.POINTER(Weights), _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _I32,
                                     _P, _P, _P, _P]
     L.pgmoe_combine.argtypes = [_P, _P, _I32, _I32, _I32, _P, _P, _P, _P]
+    kv = (ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch))
+    L.pgmoe_rope_append.argtypes = [*kv, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _I32, _P, _I32, _I32,
+                                    ctypes.c_float, _P, _P, ctypes.c_float, _P, _P]
+    L.pgmoe_attend_workspace_bytes.restype = ctypes.c_size_t
+    L.pgmoe_attend_workspace_bytes.argtypes = [*kv, _I32, _I32]
+    L.pgmoe_attend.argtypes = [*kv, _P, _I64, _I64, _I32, _I32, ctypes.c_float, _P, _P, _P, ctypes.c_size_t, _P]
+    L.pgmoe_sample_workspace_bytes.restype = ctypes.c_size_t
+    L.pgmoe_sample_workspace_bytes.argtypes = [_I32, _I32]
+    L.pgmoe_sample.argtypes = [_P, _I32, _I64, _I32, _I32, _P, ctypes.POINTER(Sampling), _P, _P, _P, ctypes.c_size_t, _P]
     for fn in ("pgmoe_moe_forward", "pgmoe_moe_forward_timed", "pgmoe_router_topk", "pgmoe_dispatch",
                "pgmoe_dispatch_ws", "pgmoe_expert_gateup",
                "pgmoe_expert_down", "pgmoe_combine", "pgmoe_relayout_weights", "pgmoe_relayout_weights_padded",
                "pgmoe_build_scale_plane",
                "pgmoe_dense_forward", "pgmoe_moe_routing", "pgmoe_moe_status", "pgmoe_moe_forward_noalloc",
                "pgmoe_add_rmsnorm", "pgmoe_linear_forward", "pgmoe_linear_forward_packed", "pgmoe_dequant_rows",
-               "pgmoe_requant_w4", "pgmoe_requant_w8_f16"):
+               "pgmoe_requant_w4", "pgmoe_requant_w8_f16", "pgmoe_rope_append", "pgmoe_attend", "pgmoe_sample"):
         getattr(L, fn).restype = ctypes.c_int
     ver = L.pgmoe_abi_version()
     if ver != ABI_VERSION:
@@ -159,7 +209,8 @@ EXPORTS = (
     "pgmoe_dense_workspace_bytes", "pgmoe_dense_forward", "pgmoe_moe_routing", "pgmoe_moe_status",
     "pgmoe_moe_forward_noalloc", "pgmoe_add_rmsnorm", "pgmoe_linear_workspace_bytes", "pgmoe_linear_forward",
     "pgmoe_dequant_rows", "pgmoe_relayout_weights_padded", "pgmoe_requant_w4", "pgmoe_requant_w8_f16",
-    "pgmoe_linear_forward_packed",
+    "pgmoe_linear_forward_packed", "pgmoe_rope_append", "pgmoe_attend_workspace_bytes", "pgmoe_attend",
+    "pgmoe_sample_workspace_bytes", "pgmoe_sample",
 )
 
 STATUS_SPIN_TIMEOUT = 1  # PGMOE_STATUS_SPIN_TIMEOUT

@@ -1,0 +1,332 @@
+"""Paged KV cache with rotary append and shared-prefix attention (pgmoe_rope_append, pgmoe_attend).
+
+The step between a layer's Q/K/V projections (FusedLinearPack) and its output projection:
+
+    rope  = HipRotary(head_dim, base=1e6)
+    cache = HipPagedKVCache(n_pages, page_size, n_kv_heads, head_dim)      # one a layer
+    batch = KVBatch(page_table, lens, q_start=..., prefix_pages=..., prefix_len=...)   # one a step, all layers
+    q = cache.append(q, k, v, batch, rope, q_norm=..., k_norm=...)   # norms + rotary + K/V rows, rotated q
+    o = cache.attend(q, batch)                                       # softmax(q K^T / sqrt(D)) V
+
+Every sequence sees the ``prefix_len`` keys of ``prefix_pages`` (a system prompt, a document) and then
+its own keys; the prefix's keys and values are read once for the whole batch.  The batch's tensors
+live on the device and are read when the kernels run: a program updates them in place between steps
+(``lens.add_(1)``), and a captured graph replays on what they then hold.  Nothing synchronises with
+the host.  There is no CPU path: CPU tensors, and types, widths and page sizes without a kernel,
+raise.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Dict, Optional, Sequence, Tuple, Union
+
+import torch
+
+from ._lib import KVBatch as _KVBatch
+from ._lib import KVCache as _KVCache
+from ._lib import check, lib
+
+_DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+_CACHE_DT = (torch.float16, torch.bfloat16)
+_DIMS = (64, 128, 256)
+_PAGES = (16, 32, 64, 128, 256)
+_MAX_SEQS = 4096
+
+_IntTensor = Union[torch.Tensor, Sequence[int]]
+
+
+def _on_device(dev: torch.device):
+    """A guard that makes `dev` current for a launch; nothing when it already is."""
+    return torch.cuda.device(dev)
+
+
+def _cuda_device(device: Optional[Union[torch.device, str]]) -> torch.device:
+    dev = torch.device("cuda" if device is None else device)
+    if dev.type != "cuda":
+        raise ValueError("pgmoe attention runs on a HIP device (torch.device('cuda', i))")
+    return torch.device("cuda", torch.cuda.current_device()) if dev.index is None else dev
+
+
+class HipRotary:
+    """Rotary positions: pair i turns by position * inv_freq[i] radians.
+
+    inv_freq: float64 [rotary_dim / 2], or None for base ** (-2 i / rotary_dim).  freq_factors (a
+    GGUF file's rope_freqs) divide it, position_scale multiplies every position (linear scaling),
+    attn_factor scales cosine and sine (YaRN).  Pairs are (i, i + rotary_dim / 2), or (2 i, 2 i + 1)
+    with interleaved."""
+
+    def __init__(self, head_dim: int, base: float = 10000.0, rotary_dim: Optional[int] = None,
+                 interleaved: bool = False, inv_freq: Optional[torch.Tensor] = None,
+                 freq_factors: Optional[torch.Tensor] = None, position_scale: float = 1.0, attn_factor: float = 1.0,
+                 device: Optional[Union[torch.device, str]] = None) -> None:
+        if inv_freq is not None:
+            if inv_freq.dim() != 1 or (rotary_dim is not None and inv_freq.numel() * 2 != rotary_dim):
+                raise ValueError("inv_freq holds one float64 frequency a pair (rotary_dim / 2)")
+            rotary_dim = 2 * inv_freq.numel()
+            if device is None:
+                device = inv_freq.device if inv_freq.device.type == "cuda" else None
+        rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
+        if rotary_dim < 16 or rotary_dim > head_dim or rotary_dim % 16:
+            raise ValueError(f"rotary_dim {rotary_dim}: a multiple of 16 up to head_dim {head_dim}")
+        if not (math.isfinite(position_scale) and math.isfinite(attn_factor) and base > 0):
+            raise ValueError("base must be positive, position_scale and attn_factor finite")
+        self.device = _cuda_device(device)
+        self.head_dim, self.rotary_dim, self.interleaved = int(head_dim), rotary_dim, bool(interleaved)
+        self.attn_factor = float(attn_factor)
+        if inv_freq is None:
+            inv_freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+        f = inv_freq.to("cpu", torch.float64)
+        if freq_factors is not None:
+            if freq_factors.numel() != rotary_dim // 2:
+                raise ValueError("freq_factors holds one factor a pair (rotary_dim / 2)")
+            f = f / freq_factors.to("cpu", torch.float64).reshape(-1)
+        self.turns = (f * (position_scale / (2.0 * math.pi))).to(self.device)
+
+
+class KVBatch:
+    """The sequences of one step (pgmoe_kv_batch): `page_table` int32 [n_seqs, max_pages], `lens`
+    int32 [n_seqs] (own keys of each sequence, this step's among them), `q_start` int32 [n_seqs + 1]
+    (first token row of each sequence and the end; None: one token each), `prefix_pages` int32 and
+    `prefix_len` (keys every sequence sees before its own).
+
+    Tensors on the device are kept, not copied, and may be updated in place.  Lists and CPU tensors
+    are checked and copied to the device."""
+
+    def __init__(self, page_table: _IntTensor, lens: _IntTensor, q_start: Optional[_IntTensor] = None,
+                 prefix_pages: Optional[_IntTensor] = None, prefix_len: int = 0,
+                 device: Optional[Union[torch.device, str]] = None) -> None:
+        given = [t for t in (page_table, lens, q_start, prefix_pages)
+                 if isinstance(t, torch.Tensor) and t.device.type == "cuda"]
+        self.device = given[0].device if given else _cuda_device(device)
+        self._table = self._int32("page_table", page_table, 2, -1)
+        self._lens = self._int32("lens", lens, 1, 0)
+        n = self._table.shape[0]
+        if not 1 <= n <= _MAX_SEQS:
+            raise NotImplementedError(f"{n} sequences (1 .. {_MAX_SEQS})")
+        if self._table.shape[1] < 1 or self._lens.shape[0] != n:
+            raise ValueError(f"page_table {tuple(self._table.shape)} and lens {tuple(self._lens.shape)} of {n} sequences")
+        self._q_start = None
+        if q_start is not None:
+            self._q_start = self._int32("q_start", q_start, 1, 0)
+            if self._q_start.shape[0] != n + 1:
+                raise ValueError(f"q_start holds {self._q_start.shape[0]} rows, {n} sequences need {n + 1}")
+            host = q_start if not isinstance(q_start, torch.Tensor) else q_start.tolist() if q_start.device.type == "cpu" else None
+            if host is not None and (host[0] != 0 or any(a > b for a, b in zip(host, host[1:]))):
+                raise ValueError("q_start begins at 0 and does not decrease")
+        self.prefix_len = int(prefix_len)
+        if self.prefix_len < 0:
+            raise ValueError("negative prefix_len")
+        self._prefix = None if prefix_pages is None else self._int32("prefix_pages", prefix_pages, 1, -1)
+        if self.prefix_len and self._prefix is None:
+            raise ValueError("prefix_len without prefix_pages")
+        self.n_seqs, self.max_pages = n, int(self._table.shape[1])
+        self._c = _KVBatch(self._table.data_ptr(), self._lens.data_ptr(),
+                           None if self._q_start is None else self._q_start.data_ptr(),
+                           None if self._prefix is None else self._prefix.data_ptr(),
+                           self._table.stride(0), n, self.max_pages, self.prefix_len)
+        self._ref = ctypes.byref(self._c)
+
+    def _int32(self, name: str, x: _IntTensor, dims: int, least: int) -> torch.Tensor:
+        t = x if isinstance(x, torch.Tensor) else torch.tensor(x, dtype=torch.int32)
+        if t.dim() != dims:
+            raise ValueError(f"{name} has {t.dim()} dimensions, not {dims}")
+        if t.device.type != "cuda":
+            if t.is_floating_point() or (t.numel() and (int(t.min()) < least or int(t.max()) > 2 ** 31 - 1)):
+                raise ValueError(f"{name} holds int32 values from {least} on")
+            return t.to(self.device, torch.int32).contiguous()
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} is an int32 tensor")
+        if t.device != self.device:
+            raise ValueError(f"{name} is on {t.device}, the batch on {self.device}")
+        if t.numel() and t.stride(-1) != 1:
+            raise ValueError(f"{name} must be contiguous along its rows")
+        return t
+
+    # the tensors the kernels read: updated in place, never replaced (the addresses are fixed)
+    page_table = property(lambda self: self._table)
+    lens = property(lambda self: self._lens)
+    q_start = property(lambda self: self._q_start)
+    prefix_pages = property(lambda self: self._prefix)
+
+
+class HipPagedKVCache:
+    """K and V pages of one attention layer: [n_pages, n_kv_heads, page_size, head_dim] each."""
+
+    def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+                 dtype: torch.dtype = torch.float16, device: Optional[Union[torch.device, str]] = None) -> None:
+        dev = _cuda_device(device)
+        self._check(n_pages, page_size, n_kv_heads, head_dim, dtype)
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        self._bind(torch.zeros(shape, dtype=dtype, device=dev), torch.zeros(shape, dtype=dtype, device=dev))
+
+    @classmethod
+    def from_tensors(cls, k: torch.Tensor, v: torch.Tensor) -> "HipPagedKVCache":
+        """A cache over existing pages, views of a larger allocation among them (a layer's slice, K and
+        V interleaved): both [n_pages, n_kv_heads, page_size, head_dim] with the same strides, the last
+        dimension contiguous, the others in multiples of 8 elements."""
+        self = cls.__new__(cls)
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
+            raise ValueError("k and v pages: [n_pages, n_kv_heads, page_size, head_dim] of one type, device and layout")
+        if k.device.type != "cuda":
+            raise ValueError("pgmoe attention runs on a HIP device tensor")
+        n, h, ps, d = k.shape
+        self._check(n, ps, h, d, k.dtype)
+        st = k.stride()
+        if st[3] != 1 or any(x % 8 for x in st[:3]) or k.data_ptr() % 16 or v.data_ptr() % 16:
+            raise ValueError("pages need a contiguous head_dim, strides of whole 16 bytes and 16-byte alignment")
+        if st[2] < d or st[2] > 1 << 22 or any(s <= 0 and m > 1 for s, m in zip(st, k.shape)):
+            raise ValueError("the rows of a page overlap or lie too far apart")
+        self._bind(k, v)
+        return self
+
+    @staticmethod
+    def _check(n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype) -> None:
+        if dtype not in _CACHE_DT:
+            raise NotImplementedError(f"KV cache of dtype {dtype} (fp16 or bf16)")
+        if head_dim not in _DIMS:
+            raise NotImplementedError(f"head_dim {head_dim} (one of {_DIMS})")
+        if page_size not in _PAGES:
+            raise NotImplementedError(f"page_size {page_size} (one of {_PAGES})")
+        if not (1 <= n_pages < 2 ** 31 and 1 <= n_kv_heads <= 1024):
+            raise ValueError(f"{n_pages} pages of {n_kv_heads} KV heads")
+
+    def _bind(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        lib()
+        self._k, self._v = k, v
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = (int(x) for x in k.shape)
+        self.dtype, self.device = k.dtype, k.device
+        st = k.stride()
+        self._c = _KVCache(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], self.n_pages, self.page_size,
+                           self.n_kv_heads, self.head_dim, _DT[k.dtype])
+        self._ref = ctypes.byref(self._c)
+        self._ws_bytes: Dict[Tuple[int, ...], int] = {}
+
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+
+    # ------------------------------------------------------------------ checks
+    def _heads(self, name: str, x: torch.Tensor, dtypes, heads: Optional[int] = None) -> torch.Tensor:
+        if x.device != self.device:
+            raise ValueError(f"{name} is on {x.device}, the cache on {self.device}")
+        if x.dtype not in dtypes:
+            raise NotImplementedError(f"{name} of dtype {x.dtype}")
+        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
+            raise ValueError(f"{name} {tuple(x.shape)}: [tokens, {'heads' if heads is None else heads}, {self.head_dim}]")
+        st = x.stride()
+        unit = 4 if x.dtype == torch.float32 else 8
+        if st[2] != 1 or st[0] % unit or st[1] % unit or x.data_ptr() % 16:
+            return x.clone(memory_format=torch.contiguous_format)  # rows the kernels cannot read 16 bytes at a time
+        return x
+
+    def _tokens(self, q: torch.Tensor, batch: KVBatch) -> Tuple[int, int]:
+        T, hq = int(q.shape[0]), int(q.shape[1])
+        if hq < 1 or hq % self.n_kv_heads:
+            raise ValueError(f"{hq} query heads on {self.n_kv_heads} KV heads")
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
+        if batch._q_start is None and T != batch.n_seqs:
+            raise ValueError(f"{T} tokens of {batch.n_seqs} sequences: q_start says which are whose")
+        if batch.prefix_len > (0 if batch._prefix is None else batch._prefix.shape[0]) * self.page_size:
+            raise ValueError(f"a prefix of {batch.prefix_len} keys on {batch._prefix.shape[0]} pages of {self.page_size}")
+        return T, hq
+
+    def _out(self, out: Optional[torch.Tensor], q: torch.Tensor, T: int, hq: int) -> torch.Tensor:
+        if out is None:
+            return torch.empty((T, hq, self.head_dim), dtype=self.dtype, device=self.device)
+        if out.shape != (T, hq, self.head_dim) or out.dtype != self.dtype or out.device != self.device:
+            raise ValueError(f"out: [{T}, {hq}, {self.head_dim}] of {self.dtype} on {self.device}")
+        if not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError("out must be contiguous and 16-byte aligned")
+        return out
+
+    @staticmethod
+    def _span(t: torch.Tensor) -> Tuple[int, int]:
+        n = sum((m - 1) * s for m, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+    def _apart(self, out: torch.Tensor, *others: torch.Tensor) -> None:
+        lo, hi = self._span(out)
+        for o in others:
+            a, b = self._span(o)
+            if lo < b and a < hi:
+                raise ValueError("out overlaps an input")
+
+    # ------------------------------------------------------------------ operators
+    def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: KVBatch,
+               rope: Optional[HipRotary] = None, q_norm: Optional[torch.Tensor] = None,
+               k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Write this step's keys and values into the pages and return the queries, q and k normalised
+        (per head, with norm weights [head_dim]) and rotated, in the cache's type [T, n_q_heads, head_dim].
+
+        q [T, n_q_heads, D], k and v [T, n_kv_heads, D]: fp32, fp16 or bf16, all of one type (the parts of
+        a fused projection's output as they are).  A token whose page does not exist (an id outside the
+        cache, a row past the page table) is not written.  Rows of `out` behind the last sequence are left
+        alone.  No two tokens may fall on one cache row."""
+        if k.dtype != q.dtype or v.dtype != q.dtype:
+            raise ValueError(f"q, k and v of one dtype, not {q.dtype}, {k.dtype}, {v.dtype}")
+        q = self._heads("q", q, _DT)
+        T, hq = self._tokens(q, batch)
+        k, v = self._heads("k", k, _DT, self.n_kv_heads), self._heads("v", v, _DT, self.n_kv_heads)
+        if k.shape[0] != T or v.shape[0] != T:
+            raise ValueError(f"{T} queries, {k.shape[0]} keys, {v.shape[0]} values")
+        turns, rot, inter, factor = None, 0, 0, 1.0
+        if rope is not None:
+            if rope.head_dim != self.head_dim or rope.device != self.device:
+                raise ValueError(f"rotary of head_dim {rope.head_dim} on {rope.device}, cache of {self.head_dim} on {self.device}")
+            turns, rot, inter, factor = rope.turns.data_ptr(), rope.rotary_dim, rope.interleaved, rope.attn_factor
+        norms = []
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None:
+                if w.numel() != self.head_dim or w.device != self.device:
+                    raise ValueError(f"{name}: {self.head_dim} weights on {self.device}")
+                w = w.to(torch.float32).contiguous()
+                if w.data_ptr() % 16:
+                    w = w.clone()
+            norms.append(w)
+        res = self._out(out, q, T, hq)
+        if out is not None:
+            self._apart(out, q, k, v, self._k, self._v)
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        with _on_device(self.device):
+            check(lib().pgmoe_rope_append(self._ref, batch._ref, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+                                          v.data_ptr(), vs[0], vs[1], _DT[q.dtype], T, hq, turns, rot, int(inter), factor,
+                                          None if norms[0] is None else norms[0].data_ptr(),
+                                          None if norms[1] is None else norms[1].data_ptr(), float(eps), res.data_ptr(),
+                                          torch.cuda.current_stream(self.device).cuda_stream), "pgmoe_rope_append")
+        return res
+
+    def attend(self, q: torch.Tensor, batch: KVBatch, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+               return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+        """softmax(scale * q K^T) V over the shared prefix and each sequence's own keys up to the query's
+        own, in the cache's type [T, n_q_heads, head_dim]; scale defaults to 1 / sqrt(head_dim).  With
+        return_lse also log(sum(exp(scale * q K^T))), fp32 [T, n_q_heads].
+
+        q [T, n_q_heads, D] in the cache's type; query head h reads KV head h // (n_q_heads / n_kv_heads).
+        A query that sees no key gets zeros and -inf; one that sees a key on a page that does not exist
+        gets NaN.  Masked keys and unused page rows may hold anything.  Rows of `out` behind the last
+        sequence are left alone."""
+        q = self._heads("q", q, (self.dtype,))
+        T, hq = self._tokens(q, batch)
+        scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        if not (0.0 < scale < 3e38):
+            raise ValueError("scale must be positive and finite")
+        res = self._out(out, q, T, hq)
+        if out is not None:
+            self._apart(out, q, self._k, self._v)
+        lse = torch.empty((T, hq), dtype=torch.float32, device=self.device) if return_lse else None
+        key = (T, hq, batch.n_seqs, batch.max_pages, batch.prefix_len, batch._q_start is None)
+        n = self._ws_bytes.get(key)
+        if n is None:
+            n = self._ws_bytes[key] = int(lib().pgmoe_attend_workspace_bytes(self._ref, batch._ref, T, hq))
+        # scratch of this call alone, from the stream's allocator: calls on other streams, and graphs that
+        # replay side by side, each have their own
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        qs = q.stride()
+        with _on_device(self.device):
+            check(lib().pgmoe_attend(self._ref, batch._ref, q.data_ptr(), qs[0], qs[1], T, hq, scale, res.data_ptr(),
+                                     None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), n,
+                                     torch.cuda.current_stream(self.device).cuda_stream), "pgmoe_attend")
+        return res if lse is None else (res, lse)
