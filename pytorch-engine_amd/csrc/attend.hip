@@ -1,95 +1,727 @@
 // Attention of a batch over a paged KV cache whose first keys are shared by every sequence.
 //
-// The simplest right form: one wave per (query, head) walks the keys with the running maximum and sum of
-// the softmax; each lane holds D / 64 columns, a score is a sum over the wave.
+// For query row (token t, head h) with visible keys j (the shared prefix, then the sequence's own up to the
+// query): o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale (q . k_j - max)), in one pass over the keys with the
+// running maximum and sum (exp2 of scores scaled by scale * log2 e in fp32).
+//
+// Rows that read the same keys are computed together: the rows of a sequence's tokens and of the query heads
+// that share a KV head, and on the prefix the rows of every sequence.  A segment is such a set of rows on one
+// KV head: up to 32 rows (kSplit: the 4 waves take different keys and meet at the end) or a tile of 128 (32
+// a wave, the waves share each tile of keys).  Segments are cut into tiles of 128 / 64 keys, and every
+// workgroup takes an equal run of the tiles of all segments in order, found on the device from lens and
+// q_start, so nothing about the lengths is known to or kept by the host.  A segment that several workgroups
+// share leaves unnormalised partial rows and their (max, sum), merged in slot order by combine_kernel.
+//
+// The products run on 32x32x16 MFMA, scores transposed: S^T = K Q^T has a query row per lane column, so the
+// maximum and sum of a row are sums over a lane's registers and one swap of wave halves, and the rounded
+// probabilities are already the B operand of O^T = V^T P^T (whose k index may be permuted as long as V's
+// rows are too).  K and V go from memory to LDS without registers, rows swizzled so that the 16-byte reads
+// of K and the transposing 8-byte reads of V meet no bank twice.
+//
+// Masked keys: a tile with a key that some row does not see takes the checked path: scores of masked keys
+// become -inf, and V values that are not finite reach only the rows that see them.  Rows past the last
+// visible key are read as copies of it.
+#include <atomic>
+
 #include "kv.h"
 #include "launch.h"
 
 namespace pgmoe {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 256;
+constexpr int kSplitKeys = 128, kSharedKeys = 64;  // keys of a tile, by kind of segment
+constexpr int kSharedRows = 128;
 
 struct AttendArgs {
     KvCache C;
     KvBatch B;
     const uint16_t* q;
     int64_t q_tok, q_head;
-    int T, hq;
-    float scale;
+    int T, hq, group;
+    float c;  // scale * log2(e)
     uint16_t* out;
     float* lse;
+    // partial rows [prefix, own][slot][T * hq][dim], their (max in log2 units, sum), and the slots a row has
+    float* part;
+    float2* ml;
+    int* slots;
+    int nslot;
+};
+
+template <int D>
+struct Geo {
+    static constexpr int RB = 2 * D;            // bytes of a row
+    static constexpr int CPB = D / 32;          // 1 KB copies of 16 rows
+    static constexpr int RPC = 16 / CPB;        // rows of a copy
+    static constexpr int LPR = 64 / RPC;        // lanes of a row in a copy
+    static constexpr int KM = D == 64 ? 7 : 15;  // K: 16-byte chunk c of row r lies at c ^ (r & KM)
+    static constexpr int LDS = 512 * D;         // both kinds of segment
+    static constexpr int OCC = D == 256 ? 1 : 2;  // waves a SIMD
+    // V: 32-byte pair p of row r lies at p ^ vswz(r)
+    __device__ static constexpr int vswz(int r) { return D == 64 ? (r >> 1) & 3 : r & 7; }
+};
+
+// 1 KB from memory to LDS, lane l's 16 bytes to lds + 16 l; waited for with vm_wait (copies are not in the
+// compiler's own count of loads, which only makes its waits longer).
+__device__ __forceinline__ void copy_lds(const void* base, uint32_t off, uint32_t lds) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(off), "s"(base), "s"(lds)
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uni64(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)uni((int)v) | (uint64_t)(uint32_t)uni((int)(v >> 32)) << 32);
+}
+// A scalar load: the index is the wave's, and nothing in this kernel writes page tables.
+__device__ __forceinline__ int sload(const int32_t* p, int64_t i) {
+    return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p)[i];
+}
+
+// One sequence's rows and keys.
+struct Seq {
+    int lo, n, len, cap, rows;
+    // keys that its token i sees: at most cap; `far` if lens says more
+    __device__ __forceinline__ int seen(int i, bool* far = nullptr) const {
+        const int64_t v = (int64_t)len - n + i + 1;
+        if (far) *far = v > cap;
+        return v < 0 ? 0 : v > cap ? cap : (int)v;
+    }
+    __device__ __forceinline__ int last_token(int tile, int group) const {
+        const int i = (kSharedRows * (tile + 1) - 1) / group;
+        return i < n - 1 ? i : n - 1;
+    }
+    __device__ __forceinline__ int tiles(int tile, int group) const {  // of row tile `tile`
+        const int k = rows <= 32 ? (seen(n - 1) + kSplitKeys - 1) / kSplitKeys
+                                 : (seen(last_token(tile, group)) + kSharedKeys - 1) / kSharedKeys;
+        return k < 1 ? 1 : k;
+    }
+};
+__device__ __forceinline__ Seq load_seq(const AttendArgs& A, int b) {
+    Seq s;
+    int hi;
+    seq_tokens(A.B, b, A.T, s.lo, hi);
+    s.n = hi - s.lo;
+    s.len = A.B.lens[b];
+    s.len = s.len < 0 ? 0 : s.len;
+    s.cap = A.B.max_pages << A.C.page_shift;
+    s.rows = s.n * A.group;
+    return s;
+}
+__device__ __forceinline__ int row_tiles(int rows) { return rows <= 32 ? (rows > 0) : (rows + kSharedRows - 1) / kSharedRows; }
+
+// What a workgroup computes at a time: tiles [j0, j1) of one segment.
+struct Work {
+    int prefix, split, lo, rows, row0, kvh, b, keys, j0, j1, slot, nslots;
+    int len, n, cap;  // own keys: Seq's
 };
 
 template <int D, bool BF16>
-__global__ __launch_bounds__(64) void attend_simple_kernel(const AttendArgs A) {
-    constexpr int N = D / 64;
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const int kvh = h / (A.hq / A.C.heads);
-    int b = t, lo = t, hi = t + 1;
-    if (A.B.q_start) {
-        int n = 0;
-        for (int i = lane; i < A.B.seqs; i += 64) n += A.B.q_start[i] <= t;
-        b = (int)group_sum<64>((float)n) - 1;
-        if (b < 0) return;
-        seq_tokens(A.B, b, A.T, lo, hi);
+struct Core {
+    using G = Geo<D>;
+    static constexpr int NK = D / 16, ND = D / 32;
+    u16x8 q[NK];
+    f32x16 o[ND];
+    float s[16];
+    u16x8 p[2];
+    float m, l, c;
+    int lane, n, h;
+    uint32_t koff, voff[ND];  // LDS byte offsets of this lane's reads
+
+    __device__ __forceinline__ static f32x16 mfma(u16x8 a, u16x8 b, f32x16 acc) {
+        if constexpr (BF16)
+            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                           acc, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), acc,
+                                                          0, 0, 0);
     }
-    if (b >= A.B.seqs || t < lo || t >= hi) return;
-    int len = A.B.lens[b];
-    len = len < 0 ? 0 : len;
-    const int cap = A.B.max_pages << A.C.page_shift;
-    int64_t seen = (int64_t)len - (hi - t) + 1;
-    const bool beyond = seen > cap;
-    const int own = seen < 0 ? 0 : seen > cap ? cap : (int)seen;
-    const uint16_t* qp = A.q + (int64_t)t * A.q_tok + (int64_t)h * A.q_head;
-    float q[N], o[N], m = -INFINITY, l = 0.0f;
+    __device__ __forceinline__ static float swap32(float v) { return xor_lane<32>(v); }
+
+    __device__ __forceinline__ void begin(int lane_) {
+        lane = lane_, n = lane & 31, h = lane >> 5;
+        m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) q[i] = from16<BF16>(qp[lane + 64 * i]) * A.scale, o[i] = 0.0f;
-    const int ps = 1 << A.C.page_shift;
-    for (int j = 0; j < A.B.prefix + own; ++j) {
-        const int jj = j < A.B.prefix ? j : j - A.B.prefix;
-        const int page = j < A.B.prefix ? A.B.prefix_pages[jj >> A.C.page_shift]
-                                        : A.B.table[(int64_t)b * A.B.table_stride + (jj >> A.C.page_shift)];
-        float s = 0.0f, v[N];
-        if (page >= 0 && page < A.C.n_pages) {
-            const int64_t at = (int64_t)page * A.C.page_stride + (int64_t)kvh * A.C.head_stride +
-                               (int64_t)(jj & (ps - 1)) * A.C.row_stride;
+        for (int i = 0; i < ND; ++i) o[i] = f32x16{};
+        koff = n * G::RB + ((h ^ (n & G::KM)) << 4);
+        // transposing read: 16 lanes take 4 rows of 16 columns, lane 4 r + i the row r and columns 4 i ..;
+        // each ends with its column of the 4 rows
+        const int r = 4 * h + ((lane & 15) >> 2);
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                s = __builtin_fmaf(q[i], from16<BF16>(A.C.k[at + lane + 64 * i]), s);
-                v[i] = from16<BF16>(A.C.v[at + lane + 64 * i]);
-            }
-        } else {
-            s = NAN;
+        for (int d = 0; d < ND; ++d)
+            voff[d] = r * G::RB + (((2 * d + ((lane >> 4) & 1)) ^ G::vswz(r)) << 5) + ((lane & 3) << 3);
+    }
+    // S^T of 32 keys: s[i] is key 8 (i / 4) + 4 h + i % 4 of this lane's row
+    __device__ __forceinline__ void scores(const uint8_t* K) {
+        f32x16 a{};
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = NAN;
+        for (int i = 0; i < NK; ++i) {
+            const u16x8 k = *(const u16x8*)(K + (koff ^ (uint32_t)(i << 5)));
+            a = mfma(k, q[i], a);
         }
-        s = group_sum<64>(s);
-        const float mn = fmaxf(m, s);
-        const float c = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(s - mn);
-        l = l * c + p;
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = o[i] * c + p * v[i];
-        m = mn;
+        for (int i = 0; i < 16; ++i) s[i] = a[i];
     }
-    const bool empty = A.B.prefix + own == 0;
-    if (beyond) l = NAN;
+    __device__ __forceinline__ static int key_of(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+    // left: visible keys of this lane's row from the tile's first on; bad: bit b: block b of 16 keys has no page
+    __device__ __forceinline__ void mask(int left, int bad) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        A.out[((int64_t)t * A.hq + h) * D + lane + 64 * i] = empty ? 0 : to16<BF16>(o[i] / l);
-    if (A.lse && lane == 0) A.lse[(int64_t)t * A.hq + h] = empty ? -INFINITY : m + logf(l);
+        for (int i = 0; i < 16; ++i) {
+            if ((bad >> (i >> 3)) & 1) s[i] = NAN;
+            if (key_of(i, h) >= left) s[i] = -INFINITY;
+        }
+    }
+    __device__ __forceinline__ void softmax() {
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        mx = fmaxf(mx, swap32(mx));
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx);
+            const float f = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * c);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= f;
+            m = mn;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -mc));
+            l += e;
+            p[i >> 3][i & 7] = to16<BF16>(e);
+        }
+    }
+    __device__ __forceinline__ u16x8 vfrag(const uint8_t* V, int st, int d) const {
+        typedef __attribute__((address_space(3))) s16x4* lp;
+        const uint8_t* at = V + voff[d] + st * 16 * G::RB;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)at);
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at + 8 * G::RB));
+        u16x8 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = (uint16_t)a[i], r[4 + i] = (uint16_t)b[i];
+        return r;
+    }
+    __device__ __forceinline__ void values(const uint8_t* V) {
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] = mfma(vfrag(V, st, d), p[st], o[d]);
+    }
+    __device__ __forceinline__ static bool odd(uint16_t v) {  // infinite or NaN
+        constexpr uint16_t e = BF16 ? 0x7f80 : 0x7c00;
+        return (v & e) == e;
+    }
+    // values() where some row does not see some key: what is not finite is left out, then added key by key to
+    // the rows that see it (0 * inf of a masked key would be NaN)
+    __device__ __forceinline__ void values_checked(const uint8_t* V, int left) {
+        uint32_t keys = 0;
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                u16x8 v = vfrag(V, st, d);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (odd(v[i])) {
+                        keys |= 1u << (16 * st + 8 * (i >> 2) + 4 * h + (i & 3));
+                        v[i] = 0;
+                    }
+                o[d] = mfma(v, p[st], o[d]);
+            }
+        if (!__any(keys != 0)) return;
+        keys |= xor_lane_u<1>(keys);
+        keys |= xor_lane_u<2>(keys);
+        keys |= xor_lane_u<4>(keys);
+        keys |= xor_lane_u<8>(keys);
+        keys |= xor_lane_u<16>(keys);
+        keys |= xor_lane_u<32>(keys);
+        for (uint32_t rest = uni((int)keys); rest; rest &= rest - 1) {
+            const int k = __builtin_ctz(rest);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                f32x16 a{};
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    u16x8 v = vfrag(V, st, d);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (!odd(v[i]) || 16 * st + 8 * (i >> 2) + 4 * h + (i & 3) != k) v[i] = 0;
+                    a = mfma(v, p[st], a);
+                }
+                if (k < left) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] += a[i];
+                }
+            }
+        }
+    }
+};
+
+// Copies the 16 rows of the key block that begins at key kb (a multiple of 16) of K or V into LDS; keys past
+// the last one are copies of it.  Returns whether the block has no page.
+template <int D, bool V>
+__device__ __forceinline__ bool copy_block(const AttendArgs& A, const uint16_t* cache, const int32_t* pages, int kvh, int kb,
+                                           int keys, int lane, uint32_t lds) {
+    using G = Geo<D>;
+    const int last = keys - 1;
+    const int ke = kb > last ? last & ~15 : kb;
+    int page = sload(pages, ke >> A.C.page_shift);
+    const bool bad = page < 0 || page >= A.C.n_pages;
+    if (bad) page = 0;
+    const uint16_t* base = cache + (int64_t)page * A.C.page_stride + (int64_t)kvh * A.C.head_stride +
+                           (int64_t)(ke & ((1 << A.C.page_shift) - 1)) * A.C.row_stride;
+    const uint32_t rs = (uint32_t)A.C.row_stride * 2;
+    const int lr = lane / G::LPR, cs = lane % G::LPR;
+    if (kb + 16 <= keys) {
+#pragma unroll
+        for (int i = 0; i < G::CPB; ++i) {
+            const int r = i * G::RPC + lr;
+            const uint32_t ch = V ? cs ^ (2 * G::vswz(r)) : cs ^ (r & G::KM);
+            copy_lds(base + (int64_t)(i * G::RPC) * A.C.row_stride, (uint32_t)lr * rs + (ch << 4), lds + i * 1024);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < G::CPB; ++i) {
+            const int r = i * G::RPC + lr;
+            const uint32_t ch = V ? cs ^ (2 * G::vswz(r)) : cs ^ (r & G::KM);
+            const int at = r + (kb - ke) < last - ke ? r + (kb - ke) : last - ke;
+            copy_lds(base, (uint32_t)at * rs + (ch << 4), lds + i * 1024);
+        }
+    }
+    return bad;
 }
 
-size_t attend_ws_bytes(const KvCache& C, const KvBatch& B, int T, int hq) { return 0; }
+// Four consecutive columns of a finished or partial row.
+template <int D, bool BF16>
+__device__ __forceinline__ void put4(const AttendArgs& A, const Work& W, bool direct, int64_t row, int d, float4 v,
+                                     float inv) {
+    if (direct) {
+        const uint32_t a = to16<BF16>(v.x * inv) | (uint32_t)to16<BF16>(v.y * inv) << 16;
+        const uint32_t b = to16<BF16>(v.z * inv) | (uint32_t)to16<BF16>(v.w * inv) << 16;
+        *(uint2*)(A.out + row * D + d) = make_uint2(a, b);
+    } else {
+        const int64_t R = (int64_t)A.T * A.hq;
+        *(float4*)(A.part + (((W.prefix ? 0 : A.nslot) + W.slot) * R + row) * D + d) = v;
+    }
+}
+// The row's statistics: lse of a finished row, (max, sum) of a partial one; slot 0 says how many there are.
+__device__ __forceinline__ void put_row(const AttendArgs& A, const Work& W, bool direct, int64_t row, float m, float l,
+                                        bool empty) {
+    if (direct) {
+        if (A.lse) A.lse[row] = empty ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    } else {
+        const int64_t R = (int64_t)A.T * A.hq;
+        A.ml[((W.prefix ? 0 : A.nslot) + W.slot) * R + row] = make_float2(m, l);
+    }
+    if (W.slot == 0 && A.slots) A.slots[(W.prefix ? 0 : (int64_t)A.T * A.hq) + row] = empty ? 0 : W.nslots;
+}
+
+template <int D, bool BF16>
+__global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const AttendArgs A) {
+    using G = Geo<D>;
+    using K = Core<D, BF16>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
+    __shared__ int64_t s_base[kThreads + 1];
+    __shared__ int64_t s_red[4];
+    __shared__ int s_max[4];
+    __shared__ float2 s_ml[4][32];
+    __shared__ Work s_work;
+    __shared__ int64_t s_start;
+    const int tid = threadIdx.x, lane = tid & 63, wv = uni(tid >> 6);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem;
+
+    // ---- the tiles of all segments: the prefix's, then each sequence's
+    const int per = (A.B.seqs + kThreads - 1) / kThreads;
+    int64_t mine = 0;
+    int most = 0;
+    for (int i = 0; i < per; ++i) {
+        const int b = tid * per + i;
+        if (b >= A.B.seqs) break;
+        const Seq s = load_seq(A, b);
+        const int rt = row_tiles(s.rows);
+        for (int t = 0; t < rt; ++t) {
+            const int k = s.tiles(t, A.group);
+            mine += k;
+            most = k > most ? k : most;
+        }
+    }
+    mine *= A.C.heads;
+    int64_t inc = mine;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t o = __shfl_up((long long)inc, d);
+        if (lane >= d) inc += o;
+        const int x = __shfl_xor(most, d);
+        most = x > most ? x : most;
+    }
+    if (lane == 63) s_red[wv] = inc, s_max[wv] = most;
+    __syncthreads();
+    int64_t before = inc - mine, own = 0;
+    most = 0;
+    for (int i = 0; i < 4; ++i) {
+        if (i < wv) before += s_red[i];
+        own += s_red[i];
+        most = s_max[i] > most ? s_max[i] : most;
+    }
+    s_base[tid] = before;
+    int Tq = A.T;
+    if (A.B.q_start) {
+        const int e = A.B.q_start[A.B.seqs];
+        Tq = e < 0 ? 0 : e < Tq ? e : Tq;
+    }
+    const int prows = A.B.prefix ? Tq * A.group : 0, prt = row_tiles(prows);
+    const int pkeys = prows <= 32 ? kSplitKeys : kSharedKeys;
+    const int ptiles = (A.B.prefix + pkeys - 1) / pkeys;
+    if (prt && ptiles > most) most = ptiles;
+    const int64_t shared = (int64_t)ptiles * prt * A.C.heads;
+    const int64_t total = uni64(shared + own);
+    // a workgroup's run of tiles: an equal share, and long enough that no segment meets more than nslot of them
+    int64_t run = (total + gridDim.x - 1) / gridDim.x;
+    if (A.nslot > 2) {
+        const int64_t least = (most + A.nslot - 3) / (A.nslot - 2);
+        run = run > least ? run : least;
+    } else {
+        run = total;
+    }
+    run = uni64(run < 1 ? 1 : run);
+
+    int64_t at = (int64_t)blockIdx.x * run;
+    const int64_t end = at + run < total ? at + run : total;
+    while (at < end) {
+        // ---- the segment that holds tile `at`
+        __syncthreads();
+        if (at < shared) {
+            if (tid == 0) {
+                const int seg = (int)(at / ptiles), j0 = (int)(at - (int64_t)seg * ptiles);
+                const int kvh = seg / prt, rt = seg % prt;
+                const int64_t left = end - at;
+                s_work = Work{1, prows <= 32, 0, prows, rt * kSharedRows, kvh, 0, A.B.prefix, j0,
+                              (int)(j0 + left < ptiles ? j0 + left : ptiles), 0, 0, 0, 0, 0};
+                s_start = at - j0;
+            }
+        } else {
+            const int64_t x = at - shared;
+            if (mine && x >= before && x < before + mine) {
+                int64_t loc = x - before;
+                for (int i = 0; i < per; ++i) {
+                    const int b = tid * per + i;
+                    const Seq s = load_seq(A, b);
+                    const int rt = row_tiles(s.rows);
+                    int64_t sum = 0;
+                    for (int t = 0; t < rt; ++t) sum += s.tiles(t, A.group);
+                    if (loc >= sum * A.C.heads) {
+                        loc -= sum * A.C.heads;
+                        continue;
+                    }
+                    const int kvh = (int)(loc / sum);
+                    int64_t j0 = loc - kvh * sum;
+                    int t = 0;
+                    while (j0 >= s.tiles(t, A.group)) j0 -= s.tiles(t++, A.group);
+                    const int nt = s.tiles(t, A.group);
+                    const int64_t left = end - at;
+                    const bool split = s.rows <= 32;
+                    s_work = Work{0, split, s.lo, s.rows, t * kSharedRows, kvh, b,
+                                  s.seen(split ? s.n - 1 : s.last_token(t, A.group)), (int)j0,
+                                  (int)(j0 + left < nt ? j0 + left : nt), 0, 0, s.len, s.n, s.cap};
+                    s_start = at - j0;
+                    s_work.nslots = nt;  // the segment's tiles, for now
+                    break;
+                }
+            }
+        }
+        __syncthreads();
+        Work W = s_work;
+        W.prefix = uni(W.prefix), W.split = uni(W.split), W.lo = uni(W.lo), W.rows = uni(W.rows), W.row0 = uni(W.row0);
+        W.kvh = uni(W.kvh), W.b = uni(W.b), W.keys = uni(W.keys), W.j0 = uni(W.j0), W.j1 = uni(W.j1);
+        W.len = uni(W.len), W.n = uni(W.n), W.cap = uni(W.cap);
+        {
+            const int64_t start = uni64(s_start);
+            const int nt = W.prefix ? ptiles : uni(W.nslots);
+            const int64_t first = start / run;
+            W.slot = (int)((int64_t)blockIdx.x - first);
+            W.nslots = (int)((start + nt - 1) / run - first) + 1;
+        }
+        const bool direct = !W.prefix && !A.B.prefix && W.nslots == 1;
+        const int32_t* pages = W.prefix ? A.B.prefix_pages : A.B.table + (int64_t)W.b * A.B.table_stride;
+
+        // ---- this lane's row
+        K core;
+        core.begin(lane);
+        core.c = A.c;
+        const int row = W.row0 + (W.split ? 0 : 32 * wv) + core.n;
+        const bool valid = row < W.rows;
+        const int rc = valid ? row : W.rows - 1;
+        const int tok = rc / A.group, head = W.kvh * A.group + rc % A.group;
+        const int64_t orow = (int64_t)(W.lo + tok) * A.hq + head;
+        bool far = false;
+        int seen = W.keys;
+        if (!W.prefix) {
+            Seq s;
+            s.len = W.len, s.n = W.n, s.cap = W.cap;
+            seen = s.seen(tok, &far);
+        }
+        const int seen0 = __builtin_amdgcn_readlane(seen, 0), seen1 = __builtin_amdgcn_readlane(seen, 31);
+        {
+            const uint16_t* qp = A.q + (int64_t)(W.lo + tok) * A.q_tok + (int64_t)head * A.q_head + 8 * core.h;
+#pragma unroll
+            for (int i = 0; i < K::NK; ++i) core.q[i] = *(const u16x8*)(qp + 16 * i);
+        }
+
+        if (W.split) {
+            // each wave its own 32 keys of every tile, K and V in buffers of its own: the next tile's K is on
+            // its way while this one's V is used, and the other way round
+            const uint32_t kb = lds0 + wv * 128 * D, vb = kb + 64 * D;
+            const uint8_t *kp = smem + wv * 128 * D, *vp = kp + 64 * D;
+            int key = W.j0 * kSplitKeys + 32 * wv;
+            const int stop = W.j1 * kSplitKeys < W.keys ? W.j1 * kSplitKeys : W.keys;
+            int bad = 0;
+            if (key < stop) {
+                bad = copy_block<D, false>(A, A.C.k, pages, W.kvh, key, W.keys, lane, kb);
+                bad |= copy_block<D, false>(A, A.C.k, pages, W.kvh, key + 16, W.keys, lane, kb + 32 * D) << 1;
+                copy_block<D, true>(A, A.C.v, pages, W.kvh, key, W.keys, lane, vb);
+                copy_block<D, true>(A, A.C.v, pages, W.kvh, key + 16, W.keys, lane, vb + 32 * D);
+            }
+            while (key < stop) {
+                const int next = key + kSplitKeys;
+                vm_wait<D / 16>();
+                core.scores(kp);
+                lds_wait();
+                int nbad = 0;
+                if (next < stop) {
+                    nbad = copy_block<D, false>(A, A.C.k, pages, W.kvh, next, W.keys, lane, kb);
+                    nbad |= copy_block<D, false>(A, A.C.k, pages, W.kvh, next + 16, W.keys, lane, kb + 32 * D) << 1;
+                }
+                const bool masked = key + 32 > seen0 || bad;
+                if (masked) core.mask(seen - key, bad);
+                core.softmax();
+                if (next < stop)
+                    vm_wait<D / 16>();
+                else
+                    vm_wait<0>();
+                if (masked)
+                    core.values_checked(vp, seen - key);
+                else
+                    core.values(vp);
+                lds_wait();
+                if (next < stop) {
+                    copy_block<D, true>(A, A.C.v, pages, W.kvh, next, W.keys, lane, vb);
+                    copy_block<D, true>(A, A.C.v, pages, W.kvh, next + 16, W.keys, lane, vb + 32 * D);
+                }
+                key = next;
+                bad = nbad;
+            }
+            // the four waves' rows meet in LDS
+            float l = core.l + K::swap32(core.l);
+            if (far) l = NAN;
+            __syncthreads();
+            float* so = (float*)smem;
+#pragma unroll
+            for (int d = 0; d < K::ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) so[(wv * (D / 2) + d * 16 + i) * 64 + lane] = core.o[d][i];
+            if (lane < 32) s_ml[wv][lane] = make_float2(core.m * A.c, l);
+            __syncthreads();
+            float f[4], mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_ml[w][core.n].x);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                f[w] = __builtin_amdgcn_exp2f(s_ml[w][core.n].x - (mx == -INFINITY ? 0.0f : mx));
+                sum = sum + f[w] * s_ml[w][core.n].y;
+            }
+            const bool empty = !W.prefix && !A.B.prefix && seen == 0;
+            const float inv = empty ? 0.0f : 1.0f / sum;
+            if (valid) {
+#pragma unroll
+                for (int g = 0; g < D / 32; ++g) {
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int reg = wv * (D / 8) + 4 * g + i;
+                        v[i] = 0.0f;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) v[i] += f[w] * so[(w * (D / 2) + reg) * 64 + lane];
+                    }
+                    const int reg = wv * (D / 8) + 4 * g;
+                    put4<D, BF16>(A, W, direct, orow, (reg >> 4) * 32 + 8 * ((reg & 15) >> 2) + 4 * core.h,
+                                  make_float4(v[0], v[1], v[2], v[3]), inv);
+                }
+                if (wv == 0 && core.h == 0) put_row(A, W, direct, orow, mx, sum, empty);
+            }
+        } else {
+            // every wave the same 64 keys, two buffers of K and V; a wave brings 16 rows of each
+            const int tile_rows = W.rows - W.row0;
+            const bool works = 32 * wv < tile_rows;
+            int bad = 0, nbad = 0;
+            auto bring = [&](int j) {
+                const uint32_t buf = lds0 + (j & 1) * 256 * D;
+                const int key = j * kSharedKeys;
+                copy_block<D, false>(A, A.C.k, pages, W.kvh, key + 16 * wv, W.keys, lane, buf + wv * 32 * D);
+                copy_block<D, true>(A, A.C.v, pages, W.kvh, key + 16 * wv, W.keys, lane, buf + 128 * D + wv * 32 * D);
+                nbad = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int kk = key + 16 * i < W.keys ? key + 16 * i : (W.keys - 1) & ~15;
+                    const int page = sload(pages, kk >> A.C.page_shift);
+                    nbad |= (page < 0 || page >= A.C.n_pages) << i;
+                }
+            };
+            if (W.j0 < W.j1 && W.keys > 0) bring(W.j0);
+            for (int j = W.j0; j < W.j1 && W.keys > 0; ++j) {
+                bad = nbad;
+                vm_wait<0>();
+                lds_barrier();
+                if (j + 1 < W.j1) bring(j + 1);
+                const uint8_t* buf = smem + (j & 1) * 256 * D;
+                if (works) {
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        const int key = j * kSharedKeys + 32 * half;
+                        if (key >= seen1) break;
+                        core.scores(buf + half * 64 * D);
+                        const int bb = (bad >> (2 * half)) & 3;
+                        const bool masked = key + 32 > seen0 || bb;
+                        if (masked) core.mask(seen - key, bb);
+                        core.softmax();
+                        if (masked)
+                            core.values_checked(buf + 128 * D + half * 64 * D, seen - key);
+                        else
+                            core.values(buf + 128 * D + half * 64 * D);
+                    }
+                }
+            }
+            float l = core.l + K::swap32(core.l);
+            if (far) l = NAN;
+            const bool empty = !W.prefix && !A.B.prefix && seen == 0;
+            const float inv = empty ? 0.0f : 1.0f / l;
+            if (valid) {
+#pragma unroll
+                for (int d = 0; d < K::ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        put4<D, BF16>(A, W, direct, orow, d * 32 + 8 * i + 4 * core.h,
+                                      make_float4(core.o[d][4 * i], core.o[d][4 * i + 1], core.o[d][4 * i + 2],
+                                                  core.o[d][4 * i + 3]),
+                                      inv);
+                if (core.h == 0) put_row(A, W, direct, orow, core.m * A.c, l, empty);
+            }
+        }
+        at += W.j1 - W.j0;
+    }
+}
+
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's slots in order; one wave a row.
+template <int D, bool BF16>
+__global__ __launch_bounds__(kThreads) void combine_rows_kernel(const AttendArgs A) {
+    constexpr int N = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t R = (int64_t)A.T * A.hq;
+    const int64_t row = (int64_t)blockIdx.x * 4 + uni(threadIdx.x >> 6);
+    if (row >= R) return;
+    if (A.B.q_start && row / A.hq >= A.B.q_start[A.B.seqs]) return;
+    if (!A.B.q_start && row / A.hq >= A.B.seqs) return;
+    int ns = A.slots[R + row], np = A.B.prefix ? A.slots[row] : 0;
+    if (!A.B.prefix && ns == 1) return;  // written by the only workgroup that had it
+    if (!A.B.prefix && ns == 0) {  // a row that sees nothing
+#pragma unroll
+        for (int i = 0; i < N; ++i) A.out[row * D + N * lane + i] = 0;
+        if (A.lse && lane == 0) A.lse[row] = -INFINITY;
+        return;
+    }
+    ns = ns < 0 ? 0 : ns > A.nslot ? A.nslot : ns;
+    np = np < 0 ? 0 : np > A.nslot ? A.nslot : np;
+    const int all = np + ns;
+    auto place = [&](int s) { return (s < np ? s : A.nslot + s - np) * R + row; };
+    float mx = -INFINITY;
+    for (int s = lane; s < all; s += 64) mx = fmaxf(mx, A.ml[place(s)].x);
+    mx = wave_max(mx);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    float o[N], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = 0.0f;
+    for (int s = 0; s < all; ++s) {
+        const int64_t at = place(s);
+        const float2 ml = A.ml[at];
+        const float f = __builtin_amdgcn_exp2f(ml.x - ref);
+        sum += f * ml.y;
+        const float* p = A.part + at * D + N * lane;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] += f * p[i];
+    }
+    const float inv = 1.0f / sum;
+    uint16_t* w = A.out + row * D + N * lane;
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = to16<BF16>(o[i] * inv);
+    if (A.lse && lane == 0) A.lse[row] = (mx + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+}
+
+static int attend_slots(int64_t rows, int D) {
+    // partial rows of at most 256 MiB a region, 130 slots (a long sequence alone on the chip), at least 4
+    int64_t n = ((int64_t)256 << 20) / (rows * D * 4);
+    return (int)(n < 4 ? 4 : n > 130 ? 130 : n);
+}
+struct AttendWs {
+    int64_t ml, slots, total;
+    int nslot;
+};
+static AttendWs attend_ws(const KvCache& C, const KvBatch& B, int T, int hq) {
+    const int64_t R = (int64_t)T * hq;
+    AttendWs w;
+    w.nslot = attend_slots(R, C.dim);
+    const int regions = 2;
+    w.ml = R * w.nslot * regions * C.dim * 4;
+    w.slots = w.ml + R * w.nslot * regions * 8;
+    w.total = (w.slots + R * 2 * 4 + 255) / 256 * 256;
+    return w;
+}
+size_t attend_ws_bytes(const KvCache& C, const KvBatch& B, int T, int hq) { return attend_ws(C, B, T, hq).total; }
+
+static int cu_count() {
+    static std::atomic<int> cached[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    int n = cached[dev].load(std::memory_order_relaxed);
+    if (!n) {
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+        cached[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
 
 int launch_attend(const KvCache& C, const KvBatch& B, const uint16_t* q, int64_t q_tok, int64_t q_head, int T, int hq,
                   float scale, uint16_t* out, float* lse, void* ws, hipStream_t st) {
     if (T == 0) return PGMOE_OK;
-    AttendArgs A{C, B, q, q_tok, q_head, T, hq, scale, out, lse};
-    const dim3 grid(T, hq), block(64);
-#define ATT(D)                                                                   \
-    do {                                                                         \
-        if (C.bf16)                                                              \
-            PG_LAUNCH((attend_simple_kernel<D, true>), grid, block, 0, st, A);   \
-        else                                                                     \
-            PG_LAUNCH((attend_simple_kernel<D, false>), grid, block, 0, st, A);  \
+    const AttendWs w = attend_ws(C, B, T, hq);
+    uint8_t* b = (uint8_t*)ws;
+    const AttendArgs A{C,   B,   q,   q_tok, q_head, T, hq, hq / C.heads, scale * 1.4426950408889634f, out,
+                       lse, (float*)b, (float2*)(b + w.ml), (int*)(b + w.slots), w.nslot};
+    const int64_t R = (int64_t)T * hq;
+    const dim3 block(kThreads);
+#define ATT(D)                                                                                                \
+    do {                                                                                                      \
+        const dim3 grid(cu_count() * Geo<D>::OCC), rows((unsigned)((R + 3) / 4));                             \
+        if (C.bf16) {                                                                                         \
+            PG_LAUNCH((attend_kernel<D, true>), grid, block, 0, st, A);                                       \
+            PG_LAUNCH((combine_rows_kernel<D, true>), rows, block, 0, st, A);                                 \
+        } else {                                                                                              \
+            PG_LAUNCH((attend_kernel<D, false>), grid, block, 0, st, A);                                      \
+            PG_LAUNCH((combine_rows_kernel<D, false>), rows, block, 0, st, A);                                \
+        }                                                                                                     \
     } while (0)
     if (C.dim == 64)
         ATT(64);
