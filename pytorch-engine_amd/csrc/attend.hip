@@ -129,15 +129,14 @@ struct Work {
     int len, n, cap;  // own keys: Seq's
 };
 
+// The products and softmax of one wave's 32 rows, N2 groups of 32 keys at a time.
 template <int D, bool BF16>
 struct Core {
     using G = Geo<D>;
     static constexpr int NK = D / 16, ND = D / 32;
     u16x8 q[NK];
     f32x16 o[ND];
-    float s[16];
-    u16x8 p[2];
-    float m, l, c;
+    float m, l, c;  // reference maximum (raw score), sum over this lane's keys, scale * log2(e)
     int lane, n, h;
     uint32_t koff, voff[ND];  // LDS byte offsets of this lane's reads
 
@@ -164,32 +163,38 @@ struct Core {
         for (int d = 0; d < ND; ++d)
             voff[d] = r * G::RB + (((2 * d + ((lane >> 4) & 1)) ^ G::vswz(r)) << 5) + ((lane & 3) << 3);
     }
-    // S^T of 32 keys: s[i] is key 8 (i / 4) + 4 h + i % 4 of this lane's row
-    __device__ __forceinline__ void scores(const uint8_t* K) {
-        f32x16 a{};
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const u16x8 k = *(const u16x8*)(K + (koff ^ (uint32_t)(i << 5)));
-            a = mfma(k, q[i], a);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = a[i];
-    }
     __device__ __forceinline__ static int key_of(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
-    // left: visible keys of this lane's row from the tile's first on; bad: bit b: block b of 16 keys has no page
-    __device__ __forceinline__ void mask(int left, int bad) {
+    // S^T of N2 * 32 keys: s[g][i] is key 32 g + key_of(i, h) of this lane's row
+    template <int N2>
+    __device__ __forceinline__ void scores(const uint8_t* K, f32x16 (&s)[N2]) {
+#pragma unroll
+        for (int g = 0; g < N2; ++g) s[g] = f32x16{};
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int g = 0; g < N2; ++g)
+                s[g] = mfma(*(const u16x8*)(K + g * 32 * G::RB + (koff ^ (uint32_t)(i << 5))), q[i], s[g]);
+    }
+    // left: visible keys of this lane's row from the group's first on; bad: bit b: block b of 16 keys has no page
+    __device__ __forceinline__ void mask(f32x16& s, int left, int bad) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             if ((bad >> (i >> 3)) & 1) s[i] = NAN;
             if (key_of(i, h) >= left) s[i] = -INFINITY;
         }
     }
-    __device__ __forceinline__ void softmax() {
-        float mx = s[0];
+    // p = 2^(c (s - m)) rounded, l += sum p.  The reference m follows the maximum only when that has grown
+    // by 2^8: p stays within fp16's range and its relative precision, and the rescaling of o (64 products a
+    // lane) all but vanishes.
+    template <int N2>
+    __device__ __forceinline__ void softmax(const f32x16 (&s)[N2], u16x8 (&p)[2 * N2]) {
+        float mx = s[0][0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        for (int g = 0; g < N2; ++g)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[g][i]);
         mx = fmaxf(mx, swap32(mx));
-        if (__any(mx > m)) {
+        if (__any((mx - m) * c > 8.0f)) {
             const float mn = fmaxf(m, mx);
             const float f = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * c);
             l *= f;
@@ -201,11 +206,13 @@ struct Core {
         }
         const float mc = m == -INFINITY ? 0.0f : m * c;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -mc));
-            l += e;
-            p[i >> 3][i & 7] = to16<BF16>(e);
-        }
+        for (int g = 0; g < N2; ++g)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][i], c, -mc));
+                l += e;
+                p[2 * g + (i >> 3)][i & 7] = to16<BF16>(e);
+            }
     }
     __device__ __forceinline__ u16x8 vfrag(const uint8_t* V, int st, int d) const {
         typedef __attribute__((address_space(3))) s16x4* lp;
@@ -217,9 +224,10 @@ struct Core {
         for (int i = 0; i < 4; ++i) r[i] = (uint16_t)a[i], r[4 + i] = (uint16_t)b[i];
         return r;
     }
-    __device__ __forceinline__ void values(const uint8_t* V) {
+    template <int N2>
+    __device__ __forceinline__ void values(const uint8_t* V, const u16x8 (&p)[2 * N2]) {
 #pragma unroll
-        for (int st = 0; st < 2; ++st)
+        for (int st = 0; st < 2 * N2; ++st)
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] = mfma(vfrag(V, st, d), p[st], o[d]);
     }
@@ -227,9 +235,9 @@ struct Core {
         constexpr uint16_t e = BF16 ? 0x7f80 : 0x7c00;
         return (v & e) == e;
     }
-    // values() where some row does not see some key: what is not finite is left out, then added key by key to
-    // the rows that see it (0 * inf of a masked key would be NaN)
-    __device__ __forceinline__ void values_checked(const uint8_t* V, int left) {
+    // values() of 32 keys where some row does not see some key: what is not finite is left out, then added
+    // key by key to the rows that see it (0 * inf of a masked key would be NaN)
+    __device__ __forceinline__ void values_checked(const uint8_t* V, const u16x8 (&p)[2], int left) {
         uint32_t keys = 0;
 #pragma unroll
         for (int st = 0; st < 2; ++st)
@@ -271,22 +279,31 @@ struct Core {
             }
         }
     }
+    // 32 keys with masks
+    __device__ __forceinline__ void checked(const uint8_t* K, const uint8_t* V, int left, int bad) {
+        f32x16 s[1];
+        u16x8 p[2];
+        scores<1>(K, s);
+        mask(s[0], left, bad);
+        softmax<1>(s, p);
+        values_checked(V, p, left);
+    }
 };
 
 // Copies the 16 rows of the key block that begins at key kb (a multiple of 16) of K or V into LDS; keys past
-// the last one are copies of it.  Returns whether the block has no page.
+// the last one are copies of it, and a page that does not exist is read as page 0.
 template <int D, bool V>
-__device__ __forceinline__ bool copy_block(const AttendArgs& A, const uint16_t* cache, const int32_t* pages, int kvh, int kb,
+__device__ __forceinline__ void copy_block(const AttendArgs& A, const uint16_t* cache, const int32_t* pages, int kvh, int kb,
                                            int keys, int lane, uint32_t lds) {
     using G = Geo<D>;
     const int last = keys - 1;
     const int ke = kb > last ? last & ~15 : kb;
     int page = sload(pages, ke >> A.C.page_shift);
-    const bool bad = page < 0 || page >= A.C.n_pages;
-    if (bad) page = 0;
+    if (page < 0 || page >= A.C.n_pages) page = 0;
     const uint16_t* base = cache + (int64_t)page * A.C.page_stride + (int64_t)kvh * A.C.head_stride +
                            (int64_t)(ke & ((1 << A.C.page_shift) - 1)) * A.C.row_stride;
     const uint32_t rs = (uint32_t)A.C.row_stride * 2;
+    asm volatile("" : "+v"(lane));  // offsets made here, not held (or spilled) across the loop
     const int lr = lane / G::LPR, cs = lane % G::LPR;
     if (kb + 16 <= keys) {
 #pragma unroll
@@ -303,6 +320,15 @@ __device__ __forceinline__ bool copy_block(const AttendArgs& A, const uint16_t* 
             const int at = r + (kb - ke) < last - ke ? r + (kb - ke) : last - ke;
             copy_lds(base, (uint32_t)at * rs + (ch << 4), lds + i * 1024);
         }
+    }
+}
+// Bit b: the block of 16 keys from key + 16 b on has no page (keys past the last one count as it).
+__device__ __forceinline__ int bad_blocks(const AttendArgs& A, const int32_t* pages, int key, int keys, int blocks) {
+    int bad = 0;
+    for (int i = 0; i < blocks; ++i) {
+        const int k = key + 16 * i < keys ? key + 16 * i : keys - 1;
+        const int page = sload(pages, k >> A.C.page_shift);
+        bad |= (page < 0 || page >= A.C.n_pages) << i;
     }
     return bad;
 }
@@ -475,55 +501,71 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             s.len = W.len, s.n = W.n, s.cap = W.cap;
             seen = s.seen(tok, &far);
         }
-        const int seen0 = __builtin_amdgcn_readlane(seen, 0), seen1 = __builtin_amdgcn_readlane(seen, 31);
+        const int seen1 = __builtin_amdgcn_readlane(seen, 31);  // the wave's last row sees most
         {
             const uint16_t* qp = A.q + (int64_t)(W.lo + tok) * A.q_tok + (int64_t)head * A.q_head + 8 * core.h;
 #pragma unroll
             for (int i = 0; i < K::NK; ++i) core.q[i] = *(const u16x8*)(qp + 16 * i);
         }
+        // tiles whose every key is there and seen by every row need no checks: [j0, jf)
+        const int tk = W.split ? kSplitKeys : kSharedKeys;
+        int jf;
+        {
+            bool ok = true;
+            const int k0 = W.j0 * tk, k1 = W.j1 * tk < W.keys ? W.j1 * tk : W.keys;
+            for (int i = (k0 >> A.C.page_shift) + lane; (int64_t)i << A.C.page_shift < k1; i += 64) {
+                const int page = pages[i];
+                ok = ok && page >= 0 && page < A.C.n_pages;
+            }
+            // the first row of the whole tile sees least
+            Seq s;
+            s.len = W.len, s.n = W.n, s.cap = W.cap;
+            const int least = W.prefix ? W.keys : uni(s.seen(W.row0 / A.group));
+            jf = __all(ok) ? least / tk : 0;
+            jf = jf < W.j0 ? W.j0 : jf < W.j1 ? jf : W.j1;
+        }
+#pragma unroll
+        for (int i = 0; i < K::NK; ++i) asm volatile("" : "+v"(core.q[i]));  // arrived before the loops
 
         if (W.split) {
             // each wave its own 32 keys of every tile, K and V in buffers of its own: the next tile's K is on
             // its way while this one's V is used, and the other way round
             const uint32_t kb = lds0 + wv * 128 * D, vb = kb + 64 * D;
             const uint8_t *kp = smem + wv * 128 * D, *vp = kp + 64 * D;
-            int key = W.j0 * kSplitKeys + 32 * wv;
-            const int stop = W.j1 * kSplitKeys < W.keys ? W.j1 * kSplitKeys : W.keys;
-            int bad = 0;
-            if (key < stop) {
-                bad = copy_block<D, false>(A, A.C.k, pages, W.kvh, key, W.keys, lane, kb);
-                bad |= copy_block<D, false>(A, A.C.k, pages, W.kvh, key + 16, W.keys, lane, kb + 32 * D) << 1;
+            auto bring_k = [&](int key) {
+                copy_block<D, false>(A, A.C.k, pages, W.kvh, key, W.keys, lane, kb);
+                copy_block<D, false>(A, A.C.k, pages, W.kvh, key + 16, W.keys, lane, kb + 32 * D);
+            };
+            auto bring_v = [&](int key) {
                 copy_block<D, true>(A, A.C.v, pages, W.kvh, key, W.keys, lane, vb);
                 copy_block<D, true>(A, A.C.v, pages, W.kvh, key + 16, W.keys, lane, vb + 32 * D);
-            }
-            while (key < stop) {
+            };
+            int key = W.j0 * kSplitKeys + 32 * wv;
+            const int stop = W.j1 * kSplitKeys < W.keys ? W.j1 * kSplitKeys : W.keys;
+            if (key < stop) bring_k(key), bring_v(key);
+            for (int j = W.j0; j < jf; ++j) {
                 const int next = key + kSplitKeys;
+                f32x16 s[1];
+                u16x8 p[2];
                 vm_wait<D / 16>();
-                core.scores(kp);
+                core.template scores<1>(kp, s);
                 lds_wait();
-                int nbad = 0;
-                if (next < stop) {
-                    nbad = copy_block<D, false>(A, A.C.k, pages, W.kvh, next, W.keys, lane, kb);
-                    nbad |= copy_block<D, false>(A, A.C.k, pages, W.kvh, next + 16, W.keys, lane, kb + 32 * D) << 1;
-                }
-                const bool masked = key + 32 > seen0 || bad;
-                if (masked) core.mask(seen - key, bad);
-                core.softmax();
+                if (next < stop) bring_k(next);
+                core.template softmax<1>(s, p);
                 if (next < stop)
                     vm_wait<D / 16>();
                 else
                     vm_wait<0>();
-                if (masked)
-                    core.values_checked(vp, seen - key);
-                else
-                    core.values(vp);
+                core.template values<1>(vp, p);
                 lds_wait();
-                if (next < stop) {
-                    copy_block<D, true>(A, A.C.v, pages, W.kvh, next, W.keys, lane, vb);
-                    copy_block<D, true>(A, A.C.v, pages, W.kvh, next + 16, W.keys, lane, vb + 32 * D);
-                }
+                if (next < stop) bring_v(next);
                 key = next;
-                bad = nbad;
+            }
+            for (; key < stop; key += kSplitKeys) {
+                vm_wait<0>();
+                core.checked(kp, vp, seen - key, bad_blocks(A, pages, key, W.keys, 2));
+                lds_wait();
+                if (key + kSplitKeys < stop) bring_k(key + kSplitKeys), bring_v(key + kSplitKeys);
             }
             // the four waves' rows meet in LDS
             float l = core.l + K::swap32(core.l);
@@ -565,44 +607,40 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             }
         } else {
             // every wave the same 64 keys, two buffers of K and V; a wave brings 16 rows of each
-            const int tile_rows = W.rows - W.row0;
-            const bool works = 32 * wv < tile_rows;
-            int bad = 0, nbad = 0;
+            const bool works = 32 * wv < W.rows - W.row0;
             auto bring = [&](int j) {
                 const uint32_t buf = lds0 + (j & 1) * 256 * D;
-                const int key = j * kSharedKeys;
-                copy_block<D, false>(A, A.C.k, pages, W.kvh, key + 16 * wv, W.keys, lane, buf + wv * 32 * D);
-                copy_block<D, true>(A, A.C.v, pages, W.kvh, key + 16 * wv, W.keys, lane, buf + 128 * D + wv * 32 * D);
-                nbad = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int kk = key + 16 * i < W.keys ? key + 16 * i : (W.keys - 1) & ~15;
-                    const int page = sload(pages, kk >> A.C.page_shift);
-                    nbad |= (page < 0 || page >= A.C.n_pages) << i;
-                }
+                const int key = j * kSharedKeys + 16 * wv;
+                copy_block<D, false>(A, A.C.k, pages, W.kvh, key, W.keys, lane, buf + wv * 32 * D);
+                copy_block<D, true>(A, A.C.v, pages, W.kvh, key, W.keys, lane, buf + 128 * D + wv * 32 * D);
             };
-            if (W.j0 < W.j1 && W.keys > 0) bring(W.j0);
-            for (int j = W.j0; j < W.j1 && W.keys > 0; ++j) {
-                bad = nbad;
+            const int stop = W.keys > 0 ? W.j1 : W.j0;
+            if (W.j0 < stop) bring(W.j0);
+            int j = W.j0;
+            for (; j < jf; ++j) {
                 vm_wait<0>();
                 lds_barrier();
-                if (j + 1 < W.j1) bring(j + 1);
+                if (j + 1 < stop) bring(j + 1);
                 const uint8_t* buf = smem + (j & 1) * 256 * D;
                 if (works) {
+                    f32x16 s[2];
+                    u16x8 p[4];
+                    core.template scores<2>(buf, s);
+                    core.template softmax<2>(s, p);
+                    core.template values<2>(buf + 128 * D, p);
+                }
+            }
+            for (; j < stop; ++j) {
+                vm_wait<0>();
+                lds_barrier();
+                if (j + 1 < stop) bring(j + 1);
+                const uint8_t* buf = smem + (j & 1) * 256 * D;
 #pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        const int key = j * kSharedKeys + 32 * half;
-                        if (key >= seen1) break;
-                        core.scores(buf + half * 64 * D);
-                        const int bb = (bad >> (2 * half)) & 3;
-                        const bool masked = key + 32 > seen0 || bb;
-                        if (masked) core.mask(seen - key, bb);
-                        core.softmax();
-                        if (masked)
-                            core.values_checked(buf + 128 * D + half * 64 * D, seen - key);
-                        else
-                            core.values(buf + 128 * D + half * 64 * D);
-                    }
+                for (int half = 0; half < 2 && works; ++half) {
+                    const int key = j * kSharedKeys + 32 * half;
+                    if (key >= seen1) break;
+                    core.checked(buf + half * 64 * D, buf + 128 * D + half * 64 * D, seen - key,
+                                 bad_blocks(A, pages, key, W.keys, 2));
                 }
             }
             float l = core.l + K::swap32(core.l);
