@@ -6,11 +6,11 @@
 //
 // Rows that read the same keys are computed together: the rows of a sequence's tokens and of the query heads
 // that share a KV head, and on the prefix the rows of every sequence.  A segment is such a set of rows on one
-// KV head: up to 32 rows (kSplit: the 4 waves take different keys and meet at the end) or a tile of 128 (32
-// a wave, the waves share each tile of keys).  Segments are cut into tiles of 128 / 64 keys, and every
-// workgroup takes an equal run of the tiles of all segments in order, found on the device from lens and
-// q_start, so nothing about the lengths is known to or kept by the host.  A segment that several workgroups
-// share leaves unnormalised partial rows and their (max, sum), merged in slot order by combine_kernel.
+// KV head: up to 32 rows (split: one wave's) or a tile of 128 (shared: 32 a wave, the four waves share each
+// tile of keys).  Every wave takes an equal run of the tiles of all split segments in order, then every
+// workgroup one of the shared segments', found on the device from lens and q_start, so nothing about the
+// lengths is known to or kept by the host.  A segment that several runs share leaves unnormalised partial
+// rows and their (max, sum), merged in slot order by combine_rows_kernel.
 //
 // The products run on 32x32x16 MFMA, scores transposed: S^T = K Q^T has a query row per lane column, so the
 // maximum and sum of a row are sums over a lane's registers and one swap of wave halves, and the rounded
@@ -34,8 +34,11 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 256;
-constexpr int kSplitKeys = 128, kSharedKeys = 64;  // keys of a tile, by kind of segment
-constexpr int kSharedRows = 128;
+constexpr int kValu = 0x2, kMfma = 0x8, kDs = 0x100;  // instruction classes of sched_group_barrier
+constexpr int kSplitKeys = 32, kSharedKeys = 64;  // keys of a tile, by kind of segment
+constexpr int kSplitRows = 32, kSharedRows = 128;
+constexpr int kSplitLeast = 4;  // tiles of a wave's run at least
+constexpr int kSplitHead = 3, kSharedHead = 5;  // what a segment costs beside its tiles, in tiles
 
 struct AttendArgs {
     KvCache C;
@@ -104,9 +107,10 @@ struct Seq {
         const int i = (kSharedRows * (tile + 1) - 1) / group;
         return i < n - 1 ? i : n - 1;
     }
-    __device__ __forceinline__ int tiles(int tile, int group) const {  // of row tile `tile`
-        const int k = rows <= 32 ? (seen(n - 1) + kSplitKeys - 1) / kSplitKeys
-                                 : (seen(last_token(tile, group)) + kSharedKeys - 1) / kSharedKeys;
+    __device__ __forceinline__ bool split() const { return rows <= kSplitRows; }
+    __device__ __forceinline__ int tiles(int tile, int group) const {  // of row tile `tile`; one at least
+        const int k = split() ? (seen(n - 1) + kSplitKeys - 1) / kSplitKeys
+                              : (seen(last_token(tile, group)) + kSharedKeys - 1) / kSharedKeys;
         return k < 1 ? 1 : k;
     }
 };
@@ -121,12 +125,117 @@ __device__ __forceinline__ Seq load_seq(const AttendArgs& A, int b) {
     s.rows = s.n * A.group;
     return s;
 }
-__device__ __forceinline__ int row_tiles(int rows) { return rows <= 32 ? (rows > 0) : (rows + kSharedRows - 1) / kSharedRows; }
+__device__ __forceinline__ int row_tiles(int rows) {
+    return rows <= kSplitRows ? (rows > 0) : (rows + kSharedRows - 1) / kSharedRows;
+}
 
-// What a workgroup computes at a time: tiles [j0, j1) of one segment.
+// Tiles [j0, j1) of one segment: what a wave (split) or a workgroup (shared) computes at a time.
 struct Work {
-    int prefix, split, lo, rows, row0, kvh, b, keys, j0, j1, slot, nslots;
+    int prefix, lo, rows, row0, kvh, b, keys, j0, j1, slot, nslots;
     int len, n, cap;  // own keys: Seq's
+    int left;         // of the run behind this work
+    __device__ __forceinline__ void scalar() {  // every lane holds the same: into scalar registers
+        prefix = uni(prefix), lo = uni(lo), rows = uni(rows), row0 = uni(row0), kvh = uni(kvh), b = uni(b);
+        keys = uni(keys), j0 = uni(j0), j1 = uni(j1), slot = uni(slot), nslots = uni(nslots);
+        len = uni(len), n = uni(n), cap = uni(cap), left = uni(left);
+    }
+};
+
+// The prefix's segments of one kind and the sequences' of that kind lie one behind the other on an axis of
+// tiles, each with kHead tiles' room before its first for what a segment costs by itself.  s_base holds
+// where each thread's sequences begin.
+template <bool SPLIT>
+struct Axis {
+    static constexpr int kHead = SPLIT ? kSplitHead : kSharedHead;
+    int ptiles, psegs, run, total;
+
+    __device__ __forceinline__ static int cost(const AttendArgs& A, const Seq& s) {  // of one KV head
+        if (s.split() != SPLIT) return 0;
+        const int rt = row_tiles(s.rows);
+        int c = 0;
+        for (int t = 0; t < rt; ++t) c += s.tiles(t, A.group) + kHead;
+        return c;
+    }
+    __device__ __forceinline__ Work fill(int start, int n, int at, int end, int who) const {
+        Work W;
+        const int first = at - start - kHead;  // a run may begin or end in the head
+        W.j0 = first < 0 ? 0 : first;
+        const int stop = end - start - kHead;
+        W.j1 = stop < n ? stop : n;
+        const int w0 = (start + kHead) / run;
+        W.slot = who - w0;
+        W.nslots = (start + kHead + n - 1) / run - w0 + 1;
+        W.left = end - (start + kHead + n);
+        return W;
+    }
+    // The work that begins at `at` of the run that ends at `end`, found by one wave.
+    __device__ __forceinline__ Work find(const AttendArgs& A, const int* s_base, int per, int Tq, int at, int end, int who,
+                                         int lane) const {
+        const int pall = psegs * (ptiles + kHead);
+        if (at < pall) {
+            const int seg = at / (ptiles + kHead);
+            Work W = fill(seg * (ptiles + kHead), ptiles, at, end, who);
+            const int rows = Tq * A.group, prt = row_tiles(rows);
+            W.prefix = 1, W.lo = 0, W.rows = rows, W.kvh = seg / prt, W.row0 = (seg - W.kvh * prt) * kSharedRows, W.b = 0;
+            W.keys = A.B.prefix, W.len = 0, W.n = 0, W.cap = 0;
+            return W;
+        }
+        // the thread, then among its sequences, then the row tile: the last that begins at or before `at`
+        int i = 0;
+#pragma unroll
+        for (int g = 0; g < kThreads / 64; ++g) i += __popcll(__ballot(s_base[64 * g + lane] <= at));
+        i -= 1;
+        int from = uni(s_base[i]);
+        i *= per;
+        Seq s;
+        int c = 0;
+        if (per == 1) {
+            s = load_seq(A, i);
+            c = cost(A, s);
+        } else {
+            const bool in = lane < per && i + lane < A.B.seqs;
+            Seq m = load_seq(A, in ? i + lane : A.B.seqs - 1);
+            const int mc = in ? cost(A, m) * A.C.heads : 0;
+            int inc = mc;
+            for (int d = 1; d < 16; d <<= 1) {
+                const int o = __shfl_up(inc, d);
+                if (lane >= d) inc += o;
+            }
+            // lanes that hold nothing end where their neighbour does
+            const int k = __popcll(__ballot(in && from + inc <= at));
+            from += uni(__shfl(inc - mc, k));
+            i += k;
+            s = load_seq(A, i);
+            c = uni(__shfl(mc, k)) / A.C.heads;
+        }
+        s.lo = uni(s.lo), s.n = uni(s.n), s.len = uni(s.len), s.rows = uni(s.rows);
+        c = uni(c);
+        const int kvh = (at - from) / c;
+        from += kvh * c;
+        int t = 0;
+        if (!SPLIT) {
+            const int rt = row_tiles(s.rows);
+            for (;; t += 64) {
+                int inc = t + lane < rt ? s.tiles(t + lane, A.group) + kHead : 0;
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int o = __shfl_up(inc, d);
+                    if (lane >= d) inc += o;
+                }
+                const int k = __popcll(__ballot(t + lane < rt && from + inc <= at));
+                if (k < 64 && t + k < rt) {
+                    if (k) from += uni(__shfl(inc, k - 1));
+                    t += k;
+                    break;
+                }
+                from += uni(__shfl(inc, 63));
+            }
+        }
+        Work W = fill(from, s.tiles(t, A.group), at, end, who);
+        W.prefix = 0, W.lo = s.lo, W.rows = s.rows, W.row0 = t * kSharedRows, W.kvh = kvh, W.b = i;
+        W.keys = s.seen(SPLIT ? s.n - 1 : s.last_token(t, A.group));
+        W.len = s.len, W.n = s.n, W.cap = s.cap;
+        return W;
+    }
 };
 
 // The products and softmax of one wave's 32 rows, N2 groups of 32 keys at a time.
@@ -174,13 +283,22 @@ struct Core {
 #pragma unroll
             for (int g = 0; g < N2; ++g)
                 s[g] = mfma(*(const u16x8*)(K + g * 32 * G::RB + (koff ^ (uint32_t)(i << 5))), q[i], s[g]);
+        // four reads ahead of the products that take them
+        __builtin_amdgcn_sched_group_barrier(kDs, 4, 0);
+#pragma unroll
+        for (int i = 0; i < N2 * NK - 4; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kDs, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
     }
     // left: visible keys of this lane's row from the group's first on; bad: bit b: block b of 16 keys has no page
     __device__ __forceinline__ void mask(f32x16& s, int left, int bad) {
+        left -= 4 * h;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             if ((bad >> (i >> 3)) & 1) s[i] = NAN;
-            if (key_of(i, h) >= left) s[i] = -INFINITY;
+            if (key_of(i, 0) >= left) s[i] = -INFINITY;
         }
     }
     // p = 2^(c (s - m)) rounded, l += sum p.  The reference m follows the maximum only when that has grown
@@ -230,14 +348,35 @@ struct Core {
         for (int st = 0; st < 2 * N2; ++st)
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] = mfma(vfrag(V, st, d), p[st], o[d]);
+        // the first 16 keys' V and probabilities, then the products with the next 16 keys' beside them
+        __builtin_amdgcn_sched_group_barrier(kDs, 2 * ND, 0);
+        __builtin_amdgcn_sched_group_barrier(kValu, 28, 0);
+#pragma unroll
+        for (int i = 0; i < (2 * N2 - 1) * ND; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kDs, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(kValu, 28 / ND, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, ND, 0);
     }
     __device__ __forceinline__ static bool odd(uint16_t v) {  // infinite or NaN
         constexpr uint16_t e = BF16 ? 0x7f80 : 0x7c00;
         return (v & e) == e;
     }
-    // values() of 32 keys where some row does not see some key: what is not finite is left out, then added
-    // key by key to the rows that see it (0 * inf of a masked key would be NaN)
-    __device__ __forceinline__ void values_checked(const uint8_t* V, const u16x8 (&p)[2], int left) {
+    // Whether one of 32 keys' values is infinite or NaN: an exponent of all ones plus one carries into bit 15.
+    __device__ __forceinline__ bool any_odd(const uint8_t* V) const {
+        constexpr uint32_t e = BF16 ? 0x7f807f80u : 0x7c007c00u, one = BF16 ? 0x00800080u : 0x04000400u;
+        uint32_t t = 0;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {  // the wave's 64 lanes cover the 32 rows, 1 KB a step
+            const uint4 v = *(const uint4*)(V + i * 1024 + lane * 16);
+            t |= ((v.x & e) + one) | ((v.y & e) + one) | ((v.z & e) + one) | ((v.w & e) + one);
+        }
+        return __any((t & 0x80008000u) != 0);
+    }
+    // values() of 32 keys of which some are not finite, and not seen by every row: those are left out, then
+    // added key by key to the rows that see them (0 * inf of a masked key would be NaN)
+    __device__ __forceinline__ void values_odd(const uint8_t* V, const u16x8 (&p)[2], int left) {
         uint32_t keys = 0;
 #pragma unroll
         for (int st = 0; st < 2; ++st)
@@ -247,12 +386,12 @@ struct Core {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (odd(v[i])) {
-                        keys |= 1u << (16 * st + 8 * (i >> 2) + 4 * h + (i & 3));
+                        keys |= 1u << (16 * st + key_of(i, 0));
                         v[i] = 0;
                     }
                 o[d] = mfma(v, p[st], o[d]);
             }
-        if (!__any(keys != 0)) return;
+        keys <<= 4 * h;
         keys |= xor_lane_u<1>(keys);
         keys |= xor_lane_u<2>(keys);
         keys |= xor_lane_u<4>(keys);
@@ -269,7 +408,7 @@ struct Core {
                     u16x8 v = vfrag(V, st, d);
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (!odd(v[i]) || 16 * st + 8 * (i >> 2) + 4 * h + (i & 3) != k) v[i] = 0;
+                        if (!odd(v[i]) || 16 * st + key_of(i, 0) != k - 4 * h) v[i] = 0;
                     a = mfma(v, p[st], a);
                 }
                 if (k < left) {
@@ -286,7 +425,10 @@ struct Core {
         scores<1>(K, s);
         mask(s[0], left, bad);
         softmax<1>(s, p);
-        values_checked(V, p, left);
+        if (any_odd(V))
+            values_odd(V, p, left);
+        else
+            values<1>(V, p);
     }
 };
 
@@ -358,180 +500,152 @@ __device__ __forceinline__ void put_row(const AttendArgs& A, const Work& W, bool
     if (W.slot == 0 && A.slots) A.slots[(W.prefix ? 0 : (int64_t)A.T * A.hq) + row] = empty ? 0 : W.nslots;
 }
 
+// A wave's rows of one piece of work.
 template <int D, bool BF16>
-__global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const AttendArgs A) {
-    using G = Geo<D>;
-    using K = Core<D, BF16>;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
-    __shared__ int64_t s_base[kThreads + 1];
-    __shared__ int64_t s_red[4];
-    __shared__ int s_max[4];
-    __shared__ float2 s_ml[4][32];
-    __shared__ Work s_work;
-    __shared__ int64_t s_start;
-    const int tid = threadIdx.x, lane = tid & 63, wv = uni(tid >> 6);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem;
-
-    // ---- the tiles of all segments: the prefix's, then each sequence's
-    const int per = (A.B.seqs + kThreads - 1) / kThreads;
-    int64_t mine = 0;
-    int most = 0;
-    for (int i = 0; i < per; ++i) {
-        const int b = tid * per + i;
-        if (b >= A.B.seqs) break;
-        const Seq s = load_seq(A, b);
-        const int rt = row_tiles(s.rows);
-        for (int t = 0; t < rt; ++t) {
-            const int k = s.tiles(t, A.group);
-            mine += k;
-            most = k > most ? k : most;
-        }
-    }
-    mine *= A.C.heads;
-    int64_t inc = mine;
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t o = __shfl_up((long long)inc, d);
-        if (lane >= d) inc += o;
-        const int x = __shfl_xor(most, d);
-        most = x > most ? x : most;
-    }
-    if (lane == 63) s_red[wv] = inc, s_max[wv] = most;
-    __syncthreads();
-    int64_t before = inc - mine, own = 0;
-    most = 0;
-    for (int i = 0; i < 4; ++i) {
-        if (i < wv) before += s_red[i];
-        own += s_red[i];
-        most = s_max[i] > most ? s_max[i] : most;
-    }
-    s_base[tid] = before;
-    int Tq = A.T;
-    if (A.B.q_start) {
-        const int e = A.B.q_start[A.B.seqs];
-        Tq = e < 0 ? 0 : e < Tq ? e : Tq;
-    }
-    const int prows = A.B.prefix ? Tq * A.group : 0, prt = row_tiles(prows);
-    const int pkeys = prows <= 32 ? kSplitKeys : kSharedKeys;
-    const int ptiles = (A.B.prefix + pkeys - 1) / pkeys;
-    if (prt && ptiles > most) most = ptiles;
-    const int64_t shared = (int64_t)ptiles * prt * A.C.heads;
-    const int64_t total = uni64(shared + own);
-    // a workgroup's run of tiles: an equal share, and long enough that no segment meets more than nslot of them
-    int64_t run = (total + gridDim.x - 1) / gridDim.x;
-    if (A.nslot > 2) {
-        const int64_t least = (most + A.nslot - 3) / (A.nslot - 2);
-        run = run > least ? run : least;
-    } else {
-        run = total;
-    }
-    run = uni64(run < 1 ? 1 : run);
-
-    int64_t at = (int64_t)blockIdx.x * run;
-    const int64_t end = at + run < total ? at + run : total;
-    while (at < end) {
-        // ---- the segment that holds tile `at`
-        __syncthreads();
-        if (at < shared) {
-            if (tid == 0) {
-                const int seg = (int)(at / ptiles), j0 = (int)(at - (int64_t)seg * ptiles);
-                const int kvh = seg / prt, rt = seg % prt;
-                const int64_t left = end - at;
-                s_work = Work{1, prows <= 32, 0, prows, rt * kSharedRows, kvh, 0, A.B.prefix, j0,
-                              (int)(j0 + left < ptiles ? j0 + left : ptiles), 0, 0, 0, 0, 0};
-                s_start = at - j0;
-            }
-        } else {
-            const int64_t x = at - shared;
-            if (mine && x >= before && x < before + mine) {
-                int64_t loc = x - before;
-                for (int i = 0; i < per; ++i) {
-                    const int b = tid * per + i;
-                    const Seq s = load_seq(A, b);
-                    const int rt = row_tiles(s.rows);
-                    int64_t sum = 0;
-                    for (int t = 0; t < rt; ++t) sum += s.tiles(t, A.group);
-                    if (loc >= sum * A.C.heads) {
-                        loc -= sum * A.C.heads;
-                        continue;
-                    }
-                    const int kvh = (int)(loc / sum);
-                    int64_t j0 = loc - kvh * sum;
-                    int t = 0;
-                    while (j0 >= s.tiles(t, A.group)) j0 -= s.tiles(t++, A.group);
-                    const int nt = s.tiles(t, A.group);
-                    const int64_t left = end - at;
-                    const bool split = s.rows <= 32;
-                    s_work = Work{0, split, s.lo, s.rows, t * kSharedRows, kvh, b,
-                                  s.seen(split ? s.n - 1 : s.last_token(t, A.group)), (int)j0,
-                                  (int)(j0 + left < nt ? j0 + left : nt), 0, 0, s.len, s.n, s.cap};
-                    s_start = at - j0;
-                    s_work.nslots = nt;  // the segment's tiles, for now
-                    break;
-                }
-            }
-        }
-        __syncthreads();
-        Work W = s_work;
-        W.prefix = uni(W.prefix), W.split = uni(W.split), W.lo = uni(W.lo), W.rows = uni(W.rows), W.row0 = uni(W.row0);
-        W.kvh = uni(W.kvh), W.b = uni(W.b), W.keys = uni(W.keys), W.j0 = uni(W.j0), W.j1 = uni(W.j1);
-        W.len = uni(W.len), W.n = uni(W.n), W.cap = uni(W.cap);
-        {
-            const int64_t start = uni64(s_start);
-            const int nt = W.prefix ? ptiles : uni(W.nslots);
-            const int64_t first = start / run;
-            W.slot = (int)((int64_t)blockIdx.x - first);
-            W.nslots = (int)((start + nt - 1) / run - first) + 1;
-        }
-        const bool direct = !W.prefix && !A.B.prefix && W.nslots == 1;
-        const int32_t* pages = W.prefix ? A.B.prefix_pages : A.B.table + (int64_t)W.b * A.B.table_stride;
-
-        // ---- this lane's row
-        K core;
-        core.begin(lane);
-        core.c = A.c;
-        const int row = W.row0 + (W.split ? 0 : 32 * wv) + core.n;
-        const bool valid = row < W.rows;
+struct Rows {
+    int tok, head, seen;
+    int64_t orow;
+    bool valid, far;
+    __device__ __forceinline__ Rows(const AttendArgs& A, const Work& W, int row) {
+        valid = row < W.rows;
         const int rc = valid ? row : W.rows - 1;
-        const int tok = rc / A.group, head = W.kvh * A.group + rc % A.group;
-        const int64_t orow = (int64_t)(W.lo + tok) * A.hq + head;
-        bool far = false;
-        int seen = W.keys;
+        tok = rc / A.group;
+        head = W.kvh * A.group + rc - tok * A.group;
+        orow = (int64_t)(W.lo + tok) * A.hq + head;
+        far = false;
+        seen = W.keys;
         if (!W.prefix) {
             Seq s;
             s.len = W.len, s.n = W.n, s.cap = W.cap;
             seen = s.seen(tok, &far);
         }
-        const int seen1 = __builtin_amdgcn_readlane(seen, 31);  // the wave's last row sees most
-        {
-            const uint16_t* qp = A.q + (int64_t)(W.lo + tok) * A.q_tok + (int64_t)head * A.q_head + 8 * core.h;
+    }
+    __device__ __forceinline__ void load_q(const AttendArgs& A, const Work& W, Core<D, BF16>& core) const {
+        const uint16_t* qp = A.q + (int64_t)(W.lo + tok) * A.q_tok + (int64_t)head * A.q_head + 8 * core.h;
 #pragma unroll
-            for (int i = 0; i < K::NK; ++i) core.q[i] = *(const u16x8*)(qp + 16 * i);
-        }
-        // tiles whose every key is there and seen by every row need no checks: [j0, jf)
-        const int tk = W.split ? kSplitKeys : kSharedKeys;
-        int jf;
-        {
-            bool ok = true;
-            const int k0 = W.j0 * tk, k1 = W.j1 * tk < W.keys ? W.j1 * tk : W.keys;
-            for (int i = (k0 >> A.C.page_shift) + lane; (int64_t)i << A.C.page_shift < k1; i += 64) {
-                const int page = pages[i];
-                ok = ok && page >= 0 && page < A.C.n_pages;
-            }
-            // the first row of the whole tile sees least
-            Seq s;
-            s.len = W.len, s.n = W.n, s.cap = W.cap;
-            const int least = W.prefix ? W.keys : uni(s.seen(W.row0 / A.group));
-            jf = __all(ok) ? least / tk : 0;
-            jf = jf < W.j0 ? W.j0 : jf < W.j1 ? jf : W.j1;
-        }
+        for (int i = 0; i < Core<D, BF16>::NK; ++i) core.q[i] = *(const u16x8*)(qp + 16 * i);
+    }
+    __device__ __forceinline__ void store(const AttendArgs& A, const Work& W, const Core<D, BF16>& core) const {
+        const bool direct = !W.prefix && !A.B.prefix && W.nslots == 1;
+        float l = core.l + core.swap32(core.l);
+        if (far) l = NAN;
+        const bool empty = !W.prefix && !A.B.prefix && seen == 0;
+        const float inv = empty ? 0.0f : 1.0f / l;
+        if (!valid) return;
 #pragma unroll
-        for (int i = 0; i < K::NK; ++i) asm volatile("" : "+v"(core.q[i]));  // arrived before the loops
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                put4<D, BF16>(A, W, direct, orow, d * 32 + 8 * i + 4 * core.h,
+                              make_float4(core.o[d][4 * i], core.o[d][4 * i + 1], core.o[d][4 * i + 2],
+                                          core.o[d][4 * i + 3]),
+                              inv);
+        if (core.h == 0) put_row(A, W, direct, orow, core.m * A.c, l, empty);
+    }
+};
 
-        if (W.split) {
-            // each wave its own 32 keys of every tile, K and V in buffers of its own: the next tile's K is on
-            // its way while this one's V is used, and the other way round
-            const uint32_t kb = lds0 + wv * 128 * D, vb = kb + 64 * D;
-            const uint8_t *kp = smem + wv * 128 * D, *vp = kp + 64 * D;
+// How many of the tiles [j0, j1) need no checks: every key on a page and seen by every row.
+__device__ __forceinline__ int plain_tiles(const AttendArgs& A, const Work& W, const int32_t* pages, int tile, int least,
+                                           int lane) {
+    bool ok = true;
+    const int k0 = W.j0 * tile, k1 = W.j1 * tile < W.keys ? W.j1 * tile : W.keys;
+    for (int i = (k0 >> A.C.page_shift) + lane; (int64_t)i << A.C.page_shift < k1; i += 64) {
+        const int page = pages[i];
+        ok = ok && page >= 0 && page < A.C.n_pages;
+    }
+    const int jf = __all(ok) ? least / tile : 0;
+    return jf < W.j0 ? W.j0 : jf < W.j1 ? jf : W.j1;
+}
+
+template <int D, bool BF16>
+__global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const AttendArgs A) {
+    using G = Geo<D>;
+    using K = Core<D, BF16>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
+    __shared__ int s_base[2][kThreads];
+    __shared__ int s_red[4][4];
+    const int tid = threadIdx.x, lane = tid & 63, wv = uni(tid >> 6);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem;
+
+    // ---- the two axes: split segments are dealt to waves, shared ones to workgroups
+    const int per = (A.B.seqs + kThreads - 1) / kThreads;
+    int mine[4] = {0, 0, 0, 0};  // split and shared cost; the longest segment of each
+    for (int i = 0; i < per; ++i) {
+        const int b = tid * per + i;
+        if (b >= A.B.seqs) break;
+        const Seq s = load_seq(A, b);
+        const int kind = s.split() ? 0 : 1, rt = row_tiles(s.rows);
+        if (!rt) continue;
+        mine[kind] += (kind ? Axis<false>::cost(A, s) : Axis<true>::cost(A, s)) * A.C.heads;
+        const int k = s.tiles(rt - 1, A.group);
+        mine[2 + kind] = k > mine[2 + kind] ? k : mine[2 + kind];
+    }
+    int inc[2] = {mine[0], mine[1]};
+    for (int d = 1; d < 64; d <<= 1) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int o = __shfl_up(inc[k], d);
+            if (lane >= d) inc[k] += o;
+            const int x = __shfl_xor(mine[2 + k], d);
+            mine[2 + k] = x > mine[2 + k] ? x : mine[2 + k];
+        }
+    }
+    if (lane == 63) s_red[wv][0] = inc[0], s_red[wv][1] = inc[1], s_red[wv][2] = mine[2], s_red[wv][3] = mine[3];
+    __syncthreads();
+    int before[2] = {inc[0] - mine[0], inc[1] - mine[1]}, own[2] = {0, 0}, most[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        for (int i = 0; i < 4; ++i) {
+            if (i < wv) before[k] += s_red[i][k];
+            own[k] += s_red[i][k];
+            most[k] = s_red[i][2 + k] > most[k] ? s_red[i][2 + k] : most[k];
+        }
+    int Tq = A.T;
+    if (A.B.q_start) {
+        const int e = A.B.q_start[A.B.seqs];
+        Tq = uni(e < 0 ? 0 : e < Tq ? e : Tq);
+    }
+    Axis<true> ax0;
+    Axis<false> ax1;
+    {
+        const int prows = A.B.prefix ? Tq * A.group : 0;
+        const bool sp = prows <= kSplitRows;
+        const int tile = sp ? kSplitKeys : kSharedKeys, pt = (A.B.prefix + tile - 1) / tile;
+        const int segs = row_tiles(prows) * A.C.heads;
+        ax0.ptiles = ax1.ptiles = pt;
+        ax0.psegs = sp ? segs : 0;
+        ax1.psegs = sp ? 0 : segs;
+        if (segs && pt > most[sp ? 0 : 1]) most[sp ? 0 : 1] = pt;
+        const int p0 = ax0.psegs * (pt + kSplitHead), p1 = ax1.psegs * (pt + kSharedHead);
+        s_base[0][tid] = p0 + before[0];
+        s_base[1][tid] = p1 + before[1];
+        ax0.total = uni(p0 + own[0]);
+        ax1.total = uni(p1 + own[1]);
+        // equal runs, long enough that no segment meets more than nslot of them
+        const int w0 = gridDim.x * 4, w1 = gridDim.x;
+        const int l0 = (most[0] + A.nslot - 3) / (A.nslot - 2), l1 = (most[1] + A.nslot - 3) / (A.nslot - 2);
+        ax0.run = (ax0.total + w0 - 1) / w0;
+        ax1.run = (ax1.total + w1 - 1) / w1;
+        ax0.run = ax0.run > l0 ? ax0.run : l0;
+        ax1.run = ax1.run > l1 ? ax1.run : l1;
+        ax0.run = uni(ax0.run > kSplitLeast ? ax0.run : kSplitLeast);
+        ax1.run = uni(ax1.run > 1 ? ax1.run : 1);
+    }
+    __syncthreads();
+
+    {  // ---- split segments: each wave by itself; the next tile's K is on its way while this one's V is used,
+       // and the other way round
+        const uint32_t kb = lds0 + wv * 128 * D, vb = kb + 64 * D;
+        const uint8_t *kp = smem + wv * 128 * D, *vp = kp + 64 * D;
+        const int who = blockIdx.x * 4 + wv;
+        int at = ax0.total / ax0.run < who ? ax0.total : who * ax0.run;
+        const int end = at + ax0.run < ax0.total ? at + ax0.run : ax0.total;
+        while (at < end) {
+            Work W = ax0.find(A, s_base[0], per, Tq, at, end, who, lane);
+            W.scalar();
+            at = end - W.left;
+            if (W.j0 >= W.j1) continue;
+            const int32_t* pages = W.prefix ? A.B.prefix_pages : A.B.table + (int64_t)W.b * A.B.table_stride;
             auto bring_k = [&](int key) {
                 copy_block<D, false>(A, A.C.k, pages, W.kvh, key, W.keys, lane, kb);
                 copy_block<D, false>(A, A.C.k, pages, W.kvh, key + 16, W.keys, lane, kb + 32 * D);
@@ -540,9 +654,17 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                 copy_block<D, true>(A, A.C.v, pages, W.kvh, key, W.keys, lane, vb);
                 copy_block<D, true>(A, A.C.v, pages, W.kvh, key + 16, W.keys, lane, vb + 32 * D);
             };
-            int key = W.j0 * kSplitKeys + 32 * wv;
+            K core;
+            core.begin(lane);
+            core.c = A.c;
+            const Rows<D, BF16> R(A, W, core.n);
+            R.load_q(A, W, core);
+            const int jf = uni(plain_tiles(A, W, pages, kSplitKeys, uni(R.seen), lane));
+            int key = W.j0 * kSplitKeys;
             const int stop = W.j1 * kSplitKeys < W.keys ? W.j1 * kSplitKeys : W.keys;
             if (key < stop) bring_k(key), bring_v(key);
+#pragma unroll
+            for (int i = 0; i < K::NK; ++i) asm volatile("" : "+v"(core.q[i]));  // arrived before the loops
             for (int j = W.j0; j < jf; ++j) {
                 const int next = key + kSplitKeys;
                 f32x16 s[1];
@@ -563,50 +685,34 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             }
             for (; key < stop; key += kSplitKeys) {
                 vm_wait<0>();
-                core.checked(kp, vp, seen - key, bad_blocks(A, pages, key, W.keys, 2));
+                core.checked(kp, vp, R.seen - key, bad_blocks(A, pages, key, W.keys, 2));
                 lds_wait();
                 if (key + kSplitKeys < stop) bring_k(key + kSplitKeys), bring_v(key + kSplitKeys);
             }
-            // the four waves' rows meet in LDS
-            float l = core.l + K::swap32(core.l);
-            if (far) l = NAN;
-            __syncthreads();
-            float* so = (float*)smem;
-#pragma unroll
-            for (int d = 0; d < K::ND; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) so[(wv * (D / 2) + d * 16 + i) * 64 + lane] = core.o[d][i];
-            if (lane < 32) s_ml[wv][lane] = make_float2(core.m * A.c, l);
-            __syncthreads();
-            float f[4], mx = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_ml[w][core.n].x);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                f[w] = __builtin_amdgcn_exp2f(s_ml[w][core.n].x - (mx == -INFINITY ? 0.0f : mx));
-                sum = sum + f[w] * s_ml[w][core.n].y;
+            R.store(A, W, core);
+        }
+    }
+    {  // ---- shared segments: the four waves take 32 rows each and every tile together, in two buffers of K and V
+        int at = ax1.total / ax1.run < (int)blockIdx.x ? ax1.total : blockIdx.x * ax1.run;
+        const int end = at + ax1.run < ax1.total ? at + ax1.run : ax1.total;
+        while (at < end) {
+            Work W = ax1.find(A, s_base[1], per, Tq, at, end, blockIdx.x, lane);
+            W.scalar();
+            at = end - W.left;
+            if (W.j0 >= W.j1) continue;
+            const int32_t* pages = W.prefix ? A.B.prefix_pages : A.B.table + (int64_t)W.b * A.B.table_stride;
+            K core;
+            core.begin(lane);
+            core.c = A.c;
+            const Rows<D, BF16> R(A, W, W.row0 + 32 * wv + core.n);
+            R.load_q(A, W, core);
+            int jf;
+            {  // the first row of the whole tile sees least
+                Seq s;
+                s.len = W.len, s.n = W.n, s.cap = W.cap;
+                jf = uni(plain_tiles(A, W, pages, kSharedKeys, W.prefix ? W.keys : s.seen(W.row0 / A.group), lane));
             }
-            const bool empty = !W.prefix && !A.B.prefix && seen == 0;
-            const float inv = empty ? 0.0f : 1.0f / sum;
-            if (valid) {
-#pragma unroll
-                for (int g = 0; g < D / 32; ++g) {
-                    float v[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int reg = wv * (D / 8) + 4 * g + i;
-                        v[i] = 0.0f;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) v[i] += f[w] * so[(w * (D / 2) + reg) * 64 + lane];
-                    }
-                    const int reg = wv * (D / 8) + 4 * g;
-                    put4<D, BF16>(A, W, direct, orow, (reg >> 4) * 32 + 8 * ((reg & 15) >> 2) + 4 * core.h,
-                                  make_float4(v[0], v[1], v[2], v[3]), inv);
-                }
-                if (wv == 0 && core.h == 0) put_row(A, W, direct, orow, mx, sum, empty);
-            }
-        } else {
-            // every wave the same 64 keys, two buffers of K and V; a wave brings 16 rows of each
+            const int seen1 = __builtin_amdgcn_readlane(R.seen, 31);  // the wave's last row sees most
             const bool works = 32 * wv < W.rows - W.row0;
             auto bring = [&](int j) {
                 const uint32_t buf = lds0 + (j & 1) * 256 * D;
@@ -615,7 +721,10 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                 copy_block<D, true>(A, A.C.v, pages, W.kvh, key, W.keys, lane, buf + 128 * D + wv * 32 * D);
             };
             const int stop = W.keys > 0 ? W.j1 : W.j0;
+            lds_barrier();  // every wave is done with the last segment's buffers
             if (W.j0 < stop) bring(W.j0);
+#pragma unroll
+            for (int i = 0; i < K::NK; ++i) asm volatile("" : "+v"(core.q[i]));  // arrived before the loops
             int j = W.j0;
             for (; j < jf; ++j) {
                 vm_wait<0>();
@@ -639,27 +748,12 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                 for (int half = 0; half < 2 && works; ++half) {
                     const int key = j * kSharedKeys + 32 * half;
                     if (key >= seen1) break;
-                    core.checked(buf + half * 64 * D, buf + 128 * D + half * 64 * D, seen - key,
+                    core.checked(buf + half * 64 * D, buf + 128 * D + half * 64 * D, R.seen - key,
                                  bad_blocks(A, pages, key, W.keys, 2));
                 }
             }
-            float l = core.l + K::swap32(core.l);
-            if (far) l = NAN;
-            const bool empty = !W.prefix && !A.B.prefix && seen == 0;
-            const float inv = empty ? 0.0f : 1.0f / l;
-            if (valid) {
-#pragma unroll
-                for (int d = 0; d < K::ND; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        put4<D, BF16>(A, W, direct, orow, d * 32 + 8 * i + 4 * core.h,
-                                      make_float4(core.o[d][4 * i], core.o[d][4 * i + 1], core.o[d][4 * i + 2],
-                                                  core.o[d][4 * i + 3]),
-                                      inv);
-                if (core.h == 0) put_row(A, W, direct, orow, core.m * A.c, l, empty);
-            }
+            R.store(A, W, core);
         }
-        at += W.j1 - W.j0;
     }
 }
 
