@@ -37,7 +37,7 @@ constexpr int kThreads = 256;
 constexpr int kValu = 0x2, kMfma = 0x8, kDs = 0x100;  // instruction classes of sched_group_barrier
 constexpr int kSplitKeys = 32, kSharedKeys = 64;  // keys of a tile, by kind of segment
 constexpr int kSplitRows = 32, kSharedRows = 128;
-constexpr int kSplitLeast = 4;  // tiles of a wave's run at least
+constexpr int kSplitLeast = 2;  // tiles of a wave's run at least
 constexpr int kSplitHead = 3, kSharedHead = 5;  // what a segment costs beside its tiles, in tiles
 
 struct AttendArgs {
@@ -607,6 +607,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
     }
     Axis<true> ax0;
     Axis<false> ax1;
+    int nsplit;
     {
         const int prows = A.B.prefix ? Tq * A.group : 0;
         const bool sp = prows <= kSplitRows;
@@ -621,8 +622,16 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
         s_base[1][tid] = p1 + before[1];
         ax0.total = uni(p0 + own[0]);
         ax1.total = uni(p1 + own[1]);
+        // the workgroups by the time that the two kinds take (a shared tile about 1.5 split ones), each kind
+        // spread evenly over the grid: the one streams the cache while the other multiplies
+        const float c0 = 2.0f * ax0.total, c1 = 3.0f * ax1.total;
+        int g0 = (int)((float)gridDim.x * c0 / (c0 + c1 + 1.0f) + 0.5f);
+        if (ax0.total && g0 < 1) g0 = 1;
+        if (ax1.total && g0 > (int)gridDim.x - 1) g0 = gridDim.x - 1;
+        if (!ax1.total) g0 = gridDim.x;
+        nsplit = uni(g0);
         // equal runs, long enough that no segment meets more than nslot of them
-        const int w0 = gridDim.x * 4, w1 = gridDim.x;
+        const int w0 = (g0 ? g0 : 1) * 4, w1 = (int)gridDim.x - g0 > 0 ? gridDim.x - g0 : 1;
         const int l0 = (most[0] + A.nslot - 3) / (A.nslot - 2), l1 = (most[1] + A.nslot - 3) / (A.nslot - 2);
         ax0.run = (ax0.total + w0 - 1) / w0;
         ax1.run = (ax1.total + w1 - 1) / w1;
@@ -633,11 +642,13 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
     }
     __syncthreads();
 
-    {  // ---- split segments: each wave by itself; the next tile's K is on its way while this one's V is used,
-       // and the other way round
+    const int before_me = (int)((int64_t)blockIdx.x * nsplit / gridDim.x);  // workgroups for split segments
+    if ((int)((int64_t)(blockIdx.x + 1) * nsplit / gridDim.x) > before_me) {
+        // ---- split segments: each wave by itself; the next tile's K is on its way while this one's V is used,
+        // and the other way round
         const uint32_t kb = lds0 + wv * 128 * D, vb = kb + 64 * D;
         const uint8_t *kp = smem + wv * 128 * D, *vp = kp + 64 * D;
-        const int who = blockIdx.x * 4 + wv;
+        const int who = wv * nsplit + before_me;  // neighbouring runs on other CUs
         int at = ax0.total / ax0.run < who ? ax0.total : who * ax0.run;
         const int end = at + ax0.run < ax0.total ? at + ax0.run : ax0.total;
         while (at < end) {
@@ -691,12 +702,13 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             }
             R.store(A, W, core);
         }
-    }
-    {  // ---- shared segments: the four waves take 32 rows each and every tile together, in two buffers of K and V
-        int at = ax1.total / ax1.run < (int)blockIdx.x ? ax1.total : blockIdx.x * ax1.run;
+    } else {
+        // ---- shared segments: the four waves take 32 rows each and every tile together, in two buffers of K and V
+        const int who = blockIdx.x - before_me;
+        int at = ax1.total / ax1.run < who ? ax1.total : who * ax1.run;
         const int end = at + ax1.run < ax1.total ? at + ax1.run : ax1.total;
         while (at < end) {
-            Work W = ax1.find(A, s_base[1], per, Tq, at, end, blockIdx.x, lane);
+            Work W = ax1.find(A, s_base[1], per, Tq, at, end, who, lane);
             W.scalar();
             at = end - W.left;
             if (W.j0 >= W.j1) continue;
@@ -757,49 +769,67 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
     }
 }
 
-// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's slots in order; one wave a row.
-template <int D, bool BF16>
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's slots: GROUPS groups of D / 4 threads take
+// every GROUPS-th slot each, then meet in group order.
+template <int D, bool BF16, int GROUPS>
 __global__ __launch_bounds__(kThreads) void combine_rows_kernel(const AttendArgs A) {
-    constexpr int N = D / 64;
-    const int lane = threadIdx.x & 63;
+    constexpr int LPR = D / 4;                       // threads of a group, 4 columns each
+    constexpr int RPB = kThreads / (LPR * GROUPS);   // rows of a workgroup
+    __shared__ float4 s_o[kThreads];
+    const int tid = threadIdx.x;
+    const int g = (tid / LPR) % GROUPS, c = tid % LPR;
     const int64_t R = (int64_t)A.T * A.hq;
-    const int64_t row = (int64_t)blockIdx.x * 4 + uni(threadIdx.x >> 6);
-    if (row >= R) return;
-    if (A.B.q_start && row / A.hq >= A.B.q_start[A.B.seqs]) return;
-    if (!A.B.q_start && row / A.hq >= A.B.seqs) return;
-    int ns = A.slots[R + row], np = A.B.prefix ? A.slots[row] : 0;
-    if (!A.B.prefix && ns == 1) return;  // written by the only workgroup that had it
-    if (!A.B.prefix && ns == 0) {  // a row that sees nothing
-#pragma unroll
-        for (int i = 0; i < N; ++i) A.out[row * D + N * lane + i] = 0;
-        if (A.lse && lane == 0) A.lse[row] = -INFINITY;
-        return;
+    const int64_t row = (int64_t)blockIdx.x * RPB + tid / (LPR * GROUPS);
+    int ns = 0, np = 0;
+    bool live = row < R;
+    if (live) {
+        const int64_t t = row / A.hq;
+        live = t < (A.B.q_start ? A.B.q_start[A.B.seqs] : A.B.seqs);
     }
-    ns = ns < 0 ? 0 : ns > A.nslot ? A.nslot : ns;
-    np = np < 0 ? 0 : np > A.nslot ? A.nslot : np;
-    const int all = np + ns;
+    if (live) {
+        ns = A.slots[R + row];
+        np = A.B.prefix ? A.slots[row] : 0;
+        live = A.B.prefix || ns != 1;  // else written by the only run that had it
+        ns = ns < 0 ? 0 : ns > A.nslot ? A.nslot : ns;
+        np = np < 0 ? 0 : np > A.nslot ? A.nslot : np;
+    }
+    const bool empty = !A.B.prefix && ns == 0;
+    const int all = live ? np + ns : 0;
     auto place = [&](int s) { return (s < np ? s : A.nslot + s - np) * R + row; };
     float mx = -INFINITY;
-    for (int s = lane; s < all; s += 64) mx = fmaxf(mx, A.ml[place(s)].x);
-    mx = wave_max(mx);
+    for (int s = c; s < all; s += LPR) mx = fmaxf(mx, A.ml[place(s)].x);
+    for (int d = LPR < 64 ? LPR / 2 : 32; d; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
     const float ref = mx == -INFINITY ? 0.0f : mx;
-    float o[N], sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = 0.0f;
-    for (int s = 0; s < all; ++s) {
+    float4 o = make_float4(0, 0, 0, 0);
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int s = g; s < all; s += GROUPS) {
         const int64_t at = place(s);
         const float2 ml = A.ml[at];
+        const float4 p = *(const float4*)(A.part + at * D + 4 * c);
         const float f = __builtin_amdgcn_exp2f(ml.x - ref);
         sum += f * ml.y;
-        const float* p = A.part + at * D + N * lane;
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] += f * p[i];
+        o.x += f * p.x, o.y += f * p.y, o.z += f * p.z, o.w += f * p.w;
     }
-    const float inv = 1.0f / sum;
-    uint16_t* w = A.out + row * D + N * lane;
+    if constexpr (GROUPS > 1) {
+        __shared__ float s_l[kThreads];
+        s_o[tid] = o;
+        s_l[tid] = sum;
+        __syncthreads();
+        if (g == 0)
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = to16<BF16>(o[i] * inv);
-    if (A.lse && lane == 0) A.lse[row] = (mx + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+            for (int i = 1; i < GROUPS; ++i) {
+                const float4 p = s_o[tid + i * LPR];
+                o.x += p.x, o.y += p.y, o.z += p.z, o.w += p.w;
+                sum += s_l[tid + i * LPR];
+            }
+    }
+    if (!live || g) return;
+    const float inv = empty ? 0.0f : 1.0f / sum;
+    const uint32_t a = to16<BF16>(o.x * inv) | (uint32_t)to16<BF16>(o.y * inv) << 16;
+    const uint32_t b = to16<BF16>(o.z * inv) | (uint32_t)to16<BF16>(o.w * inv) << 16;
+    *(uint2*)(A.out + row * D + 4 * c) = make_uint2(a, b);
+    if (A.lse && c == 0) A.lse[row] = empty ? -INFINITY : (mx + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
 static int attend_slots(int64_t rows, int D) {
@@ -844,16 +874,25 @@ int launch_attend(const KvCache& C, const KvBatch& B, const uint16_t* q, int64_t
                        lse, (float*)b, (float2*)(b + w.ml), (int*)(b + w.slots), w.nslot};
     const int64_t R = (int64_t)T * hq;
     const dim3 block(kThreads);
-#define ATT(D)                                                                                                \
-    do {                                                                                                      \
-        const dim3 grid(cu_count() * Geo<D>::OCC), rows((unsigned)((R + 3) / 4));                             \
-        if (C.bf16) {                                                                                         \
-            PG_LAUNCH((attend_kernel<D, true>), grid, block, 0, st, A);                                       \
-            PG_LAUNCH((combine_rows_kernel<D, true>), rows, block, 0, st, A);                                 \
-        } else {                                                                                              \
-            PG_LAUNCH((attend_kernel<D, false>), grid, block, 0, st, A);                                      \
-            PG_LAUNCH((combine_rows_kernel<D, false>), rows, block, 0, st, A);                                \
-        }                                                                                                     \
+    // few rows have many slots each: 1024 / D groups a row, one row a workgroup; many have few
+    const bool few = R <= 2048;
+#define COMBINE(D, BF)                                                                                           \
+    do {                                                                                                         \
+        if (few)                                                                                                 \
+            PG_LAUNCH((combine_rows_kernel<D, BF, 1024 / D>), dim3((unsigned)R), block, 0, st, A);               \
+        else                                                                                                     \
+            PG_LAUNCH((combine_rows_kernel<D, BF, 1>), dim3((unsigned)((R * D + 1023) / 1024)), block, 0, st, A); \
+    } while (0)
+#define ATT(D)                                                               \
+    do {                                                                     \
+        const dim3 grid(cu_count() * Geo<D>::OCC);                           \
+        if (C.bf16) {                                                        \
+            PG_LAUNCH((attend_kernel<D, true>), grid, block, 0, st, A);      \
+            COMBINE(D, true);                                                \
+        } else {                                                             \
+            PG_LAUNCH((attend_kernel<D, false>), grid, block, 0, st, A);     \
+            COMBINE(D, false);                                               \
+        }                                                                    \
     } while (0)
     if (C.dim == 64)
         ATT(64);
@@ -862,6 +901,7 @@ int launch_attend(const KvCache& C, const KvBatch& B, const uint16_t* q, int64_t
     else
         ATT(256);
 #undef ATT
+#undef COMBINE
     return check_launch("attend");
 }
 
