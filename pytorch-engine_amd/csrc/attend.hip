@@ -78,6 +78,32 @@ __device__ __forceinline__ void copy_lds(const void* base, uint32_t off, uint32_
                  : "v"(off), "s"(base), "s"(lds)
                  : "memory");
 }
+// Four of them from rows that follow each other without gaps: the instruction's offset moves both addresses.
+__device__ __forceinline__ void copy_lds4(const void* base, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3,
+                                          uint32_t lds) {
+    uint32_t keep;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\t"
+        "global_load_lds_dwordx4 %1, %5\n\t"
+        "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+        "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+        "global_load_lds_dwordx4 %4, %5 offset:3072\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(base), "s"(lds)
+        : "memory");
+}
+__device__ __forceinline__ void copy_lds2(const void* base, uint32_t o0, uint32_t o1, uint32_t lds) {
+    uint32_t keep;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\t"
+        "global_load_lds_dwordx4 %1, %3\n\t"
+        "global_load_lds_dwordx4 %2, %3 offset:1024\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "v"(o0), "v"(o1), "s"(base), "s"(lds)
+        : "memory");
+}
 template <int N>
 __device__ __forceinline__ void vm_wait() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -275,7 +301,7 @@ struct Core {
     __device__ __forceinline__ static int key_of(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
     // S^T of N2 * 32 keys: s[g][i] is key 32 g + key_of(i, h) of this lane's row
     template <int N2>
-    __device__ __forceinline__ void scores(const uint8_t* K, f32x16 (&s)[N2]) {
+    __device__ __forceinline__ void score_products(const uint8_t* K, f32x16 (&s)[N2]) {
 #pragma unroll
         for (int g = 0; g < N2; ++g) s[g] = f32x16{};
 #pragma unroll
@@ -283,6 +309,10 @@ struct Core {
 #pragma unroll
             for (int g = 0; g < N2; ++g)
                 s[g] = mfma(*(const u16x8*)(K + g * 32 * G::RB + (koff ^ (uint32_t)(i << 5))), q[i], s[g]);
+    }
+    template <int N2>
+    __device__ __forceinline__ void scores(const uint8_t* K, f32x16 (&s)[N2]) {
+        score_products<N2>(K, s);
         // four reads ahead of the products that take them
         __builtin_amdgcn_sched_group_barrier(kDs, 4, 0);
 #pragma unroll
@@ -301,11 +331,11 @@ struct Core {
             if (key_of(i, 0) >= left) s[i] = -INFINITY;
         }
     }
-    // p = 2^(c (s - m)) rounded, l += sum p.  The reference m follows the maximum only when that has grown
-    // by 2^8: p stays within fp16's range and its relative precision, and the rescaling of o (64 products a
-    // lane) all but vanishes.
+    // The reference m follows the running maximum only when that has grown by 2^8: p = 2^(c (s - m)) stays
+    // within fp16's range and its relative precision, and the rescaling of o (64 products a lane) all but
+    // vanishes.
     template <int N2>
-    __device__ __forceinline__ void softmax(const f32x16 (&s)[N2], u16x8 (&p)[2 * N2]) {
+    __device__ __forceinline__ void grow(const f32x16 (&s)[N2]) {
         float mx = s[0][0];
 #pragma unroll
         for (int g = 0; g < N2; ++g)
@@ -322,6 +352,10 @@ struct Core {
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
             m = mn;
         }
+    }
+    // p = 2^(c (s - m)) rounded, l += sum p
+    template <int N2>
+    __device__ __forceinline__ void weigh(const f32x16 (&s)[N2], u16x8 (&p)[2 * N2]) {
         const float mc = m == -INFINITY ? 0.0f : m * c;
 #pragma unroll
         for (int g = 0; g < N2; ++g)
@@ -424,7 +458,8 @@ struct Core {
         u16x8 p[2];
         scores<1>(K, s);
         mask(s[0], left, bad);
-        softmax<1>(s, p);
+        grow<1>(s);
+        weigh<1>(s, p);
         if (any_odd(V))
             values_odd(V, p, left);
         else
@@ -432,35 +467,50 @@ struct Core {
     }
 };
 
-// Copies the 16 rows of the key block that begins at key kb (a multiple of 16) of K or V into LDS; keys past
-// the last one are copies of it, and a page that does not exist is read as page 0.
-template <int D, bool V>
-__device__ __forceinline__ void copy_block(const AttendArgs& A, const uint16_t* cache, const int32_t* pages, int kvh, int kb,
-                                           int keys, int lane, uint32_t lds) {
-    using G = Geo<D>;
+// Where the block of 16 keys from kb on (a multiple of 16) lies: element offset of its first row in k and v,
+// and how many of its rows hold keys (all behind the last key: none; it then stands on the last key's block).
+struct Block {
+    int64_t at;
+    int have, first;  // rows [0, have) are keys; the block's key 0 is row `first` of the rows at `at`
+};
+__device__ __forceinline__ Block find_block(const AttendArgs& A, const int32_t* pages, int kvh, int kb, int keys) {
     const int last = keys - 1;
     const int ke = kb > last ? last & ~15 : kb;
     int page = sload(pages, ke >> A.C.page_shift);
     if (page < 0 || page >= A.C.n_pages) page = 0;
-    const uint16_t* base = cache + (int64_t)page * A.C.page_stride + (int64_t)kvh * A.C.head_stride +
-                           (int64_t)(ke & ((1 << A.C.page_shift) - 1)) * A.C.row_stride;
+    Block b;
+    b.at = (int64_t)page * A.C.page_stride + (int64_t)kvh * A.C.head_stride +
+           (int64_t)(ke & ((1 << A.C.page_shift) - 1)) * A.C.row_stride;
+    b.have = keys - ke, b.first = kb - ke;
+    return b;
+}
+// Copies a block's 16 rows of K or V into LDS; rows past the last key are copies of it.
+template <int D, bool V>
+__device__ __forceinline__ void copy_block(const AttendArgs& A, const uint16_t* cache, const Block& b, int lane, uint32_t lds) {
+    using G = Geo<D>;
+    const uint16_t* base = cache + b.at;
     const uint32_t rs = (uint32_t)A.C.row_stride * 2;
     asm volatile("" : "+v"(lane));  // offsets made here, not held (or spilled) across the loop
     const int lr = lane / G::LPR, cs = lane % G::LPR;
-    if (kb + 16 <= keys) {
+    auto chunk = [&](int i) {  // the 16-byte chunk that lane's place of copy i holds
+        const int r = i * G::RPC + lr;
+        return (uint32_t)(V ? cs ^ (2 * G::vswz(r)) : cs ^ (r & G::KM)) << 4;
+    };
+    if (b.have >= 16 && A.C.row_stride == D) {
+        const uint32_t row = (uint32_t)lr * (2 * D);
+        if constexpr (G::CPB == 2) {
+            copy_lds2(base, row + chunk(0), row + chunk(1), lds);
+        } else {
 #pragma unroll
-        for (int i = 0; i < G::CPB; ++i) {
-            const int r = i * G::RPC + lr;
-            const uint32_t ch = V ? cs ^ (2 * G::vswz(r)) : cs ^ (r & G::KM);
-            copy_lds(base + (int64_t)(i * G::RPC) * A.C.row_stride, (uint32_t)lr * rs + (ch << 4), lds + i * 1024);
+            for (int i = 0; i < G::CPB; i += 4)
+                copy_lds4(base + i * 512, row + chunk(i), row + chunk(i + 1), row + chunk(i + 2), row + chunk(i + 3),
+                          lds + i * 1024);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < G::CPB; ++i) {
-            const int r = i * G::RPC + lr;
-            const uint32_t ch = V ? cs ^ (2 * G::vswz(r)) : cs ^ (r & G::KM);
-            const int at = r + (kb - ke) < last - ke ? r + (kb - ke) : last - ke;
-            copy_lds(base, (uint32_t)at * rs + (ch << 4), lds + i * 1024);
+            const int r = i * G::RPC + lr + b.first;
+            copy_lds(base, (uint32_t)(r < b.have ? r : b.have - 1) * rs + chunk(i), lds + i * 1024);
         }
     }
 }
@@ -657,13 +707,16 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             at = end - W.left;
             if (W.j0 >= W.j1) continue;
             const int32_t* pages = W.prefix ? A.B.prefix_pages : A.B.table + (int64_t)W.b * A.B.table_stride;
-            auto bring_k = [&](int key) {
-                copy_block<D, false>(A, A.C.k, pages, W.kvh, key, W.keys, lane, kb);
-                copy_block<D, false>(A, A.C.k, pages, W.kvh, key + 16, W.keys, lane, kb + 32 * D);
+            Block b0, b1;
+            auto bring_k = [&](int key) {  // and where the same keys' values are
+                b0 = find_block(A, pages, W.kvh, key, W.keys);
+                b1 = find_block(A, pages, W.kvh, key + 16, W.keys);
+                copy_block<D, false>(A, A.C.k, b0, lane, kb);
+                copy_block<D, false>(A, A.C.k, b1, lane, kb + 32 * D);
             };
-            auto bring_v = [&](int key) {
-                copy_block<D, true>(A, A.C.v, pages, W.kvh, key, W.keys, lane, vb);
-                copy_block<D, true>(A, A.C.v, pages, W.kvh, key + 16, W.keys, lane, vb + 32 * D);
+            auto bring_v = [&]() {
+                copy_block<D, true>(A, A.C.v, b0, lane, vb);
+                copy_block<D, true>(A, A.C.v, b1, lane, vb + 32 * D);
             };
             K core;
             core.begin(lane);
@@ -673,7 +726,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             const int jf = uni(plain_tiles(A, W, pages, kSplitKeys, uni(R.seen), lane));
             int key = W.j0 * kSplitKeys;
             const int stop = W.j1 * kSplitKeys < W.keys ? W.j1 * kSplitKeys : W.keys;
-            if (key < stop) bring_k(key), bring_v(key);
+            if (key < stop) bring_k(key), bring_v();
 #pragma unroll
             for (int i = 0; i < K::NK; ++i) asm volatile("" : "+v"(core.q[i]));  // arrived before the loops
             for (int j = W.j0; j < jf; ++j) {
@@ -684,21 +737,22 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                 core.template scores<1>(kp, s);
                 lds_wait();
                 if (next < stop) bring_k(next);
-                core.template softmax<1>(s, p);
+                core.template grow<1>(s);
+                core.template weigh<1>(s, p);
                 if (next < stop)
                     vm_wait<D / 16>();
                 else
                     vm_wait<0>();
                 core.template values<1>(vp, p);
                 lds_wait();
-                if (next < stop) bring_v(next);
+                if (next < stop) bring_v();
                 key = next;
             }
             for (; key < stop; key += kSplitKeys) {
                 vm_wait<0>();
                 core.checked(kp, vp, R.seen - key, bad_blocks(A, pages, key, W.keys, 2));
                 lds_wait();
-                if (key + kSplitKeys < stop) bring_k(key + kSplitKeys), bring_v(key + kSplitKeys);
+                if (key + kSplitKeys < stop) bring_k(key + kSplitKeys), bring_v();
             }
             R.store(A, W, core);
         }
@@ -727,10 +781,10 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             const int seen1 = __builtin_amdgcn_readlane(R.seen, 31);  // the wave's last row sees most
             const bool works = 32 * wv < W.rows - W.row0;
             auto bring = [&](int j) {
-                const uint32_t buf = lds0 + (j & 1) * 256 * D;
-                const int key = j * kSharedKeys + 16 * wv;
-                copy_block<D, false>(A, A.C.k, pages, W.kvh, key, W.keys, lane, buf + wv * 32 * D);
-                copy_block<D, true>(A, A.C.v, pages, W.kvh, key, W.keys, lane, buf + 128 * D + wv * 32 * D);
+                const uint32_t buf = lds0 + (j & 1) * 256 * D + wv * 32 * D;
+                const Block b = find_block(A, pages, W.kvh, j * kSharedKeys + 16 * wv, W.keys);
+                copy_block<D, false>(A, A.C.k, b, lane, buf);
+                copy_block<D, true>(A, A.C.v, b, lane, buf + 128 * D);
             };
             const int stop = W.keys > 0 ? W.j1 : W.j0;
             lds_barrier();  // every wave is done with the last segment's buffers
@@ -747,7 +801,8 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                     f32x16 s[2];
                     u16x8 p[4];
                     core.template scores<2>(buf, s);
-                    core.template softmax<2>(s, p);
+                    core.template grow<2>(s);
+                    core.template weigh<2>(s, p);
                     core.template values<2>(buf + 128 * D, p);
                 }
             }
