@@ -37,6 +37,7 @@ constexpr int kThreads = 256;
 constexpr int kValu = 0x2, kMfma = 0x8, kDs = 0x100;  // instruction classes of sched_group_barrier
 constexpr int kSplitKeys = 32, kSharedKeys = 64;  // keys of a tile, by kind of segment
 constexpr int kSplitRows = 32, kSharedRows = 128;
+constexpr int kAlone = 16;  // row tiles that a lane sums by itself
 constexpr int kSplitLeast = 2;  // tiles of a wave's run at least
 constexpr int kSplitHead = 3, kSharedHead = 5;  // what a segment costs beside its tiles, in tiles
 
@@ -46,7 +47,8 @@ struct AttendArgs {
     const uint16_t* q;
     int64_t q_tok, q_head;
     int T, hq, group;
-    float c;  // scale * log2(e)
+    uint32_t by_group;  // ceil(2^32 / group): x / group = (x * by_group) >> 32 while x * group < 2^32
+    float c;            // scale * log2(e)
     uint16_t* out;
     float* lse;
     // partial rows [prefix, own][slot][T * hq][dim], their (max in log2 units, sum), and the slots a row has
@@ -120,6 +122,10 @@ __device__ __forceinline__ int sload(const int32_t* p, int64_t i) {
     return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p)[i];
 }
 
+__device__ __forceinline__ int group_of(const AttendArgs& A, int x) {  // x / group
+    return A.group == 1 ? x : (int)__umulhi((uint32_t)x, A.by_group);
+}
+
 // One sequence's rows and keys.
 struct Seq {
     int lo, n, len, cap, rows;
@@ -129,14 +135,14 @@ struct Seq {
         if (far) *far = v > cap;
         return v < 0 ? 0 : v > cap ? cap : (int)v;
     }
-    __device__ __forceinline__ int last_token(int tile, int group) const {
-        const int i = (kSharedRows * (tile + 1) - 1) / group;
-        return i < n - 1 ? i : n - 1;
+    __device__ __forceinline__ int last_token(const AttendArgs& A, int tile) const {
+        const int r = kSharedRows * (tile + 1);
+        return r < rows ? group_of(A, r - 1) : n - 1;
     }
     __device__ __forceinline__ bool split() const { return rows <= kSplitRows; }
-    __device__ __forceinline__ int tiles(int tile, int group) const {  // of row tile `tile`; one at least
+    __device__ __forceinline__ int tiles(const AttendArgs& A, int tile) const {  // of row tile `tile`; one at least
         const int k = split() ? (seen(n - 1) + kSplitKeys - 1) / kSplitKeys
-                              : (seen(last_token(tile, group)) + kSharedKeys - 1) / kSharedKeys;
+                              : (seen(last_token(A, tile)) + kSharedKeys - 1) / kSharedKeys;
         return k < 1 ? 1 : k;
     }
 };
@@ -175,11 +181,28 @@ struct Axis {
     static constexpr int kHead = SPLIT ? kSplitHead : kSharedHead;
     int ptiles, psegs, run, total;
 
-    __device__ __forceinline__ static int cost(const AttendArgs& A, const Seq& s) {  // of one KV head
-        if (s.split() != SPLIT) return 0;
-        const int rt = row_tiles(s.rows);
+    // The cost of one KV head of this lane's sequence (`in`: it has one).  A wave sums the row tiles of a long
+    // prompt together.
+    __device__ __forceinline__ static int cost(const AttendArgs& A, const Seq& s, bool in, int lane) {
+        const int rt = in && s.split() == SPLIT ? row_tiles(s.rows) : 0;
         int c = 0;
-        for (int t = 0; t < rt; ++t) c += s.tiles(t, A.group) + kHead;
+        if constexpr (SPLIT) {
+            if (rt) c = s.tiles(A, 0) + kHead;
+        } else {
+            if (rt <= kAlone)
+                for (int t = 0; t < rt; ++t) c += s.tiles(A, t) + kHead;
+            for (uint64_t big = __ballot(rt > kAlone); big; big &= big - 1) {
+                const int who = __builtin_ctzll(big);
+                Seq m;
+                m.n = __builtin_amdgcn_readlane(s.n, who), m.len = __builtin_amdgcn_readlane(s.len, who);
+                m.rows = __builtin_amdgcn_readlane(s.rows, who), m.cap = s.cap;
+                const int all = row_tiles(m.rows);
+                int sum = 0;
+                for (int t = lane; t < all; t += 64) sum += m.tiles(A, t) + kHead;
+                for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+                if (lane == who) c = sum;
+            }
+        }
         return c;
     }
     __device__ __forceinline__ Work fill(int start, int n, int at, int end, int who) const {
@@ -217,11 +240,11 @@ struct Axis {
         int c = 0;
         if (per == 1) {
             s = load_seq(A, i);
-            c = cost(A, s);
+            c = uni(cost(A, s, lane == 0, lane));
         } else {
             const bool in = lane < per && i + lane < A.B.seqs;
             Seq m = load_seq(A, in ? i + lane : A.B.seqs - 1);
-            const int mc = in ? cost(A, m) * A.C.heads : 0;
+            const int mc = cost(A, m, in, lane) * A.C.heads;
             int inc = mc;
             for (int d = 1; d < 16; d <<= 1) {
                 const int o = __shfl_up(inc, d);
@@ -242,7 +265,7 @@ struct Axis {
         if (!SPLIT) {
             const int rt = row_tiles(s.rows);
             for (;; t += 64) {
-                int inc = t + lane < rt ? s.tiles(t + lane, A.group) + kHead : 0;
+                int inc = t + lane < rt ? s.tiles(A, t + lane) + kHead : 0;
                 for (int d = 1; d < 64; d <<= 1) {
                     const int o = __shfl_up(inc, d);
                     if (lane >= d) inc += o;
@@ -256,9 +279,9 @@ struct Axis {
                 from += uni(__shfl(inc, 63));
             }
         }
-        Work W = fill(from, s.tiles(t, A.group), at, end, who);
+        Work W = fill(from, s.tiles(A, t), at, end, who);
         W.prefix = 0, W.lo = s.lo, W.rows = s.rows, W.row0 = t * kSharedRows, W.kvh = kvh, W.b = i;
-        W.keys = s.seen(SPLIT ? s.n - 1 : s.last_token(t, A.group));
+        W.keys = s.seen(SPLIT ? s.n - 1 : s.last_token(A, t));
         W.len = s.len, W.n = s.n, W.cap = s.cap;
         return W;
     }
@@ -559,7 +582,7 @@ struct Rows {
     __device__ __forceinline__ Rows(const AttendArgs& A, const Work& W, int row) {
         valid = row < W.rows;
         const int rc = valid ? row : W.rows - 1;
-        tok = rc / A.group;
+        tok = group_of(A, rc);
         head = W.kvh * A.group + rc - tok * A.group;
         orow = (int64_t)(W.lo + tok) * A.hq + head;
         far = false;
@@ -622,13 +645,14 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
     int mine[4] = {0, 0, 0, 0};  // split and shared cost; the longest segment of each
     for (int i = 0; i < per; ++i) {
         const int b = tid * per + i;
-        if (b >= A.B.seqs) break;
-        const Seq s = load_seq(A, b);
-        const int kind = s.split() ? 0 : 1, rt = row_tiles(s.rows);
-        if (!rt) continue;
-        mine[kind] += (kind ? Axis<false>::cost(A, s) : Axis<true>::cost(A, s)) * A.C.heads;
-        const int k = s.tiles(rt - 1, A.group);
-        mine[2 + kind] = k > mine[2 + kind] ? k : mine[2 + kind];
+        const bool in = b < A.B.seqs;
+        const Seq s = load_seq(A, in ? b : A.B.seqs - 1);
+        mine[0] += Axis<true>::cost(A, s, in, lane) * A.C.heads;
+        mine[1] += Axis<false>::cost(A, s, in, lane) * A.C.heads;
+        if (in && s.rows) {
+            const int k = s.tiles(A, row_tiles(s.rows) - 1), kind = s.split() ? 2 : 3;
+            mine[kind] = k > mine[kind] ? k : mine[kind];
+        }
     }
     int inc[2] = {mine[0], mine[1]};
     for (int d = 1; d < 64; d <<= 1) {
@@ -776,7 +800,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             {  // the first row of the whole tile sees least
                 Seq s;
                 s.len = W.len, s.n = W.n, s.cap = W.cap;
-                jf = uni(plain_tiles(A, W, pages, kSharedKeys, W.prefix ? W.keys : s.seen(W.row0 / A.group), lane));
+                jf = uni(plain_tiles(A, W, pages, kSharedKeys, W.prefix ? W.keys : s.seen(group_of(A, W.row0)), lane));
             }
             const int seen1 = __builtin_amdgcn_readlane(R.seen, 31);  // the wave's last row sees most
             const bool works = 32 * wv < W.rows - W.row0;
@@ -925,8 +949,9 @@ int launch_attend(const KvCache& C, const KvBatch& B, const uint16_t* q, int64_t
     if (T == 0) return PGMOE_OK;
     const AttendWs w = attend_ws(C, B, T, hq);
     uint8_t* b = (uint8_t*)ws;
-    const AttendArgs A{C,   B,   q,   q_tok, q_head, T, hq, hq / C.heads, scale * 1.4426950408889634f, out,
-                       lse, (float*)b, (float2*)(b + w.ml), (int*)(b + w.slots), w.nslot};
+    const int group = hq / C.heads;
+    const AttendArgs A{C,   B,         q,   q_tok, q_head, T, hq, group, (uint32_t)(0x100000000ull / group + (group > 1)),
+                       scale * 1.4426950408889634f, out, lse, (float*)b, (float2*)(b + w.ml), (int*)(b + w.slots), w.nslot};
     const int64_t R = (int64_t)T * hq;
     const dim3 block(kThreads);
     // few rows have many slots each: 1024 / D groups a row, one row a workgroup; many have few
