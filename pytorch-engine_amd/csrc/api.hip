@@ -833,7 +833,7 @@ int pgmoe_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t 
         return fail(PGMOE_E_WORKSPACE, "workspace %zu bytes, need %zu", ws_bytes, need);
     int bits = 0;
     while ((1 << bits) < vocab) ++bits;
-    const SampleArgs A{logits, dtype, row_stride, rows, vocab, u, *S, token, logprob, 62 - bits, ws};
+    const SampleArgs A{logits, dtype, row_stride, rows, vocab, u, *S, token, logprob, bits < 11 ? 51 : 62 - bits, ws};
     return launch_sample(A, as_stream(stream));
 }
 

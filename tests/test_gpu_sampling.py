@@ -1,6 +1,8 @@
 """sample_tokens against a float64 reference (tests/kv_helpers.sample_reference): tokens equal,
 log-probabilities to an fp32 step (2^-23 relative, twice the rounding of the result) and the fixed
-point: each of V weights is off by half of 2^-(62 - ceil(log2 V)) at most, beside a total of 1 and more."""
+point: weights are multiples of 2^-s with s = min(51, 62 - ceil(log2 V)) (51: what the 52-bit fraction of a
+double holds), so each of V is off by 2^-(s + 1) at most, their total, 1 and more, by V 2^-(s + 1), and its
+logarithm by no more."""
 
 import math
 
@@ -30,7 +32,7 @@ def _check(dev, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     tok, lp = sample_tokens(x.to(dev), u.to(dev), temperature=to(temperature, 0), top_k=to(top_k, 0), top_p=to(top_p, 0),
                             min_p=to(min_p, 0))
     tok, lp = tok.cpu().numpy(), lp.cpu().numpy().astype(np.float64)
-    fixed = x.shape[1] * 2.0 ** (math.ceil(math.log2(x.shape[1])) - 63) + 2.0 ** -50
+    fixed = x.shape[1] * 2.0 ** -(min(51, 62 - math.ceil(math.log2(x.shape[1]))) + 1) + 2.0 ** -50
     for r in range(x.shape[0]):
         par = [float(v[r]) if isinstance(v, torch.Tensor) else v for v in (temperature, top_k, top_p, min_p)]
         par[1] = int(par[1])
