@@ -16,13 +16,16 @@
 namespace pgmoe {
 
 constexpr int kSlice = 8192;                   // tokens of a slice
-constexpr int kSliceThreads = 256;
-constexpr int kRowThreads = 1024;
-constexpr int kPer = kSlice / kRowThreads;     // consecutive tokens of a row_kernel thread
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kPer = kSlice / kThreads;        // tokens of a thread
 constexpr int kBins = 256;                     // of the distance; the last holds all that lies further
 constexpr float kPerNat = 8.0f;                // bins a unit of x / T
-constexpr int kDigits = 2048;
-constexpr int kList = 6144;                    // tokens of one bin that fit LDS
+constexpr int kDigitBits = 9;                  // of a level of the descent
+constexpr int kDigits = 1 << kDigitBits;
+constexpr int kList = 7168;                    // tokens of one bin that fit LDS
+constexpr int kBatch = 4;                      // slices that row_kernel reads at a time
+constexpr int kHeld = 12;                      // histogram entries that a thread keeps in registers
 constexpr int kMaxSlices = kMaxVocab / kSlice;
 
 struct Slice {
@@ -58,9 +61,9 @@ __device__ __forceinline__ void load_logits(const SampleArgs& A, int64_t row, in
     const int64_t at = row + i;
     if (A.dtype == PGMOE_DT_F32) {
         const float* p = (const float*)A.logits + at;
-        if (i + N <= A.vocab && ((uintptr_t)p & 15) == 0) {
+        if (N % 4 == 0 && i + N <= A.vocab && ((uintptr_t)p & 15) == 0) {
 #pragma unroll
-            for (int j = 0; j < N; j += 4) {
+            for (int j = 0; j + 3 < N; j += 4) {
                 const float4 v = *(const float4*)(p + j);
                 x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
             }
@@ -72,9 +75,9 @@ __device__ __forceinline__ void load_logits(const SampleArgs& A, int64_t row, in
     }
     const uint16_t* p = (const uint16_t*)A.logits + at;
     uint16_t h[N];
-    if (i + N <= A.vocab && ((uintptr_t)p & 15) == 0) {
+    if (N % 8 == 0 && i + N <= A.vocab && ((uintptr_t)p & 15) == 0) {
 #pragma unroll
-        for (int j = 0; j < N; j += 8) {
+        for (int j = 0; j + 7 < N; j += 8) {
             const uint4 v = *(const uint4*)(p + j);
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -105,28 +108,28 @@ struct Settings {
     }
 };
 
-// w = exp((x - top) / T) = 2^(q / 32) e^g with |g| <= ln 2 / 64: a table of 32 powers and five terms of the
-// series, relative error 2^-48; fixed point by adding 2^52.
+// w = exp((x - top) / T) = 2^(q / 256) e^g with |g| <= ln 2 / 512: a table of 256 powers and four terms of the
+// series, relative error 2^-50; fixed point by adding 2^52.
+constexpr int kPowers = 256;
 struct Weigh {
-    const double* powers;  // 2^(i / 32), LDS
+    const double* powers;  // 2^(i / 256), LDS
     float top;
-    double k32;  // 32 log2(e) / T
+    double k;  // 256 log2(e) / T
     int shift;
     __device__ __forceinline__ Weigh(const double* powers_, float top_, double inv_t, int shift_)
-        : powers(powers_), top(top_), k32(inv_t * 46.16624130844683), shift(shift_) {}
+        : powers(powers_), top(top_), k(inv_t * 369.32993046757464), shift(shift_) {}
     __device__ __forceinline__ double scaled(float x, int shift_) const {
         if (x == top) return __builtin_ldexp(1.0, shift_);
-        const double t = ((double)x - (double)top) * k32;
-        if (!(t > -2048.0)) return 0.0;  // also -inf, NaN, and everything beside +inf; 2^-64
+        const double t = ((double)x - (double)top) * k;
+        if (!(t > -16384.0)) return 0.0;  // also -inf, NaN, and everything beside +inf; 2^-64
         const double q = __builtin_rint(t);
-        const double g = (t - q) * 0.021660849392498290;
-        double p = __builtin_fma(g, 1.0 / 120.0, 1.0 / 24.0);
-        p = __builtin_fma(p, g, 1.0 / 6.0);
+        const double g = (t - q) * 0.0027076061740622863;
+        double p = __builtin_fma(g, 1.0 / 24.0, 1.0 / 6.0);
         p = __builtin_fma(p, g, 0.5);
         p = __builtin_fma(p, g, 1.0);
         p = __builtin_fma(p, g, 1.0);
         const int n = (int)q;
-        return __builtin_ldexp(powers[n & 31] * p, (n >> 5) + shift_);
+        return __builtin_ldexp(powers[n & (kPowers - 1)] * p, (n >> 8) + shift_);
     }
     __device__ __forceinline__ double w(float x) const { return scaled(x, 0); }
     __device__ __forceinline__ uint64_t fix(float x) const {
@@ -135,7 +138,7 @@ struct Weigh {
     }
 };
 __device__ __forceinline__ void fill_powers(double* p, int tid) {
-    if (tid < 32) p[tid] = exp2((double)tid / 32.0);
+    if (tid < kPowers) p[tid] = exp2((double)tid / kPowers);
 }
 
 // The grid of the histogram: bins of 1/8 in x / T, counted down from the bin of `top`.
@@ -153,20 +156,33 @@ __device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
     return v;
 }
 
-__global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const SampleArgs A) {
-    constexpr int G = 8, N = kSlice / kSliceThreads / G;  // groups of 8 tokens a thread
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) { return __shfl((unsigned long long)v, lane); }
+// Sum over the lanes below this one, and over all.
+__device__ __forceinline__ uint64_t wave_before(uint64_t v, uint64_t* all) {
+    const int lane = threadIdx.x & 63;
+    uint64_t x = v;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t p = __shfl_up((unsigned long long)x, d);
+        if (lane >= d) x += p;
+    }
+    *all = shfl64(x, 63);
+    return x - v;
+}
+
+__global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs A) {
+    constexpr int G = 8, N = kPer / G;  // groups of 8 tokens a thread
     __shared__ uint32_t cnt[kBins];
     __shared__ unsigned long long wgt[kBins];
-    __shared__ double powers[32];
-    __shared__ float s_max[kSliceThreads / 64];
-    __shared__ uint64_t s_sum[kSliceThreads / 64];
+    __shared__ double powers[kPowers];
+    __shared__ float s_max[kWaves];
+    __shared__ uint64_t s_sum[kWaves];
     __shared__ int s_first;
     const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, base = blockIdx.x * kSlice;
     const int64_t row = (int64_t)r * A.row_stride;
     float x[N][G];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const int i = base + (j * kSliceThreads + tid) * G;
+        const int i = base + (j * kThreads + tid) * G;
         if (i < A.vocab)
             load_logits<G>(A, row, i, x[j]);
         else
@@ -175,7 +191,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
     const Settings S(A, r);
     fill_powers(powers, tid);
     if (tid == 0) s_first = 0x7fffffff;
-    cnt[tid] = 0, wgt[tid] = 0;
+    if (tid < kBins) cnt[tid] = 0, wgt[tid] = 0;
     float mx = -INFINITY;
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -185,7 +201,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
     if (lane == 0) s_max[tid >> 6] = mx;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kSliceThreads / 64; ++i) mx = fmaxf(mx, s_max[i]);
+    for (int i = 0; i < kWaves; ++i) mx = fmaxf(mx, s_max[i]);
 
     const int64_t at = (int64_t)r * gridDim.x + blockIdx.x;
     const Layout o = layout(A.rows, A.vocab);
@@ -197,7 +213,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
 #pragma unroll
             for (int e = 0; e < G; ++e)
                 if (x[j][e] == mx) {
-                    const int i = base + (j * kSliceThreads + tid) * G + e;
+                    const int i = base + (j * kThreads + tid) * G + e;
                     first = i < first ? i : first;
                 }
         if (first != 0x7fffffff) atomicMin(&s_first, first);
@@ -222,53 +238,64 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slice_kernel(const Sampl
         sum = wave_sum(sum);
         if (lane == 0) s_sum[tid >> 6] = sum;
         __syncthreads();
-        if (tid == 0) *out = Slice{s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], mx, 0};
+        if (tid == 0) {
+            sum = 0;
+            for (int i = 0; i < kWaves; ++i) sum += s_sum[i];
+            *out = Slice{sum, mx, 0};
+        }
     }
     if (S.filters) {
         __syncthreads();
-        ((uint32_t*)((uint8_t*)A.ws + o.cnt))[at * kBins + tid] = cnt[tid];
-        ((uint64_t*)((uint8_t*)A.ws + o.wgt))[at * kBins + tid] = wgt[tid];
+        if (tid < kBins) {
+            ((uint32_t*)((uint8_t*)A.ws + o.cnt))[at * kBins + tid] = cnt[tid];
+            ((uint64_t*)((uint8_t*)A.ws + o.wgt))[at * kBins + tid] = wgt[tid];
+        }
     }
 }
 
-__device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t* s) {
-    __syncthreads();
-    v = wave_sum(v);
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t t = 0;
-    for (int i = 0; i < kRowThreads / 64; ++i) t += s[i];
-    return t;
-}
-// Sums of two values over the threads below this one.
-__device__ __forceinline__ void block_before(uint64_t& a, uint64_t& b, uint64_t (*s)[2]) {
-    __syncthreads();
-    const int lane = threadIdx.x & 63;
-    uint64_t x = a, y = b;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t p = __shfl_up((unsigned long long)x, d), q = __shfl_up((unsigned long long)y, d);
-        if (lane >= d) x += p, y += q;
+// Where the order of the tokens leaves the kept ones, among N places (bins or digits) a lane of one wave, in
+// order: the first place that is not kept whole, with the count and weight before it; -1: all are.
+template <int N>
+struct Border {
+    int place;
+    uint64_t cb, wb, all;
+    template <class Stop>
+    __device__ __forceinline__ Border(const uint64_t (&c)[N], const uint64_t (&w)[N], uint64_t cb0, uint64_t wb0,
+                                      Stop&& stop) {
+        const int lane = threadIdx.x & 63;
+        uint64_t cs = 0, ws = 0, unused;
+#pragma unroll
+        for (int i = 0; i < N; ++i) cs += c[i], ws += w[i];
+        uint64_t c1 = cb0 + wave_before(cs, &unused), w1 = wb0 + wave_before(ws, &all);
+        int at = -1;
+        uint64_t ca = 0, wa = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (at < 0 && c[i] && stop(lane * N + i, c1 + c[i], w1 + w[i], all)) at = lane * N + i, ca = c1, wa = w1;
+            c1 += c[i], w1 += w[i];
+        }
+        const uint64_t who = __ballot(at >= 0);
+        const int l = who ? __builtin_ctzll(who) : 0;
+        place = who ? __shfl(at, l) : -1;
+        cb = shfl64(ca, l), wb = shfl64(wa, l);
     }
-    if (lane == 63) s[threadIdx.x >> 6][0] = x, s[threadIdx.x >> 6][1] = y;
-    __syncthreads();
-    a = x - a, b = y - b;
-    for (int i = 0; i < (int)(threadIdx.x >> 6); ++i) a += s[i][0], b += s[i][1];
-}
+};
 
-__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArgs A) {
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A) {
+    constexpr int kLaneSlices = kMaxSlices / 64;
     __shared__ uint2 list[kList];  // (key, index) of the tokens of the last kept one's bin
-    __shared__ unsigned long long wsum[kDigits];
-    __shared__ uint32_t cnt[kDigits];
-    __shared__ unsigned long long slice_w[kMaxSlices];
+    __shared__ unsigned long long wsum[2][kDigits];
+    __shared__ uint32_t cnt[2][kDigits];
+    __shared__ unsigned long long slice_w[kMaxSlices];  // what a slice keeps
+    __shared__ uint32_t slice_n[kMaxSlices];            // its tokens of key `edge`
     __shared__ double slice_s[kMaxSlices];  // the slice's weights to the row's: exp((its max - max) / T)
     __shared__ float slice_d[kMaxSlices];   // the slice's bins to the row's
-    __shared__ uint32_t slice_n[kMaxSlices];
-    __shared__ double powers[32];
-    __shared__ uint64_t red[kRowThreads / 64][2];
-    __shared__ float redf[kRowThreads / 64];
-    __shared__ int s_bin, s_n, s_first, s_slice;
-    __shared__ uint64_t s_cb, s_wb;
-    const int r = blockIdx.x, tid = threadIdx.x, V = A.vocab;
+    __shared__ uint8_t slice_in[kMaxSlices];
+    __shared__ double powers[kPowers];
+    __shared__ uint64_t red[kWaves][2];
+    __shared__ int s_n;
+    __shared__ uint32_t s_lo, s_hi;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, V = A.vocab;
     const int slices = (V + kSlice - 1) / kSlice;
     const int64_t row = (int64_t)r * A.row_stride;
     const Layout o = layout(A.rows, V);
@@ -277,14 +304,24 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
     const uint64_t* hw = (const uint64_t*)((uint8_t*)A.ws + o.wgt) + (int64_t)r * slices * kBins;
     const Settings S(A, r);
 
-    Slice mine{0, -INFINITY, 0x7fffffff};
-    if (tid < slices) mine = sl[tid];
+    // every wave holds the slices' maxima, so that the row's needs no meeting
+    float mx = -INFINITY;
+    int first = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < kLaneSlices; ++i)
+        if (64 * i + lane < slices) mx = fmaxf(mx, sl[64 * i + lane].max);
+    uint32_t hold_c[kHeld];
+    uint64_t hold_w[kHeld];
+    if (S.filters) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int e = i * kThreads + tid;
+            hold_c[i] = e < slices * kBins ? hc[e] : 0;
+            hold_w[i] = e < slices * kBins ? hw[e] : 0;
+        }
+    }
     fill_powers(powers, tid);
-    if (tid == 0) s_first = 0x7fffffff, s_n = 0, s_bin = 0x7fffffff;
-    float mx = wave_max(mine.max);
-    if ((tid & 63) == 0) redf[tid >> 6] = mx;
-    __syncthreads();
-    for (int i = 0; i < kRowThreads / 64; ++i) mx = fmaxf(mx, redf[i]);
+    mx = wave_max(mx);
     if (mx == -INFINITY) {
         if (tid == 0) {
             A.token[r] = -1;
@@ -293,10 +330,18 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
         return;
     }
     if (S.greedy) {
-        if (mine.max == mx) atomicMin(&s_first, mine.first);
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kLaneSlices; ++i)
+            if (64 * i + lane < slices && sl[64 * i + lane].max == mx) {
+                const int f = sl[64 * i + lane].first;
+                first = f < first ? f : first;
+            }
+        for (int d = 32; d; d >>= 1) {
+            const int f = __shfl_xor(first, d);
+            first = f < first ? f : first;
+        }
         if (tid == 0) {
-            A.token[r] = s_first;
+            A.token[r] = first;
             if (A.logprob) A.logprob[r] = 0.0f;
         }
         return;
@@ -305,33 +350,38 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
     const Grid g(mx, S.inv_t);
     auto to_row = [&](uint64_t w, int s) { return slice_s[s] == 1.0 ? w : (uint64_t)llrint((double)w * slice_s[s]); };
     if (tid < slices) {
-        const bool top = mine.max == mx;
-        slice_s[tid] = top ? 1.0 : mine.max == -INFINITY || mx == INFINITY ? 0.0 : exp(((double)mine.max - (double)mx) * S.inv_t);
-        slice_d[tid] = top ? 0.0f : g.at - floorf(mine.max * g.g);
-        slice_w[tid] = to_row(mine.sum, tid);  // without filters: everything is kept
-        slice_n[tid] = 0;
+        const Slice m = sl[tid];
+        const bool top = m.max == mx;
+        const double f = top ? 1.0 : m.max == -INFINITY || mx == INFINITY ? 0.0 : exp(((double)m.max - (double)mx) * S.inv_t);
+        slice_s[tid] = f;
+        slice_d[tid] = top ? 0.0f : g.at - floorf(m.max * g.g);
+        slice_w[tid] = S.filters ? 0 : f == 1.0 ? m.sum : (uint64_t)llrint((double)m.sum * f);
+        slice_n[tid] = 0, slice_in[tid] = 0;
     }
+    for (int i = tid; i < kDigits; i += kThreads) cnt[0][i] = cnt[1][i] = 0, wsum[0][i] = wsum[1][i] = 0;
+    if (tid == 0) s_n = 0, s_lo = 0xffffffffu, s_hi = 0;
     __syncthreads();
 
     // The last kept token: key `edge`, of which the first `ties` in index order are kept; every greater key is.
     uint32_t edge = 0;
     uint64_t ties = 0;
     if (S.filters) {
-        for (int i = tid; i < kBins; i += kRowThreads) cnt[i] = 0, wsum[i] = 0;
-        __syncthreads();
         auto row_bin = [&](int s, int b) {
             const float d = (float)b + slice_d[s];
             return d < (float)(kBins - 1) ? (int)d : kBins - 1;
         };
-        for (int i = tid; i < slices * kBins; i += kRowThreads) {
-            const int s = i / kBins;
-            const uint32_t c = hc[i];
-            if (c && sl[s].max > -INFINITY) {
-                const int b = row_bin(s, i % kBins);
-                atomicAdd(&cnt[b], c);
-                atomicAdd(&wsum[b], (unsigned long long)to_row(hw[i], s));
-            }
-        }
+        auto entries = [&](auto&& take) {  // the slices' histograms, entry by entry
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (hold_c[i]) take(i * kThreads + tid, hold_c[i], hold_w[i]);
+            for (int e = kHeld * kThreads + tid; e < slices * kBins; e += kThreads)
+                if (hc[e]) take(e, hc[e], hw[e]);
+        };
+        entries([&](int e, uint32_t c, uint64_t w) {
+            const int s = e / kBins, b = row_bin(s, e % kBins);
+            atomicAdd(&cnt[0][b], c);
+            atomicAdd(&wsum[0][b], (unsigned long long)to_row(w, s));
+        });
         // the least key that min_p keeps: bisection to the border of w >= min_p, from its logarithm
         uint32_t least = 0;
         int least_bin = kBins;
@@ -351,136 +401,232 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
             least_bin = g.bin(of_key(least));
         }
         __syncthreads();
-        const uint64_t all = block_sum(tid < kBins ? wsum[tid] : 0, (uint64_t*)red);
-        const uint64_t target = S.top_p < 1.0 ? (S.top_p > 0.0 ? (uint64_t)ceil(S.top_p * (double)all) : 0) : ~0ull;
-        uint64_t cb, wb;
+        uint64_t target = ~0ull, cb, wb;
+        int bin;
         {
-            const uint64_t c = tid < kBins ? cnt[tid] : 0, w = tid < kBins ? wsum[tid] : 0;
-            uint64_t c0 = c, w0 = w;
-            block_before(c0, w0, red);
-            if (c && (c0 + c >= S.top_k || w0 + w >= target || tid >= least_bin)) atomicMin(&s_bin, tid);
-            __syncthreads();
-            if (tid == s_bin) s_cb = c0, s_wb = w0;
-        }
-        __syncthreads();
-        const int bin = s_bin;
-        if (bin < kBins) {
-            cb = s_cb, wb = s_wb;
-            const bool listed = cnt[bin] <= kList;
-            // what each slice keeps above the bin, and the bin's tokens
-            if (tid < slices) slice_w[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < slices * kBins; i += kRowThreads) {
-                const int s = i / kBins;
-                if (hc[i] && sl[s].max > -INFINITY && row_bin(s, i % kBins) < bin)
-                    atomicAdd(&slice_w[s], (unsigned long long)to_row(hw[i], s));
-            }
-            auto scan = [&](auto&& take) {  // every token of the bin, in no order
-                if (listed) {
-                    for (int i = tid; i < s_n && i < kList; i += kRowThreads) take(list[i].x, (int)list[i].y);
-                } else {
-                    for (int s = 0; s < slices; ++s) {
-                        float x[kPer];
-                        const int i0 = s * kSlice + tid * kPer;
-                        if (i0 >= V) continue;
-                        load_logits<kPer>(A, row, i0, x);
+            constexpr int N = kBins / 64;
+            uint64_t c[N], w[N];
 #pragma unroll
-                        for (int e = 0; e < kPer; ++e)
-                            if (x[e] > -INFINITY && g.bin(x[e]) == bin) take(key_of(x[e]), i0 + e);
+            for (int i = 0; i < N; ++i) c[i] = cnt[0][lane * N + i], w[i] = wsum[0][lane * N + i];
+            auto aim = [&](uint64_t all) {
+                return S.top_p < 1.0 ? (S.top_p > 0.0 ? (uint64_t)ceil(S.top_p * (double)all) : 0) : ~0ull;
+            };
+            const Border<N> B(c, w, 0, 0, [&](int b, uint64_t ce, uint64_t we, uint64_t all) {
+                return ce >= S.top_k || we >= aim(all) || b >= least_bin;
+            });
+            target = aim(B.all);
+            bin = B.place, cb = B.cb, wb = B.wb;
+        }
+        const bool some = bin >= 0;
+        const uint32_t cnt_bin = some ? cnt[0][bin] : 0;
+        const bool listed = cnt_bin <= kList;
+        __syncthreads();
+        for (int i = tid; i < kBins; i += kThreads) cnt[0][i] = 0, wsum[0][i] = 0;
+        // what each slice keeps above the bin, and which have tokens in it
+        entries([&](int e, uint32_t c, uint64_t w) {
+            const int s = e / kBins, b = row_bin(s, e % kBins);
+            if (!some || b < bin)
+                atomicAdd(&slice_w[s], (unsigned long long)to_row(w, s));
+            else if (b == bin)
+                slice_in[s] = 1;
+        });
+        __syncthreads();
+        if (some) {
+            // The slices that have tokens in the bin, kBatch of them on their way at a time: a thread's tokens
+            // of one slice, and the index of the first of each eight
+            auto read_slices = [&](auto&& look) {
+                int s = -1;
+                while (s < slices) {
+                    float x[kBatch][kPer / 8][8];
+                    int at[kBatch];
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b) {
+                        do ++s;
+                        while (s < slices && !slice_in[s]);
+                        s = s < slices ? s : slices;
+                        at[b] = s;
+#pragma unroll
+                        for (int j = 0; j < kPer / 8; ++j) {
+                            const int i = s * kSlice + (j * kThreads + tid) * 8;
+                            if (s < slices && i < V)
+                                load_logits<8>(A, row, i, x[b][j]);
+                            else
+                                for (int q = 0; q < 8; ++q) x[b][j][q] = -INFINITY;
+                        }
                     }
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b)
+                        if (at[b] < slices) look(x[b], at[b] * kSlice + tid * 8);
                 }
             };
-            if (listed) {
-#pragma unroll 4
-                for (int s = 0; s < slices; ++s) {
-                    // only slices that have tokens there
-                    const float b = (float)bin - slice_d[s];
-                    if (bin < kBins - 1 && (!(b >= 0.0f) || !hc[s * kBins + (int)b])) continue;
-                    float x[kPer];
-                    const int i0 = s * kSlice + tid * kPer;
-                    if (i0 >= V) continue;
-                    load_logits<kPer>(A, row, i0, x);
-#pragma unroll
-                    for (int e = 0; e < kPer; ++e)
-                        if (x[e] > -INFINITY && g.bin(x[e]) == bin) {
-                            const int at = atomicAdd(&s_n, 1);
-                            if (at < kList) list[at] = make_uint2(key_of(x[e]), (uint32_t)(i0 + e));
-                        }
+            auto place = [&](int i0, int j, int q) { return i0 + j * kThreads * 8 + q; };
+            // the bin's logits are those from xl to xh: the borders of its keys, by bisection near its place
+            auto first_key = [&](int b) {  // the least key of bin b or a nearer one
+                uint32_t out = key_of(-INFINITY), in = key_of(mx);
+                if (b >= kBins - 1) return out + 1;
+                if (b < 0) return in + 1;
+                const uint32_t k = key_of((g.at - (float)b) / g.g);
+                if (k > out + 8 && k < in && g.bin(of_key(k - 8)) > b) out = k - 8;
+                if (k > out && k + 8 < in && g.bin(of_key(k + 8)) <= b) in = k + 8;
+                while (in - out > 1) {
+                    const uint32_t mid = out + (in - out) / 2;
+                    (g.bin(of_key(mid)) <= b ? in : out) = mid;
                 }
-            }
-            __syncthreads();
-            uint32_t prefix = 0;
-            int low = 32;  // bits below the prefix
-            const int bits[3] = {11, 11, 10};
-            bool whole = false;
-            for (int level = 0; level < 3 && !whole; ++level) {
-                const int sh = low - bits[level], n = 1 << bits[level];
-                for (int i = tid; i < n; i += kRowThreads) cnt[i] = 0, wsum[i] = 0;
-                if (tid == 0) s_bin = -1;
-                __syncthreads();
-                scan([&](uint32_t u, int) {
-                    if (level == 0 || (u >> low) == prefix) {
-                        const int d = (u >> sh) & (n - 1);
-                        atomicAdd(&cnt[d], 1u);
-                        atomicAdd(&wsum[d], (unsigned long long)W.fix(of_key(u)));
+                return in;
+            };
+            const float xl = of_key(first_key(bin)), xh = of_key(first_key(bin - 1) - 1);
+            auto read_bin = [&](auto&& take) {  // the bin's tokens from memory
+                read_slices([&](const float (&x)[kPer / 8][8], int i0) {
+                    for (int j = 0; j < kPer / 8; ++j)
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            if (x[j][q] >= xl && x[j][q] <= xh) take(key_of(x[j][q]), place(i0, j, q));
+                });
+            };
+            uint32_t lo = 0xffffffffu, hi = 0;
+            if (listed) {  // their indexes into the list, then their keys
+                read_slices([&](const float (&x)[kPer / 8][8], int i0) {
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int j = 0; j < kPer / 8; ++j)
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) m |= (uint32_t)(x[j][q] >= xl && x[j][q] <= xh) << (8 * j + q);
+                    if (!__any(m != 0)) return;
+                    int n = __popc(m);
+                    const int own = n;
+                    for (int d = 1; d < 64; d <<= 1) {
+                        const int p = __shfl_up(n, d);
+                        if (lane >= d) n += p;
                     }
+                    int at = 0;
+                    if (lane == 63) at = atomicAdd(&s_n, n);
+                    at = __builtin_amdgcn_readlane(at, 63) + n - own;
+#pragma unroll
+                    for (int j = 0; j < kPer / 8; ++j)
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            if ((m >> (8 * j + q)) & 1) {
+                                if (at < kList) list[at].y = (uint32_t)place(i0, j, q);
+                                ++at;
+                            }
                 });
                 __syncthreads();
-                // thread i holds digits n - 1 - 2 i and n - 2 - 2 i: the order of the tokens
-                uint64_t c[2] = {0, 0}, w[2] = {0, 0};
-                for (int q = 0; q < 2; ++q) {
-                    const int d = n - 1 - 2 * tid - q;
-                    if (d >= 0) c[q] = cnt[d], w[q] = wsum[d];
+                for (int i = tid; i < s_n && i < kList; i += kThreads) {
+                    float y[1];
+                    load_logits<1>(A, row, (int)list[i].y, y);
+                    const uint32_t k = key_of(y[0]);
+                    list[i].x = k;
+                    lo = k < lo ? k : lo;
+                    hi = k > hi ? k : hi;
                 }
-                uint64_t c0 = c[0] + c[1], w0 = w[0] + w[1];
-                block_before(c0, w0, red);
-                c0 += cb, w0 += wb;
-                uint64_t c1 = c0, w1 = w0;
-                for (int q = 0; q < 2; ++q) {
-                    const int d = n - 1 - 2 * tid - q;
-                    if (d >= 0 && c[q]) {
-                        const uint32_t lowest = (low == 32 ? 0u : prefix << low) | (uint32_t)d << sh;
-                        if (c1 + c[q] >= S.top_k || w1 + w[q] >= target || lowest < least) atomicMax(&s_bin, d);
-                    }
-                    c1 += c[q], w1 += w[q];
+            } else {
+                read_bin([&](uint32_t k, int) {
+                    lo = k < lo ? k : lo;
+                    hi = k > hi ? k : hi;
+                });
+            }
+            if (lo <= hi) atomicMin(&s_lo, lo), atomicMax(&s_hi, hi);
+            __syncthreads();
+            lo = s_lo, hi = s_hi;
+            const int held = s_n < kList ? s_n : kList;
+            auto scan = [&](auto&& take) {  // every token of the bin, in no order
+                if (listed)
+                    for (int i = tid; i < held; i += kThreads) take(list[i].x, (int)list[i].y);
+                else
+                    read_bin(take);
+            };
+            constexpr int N = kDigits / 64;
+            int buf = 0;
+            bool open = true;  // the border lies in what is left; else all of that is kept
+            auto border = [&](auto&& below) {  // among the digits of cnt[buf], the greatest first; below: min_p ends there
+                uint64_t c[N], w[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int d = kDigits - 1 - (lane * N + i);
+                    c[i] = cnt[buf][d], w[i] = wsum[buf][d];
                 }
+                const Border<N> B(c, w, cb, wb, [&](int p, uint64_t ce, uint64_t we, uint64_t) {
+                    return ce >= S.top_k || we >= target || below(kDigits - 1 - p);
+                });
+                open = B.place >= 0;
+                if (open) cb = B.cb, wb = B.wb, ties = cnt[buf][kDigits - 1 - B.place];
+                return kDigits - 1 - B.place;
+            };
+            auto turn = [&]() {  // to the other buffer; this one, which every wave has left, is cleared
                 __syncthreads();
-                whole = s_bin < 0;  // every token of this prefix is kept, and none below it
-                if (whole) {
-                    // the greatest key below the bin's: keys of lower bins are smaller than the bin's least
-                    uint32_t lowest = 0xffffffffu;
+                for (int i = tid; i < kDigits; i += kThreads) cnt[buf][i] = 0, wsum[buf][i] = 0;
+                buf ^= 1;
+            };
+            // first by the place within the bin, which spreads keys of any exponent (the last bin has none)
+            int part = -1;
+            auto part_of = [&](uint32_t u) {
+                const float v = of_key(u) * g.g;
+                const int d = (int)((v - floorf(v)) * kDigits);
+                return d < 0 ? 0 : d < kDigits ? d : kDigits - 1;
+            };
+            auto mine = [&](uint32_t u) { return part < 0 || part_of(u) == part; };
+            ties = cnt_bin;
+            edge = lo - 1;
+            if (bin < kBins - 1 && lo < hi) {
+                scan([&](uint32_t u, int) {
+                    atomicAdd(&cnt[buf][part_of(u)], 1u);
+                    atomicAdd(&wsum[buf][part_of(u)], (unsigned long long)W.fix(of_key(u)));
+                });
+                __syncthreads();
+                const int least_part = least_bin > bin ? -1 : least_bin < bin || S.min_p > 1.0 ? kDigits : part_of(least);
+                part = border([&](int d) { return d <= least_part; });
+                if (open) {
+                    if (tid == 0) s_lo = 0xffffffffu, s_hi = 0;
+                    turn();
+                    uint32_t l = 0xffffffffu, h = 0;
                     scan([&](uint32_t u, int) {
-                        if (level == 0 || (u >> low) == prefix) lowest = u < lowest ? u : lowest;
+                        if (!mine(u)) return;
+                        l = u < l ? u : l;
+                        h = u > h ? u : h;
                     });
-                    if (tid == 0) s_first = -1;  // as unsigned: the greatest
+                    if (l <= h) atomicMin(&s_lo, l), atomicMax(&s_hi, h);
                     __syncthreads();
-                    atomicMin((unsigned*)&s_first, lowest);
+                    lo = s_lo, hi = s_hi;
+                }
+            }
+            if (open) {
+                // then by key - lo, nine bits a level from the highest that the keys left use
+                int low = 0;
+                while (low < 32 && (hi - lo) >> low) low += kDigitBits;
+                uint32_t from = lo;  // the least key of what is left
+                edge = lo;
+                while (low > 0 && open) {
+                    const int sh = low - kDigitBits;
+                    scan([&](uint32_t u, int) {
+                        const uint32_t d = u - from;
+                        if (u >= from && (low >= 32 || d >> low == 0) && mine(u)) {
+                            atomicAdd(&cnt[buf][d >> sh], 1u);
+                            atomicAdd(&wsum[buf][d >> sh], (unsigned long long)W.fix(of_key(u)));
+                        }
+                    });
                     __syncthreads();
-                    edge = (uint32_t)s_first - 1u;
-                    ties = 0;
-                    break;
-                }
-                for (int q = 0; q < 2; ++q) {
-                    if (n - 1 - 2 * tid - q == s_bin) s_cb = c0, s_wb = w0;
-                    c0 += c[q], w0 += w[q];
-                }
-                __syncthreads();
-                prefix = (low == 32 ? 0u : prefix << bits[level]) | (uint32_t)s_bin;
-                low = sh;
-                cb = s_cb, wb = s_wb;
-                if (level == 2) {
-                    edge = prefix;
-                    const uint64_t f = W.fix(of_key(edge));
-                    ties = cnt[s_bin];
-                    if (S.top_k != ~0ull) ties = ties < S.top_k - cb ? ties : S.top_k - cb;
-                    if (f && target != ~0ull) {
-                        const uint64_t m = target > wb ? (target - wb + f - 1) / f : 0;
-                        ties = ties < m ? ties : m;
+                    const int d = border([&](int i) { return from + ((uint32_t)i << sh) < least; });
+                    if (open) {
+                        from += (uint32_t)d << sh;
+                        low = sh;
+                        edge = from;
+                    } else {
+                        edge = from - 1;  // what is left lies above; lower digits, parts and bins at this or below
                     }
-                    if (edge < least) ties = 0;
-                    if (cb == 0 && ties == 0) ties = 1;
+                    if (low > 0 && open) turn();
                 }
-                __syncthreads();
+            }
+            if (open) {  // one key is left: how many of it are kept
+                const uint64_t f = W.fix(of_key(edge));
+                if (S.top_k != ~0ull) ties = ties < S.top_k - cb ? ties : S.top_k - cb;
+                if (f && target != ~0ull) {
+                    const uint64_t m = target > wb ? (target - wb + f - 1) / f : 0;
+                    ties = ties < m ? ties : m;
+                }
+                if (edge < least) ties = 0;
+                if (cb == 0 && ties == 0) ties = 1;
+            } else {
+                ties = 0;
             }
             scan([&](uint32_t u, int i) {
                 if (u > edge) atomicAdd(&slice_w[i / kSlice], (unsigned long long)W.fix(of_key(u)));
@@ -490,83 +636,91 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
         }
     }
 
-    // Along the index: the slice that holds the token, then the token.
-    const uint64_t fe = W.fix(of_key(edge));
-    auto tied = [&](uint64_t before, uint64_t n) {  // how many of n equal ones behind `before` others are kept
-        const uint64_t a = before < ties ? before : ties, b = before + n < ties ? before + n : ties;
-        return b - a;
-    };
+    // Along the index, equal ones of key `edge` until `ties` are used up: the slice that holds the token ...
+    const uint64_t fe = ties ? W.fix(of_key(edge)) : 0;
     double u = (double)A.u[r];
     u = u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;
-    uint64_t total;
+    uint64_t total, goal, nb;
+    int slice;
     {
-        const uint64_t n = tid < slices ? slice_n[tid] : 0, w = tid < slices ? slice_w[tid] : 0;
-        uint64_t nb = n, unused = 0;
-        block_before(nb, unused, red);
-        const uint64_t m = w + tied(nb, n) * fe;
-        total = block_sum(m, (uint64_t*)red);
-        uint64_t goal = (uint64_t)floor(u * (double)total);
+        uint64_t w[kLaneSlices], n[kLaneSlices], ws = 0, ns = 0, unused;
+#pragma unroll
+        for (int i = 0; i < kLaneSlices; ++i) {
+            const int s = lane * kLaneSlices + i;
+            w[i] = s < slices ? slice_w[s] : 0, n[i] = s < slices ? slice_n[s] : 0;
+            ws += w[i], ns += n[i];
+        }
+        uint64_t n0 = wave_before(ns, &unused), w0 = wave_before(ws, &total);
+        total += (ties < unused ? ties : unused) * fe;
+        goal = (uint64_t)floor(u * (double)total);
         goal = goal < total ? goal : total - 1;  // u of one and above: the last kept token
-        uint64_t at = m;
-        unused = 0;
-        block_before(at, unused, red);
-        if (tid == 0) s_slice = slices - 1;
-        __syncthreads();
-        if (at <= goal && at + m > goal) s_slice = tid, s_wb = goal - at, s_cb = nb;
+        int mine = -1;
+        uint64_t mg = 0, mn = 0;
+#pragma unroll
+        for (int i = 0; i < kLaneSlices; ++i) {
+            const uint64_t a = w0 + (n0 < ties ? n0 : ties) * fe;
+            const uint64_t n1 = n0 + n[i], z = w0 + w[i] + (n1 < ties ? n1 : ties) * fe;
+            if (a <= goal && goal < z) mine = lane * kLaneSlices + i, mg = goal - a, mn = n0;
+            n0 = n1, w0 += w[i];
+        }
+        const uint64_t who = __ballot(mine >= 0);
+        const int l = who ? __builtin_ctzll(who) : 0;
+        slice = who ? __shfl(mine, l) : 0;
+        goal = shfl64(mg, l);  // within the slice
+        nb = shfl64(mn, l);    // equal ones before it
     }
-    __syncthreads();
-    const int i0 = s_slice * kSlice + tid * kPer;
-    const uint64_t goal = s_wb;  // within the slice
+    // ... then the token
+    const int i0 = slice * kSlice + tid * kPer;
     float x[kPer];
     if (i0 < V)
         load_logits<kPer>(A, row, i0, x);
     else
         for (int e = 0; e < kPer; ++e) x[e] = -INFINITY;
-    uint64_t w = 0, n = 0;
-    int last = -1;  // of this thread's kept tokens
-#pragma unroll
-    for (int e = 0; e < kPer; ++e)
-        if (x[e] > -INFINITY) {
-            const uint32_t k = key_of(x[e]);
-            if (k > edge) w += W.fix(x[e]);
-            n += k == edge;
-        }
-    uint64_t nb = n, unused = 0;
-    block_before(nb, unused, red);
-    nb += s_cb;
-    const uint64_t m = w + tied(nb, n) * fe;
-    uint64_t at = m;
-    unused = 0;
-    block_before(at, unused, red);
-    // the slice's sum was rounded apart from its tokens' by some units of 2^-44: the last kept one then
-    if (tid == 0) s_first = -1, s_n = 0x7fffffff;
-    __syncthreads();
+    uint64_t f[kPer], w = 0, n = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-        if (!(x[e] > -INFINITY)) continue;
-        const uint32_t k = key_of(x[e]);
-        const uint64_t f = k > edge ? W.fix(x[e]) : k == edge && nb < ties ? fe : 0;
-        nb += k == edge;
-        at += f;
-        if (f) last = i0 + e;
-        if (f && at > goal) {
-            atomicMin(&s_n, i0 + e);
-            break;
-        }
+        const uint32_t k = x[e] > -INFINITY ? key_of(x[e]) : 0;
+        f[e] = k > edge ? W.fix(x[e]) : 0;
+        w += f[e];
+        n += k && k == edge;
     }
-    if (last >= 0) atomicMax(&s_first, last);
+    uint64_t wa, na;
+    uint64_t w0 = wave_before(w, &wa), n0 = nb + wave_before(n, &na);
+    if (lane == 0) red[tid >> 6][0] = wa, red[tid >> 6][1] = na;
     __syncthreads();
-    const int tok = s_n != 0x7fffffff ? s_n : s_first;
-    if (tok >= i0 && tok < i0 + kPer) {
+    uint64_t sw = 0, sn = nb;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e)
-            if (tok == i0 + e) {
-                A.token[r] = tok;
-                if (A.logprob) {
-                    const double d = x[e] == mx ? 0.0 : ((double)x[e] - (double)mx) * S.inv_t;
-                    A.logprob[r] = (float)(d - log(__builtin_ldexp((double)total, -A.shift)));
-                }
+    for (int i = 0; i < kWaves; ++i) {
+        if (i < (tid >> 6)) w0 += red[i][0], n0 += red[i][1];
+        sw += red[i][0], sn += red[i][1];
+    }
+    auto kept = [&](uint64_t before) { return ((before < ties ? before : ties) - (nb < ties ? nb : ties)) * fe; };
+    const uint64_t all = sw + kept(sn);
+    // the slice's sum was rounded apart from its tokens', by some units of 2^-shift
+    goal = goal < all ? goal : all - 1;
+    uint64_t at = w0 + kept(n0);
+    if (all ? at <= goal && goal < w0 + w + kept(n0 + n) : tid == 0) {
+        int tok = -1;
+        float xt = 0.0f;
+        if (all) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                at += f[e];
+                if (x[e] > -INFINITY && key_of(x[e]) == edge) at += n0++ < ties ? fe : 0;
+                if (tok < 0 && at > goal) tok = i0 + e, xt = x[e];
             }
+        } else {  // every weight of the slice rounds to nothing: its largest logit
+            for (int i = slice * kSlice; i < (slice + 1) * kSlice && i < V; ++i) {
+                float y[1];
+                load_logits<1>(A, row, i, y);
+                if (y[0] > -INFINITY && (tok < 0 || y[0] > xt)) tok = i, xt = y[0];
+            }
+        }
+        A.token[r] = tok;
+        if (A.logprob) {
+            const double d = xt == mx ? 0.0 : ((double)xt - (double)mx) * S.inv_t;
+            A.logprob[r] = (float)(d - log(__builtin_ldexp((double)total, -A.shift)));
+        }
     }
 }
 
@@ -574,8 +728,8 @@ size_t sample_ws_bytes(int rows, int vocab) { return (size_t)layout(rows, vocab)
 
 int launch_sample(const SampleArgs& A, hipStream_t st) {
     if (A.rows == 0) return PGMOE_OK;
-    PG_LAUNCH(sample_slice_kernel, dim3((A.vocab + kSlice - 1) / kSlice, A.rows), dim3(kSliceThreads), 0, st, A);
-    PG_LAUNCH(sample_row_kernel, dim3(A.rows), dim3(kRowThreads), 0, st, A);
+    PG_LAUNCH(sample_slice_kernel, dim3((A.vocab + kSlice - 1) / kSlice, A.rows), dim3(kThreads), 0, st, A);
+    PG_LAUNCH(sample_row_kernel, dim3(A.rows), dim3(kThreads), 0, st, A);
     return check_launch("sample");
 }
 
