@@ -55,40 +55,67 @@ __device__ __forceinline__ float of_key(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// N consecutive logits from element i of a row on, -inf behind the last.
-template <int N>
-__device__ __forceinline__ void load_logits(const SampleArgs& A, int64_t row, int i, float (&x)[N]) {
-    const int64_t at = row + i;
-    if (A.dtype == PGMOE_DT_F32) {
-        const float* p = (const float*)A.logits + at;
-        if (N % 4 == 0 && i + N <= A.vocab && ((uintptr_t)p & 15) == 0) {
+// Eight consecutive logits as they lie in memory.
+template <int DT>
+struct Eight {
+    static constexpr int SZ = DT == PGMOE_DT_F32 ? 4 : 2;
+    uint4 v[SZ / 2];
+    // aligned and inside the row: straight loads, nothing that waits for them
+    __device__ __forceinline__ void load(const void* logits, int64_t at) {
+        const uint4* p = (const uint4*)((const uint8_t*)logits + at * SZ);
 #pragma unroll
-            for (int j = 0; j + 3 < N; j += 4) {
-                const float4 v = *(const float4*)(p + j);
-                x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = i + j < A.vocab ? p[j] : -INFINITY;
-        }
-        return;
+        for (int i = 0; i < SZ / 2; ++i) v[i] = p[i];
     }
-    const uint16_t* p = (const uint16_t*)A.logits + at;
-    uint16_t h[N];
-    if (N % 8 == 0 && i + N <= A.vocab && ((uintptr_t)p & 15) == 0) {
+    // any alignment; -inf behind the last
+    __device__ __forceinline__ void load_checked(const SampleArgs& A, int64_t row, int i) {
+        uint32_t* w = (uint32_t*)v;
+        if constexpr (DT == PGMOE_DT_F32) {
 #pragma unroll
-        for (int j = 0; j + 7 < N; j += 8) {
-            const uint4 v = *(const uint4*)(p + j);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            for (int j = 0; j < 8; ++j)
+                w[j] = i + j < A.vocab ? ((const uint32_t*)A.logits)[row + i + j] : 0xff800000u;
+        } else {
+            constexpr uint32_t out = DT == PGMOE_DT_F16 ? 0xfc00 : 0xff80;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) h[j + k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t a = i + 2 * j < A.vocab ? ((const uint16_t*)A.logits)[row + i + 2 * j] : out;
+                const uint32_t b = i + 2 * j + 1 < A.vocab ? ((const uint16_t*)A.logits)[row + i + 2 * j + 1] : out;
+                w[j] = a | b << 16;
+            }
         }
+    }
+    __device__ __forceinline__ float operator[](int j) const {
+        const uint32_t* w = (const uint32_t*)v;
+        if constexpr (DT == PGMOE_DT_F32)
+            return __builtin_bit_cast(float, w[j]);
+        else if constexpr (DT == PGMOE_DT_F16)
+            return h2f((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+        else
+            return __builtin_bit_cast(float, j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+    }
+};
+template <int DT>
+__device__ __forceinline__ float one_logit(const SampleArgs& A, int64_t at) {
+    if constexpr (DT == PGMOE_DT_F32)
+        return ((const float*)A.logits)[at];
+    else if constexpr (DT == PGMOE_DT_F16)
+        return h2f(((const uint16_t*)A.logits)[at]);
+    else
+        return __builtin_bit_cast(float, (uint32_t)((const uint16_t*)A.logits)[at] << 16);
+}
+// A thread's tokens of slice s (kPer / 8 times eight), -inf where there are none.
+template <int DT>
+__device__ __forceinline__ void load_slice(const SampleArgs& A, int64_t row, int s, bool aligned, Eight<DT> (&x)[kPer / 8]) {
+    if (aligned && (s + 1) * kSlice <= A.vocab) {
+#pragma unroll
+        for (int j = 0; j < kPer / 8; ++j) x[j].load(A.logits, row + s * kSlice + (j * kThreads + (int)threadIdx.x) * 8);
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) h[j] = i + j < A.vocab ? p[j] : A.dtype == PGMOE_DT_F16 ? 0xfc00 : 0xff80;
+        for (int j = 0; j < kPer / 8; ++j) x[j].load_checked(A, row, s * kSlice + (j * kThreads + (int)threadIdx.x) * 8);
     }
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = A.dtype == PGMOE_DT_F16 ? h2f(h[j]) : __builtin_bit_cast(float, (uint32_t)h[j] << 16);
+}
+template <int DT>
+__device__ __forceinline__ bool row_aligned(const SampleArgs& A, int64_t row) {
+    return (((uintptr_t)A.logits + row * Eight<DT>::SZ) & 15) == 0;
 }
 
 // The settings of a row.
@@ -169,6 +196,7 @@ __device__ __forceinline__ uint64_t wave_before(uint64_t v, uint64_t* all) {
     return x - v;
 }
 
+template <int DT>
 __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs A) {
     constexpr int G = 8, N = kPer / G;  // groups of 8 tokens a thread
     __shared__ uint32_t cnt[kBins];
@@ -179,15 +207,8 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
     __shared__ int s_first;
     const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, base = blockIdx.x * kSlice;
     const int64_t row = (int64_t)r * A.row_stride;
-    float x[N][G];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const int i = base + (j * kThreads + tid) * G;
-        if (i < A.vocab)
-            load_logits<G>(A, row, i, x[j]);
-        else
-            for (int e = 0; e < G; ++e) x[j][e] = -INFINITY;
-    }
+    Eight<DT> x[N];
+    load_slice<DT>(A, row, blockIdx.x, row_aligned<DT>(A, row), x);
     const Settings S(A, r);
     fill_powers(powers, tid);
     if (tid == 0) s_first = 0x7fffffff;
@@ -281,6 +302,7 @@ struct Border {
     }
 };
 
+template <int DT>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A) {
     constexpr int kLaneSlices = kMaxSlices / 64;
     __shared__ uint2 list[kList];  // (key, index) of the tokens of the last kept one's bin
@@ -303,6 +325,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
     const uint32_t* hc = (const uint32_t*)((uint8_t*)A.ws + o.cnt) + (int64_t)r * slices * kBins;
     const uint64_t* hw = (const uint64_t*)((uint8_t*)A.ws + o.wgt) + (int64_t)r * slices * kBins;
     const Settings S(A, r);
+    const bool aligned = row_aligned<DT>(A, row);
 
     // every wave holds the slices' maxima, so that the row's needs no meeting
     float mx = -INFINITY;
@@ -437,7 +460,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
             auto read_slices = [&](auto&& look) {
                 int s = -1;
                 while (s < slices) {
-                    float x[kBatch][kPer / 8][8];
+                    Eight<DT> x[kBatch][kPer / 8];
                     int at[kBatch];
 #pragma unroll
                     for (int b = 0; b < kBatch; ++b) {
@@ -445,18 +468,23 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                         while (s < slices && !slice_in[s]);
                         s = s < slices ? s : slices;
                         at[b] = s;
+                    }
+                    if (aligned && at[kBatch - 1] < slices && (at[kBatch - 1] + 1) * kSlice <= V) {
 #pragma unroll
-                        for (int j = 0; j < kPer / 8; ++j) {
-                            const int i = s * kSlice + (j * kThreads + tid) * 8;
-                            if (s < slices && i < V)
-                                load_logits<8>(A, row, i, x[b][j]);
-                            else
-                                for (int q = 0; q < 8; ++q) x[b][j][q] = -INFINITY;
+                        for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                            for (int j = 0; j < kPer / 8; ++j)
+                                x[b][j].load(A.logits, row + at[b] * kSlice + (j * kThreads + tid) * 8);
+#pragma unroll
+                        for (int b = 0; b < kBatch; ++b) look(x[b], at[b] * kSlice + tid * 8);
+                    } else {
+#pragma unroll 1
+                        for (int b = 0; b < kBatch; ++b) {
+                            if (at[b] >= slices) break;
+                            load_slice<DT>(A, row, at[b], aligned, x[0]);
+                            look(x[0], at[b] * kSlice + tid * 8);
                         }
                     }
-#pragma unroll
-                    for (int b = 0; b < kBatch; ++b)
-                        if (at[b] < slices) look(x[b], at[b] * kSlice + tid * 8);
                 }
             };
             auto place = [&](int i0, int j, int q) { return i0 + j * kThreads * 8 + q; };
@@ -476,7 +504,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
             };
             const float xl = of_key(first_key(bin)), xh = of_key(first_key(bin - 1) - 1);
             auto read_bin = [&](auto&& take) {  // the bin's tokens from memory
-                read_slices([&](const float (&x)[kPer / 8][8], int i0) {
+                read_slices([&](const Eight<DT> (&x)[kPer / 8], int i0) {
                     for (int j = 0; j < kPer / 8; ++j)
 #pragma unroll
                         for (int q = 0; q < 8; ++q)
@@ -485,7 +513,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
             };
             uint32_t lo = 0xffffffffu, hi = 0;
             if (listed) {  // their indexes into the list, then their keys
-                read_slices([&](const float (&x)[kPer / 8][8], int i0) {
+                read_slices([&](const Eight<DT> (&x)[kPer / 8], int i0) {
                     uint32_t m = 0;
 #pragma unroll
                     for (int j = 0; j < kPer / 8; ++j)
@@ -512,9 +540,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                 });
                 __syncthreads();
                 for (int i = tid; i < s_n && i < kList; i += kThreads) {
-                    float y[1];
-                    load_logits<1>(A, row, (int)list[i].y, y);
-                    const uint32_t k = key_of(y[0]);
+                    const uint32_t k = key_of(one_logit<DT>(A, row + list[i].y));
                     list[i].x = k;
                     lo = k < lo ? k : lo;
                     hi = k > hi ? k : hi;
@@ -672,10 +698,16 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
     // ... then the token
     const int i0 = slice * kSlice + tid * kPer;
     float x[kPer];
-    if (i0 < V)
-        load_logits<kPer>(A, row, i0, x);
-    else
-        for (int e = 0; e < kPer; ++e) x[e] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kPer / 8; ++j) {
+        Eight<DT> v;
+        if (aligned && i0 + kPer <= V)
+            v.load(A.logits, row + i0 + 8 * j);
+        else
+            v.load_checked(A, row, i0 + 8 * j);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[8 * j + q] = v[q];
+    }
     uint64_t f[kPer], w = 0, n = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
@@ -711,9 +743,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
             }
         } else {  // every weight of the slice rounds to nothing: its largest logit
             for (int i = slice * kSlice; i < (slice + 1) * kSlice && i < V; ++i) {
-                float y[1];
-                load_logits<1>(A, row, i, y);
-                if (y[0] > -INFINITY && (tok < 0 || y[0] > xt)) tok = i, xt = y[0];
+                const float y = one_logit<DT>(A, row + i);
+                if (y > -INFINITY && (tok < 0 || y > xt)) tok = i, xt = y;
             }
         }
         A.token[r] = tok;
@@ -728,8 +759,19 @@ size_t sample_ws_bytes(int rows, int vocab) { return (size_t)layout(rows, vocab)
 
 int launch_sample(const SampleArgs& A, hipStream_t st) {
     if (A.rows == 0) return PGMOE_OK;
-    PG_LAUNCH(sample_slice_kernel, dim3((A.vocab + kSlice - 1) / kSlice, A.rows), dim3(kThreads), 0, st, A);
-    PG_LAUNCH(sample_row_kernel, dim3(A.rows), dim3(kThreads), 0, st, A);
+    const dim3 slices((A.vocab + kSlice - 1) / kSlice, A.rows), rows(A.rows), block(kThreads);
+#define SAMPLE(DT)                                                              \
+    do {                                                                        \
+        PG_LAUNCH((sample_slice_kernel<DT>), slices, block, 0, st, A);          \
+        PG_LAUNCH((sample_row_kernel<DT>), rows, block, 0, st, A);              \
+    } while (0)
+    if (A.dtype == PGMOE_DT_F32)
+        SAMPLE(PGMOE_DT_F32);
+    else if (A.dtype == PGMOE_DT_F16)
+        SAMPLE(PGMOE_DT_F16);
+    else
+        SAMPLE(PGMOE_DT_BF16);
+#undef SAMPLE
     return check_launch("sample");
 }
 
