@@ -274,6 +274,22 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
     }
 }
 
+// The least key above `out` of which `in` (which is true, as all above the border are) holds: a wave tries 64 keys
+// around `near`, and bisects where the border lies elsewhere.
+template <class In>
+__device__ __forceinline__ uint32_t first_that(uint32_t near, uint32_t out, uint32_t top, In&& in) {
+    const int lane = threadIdx.x & 63;
+    if (near > out + 32 && near < top && top - near > 32) {
+        const uint64_t m = __ballot(in(near - 32 + lane));
+        if (m && !(m & 1)) return near - 32 + __builtin_ctzll(m);
+    }
+    while (top - out > 1) {
+        const uint32_t mid = out + (top - out) / 2;
+        (in(mid) ? top : out) = mid;
+    }
+    return top;
+}
+
 // Where the order of the tokens leaves the kept ones, among N places (bins or digits) a lane of one wave, in
 // order: the first place that is not kept whole, with the count and weight before it; -1: all are.
 template <int N>
@@ -305,6 +321,7 @@ struct Border {
 template <int DT>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A) {
     constexpr int kLaneSlices = kMaxSlices / 64;
+    __shared__ uint2 few[64];
     __shared__ uint2 list[kList];  // (key, index) of the tokens of the last kept one's bin
     __shared__ unsigned long long wsum[2][kDigits];
     __shared__ uint32_t cnt[2][kDigits];
@@ -405,22 +422,15 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
             atomicAdd(&cnt[0][b], c);
             atomicAdd(&wsum[0][b], (unsigned long long)to_row(w, s));
         });
-        // the least key that min_p keeps: bisection to the border of w >= min_p, from its logarithm
+        // the least key that min_p keeps: the border of w >= min_p, near its logarithm
         uint32_t least = 0;
         int least_bin = kBins;
         if (S.min_p >= 1.0) {
             least = key_of(mx) + (S.min_p > 1.0);
             least_bin = 0;
         } else if (S.min_p > 0.0) {
-            const uint32_t k = key_of((float)((double)mx + log(S.min_p) / S.inv_t));
-            uint32_t out = key_of(-INFINITY), in = key_of(mx);  // falls short, is kept
-            if (k > out + 8 && k < in && !(W.w(of_key(k - 8)) >= S.min_p)) out = k - 8;
-            if (k > out && k + 8 < in && W.w(of_key(k + 8)) >= S.min_p) in = k + 8;
-            while (in - out > 1) {
-                const uint32_t mid = out + (in - out) / 2;
-                (W.w(of_key(mid)) >= S.min_p ? in : out) = mid;
-            }
-            least = in;
+            least = first_that(key_of((float)((double)mx + log(S.min_p) / S.inv_t)), key_of(-INFINITY), key_of(mx),
+                               [&](uint32_t k) { return W.w(of_key(k)) >= S.min_p; });
             least_bin = g.bin(of_key(least));
         }
         __syncthreads();
@@ -441,7 +451,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
             bin = B.place, cb = B.cb, wb = B.wb;
         }
         const bool some = bin >= 0;
-        const uint32_t cnt_bin = some ? cnt[0][bin] : 0;
+        const int cnt_bin = some ? (int)cnt[0][bin] : 0;
         const bool listed = cnt_bin <= kList;
         __syncthreads();
         for (int i = tid; i < kBins; i += kThreads) cnt[0][i] = 0, wsum[0][i] = 0;
@@ -469,14 +479,20 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                         s = s < slices ? s : slices;
                         at[b] = s;
                     }
-                    if (aligned && at[kBatch - 1] < slices && (at[kBatch - 1] + 1) * kSlice <= V) {
+                    // a short batch reads its first slice again
+                    bool whole = aligned && at[0] < slices;
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b) whole = whole && (at[b] >= slices || (at[b] + 1) * kSlice <= V);
+                    if (whole) {
 #pragma unroll
                         for (int b = 0; b < kBatch; ++b)
 #pragma unroll
                             for (int j = 0; j < kPer / 8; ++j)
-                                x[b][j].load(A.logits, row + at[b] * kSlice + (j * kThreads + tid) * 8);
+                                x[b][j].load(A.logits,
+                                             row + (at[b] < slices ? at[b] : at[0]) * kSlice + (j * kThreads + tid) * 8);
 #pragma unroll
-                        for (int b = 0; b < kBatch; ++b) look(x[b], at[b] * kSlice + tid * 8);
+                        for (int b = 0; b < kBatch; ++b)
+                            if (at[b] < slices) look(x[b], at[b] * kSlice + tid * 8);
                     } else {
 #pragma unroll 1
                         for (int b = 0; b < kBatch; ++b) {
@@ -490,17 +506,10 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
             auto place = [&](int i0, int j, int q) { return i0 + j * kThreads * 8 + q; };
             // the bin's logits are those from xl to xh: the borders of its keys, by bisection near its place
             auto first_key = [&](int b) {  // the least key of bin b or a nearer one
-                uint32_t out = key_of(-INFINITY), in = key_of(mx);
-                if (b >= kBins - 1) return out + 1;
-                if (b < 0) return in + 1;
-                const uint32_t k = key_of((g.at - (float)b) / g.g);
-                if (k > out + 8 && k < in && g.bin(of_key(k - 8)) > b) out = k - 8;
-                if (k > out && k + 8 < in && g.bin(of_key(k + 8)) <= b) in = k + 8;
-                while (in - out > 1) {
-                    const uint32_t mid = out + (in - out) / 2;
-                    (g.bin(of_key(mid)) <= b ? in : out) = mid;
-                }
-                return in;
+                if (b >= kBins - 1) return key_of(-INFINITY) + 1;
+                if (b < 0) return key_of(mx) + 1;
+                return first_that(key_of((g.at - (float)b) / g.g), key_of(-INFINITY), key_of(mx),
+                                  [&](uint32_t k) { return g.bin(of_key(k)) <= b; });
             };
             const float xl = of_key(first_key(bin)), xh = of_key(first_key(bin - 1) - 1);
             auto read_bin = [&](auto&& take) {  // the bin's tokens from memory
@@ -512,15 +521,16 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                 });
             };
             uint32_t lo = 0xffffffffu, hi = 0;
-            if (listed) {  // their indexes into the list, then their keys
+            if (listed) {  // their indexes, then their keys
                 read_slices([&](const Eight<DT> (&x)[kPer / 8], int i0) {
                     uint32_t m = 0;
 #pragma unroll
                     for (int j = 0; j < kPer / 8; ++j)
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) m |= (uint32_t)(x[j][q] >= xl && x[j][q] <= xh) << (8 * j + q);
+                        for (int q = 0; q < 8; ++q)
+                            m |= (uint32_t)(__builtin_amdgcn_fmed3f(x[j][q], xl, xh) == x[j][q]) << (8 * j + q);
                     if (!__any(m != 0)) return;
-                    int n = __popc(m);
+                    int n = __popc(m);  // room in the list: one request a wave and slice
                     const int own = n;
                     for (int d = 1; d < 64; d <<= 1) {
                         const int p = __shfl_up(n, d);
@@ -529,21 +539,28 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                     int at = 0;
                     if (lane == 63) at = atomicAdd(&s_n, n);
                     at = __builtin_amdgcn_readlane(at, 63) + n - own;
-#pragma unroll
-                    for (int j = 0; j < kPer / 8; ++j)
-#pragma unroll
-                        for (int q = 0; q < 8; ++q)
-                            if ((m >> (8 * j + q)) & 1) {
-                                if (at < kList) list[at].y = (uint32_t)place(i0, j, q);
-                                ++at;
-                            }
+                    for (; m; m &= m - 1, ++at) {
+                        const int q = __builtin_ctz(m);
+                        if (at < kList) list[at].y = (uint32_t)place(i0, q >> 3, q & 7);
+                    }
                 });
                 __syncthreads();
-                for (int i = tid; i < s_n && i < kList; i += kThreads) {
-                    const uint32_t k = key_of(one_logit<DT>(A, row + list[i].y));
-                    list[i].x = k;
-                    lo = k < lo ? k : lo;
-                    hi = k > hi ? k : hi;
+                constexpr int U = 8;  // keys on their way at a time
+                for (int i = tid; i < cnt_bin; i += U * kThreads) {
+                    float y[U];
+#pragma unroll
+                    for (int q = 0; q < U; ++q) {
+                        const int e = i + q * kThreads < cnt_bin ? i + q * kThreads : i;
+                        y[q] = one_logit<DT>(A, row + list[e].y);
+                    }
+#pragma unroll
+                    for (int q = 0; q < U; ++q)
+                        if (i + q * kThreads < cnt_bin) {
+                            const uint32_t k = key_of(y[q]);
+                            list[i + q * kThreads].x = k;
+                            lo = k < lo ? k : lo;
+                            hi = k > hi ? k : hi;
+                        }
                 }
             } else {
                 read_bin([&](uint32_t k, int) {
@@ -554,10 +571,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
             if (lo <= hi) atomicMin(&s_lo, lo), atomicMax(&s_hi, hi);
             __syncthreads();
             lo = s_lo, hi = s_hi;
-            const int held = s_n < kList ? s_n : kList;
             auto scan = [&](auto&& take) {  // every token of the bin, in no order
                 if (listed)
-                    for (int i = tid; i < held; i += kThreads) take(list[i].x, (int)list[i].y);
+                    for (int i = tid; i < cnt_bin; i += kThreads) take(list[i].x, (int)list[i].y);
                 else
                     read_bin(take);
             };
@@ -591,9 +607,38 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                 return d < 0 ? 0 : d < kDigits ? d : kDigits - 1;
             };
             auto mine = [&](uint32_t u) { return part < 0 || part_of(u) == part; };
+            // up to 64 tokens: each wave ranks them by key and index; the kept ones are the first of that order
+            bool settled = false;
+            auto rank = [&](uint2 e, int n) {
+                const uint64_t f = lane < n ? W.fix(of_key(e.x)) : 0;
+                uint64_t before = wb;
+                int ahead = 0;
+                for (int j = 0; j < n; ++j) {
+                    const uint32_t k = __builtin_amdgcn_readlane(e.x, j), i = __builtin_amdgcn_readlane(e.y, j);
+                    const uint64_t w = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)f, j) |
+                                       (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(f >> 32), j) << 32;
+                    const bool first = k > e.x || (k == e.x && i < e.y);
+                    ahead += first;
+                    before += first ? w : 0;
+                }
+                const bool keep = lane < n && ((cb == 0 && ahead == 0) ||
+                                               (cb + ahead < S.top_k && before < target && e.x >= least));
+                const uint64_t kept = __ballot(keep);
+                uint32_t k = keep ? e.x : 0xffffffffu, top = lane < n ? e.x : 0;
+                for (int d = 32; d; d >>= 1) {
+                    const uint32_t p = __shfl_xor(k, d), q = __shfl_xor(top, d);
+                    k = p < k ? p : k;
+                    top = q > top ? q : top;
+                }
+                edge = kept ? k : top;
+                ties = kept ? __popcll(__ballot(keep && e.x == edge)) : 0;
+                settled = true;
+            };
             ties = cnt_bin;
             edge = lo - 1;
-            if (bin < kBins - 1 && lo < hi) {
+            if (cnt_bin <= 64) {
+                rank(lane < cnt_bin ? list[lane] : make_uint2(0u, 0u), cnt_bin);
+            } else if (bin < kBins - 1 && lo < hi) {
                 scan([&](uint32_t u, int) {
                     atomicAdd(&cnt[buf][part_of(u)], 1u);
                     atomicAdd(&wsum[buf][part_of(u)], (unsigned long long)W.fix(of_key(u)));
@@ -601,7 +646,15 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                 __syncthreads();
                 const int least_part = least_bin > bin ? -1 : least_bin < bin || S.min_p > 1.0 ? kDigits : part_of(least);
                 part = border([&](int d) { return d <= least_part; });
-                if (open) {
+                if (open && ties <= 64) {
+                    if (tid == 0) s_n = 0;
+                    __syncthreads();
+                    scan([&](uint32_t u, int i) {
+                        if (mine(u)) few[atomicAdd(&s_n, 1)] = make_uint2(u, (uint32_t)i);
+                    });
+                    __syncthreads();
+                    rank(lane < (int)ties ? few[lane] : make_uint2(0u, 0u), (int)ties);
+                } else if (open) {
                     if (tid == 0) s_lo = 0xffffffffu, s_hi = 0;
                     turn();
                     uint32_t l = 0xffffffffu, h = 0;
@@ -615,7 +668,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                     lo = s_lo, hi = s_hi;
                 }
             }
-            if (open) {
+            if (open && !settled) {
                 // then by key - lo, nine bits a level from the highest that the keys left use
                 int low = 0;
                 while (low < 32 && (hi - lo) >> low) low += kDigitBits;
@@ -642,7 +695,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                     if (low > 0 && open) turn();
                 }
             }
-            if (open) {  // one key is left: how many of it are kept
+            if (settled) {
+            } else if (open) {  // one key is left: how many of it are kept
                 const uint64_t f = W.fix(of_key(edge));
                 if (S.top_k != ~0ull) ties = ties < S.top_k - cb ? ties : S.top_k - cb;
                 if (f && target != ~0ull) {
