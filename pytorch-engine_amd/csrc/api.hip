@@ -79,6 +79,19 @@ static int check_kv(const char* what, const pgmoe_kv_cache* C, const pgmoe_kv_ba
     return PGMOE_OK;
 }
 
+// What the attention kernel's 32-bit arithmetic holds: row numbers divided by the group as a product of 32
+// bits, and the tiles of all segments, from 32 keys of 128 rows on, on one axis.
+static int check_attend(const KvCache& c, const KvBatch& b, int T, int hq) {
+    const int64_t group = hq / c.heads, keys = ((int64_t)b.max_pages << c.page_shift) + b.prefix;
+    const int64_t rows = T * group;
+    if (rows * group >= (int64_t)1 << 31)
+        return fail(PGMOE_E_UNSUPPORTED, "attend: %d tokens of %d query heads a KV head in one call", T, (int)group);
+    if ((rows / 128 + 1 + b.seqs) * c.heads > ((int64_t)1 << 30) / (keys / 32 + 16))
+        return fail(PGMOE_E_UNSUPPORTED, "attend: %d sequences, %d tokens on page tables of %lld keys", b.seqs, T,
+                    (long long)keys);
+    return PGMOE_OK;
+}
+
 int check_weights(const pgmoe_weights* w, const char* what, Mats* out) {
     if (!w) return fail(PGMOE_E_INVALID, "%s: NULL weights", what);
     if (w->qtype != PGMOE_Q4_1 && w->qtype != PGMOE_Q4_K && w->qtype != PGMOE_Q5_K && w->qtype != PGMOE_Q6_K &&
@@ -784,7 +797,9 @@ size_t pgmoe_attend_workspace_bytes(const pgmoe_kv_cache* C, const pgmoe_kv_batc
                                     int32_t n_q_heads) {
     KvCache kc;
     KvBatch kb;
-    if (check_kv("attend", C, B, n_tokens, n_q_heads, &kc, &kb) || n_tokens == 0) return 0;
+    if (check_kv("attend", C, B, n_tokens, n_q_heads, &kc, &kb) || check_attend(kc, kb, n_tokens, n_q_heads) ||
+        n_tokens == 0)
+        return 0;
     return attend_ws_bytes(kc, kb, n_tokens, n_q_heads);
 }
 
@@ -794,6 +809,7 @@ int pgmoe_attend(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, const void* q
     KvCache kc;
     KvBatch kb;
     int rc = check_kv("attend", C, B, n_tokens, n_q_heads, &kc, &kb);
+    if (!rc) rc = check_attend(kc, kb, n_tokens, n_q_heads);
     if (rc) return rc;
     if (!(scale > 0.0f) || scale > 3e38f) return fail(PGMOE_E_INVALID, "attend: scale must be positive and finite");
     if (n_tokens == 0) return PGMOE_OK;

@@ -37,9 +37,20 @@ _MAX_SEQS = 4096
 _IntTensor = Union[torch.Tensor, Sequence[int]]
 
 
-def _on_device(dev: torch.device):
-    """A guard that makes `dev` current for a launch; nothing when it already is."""
-    return torch.cuda.device(dev)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def launch(dev: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, stream) of the C ABI on `dev`'s current stream, with `dev` the current device; raises on a
+    status other than 0.  (The stream's handle by itself: a Stream object costs 2 us more.)"""
+    stream = _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        check(rc, what)
 
 
 def _cuda_device(device: Optional[Union[torch.device, str]]) -> torch.device:
@@ -207,21 +218,23 @@ class HipPagedKVCache:
     v = property(lambda self: self._v)
 
     # ------------------------------------------------------------------ checks
-    def _heads(self, name: str, x: torch.Tensor, dtypes, heads: Optional[int] = None) -> torch.Tensor:
+    def _heads(self, name: str, x: torch.Tensor, dtypes, heads: Optional[int] = None) -> Tuple[torch.Tensor, int, int]:
+        """x checked, and its token and head strides; copied where its rows cannot be read 16 bytes at a time."""
+        shape, dtype = x.shape, x.dtype
         if x.device != self.device:
             raise ValueError(f"{name} is on {x.device}, the cache on {self.device}")
-        if x.dtype not in dtypes:
-            raise NotImplementedError(f"{name} of dtype {x.dtype}")
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
-            raise ValueError(f"{name} {tuple(x.shape)}: [tokens, {'heads' if heads is None else heads}, {self.head_dim}]")
-        st = x.stride()
-        unit = 4 if x.dtype == torch.float32 else 8
-        if st[2] != 1 or st[0] % unit or st[1] % unit or x.data_ptr() % 16:
-            return x.clone(memory_format=torch.contiguous_format)  # rows the kernels cannot read 16 bytes at a time
-        return x
+        if dtype not in dtypes:
+            raise NotImplementedError(f"{name} of dtype {dtype}")
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
+            raise ValueError(f"{name} {tuple(shape)}: [tokens, {'heads' if heads is None else heads}, {self.head_dim}]")
+        a, b, c = x.stride()
+        if c != 1 or (a | b) & (3 if dtype is torch.float32 else 7) or x.data_ptr() & 15:
+            x = x.clone(memory_format=torch.contiguous_format)
+            a, b, c = x.stride()
+        return x, a, b
 
     def _tokens(self, q: torch.Tensor, batch: KVBatch) -> Tuple[int, int]:
-        T, hq = int(q.shape[0]), int(q.shape[1])
+        T, hq, _ = q.shape
         if hq < 1 or hq % self.n_kv_heads:
             raise ValueError(f"{hq} query heads on {self.n_kv_heads} KV heads")
         if batch.device != self.device:
@@ -232,7 +245,7 @@ class HipPagedKVCache:
             raise ValueError(f"a prefix of {batch.prefix_len} keys on {batch._prefix.shape[0]} pages of {self.page_size}")
         return T, hq
 
-    def _out(self, out: Optional[torch.Tensor], q: torch.Tensor, T: int, hq: int) -> torch.Tensor:
+    def _out(self, out: Optional[torch.Tensor], T: int, hq: int) -> torch.Tensor:
         if out is None:
             return torch.empty((T, hq, self.head_dim), dtype=self.dtype, device=self.device)
         if out.shape != (T, hq, self.head_dim) or out.dtype != self.dtype or out.device != self.device:
@@ -267,9 +280,10 @@ class HipPagedKVCache:
         alone.  No two tokens may fall on one cache row."""
         if k.dtype != q.dtype or v.dtype != q.dtype:
             raise ValueError(f"q, k and v of one dtype, not {q.dtype}, {k.dtype}, {v.dtype}")
-        q = self._heads("q", q, _DT)
+        q, qt, qh = self._heads("q", q, _DT)
         T, hq = self._tokens(q, batch)
-        k, v = self._heads("k", k, _DT, self.n_kv_heads), self._heads("v", v, _DT, self.n_kv_heads)
+        k, kt, kh = self._heads("k", k, _DT, self.n_kv_heads)
+        v, vt, vh = self._heads("v", v, _DT, self.n_kv_heads)
         if k.shape[0] != T or v.shape[0] != T:
             raise ValueError(f"{T} queries, {k.shape[0]} keys, {v.shape[0]} values")
         turns, rot, inter, factor = None, 0, 0, 1.0
@@ -277,26 +291,22 @@ class HipPagedKVCache:
             if rope.head_dim != self.head_dim or rope.device != self.device:
                 raise ValueError(f"rotary of head_dim {rope.head_dim} on {rope.device}, cache of {self.head_dim} on {self.device}")
             turns, rot, inter, factor = rope.turns.data_ptr(), rope.rotary_dim, rope.interleaved, rope.attn_factor
-        norms = []
-        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if w is not None:
-                if w.numel() != self.head_dim or w.device != self.device:
-                    raise ValueError(f"{name}: {self.head_dim} weights on {self.device}")
-                w = w.to(torch.float32).contiguous()
-                if w.data_ptr() % 16:
-                    w = w.clone()
-            norms.append(w)
-        res = self._out(out, q, T, hq)
+        qn = None if q_norm is None else self._norm("q_norm", q_norm)
+        kn = None if k_norm is None else self._norm("k_norm", k_norm)
+        res = self._out(out, T, hq)
         if out is not None:
             self._apart(out, q, k, v, self._k, self._v)
-        qs, ks, vs = q.stride(), k.stride(), v.stride()
-        with _on_device(self.device):
-            check(lib().pgmoe_rope_append(self._ref, batch._ref, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
-                                          v.data_ptr(), vs[0], vs[1], _DT[q.dtype], T, hq, turns, rot, int(inter), factor,
-                                          None if norms[0] is None else norms[0].data_ptr(),
-                                          None if norms[1] is None else norms[1].data_ptr(), float(eps), res.data_ptr(),
-                                          torch.cuda.current_stream(self.device).cuda_stream), "pgmoe_rope_append")
+        launch(self.device, "pgmoe_rope_append", lib().pgmoe_rope_append, self._ref, batch._ref, q.data_ptr(), qt, qh,
+               k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DT[q.dtype], T, hq, turns, rot, inter, factor,
+               None if qn is None else qn.data_ptr(), None if kn is None else kn.data_ptr(), eps, res.data_ptr())
         return res
+
+    def _norm(self, name: str, w: torch.Tensor) -> torch.Tensor:
+        if w.numel() != self.head_dim or w.device != self.device:
+            raise ValueError(f"{name}: {self.head_dim} weights on {self.device}")
+        if w.dtype is not torch.float32 or not w.is_contiguous():
+            w = w.to(torch.float32).contiguous()
+        return w.clone() if w.data_ptr() & 15 else w
 
     def attend(self, q: torch.Tensor, batch: KVBatch, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
@@ -308,12 +318,12 @@ class HipPagedKVCache:
         A query that sees no key gets zeros and -inf; one that sees a key on a page that does not exist
         gets NaN.  Masked keys and unused page rows may hold anything.  Rows of `out` behind the last
         sequence are left alone."""
-        q = self._heads("q", q, (self.dtype,))
+        q, qt, qh = self._heads("q", q, (self.dtype,))
         T, hq = self._tokens(q, batch)
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
         if not (0.0 < scale < 3e38):
             raise ValueError("scale must be positive and finite")
-        res = self._out(out, q, T, hq)
+        res = self._out(out, T, hq)
         if out is not None:
             self._apart(out, q, self._k, self._v)
         lse = torch.empty((T, hq), dtype=torch.float32, device=self.device) if return_lse else None
@@ -323,10 +333,7 @@ class HipPagedKVCache:
             n = self._ws_bytes[key] = int(lib().pgmoe_attend_workspace_bytes(self._ref, batch._ref, T, hq))
         # scratch of this call alone, from the stream's allocator: calls on other streams, and graphs that
         # replay side by side, each have their own
-        ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
-        qs = q.stride()
-        with _on_device(self.device):
-            check(lib().pgmoe_attend(self._ref, batch._ref, q.data_ptr(), qs[0], qs[1], T, hq, scale, res.data_ptr(),
-                                     None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), n,
-                                     torch.cuda.current_stream(self.device).cuda_stream), "pgmoe_attend")
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        launch(self.device, "pgmoe_attend", lib().pgmoe_attend, self._ref, batch._ref, q.data_ptr(), qt, qh, T, hq, scale,
+               res.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), n)
         return res if lse is None else (res, lse)

@@ -15,7 +15,8 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from ._lib import Sampling, check, lib
+from ._lib import Sampling, lib
+from .attention import launch
 
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _MAX_VOCAB = 1 << 20
@@ -47,7 +48,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Union[floa
         raise ValueError("logits: [rows, vocab] on a HIP device")
     if logits.dtype not in _DT:
         raise NotImplementedError(f"logits of dtype {logits.dtype} (fp32, fp16 or bf16)")
-    rows, vocab = int(logits.shape[0]), int(logits.shape[1])
+    rows, vocab = logits.shape
     if not 1 <= vocab <= _MAX_VOCAB:
         raise NotImplementedError(f"vocabulary of {vocab} (1 .. {_MAX_VOCAB})")
     dev = logits.device
@@ -61,15 +62,14 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Union[floa
     k, kv = _param("top_k", top_k, rows, dev, torch.int32)
     p, pv = _param("top_p", top_p, rows, dev, torch.float32)
     m, mv = _param("min_p", min_p, rows, dev, torch.float32)
-    par = Sampling(*(None if x is None else x.data_ptr() for x in (t, k, p, m)), float(tv), float(pv), float(mv),
-                   max(0, min(int(kv), 2 ** 31 - 1)))
+    par = Sampling(None if t is None else t.data_ptr(), None if k is None else k.data_ptr(),
+                   None if p is None else p.data_ptr(), None if m is None else m.data_ptr(), tv, pv, mv,
+                   0 if kv < 0 else min(int(kv), 2 ** 31 - 1))
     token = torch.empty(rows, dtype=torch.int64, device=dev)
     logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    n = int(lib().pgmoe_sample_workspace_bytes(rows, vocab))
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    with torch.cuda.device(dev):
-        check(lib().pgmoe_sample(logits.data_ptr(), _DT[logits.dtype], logits.stride(0), rows, vocab, u.data_ptr(),
-                                 ctypes.byref(par), token.data_ptr(), logprob.data_ptr(),
-                                 None if ws is None else ws.data_ptr(), n,
-                                 torch.cuda.current_stream(dev).cuda_stream), "pgmoe_sample")
+    L = lib()
+    n = int(L.pgmoe_sample_workspace_bytes(rows, vocab))
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)  # of this call alone
+    launch(dev, "pgmoe_sample", L.pgmoe_sample, logits.data_ptr(), _DT[logits.dtype], logits.stride(0), rows, vocab,
+           u.data_ptr(), ctypes.byref(par), token.data_ptr(), logprob.data_ptr(), ws.data_ptr(), n)
     return token, logprob

@@ -74,6 +74,11 @@ def test_attend_refusals():
     assert go(q=None) == -1 and go(q=0x1002) == -1 and go(qs=4100) == -1 and go(out=None) == -1 and go(out=0x2008) == -1
     assert go(T=-1) == -1 and go(hq=0) == -1 and go(hq=34) == -1 and go(T=4) == -1
     assert go(ws=0x110) == -1
+    B.q_start = 0x50000
+    assert go(T=1 << 24, hq=4 * 64) == -2 and "tokens" in L.pgmoe_last_error().decode()
+    B.n_seqs, B.max_pages, B.table_stride = 4096, 1 << 18, 1 << 18  # 4 million keys each of 4096 sequences
+    assert go(T=4096) == -2 and "page tables" in L.pgmoe_last_error().decode()
+    assert L.pgmoe_attend_workspace_bytes(C, B, 4096, 32) == 0
 
 
 def test_sample_refusals():
