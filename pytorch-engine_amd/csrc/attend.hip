@@ -822,12 +822,16 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                 if (j + 1 < stop) bring(j + 1);
                 const uint8_t* buf = smem + (j & 1) * 256 * D;
                 if (works) {
-                    f32x16 s[2];
-                    u16x8 p[4];
-                    core.template scores<2>(buf, s);
-                    core.template grow<2>(s);
-                    core.template weigh<2>(s, p);
-                    core.template values<2>(buf + 128 * D, p);
+                    constexpr int NG = D == 256 ? 1 : 2;  // groups of 32 keys at a time; at 256 the registers hold one
+#pragma unroll 1
+                    for (int half = 0; half < 2; half += NG) {
+                        f32x16 s[NG];
+                        u16x8 p[2 * NG];
+                        core.template scores<NG>(buf + half * 64 * D, s);
+                        core.template grow<NG>(s);
+                        core.template weigh<NG>(s, p);
+                        core.template values<NG>(buf + 128 * D + half * 64 * D, p);
+                    }
                 }
             }
             for (; j < stop; ++j) {
