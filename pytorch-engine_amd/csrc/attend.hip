@@ -365,7 +365,7 @@ struct Core {
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[g][i]);
         mx = fmaxf(mx, swap32(mx));
-        if (__any((mx - m) * c > 8.0f)) {
+        if (__builtin_expect(__any((mx - m) * c > 8.0f), 0)) {
             const float mn = fmaxf(m, mx);
             const float f = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * c);
             l *= f;
@@ -483,7 +483,7 @@ struct Core {
         mask(s[0], left, bad);
         grow<1>(s);
         weigh<1>(s, p);
-        if (any_odd(V))
+        if (__builtin_expect(any_odd(V), 0))
             values_odd(V, p, left);
         else
             values<1>(V, p);
