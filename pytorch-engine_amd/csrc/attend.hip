@@ -164,12 +164,13 @@ __device__ __forceinline__ int row_tiles(int rows) {
 // Tiles [j0, j1) of one segment: what a wave (split) or a workgroup (shared) computes at a time.
 struct Work {
     int prefix, lo, rows, row0, kvh, b, keys, j0, j1, slot, nslots;
+    int pre;          // tiles of the prefix before the own keys'
     int len, n, cap;  // own keys: Seq's
     int left;         // of the run behind this work
     __device__ __forceinline__ void scalar() {  // every lane holds the same: into scalar registers
         prefix = uni(prefix), lo = uni(lo), rows = uni(rows), row0 = uni(row0), kvh = uni(kvh), b = uni(b);
         keys = uni(keys), j0 = uni(j0), j1 = uni(j1), slot = uni(slot), nslots = uni(nslots);
-        len = uni(len), n = uni(n), cap = uni(cap), left = uni(left);
+        len = uni(len), n = uni(n), cap = uni(cap), left = uni(left), pre = uni(pre);
     }
 };
 
@@ -180,17 +181,18 @@ template <bool SPLIT>
 struct Axis {
     static constexpr int kHead = SPLIT ? kSplitHead : kSharedHead;
     int ptiles, psegs, run, total;
+    int pre;  // the prefix's tiles where every row tile takes them before its own keys
 
     // The cost of one KV head of this lane's sequence (`in`: it has one).  A wave sums the row tiles of a long
     // prompt together.
-    __device__ __forceinline__ static int cost(const AttendArgs& A, const Seq& s, bool in, int lane) {
+    __device__ __forceinline__ int cost(const AttendArgs& A, const Seq& s, bool in, int lane) const {
         const int rt = in && s.split() == SPLIT ? row_tiles(s.rows) : 0;
         int c = 0;
         if constexpr (SPLIT) {
             if (rt) c = s.tiles(A, 0) + kHead;
         } else {
             if (rt <= kAlone)
-                for (int t = 0; t < rt; ++t) c += s.tiles(A, t) + kHead;
+                for (int t = 0; t < rt; ++t) c += s.tiles(A, t) + pre + kHead;
             for (uint64_t big = __ballot(rt > kAlone); big; big &= big - 1) {
                 const int who = __builtin_ctzll(big);
                 Seq m;
@@ -198,7 +200,7 @@ struct Axis {
                 m.rows = __builtin_amdgcn_readlane(s.rows, who), m.cap = s.cap;
                 const int all = row_tiles(m.rows);
                 int sum = 0;
-                for (int t = lane; t < all; t += 64) sum += m.tiles(A, t) + kHead;
+                for (int t = lane; t < all; t += 64) sum += m.tiles(A, t) + pre + kHead;
                 for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
                 if (lane == who) c = sum;
             }
@@ -218,15 +220,15 @@ struct Axis {
         return W;
     }
     // The work that begins at `at` of the run that ends at `end`, found by one wave.
-    __device__ __forceinline__ Work find(const AttendArgs& A, const int* s_base, int per, int Tq, int at, int end, int who,
-                                         int lane) const {
+    __device__ __forceinline__ Work find(const AttendArgs& A, const int* s_base, const int (*s_seq)[3], int per, int Tq,
+                                         int at, int end, int who, int lane) const {
         const int pall = psegs * (ptiles + kHead);
         if (at < pall) {
             const int seg = at / (ptiles + kHead);
             Work W = fill(seg * (ptiles + kHead), ptiles, at, end, who);
             const int rows = Tq * A.group, prt = row_tiles(rows);
             W.prefix = 1, W.lo = 0, W.rows = rows, W.kvh = seg / prt, W.row0 = (seg - W.kvh * prt) * kSharedRows, W.b = 0;
-            W.keys = A.B.prefix, W.len = 0, W.n = 0, W.cap = 0;
+            W.keys = A.B.prefix, W.len = 0, W.n = 0, W.cap = 0, W.pre = 0;
             return W;
         }
         // the thread, then among its sequences, then the row tile: the last that begins at or before `at`
@@ -239,7 +241,8 @@ struct Axis {
         Seq s;
         int c = 0;
         if (per == 1) {
-            s = load_seq(A, i);
+            s.lo = s_seq[i][0], s.n = s_seq[i][1], s.len = s_seq[i][2];
+            s.cap = A.B.max_pages << A.C.page_shift, s.rows = s.n * A.group;
             c = uni(cost(A, s, lane == 0, lane));
         } else {
             const bool in = lane < per && i + lane < A.B.seqs;
@@ -265,7 +268,7 @@ struct Axis {
         if (!SPLIT) {
             const int rt = row_tiles(s.rows);
             for (;; t += 64) {
-                int inc = t + lane < rt ? s.tiles(A, t + lane) + kHead : 0;
+                int inc = t + lane < rt ? s.tiles(A, t + lane) + pre + kHead : 0;
                 for (int d = 1; d < 64; d <<= 1) {
                     const int o = __shfl_up(inc, d);
                     if (lane >= d) inc += o;
@@ -279,8 +282,8 @@ struct Axis {
                 from += uni(__shfl(inc, 63));
             }
         }
-        Work W = fill(from, s.tiles(A, t), at, end, who);
-        W.prefix = 0, W.lo = s.lo, W.rows = s.rows, W.row0 = t * kSharedRows, W.kvh = kvh, W.b = i;
+        Work W = fill(from, s.tiles(A, t) + pre, at, end, who);
+        W.pre = pre, W.prefix = 0, W.lo = s.lo, W.rows = s.rows, W.row0 = t * kSharedRows, W.kvh = kvh, W.b = i;
         W.keys = s.seen(SPLIT ? s.n - 1 : s.last_token(A, t));
         W.len = s.len, W.n = s.n, W.cap = s.cap;
         return W;
@@ -570,7 +573,10 @@ __device__ __forceinline__ void put_row(const AttendArgs& A, const Work& W, bool
         const int64_t R = (int64_t)A.T * A.hq;
         A.ml[((W.prefix ? 0 : A.nslot) + W.slot) * R + row] = make_float2(m, l);
     }
-    if (W.slot == 0 && A.slots) A.slots[(W.prefix ? 0 : (int64_t)A.T * A.hq) + row] = empty ? 0 : W.nslots;
+    if (W.slot == 0) {
+        A.slots[(W.prefix ? 0 : (int64_t)A.T * A.hq) + row] = empty ? 0 : W.nslots;
+        if (W.pre) A.slots[row] = 0;
+    }
 }
 
 // A wave's rows of one piece of work.
@@ -599,7 +605,7 @@ struct Rows {
         for (int i = 0; i < Core<D, BF16>::NK; ++i) core.q[i] = *(const u16x8*)(qp + 16 * i);
     }
     __device__ __forceinline__ void store(const AttendArgs& A, const Work& W, const Core<D, BF16>& core) const {
-        const bool direct = !W.prefix && !A.B.prefix && W.nslots == 1;
+        const bool direct = !W.prefix && (!A.B.prefix || W.pre) && W.nslots == 1;
         float l = core.l + core.swap32(core.l);
         if (far) l = NAN;
         const bool empty = !W.prefix && !A.B.prefix && seen == 0;
@@ -617,17 +623,18 @@ struct Rows {
     }
 };
 
-// How many of the tiles [j0, j1) need no checks: every key on a page and seen by every row.
-__device__ __forceinline__ int plain_tiles(const AttendArgs& A, const Work& W, const int32_t* pages, int tile, int least,
-                                           int lane) {
+// Where the tiles from j0 on need no checks any more, up to j1: every key on a page, and of the `least` that
+// every row sees.
+__device__ __forceinline__ int plain_tiles(const AttendArgs& A, const int32_t* pages, int j0, int j1, int tile, int keys,
+                                           int least, int lane) {
     bool ok = true;
-    const int k0 = W.j0 * tile, k1 = W.j1 * tile < W.keys ? W.j1 * tile : W.keys;
+    const int k0 = j0 * tile, k1 = j1 * tile < keys ? j1 * tile : keys;
     for (int i = (k0 >> A.C.page_shift) + lane; (int64_t)i << A.C.page_shift < k1; i += 64) {
         const int page = pages[i];
         ok = ok && page >= 0 && page < A.C.n_pages;
     }
     const int jf = __all(ok) ? least / tile : 0;
-    return jf < W.j0 ? W.j0 : jf < W.j1 ? jf : W.j1;
+    return uni(jf < j0 ? j0 : jf < j1 ? jf : j1);
 }
 
 template <int D, bool BF16>
@@ -636,56 +643,78 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
     using K = Core<D, BF16>;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
     __shared__ int s_base[2][kThreads];
-    __shared__ int s_red[4][4];
+    __shared__ int s_seq[kThreads][3];
+    __shared__ int s_red[4][5];
     const int tid = threadIdx.x, lane = tid & 63, wv = uni(tid >> 6);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem;
 
     // ---- the two axes: split segments are dealt to waves, shared ones to workgroups
+    Axis<true> ax0;
+    Axis<false> ax1;
+    ax0.pre = ax1.pre = 0;
     const int per = (A.B.seqs + kThreads - 1) / kThreads;
-    int mine[4] = {0, 0, 0, 0};  // split and shared cost; the longest segment of each
+    int mine[5] = {0, 0, 0, 0, 0};  // split and shared cost, shared row tiles; the longest segment of each kind
     for (int i = 0; i < per; ++i) {
         const int b = tid * per + i;
         const bool in = b < A.B.seqs;
         const Seq s = load_seq(A, in ? b : A.B.seqs - 1);
-        mine[0] += Axis<true>::cost(A, s, in, lane) * A.C.heads;
-        mine[1] += Axis<false>::cost(A, s, in, lane) * A.C.heads;
+        if (per == 1) s_seq[tid][0] = s.lo, s_seq[tid][1] = s.n, s_seq[tid][2] = s.len;
+        mine[0] += ax0.cost(A, s, in, lane) * A.C.heads;
+        mine[1] += ax1.cost(A, s, in, lane) * A.C.heads;
         if (in && s.rows) {
-            const int k = s.tiles(A, row_tiles(s.rows) - 1), kind = s.split() ? 2 : 3;
+            const int k = s.tiles(A, row_tiles(s.rows) - 1), kind = s.split() ? 3 : 4;
             mine[kind] = k > mine[kind] ? k : mine[kind];
+            if (!s.split()) mine[2] += row_tiles(s.rows) * A.C.heads;
         }
     }
-    int inc[2] = {mine[0], mine[1]};
+    int inc[3] = {mine[0], mine[1], mine[2]};
     for (int d = 1; d < 64; d <<= 1) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < 3; ++k) {
             const int o = __shfl_up(inc[k], d);
             if (lane >= d) inc[k] += o;
-            const int x = __shfl_xor(mine[2 + k], d);
-            mine[2 + k] = x > mine[2 + k] ? x : mine[2 + k];
+        }
+#pragma unroll
+        for (int k = 3; k < 5; ++k) {
+            const int x = __shfl_xor(mine[k], d);
+            mine[k] = x > mine[k] ? x : mine[k];
         }
     }
-    if (lane == 63) s_red[wv][0] = inc[0], s_red[wv][1] = inc[1], s_red[wv][2] = mine[2], s_red[wv][3] = mine[3];
-    __syncthreads();
-    int before[2] = {inc[0] - mine[0], inc[1] - mine[1]}, own[2] = {0, 0}, most[2] = {0, 0};
+    if (lane == 63) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-        for (int i = 0; i < 4; ++i) {
+        for (int k = 0; k < 3; ++k) s_red[wv][k] = inc[k];
+        s_red[wv][3] = mine[3], s_red[wv][4] = mine[4];
+    }
+    __syncthreads();
+    int before[3] = {inc[0] - mine[0], inc[1] - mine[1], inc[2] - mine[2]}, own[3] = {0, 0, 0}, most[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
             if (i < wv) before[k] += s_red[i][k];
             own[k] += s_red[i][k];
-            most[k] = s_red[i][2 + k] > most[k] ? s_red[i][2 + k] : most[k];
         }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) most[k] = s_red[i][3 + k] > most[k] ? s_red[i][3 + k] : most[k];
+    }
     int Tq = A.T;
     if (A.B.q_start) {
         const int e = A.B.q_start[A.B.seqs];
         Tq = uni(e < 0 ? 0 : e < Tq ? e : Tq);
     }
-    Axis<true> ax0;
-    Axis<false> ax1;
     int nsplit;
     {
-        const int prows = A.B.prefix ? Tq * A.group : 0;
+        int prows = A.B.prefix ? Tq * A.group : 0;
         const bool sp = prows <= kSplitRows;
         const int tile = sp ? kSplitKeys : kSharedKeys, pt = (A.B.prefix + tile - 1) / tile;
+        // Prompts: where every sequence fills row tiles of its own, the prefix has as few readers when each
+        // row tile goes through it on the way to its own keys, and no row is left in two parts (six prompts of
+        // 200 to 1201 tokens on a prefix of 4097 keys: 444 -> 409 us).
+        if (prows && !own[0] && own[2] * 8 <= (row_tiles(prows) * A.C.heads) * 10) {
+            ax1.pre = pt;
+            prows = 0;
+            own[1] += own[2] * pt, before[1] += before[2] * pt, most[1] += pt;
+        }
         const int segs = row_tiles(prows) * A.C.heads;
         ax0.ptiles = ax1.ptiles = pt;
         ax0.psegs = sp ? segs : 0;
@@ -696,9 +725,11 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
         s_base[1][tid] = p1 + before[1];
         ax0.total = uni(p0 + own[0]);
         ax1.total = uni(p1 + own[1]);
-        // the workgroups by the time that the two kinds take (a shared tile about 1.5 split ones), each kind
-        // spread evenly over the grid: the one streams the cache while the other multiplies
-        const float c0 = 2.0f * ax0.total, c1 = 3.0f * ax1.total;
+        // the workgroups by the time that the two kinds take, each kind spread evenly over the grid: the one
+        // streams the cache while the other multiplies.  A shared tile counts as 3 split ones: 128 us for 256
+        // rows of one token behind 16000 shared keys, against 138 at 1.5, 127 at 2, 130 at 4, 143 at 1; for 64
+        // behind 8192 39.5 against 42.9, 40.9, 39.5, 45
+        const float c0 = ax0.total, c1 = 3.0f * ax1.total;
         int g0 = (int)((float)gridDim.x * c0 / (c0 + c1 + 1.0f) + 0.5f);
         if (ax0.total && g0 < 1) g0 = 1;
         if (ax1.total && g0 > (int)gridDim.x - 1) g0 = gridDim.x - 1;
@@ -726,7 +757,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
         int at = ax0.total / ax0.run < who ? ax0.total : who * ax0.run;
         const int end = at + ax0.run < ax0.total ? at + ax0.run : ax0.total;
         while (at < end) {
-            Work W = ax0.find(A, s_base[0], per, Tq, at, end, who, lane);
+            Work W = ax0.find(A, s_base[0], s_seq, per, Tq, at, end, who, lane);
             W.scalar();
             at = end - W.left;
             if (W.j0 >= W.j1) continue;
@@ -742,15 +773,15 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                 copy_block<D, true>(A, A.C.v, b0, lane, vb);
                 copy_block<D, true>(A, A.C.v, b1, lane, vb + 32 * D);
             };
+            int key = W.j0 * kSplitKeys;
+            const int stop = W.j1 * kSplitKeys < W.keys ? W.j1 * kSplitKeys : W.keys;
             K core;
             core.begin(lane);
             core.c = A.c;
             const Rows<D, BF16> R(A, W, core.n);
             R.load_q(A, W, core);
-            const int jf = uni(plain_tiles(A, W, pages, kSplitKeys, uni(R.seen), lane));
-            int key = W.j0 * kSplitKeys;
-            const int stop = W.j1 * kSplitKeys < W.keys ? W.j1 * kSplitKeys : W.keys;
             if (key < stop) bring_k(key), bring_v();
+            const int jf = plain_tiles(A, pages, W.j0, W.j1, kSplitKeys, W.keys, uni(R.seen), lane);
 #pragma unroll
             for (int i = 0; i < K::NK; ++i) asm volatile("" : "+v"(core.q[i]));  // arrived before the loops
             for (int j = W.j0; j < jf; ++j) {
@@ -786,65 +817,78 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
         int at = ax1.total / ax1.run < who ? ax1.total : who * ax1.run;
         const int end = at + ax1.run < ax1.total ? at + ax1.run : ax1.total;
         while (at < end) {
-            Work W = ax1.find(A, s_base[1], per, Tq, at, end, who, lane);
+            Work W = ax1.find(A, s_base[1], s_seq, per, Tq, at, end, who, lane);
             W.scalar();
             at = end - W.left;
             if (W.j0 >= W.j1) continue;
             const int32_t* pages = W.prefix ? A.B.prefix_pages : A.B.table + (int64_t)W.b * A.B.table_stride;
+            const bool works = 32 * wv < W.rows - W.row0;
+            auto bring = [&](int j) {
+                const uint32_t buf = lds0 + (j & 1) * 256 * D + wv * 32 * D;
+                const bool p = j < W.pre;
+                const Block b = find_block(A, p ? A.B.prefix_pages : pages, W.kvh,
+                                           (p ? j : j - W.pre) * kSharedKeys + 16 * wv, p ? A.B.prefix : W.keys);
+                copy_block<D, false>(A, A.C.k, b, lane, buf);
+                copy_block<D, true>(A, A.C.v, b, lane, buf + 128 * D);
+            };
+            // a segment without own keys still has a tile for them, which is skipped
+            const int last = W.keys > 0 ? W.j1 : W.pre < W.j1 ? W.pre : W.j1;
+            const int stop = last > W.j0 ? last : W.j0;
             K core;
             core.begin(lane);
             core.c = A.c;
             const Rows<D, BF16> R(A, W, W.row0 + 32 * wv + core.n);
             R.load_q(A, W, core);
-            int jf;
-            {  // the first row of the whole tile sees least
-                Seq s;
-                s.len = W.len, s.n = W.n, s.cap = W.cap;
-                jf = uni(plain_tiles(A, W, pages, kSharedKeys, W.prefix ? W.keys : s.seen(group_of(A, W.row0)), lane));
-            }
-            const int seen1 = __builtin_amdgcn_readlane(R.seen, 31);  // the wave's last row sees most
-            const bool works = 32 * wv < W.rows - W.row0;
-            auto bring = [&](int j) {
-                const uint32_t buf = lds0 + (j & 1) * 256 * D + wv * 32 * D;
-                const Block b = find_block(A, pages, W.kvh, j * kSharedKeys + 16 * wv, W.keys);
-                copy_block<D, false>(A, A.C.k, b, lane, buf);
-                copy_block<D, true>(A, A.C.v, b, lane, buf + 128 * D);
-            };
-            const int stop = W.keys > 0 ? W.j1 : W.j0;
             lds_barrier();  // every wave is done with the last segment's buffers
             if (W.j0 < stop) bring(W.j0);
-#pragma unroll
-            for (int i = 0; i < K::NK; ++i) asm volatile("" : "+v"(core.q[i]));  // arrived before the loops
             int j = W.j0;
-            for (; j < jf; ++j) {
-                vm_wait<0>();
-                lds_barrier();
-                if (j + 1 < stop) bring(j + 1);
-                const uint8_t* buf = smem + (j & 1) * 256 * D;
-                if (works) {
-                    constexpr int NG = D == 256 ? 1 : 2;  // groups of 32 keys at a time; at 256 the registers hold one
 #pragma unroll 1
-                    for (int half = 0; half < 2; half += NG) {
-                        f32x16 s[NG];
-                        u16x8 p[2 * NG];
-                        core.template scores<NG>(buf + half * 64 * D, s);
-                        core.template grow<NG>(s);
-                        core.template weigh<NG>(s, p);
-                        core.template values<NG>(buf + 128 * D + half * 64 * D, p);
+            for (int part = 0; part < 2; ++part) {  // the prefix's tiles, which every row sees, then the own keys'
+                const int from = part ? W.pre : 0, to = part || stop < W.pre ? stop : W.pre;
+                if (j >= to) continue;
+                const int32_t* where = part ? pages : A.B.prefix_pages;
+                const int keys = part ? W.keys : A.B.prefix;
+                const int seen = part ? R.seen : keys;
+                const int seen1 = __builtin_amdgcn_readlane(seen, 31);  // the wave's last row sees most
+                int least = keys;
+                if (part && !W.prefix) {  // the first row of the whole tile sees least
+                    Seq s;
+                    s.len = W.len, s.n = W.n, s.cap = W.cap;
+                    least = s.seen(group_of(A, W.row0));
+                }
+                const int jf = from + plain_tiles(A, where, j - from, to - from, kSharedKeys, keys, least, lane);
+#pragma unroll
+                for (int i = 0; i < K::NK; ++i) asm volatile("" : "+v"(core.q[i]));  // arrived before the loops
+                for (; j < jf; ++j) {
+                    vm_wait<0>();
+                    lds_barrier();
+                    if (j + 1 < stop) bring(j + 1);
+                    const uint8_t* buf = smem + (j & 1) * 256 * D;
+                    if (works) {
+                        constexpr int NG = D == 256 ? 1 : 2;  // groups of 32 keys at a time; at 256 the registers hold one
+#pragma unroll 1
+                        for (int half = 0; half < 2; half += NG) {
+                            f32x16 s[NG];
+                            u16x8 p[2 * NG];
+                            core.template scores<NG>(buf + half * 64 * D, s);
+                            core.template grow<NG>(s);
+                            core.template weigh<NG>(s, p);
+                            core.template values<NG>(buf + 128 * D + half * 64 * D, p);
+                        }
                     }
                 }
-            }
-            for (; j < stop; ++j) {
-                vm_wait<0>();
-                lds_barrier();
-                if (j + 1 < stop) bring(j + 1);
-                const uint8_t* buf = smem + (j & 1) * 256 * D;
+                for (; j < to; ++j) {
+                    vm_wait<0>();
+                    lds_barrier();
+                    if (j + 1 < stop) bring(j + 1);
+                    const uint8_t* buf = smem + (j & 1) * 256 * D;
 #pragma unroll 1
-                for (int half = 0; half < 2 && works; ++half) {
-                    const int key = j * kSharedKeys + 32 * half;
-                    if (key >= seen1) break;
-                    core.checked(buf + half * 64 * D, buf + 128 * D + half * 64 * D, R.seen - key,
-                                 bad_blocks(A, pages, key, W.keys, 2));
+                    for (int half = 0; half < 2 && works; ++half) {
+                        const int key = (j - from) * kSharedKeys + 32 * half;
+                        if (key >= seen1) break;
+                        core.checked(buf + half * 64 * D, buf + 128 * D + half * 64 * D, seen - key,
+                                     bad_blocks(A, where, key, keys, 2));
+                    }
                 }
             }
             R.store(A, W, core);
@@ -872,7 +916,7 @@ __global__ __launch_bounds__(kThreads) void combine_rows_kernel(const AttendArgs
     if (live) {
         ns = A.slots[R + row];
         np = A.B.prefix ? A.slots[row] : 0;
-        live = A.B.prefix || ns != 1;  // else written by the only run that had it
+        live = np || ns != 1;  // else written by the only run that had it
         ns = ns < 0 ? 0 : ns > A.nslot ? A.nslot : ns;
         np = np < 0 ? 0 : np > A.nslot ? A.nslot : np;
     }
