@@ -520,6 +520,14 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                             if (x[j][q] >= xl && x[j][q] <= xh) take(key_of(x[j][q]), place(i0, j, q));
                 });
             };
+            auto meet = [&](uint32_t l, uint32_t h) {  // the least and greatest key of the workgroup
+                for (int d = 32; d; d >>= 1) {
+                    const uint32_t p = __shfl_xor(l, d), q = __shfl_xor(h, d);
+                    l = p < l ? p : l;
+                    h = q > h ? q : h;
+                }
+                if (lane == 0 && l <= h) atomicMin(&s_lo, l), atomicMax(&s_hi, h);
+            };
             uint32_t lo = 0xffffffffu, hi = 0;
             if (listed) {  // their indexes, then their keys
                 read_slices([&](const Eight<DT> (&x)[kPer / 8], int i0) {
@@ -568,7 +576,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                     hi = k > hi ? k : hi;
                 });
             }
-            if (lo <= hi) atomicMin(&s_lo, lo), atomicMax(&s_hi, hi);
+            meet(lo, hi);
             __syncthreads();
             lo = s_lo, hi = s_hi;
             auto scan = [&](auto&& take) {  // every token of the bin, in no order
@@ -663,7 +671,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                         l = u < l ? u : l;
                         h = u > h ? u : h;
                     });
-                    if (l <= h) atomicMin(&s_lo, l), atomicMax(&s_hi, h);
+                    meet(l, h);
                     __syncthreads();
                     lo = s_lo, hi = s_hi;
                 }
