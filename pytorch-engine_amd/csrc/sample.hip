@@ -1,15 +1,22 @@
 // Token sampling: temperature, top-k, top-p, min-p and a given uniform number a row.
 //
 // Weights w = exp((x - max) / T) are held as 64-bit fixed point (2^-44 for vocabularies of 2^18, finer for
-// smaller ones: a sum stays below 2^63): integer sums have no order, and a row's result is the same bits however it is cut.  No
-// row is sorted: the last kept token is found from a histogram over the distance to the maximum, then by a
-// radix descent over the float keys of the one bin that holds it.
+// smaller ones: a sum stays below 2^63): integer sums have no order, and a row's result is the same bits however
+// it is cut.  No row is sorted: the last kept token is found from a histogram over the distance to the maximum,
+// then from the tokens of the one bin that holds it.
 //
-// slice_kernel, a workgroup for 8192 tokens of a row, reads the logits once into registers: the slice's
-// maximum, and against it the tokens' weights, their sum and the histogram (256 bins of 1/8 in x / T on a grid
-// that all slices share).  row_kernel, a workgroup a row: the slices' sums brought to the row's maximum (a
-// slice that holds the maximum exactly, so that equal logits stay equal weights), the bin of the last kept
-// token, its tokens read again into LDS, the descent, and the sums along the index down to the token.
+// sample_slice_kernel, a workgroup for 8192 tokens of a row, reads the logits once into registers: the slice's
+// maximum, and against it the tokens' weights, their sum, the histogram (256 bins of 1/8 in x / T on a grid that
+// all slices share) and the tokens' indexes, sorted by bin as they are counted.  sample_row_kernel, a workgroup a
+// row: the slices' sums brought to the row's maximum (a slice that holds the maximum exactly, so that equal logits
+// stay equal weights), the bin of the last kept token, its tokens by the slices' lists into LDS, the border among
+// them, and the sums along the index down to the token.
+//
+// Bound: the slices by the bytes of the logits where a row is not filtered (256 rows of 131072 in fp32: 41 us for
+// 134 MB), by the shared-memory atomics of the histogram where it is (64 us); the rows by a chain of some twelve
+// steps that wait for each other (15 to 40 us, whatever the rows).  The lists cost the slices 2 bytes a token and
+// save the rows a second look at their logits: 48 rows with all filters 69 -> 57 us, 64 rows whose bin holds more
+// than LDS does 186 -> 84, 256 rows 107 -> 104.
 #include "launch.h"
 #include "sample.h"
 
@@ -24,7 +31,6 @@ constexpr float kPerNat = 8.0f;                // bins a unit of x / T
 constexpr int kDigitBits = 9;                  // of a level of the descent
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kList = 7168;                    // tokens of one bin that fit LDS
-constexpr int kBatch = 4;                      // slices that row_kernel reads at a time
 constexpr int kHeld = 12;                      // histogram entries that a thread keeps in registers
 constexpr int kMaxSlices = kMaxVocab / kSlice;
 
@@ -34,7 +40,7 @@ struct Slice {
     int first;  // lowest index of the maximum
 };
 struct Layout {
-    int64_t slices, cnt, wgt, total;
+    int64_t slices, cnt, wgt, off, idx, total;
 };
 static __host__ __device__ Layout layout(int rows, int vocab) {
     const int64_t n = (int64_t)rows * ((vocab + kSlice - 1) / kSlice);
@@ -42,7 +48,9 @@ static __host__ __device__ Layout layout(int rows, int vocab) {
     o.slices = 0;
     o.wgt = (n * (int64_t)sizeof(Slice) + 255) / 256 * 256;
     o.cnt = o.wgt + n * kBins * 8;
-    o.total = o.cnt + n * kBins * 4;
+    o.off = o.cnt + n * kBins * 4;
+    o.idx = o.off + n * kBins * 2;
+    o.total = o.idx + n * kSlice * 2;
     return o;
 }
 
@@ -204,6 +212,8 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
     __shared__ double powers[kPowers];
     __shared__ float s_max[kWaves];
     __shared__ uint64_t s_sum[kWaves];
+    __shared__ uint16_t off[kBins];                              // where a bin's tokens begin in idx
+    __shared__ __attribute__((aligned(16))) uint16_t idx[kSlice];  // the tokens by bin
     __shared__ int s_first;
     const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, base = blockIdx.x * kSlice;
     const int64_t row = (int64_t)r * A.row_stride;
@@ -244,17 +254,26 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
         const Weigh W(powers, mx, S.inv_t, A.shift);
         const Grid g(mx, S.inv_t);
         uint64_t sum = 0;
+        uint32_t rank[N][G];  // of a token within its bin, in no order, beside the bin; none: no bin
+        if (S.filters) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+#pragma unroll
+                for (int e = 0; e < G; ++e) {
+                    rank[j][e] = ~0u;
+                    if (x[j][e] > -INFINITY) {
+                        const uint32_t b = g.bin(x[j][e]);
+                        rank[j][e] = atomicAdd(&cnt[b], 1u) | b << 16;
+                    }
+                }
+        }
 #pragma unroll
         for (int j = 0; j < N; ++j)
 #pragma unroll
             for (int e = 0; e < G; ++e) {
                 const uint64_t f = W.fix(x[j][e]);
                 sum += f;
-                if (S.filters && x[j][e] > -INFINITY) {
-                    const int b = g.bin(x[j][e]);
-                    atomicAdd(&cnt[b], 1u);
-                    if (f) atomicAdd(&wgt[b], (unsigned long long)f);
-                }
+                if (S.filters && f) atomicAdd(&wgt[rank[j][e] >> 16], (unsigned long long)f);
             }
         sum = wave_sum(sum);
         if (lane == 0) s_sum[tid >> 6] = sum;
@@ -264,12 +283,42 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
             for (int i = 0; i < kWaves; ++i) sum += s_sum[i];
             *out = Slice{sum, mx, 0};
         }
+        if (S.filters) {
+            if (tid < 64) {
+                constexpr int B = kBins / 64;
+                uint32_t n[B], own = 0;
+#pragma unroll
+                for (int i = 0; i < B; ++i) n[i] = cnt[lane * B + i], own += n[i];
+                uint32_t at = own;
+                for (int d = 1; d < 64; d <<= 1) {
+                    const uint32_t p = __shfl_up(at, d);
+                    if (lane >= d) at += p;
+                }
+                at -= own;
+#pragma unroll
+                for (int i = 0; i < B; ++i) off[lane * B + i] = (uint16_t)at, at += n[i];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+#pragma unroll
+                for (int e = 0; e < G; ++e)
+                    if (rank[j][e] != ~0u)
+                        idx[off[rank[j][e] >> 16] + (rank[j][e] & 0xffff)] = (uint16_t)((j * kThreads + tid) * G + e);
+            __syncthreads();
+            uint4* to = (uint4*)((uint16_t*)((uint8_t*)A.ws + o.idx) + at * kSlice);
+            for (int i = tid; i * 8 < off[kBins - 1] + (int)cnt[kBins - 1]; i += kThreads) to[i] = ((const uint4*)idx)[i];
+        }
     }
     if (S.filters) {
-        __syncthreads();
+        if (mx == -INFINITY) {
+            if (tid < kBins) off[tid] = 0;
+            __syncthreads();
+        }
         if (tid < kBins) {
             ((uint32_t*)((uint8_t*)A.ws + o.cnt))[at * kBins + tid] = cnt[tid];
             ((uint64_t*)((uint8_t*)A.ws + o.wgt))[at * kBins + tid] = wgt[tid];
+            ((uint16_t*)((uint8_t*)A.ws + o.off))[at * kBins + tid] = off[tid];
         }
     }
 }
@@ -329,7 +378,6 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
     __shared__ uint32_t slice_n[kMaxSlices];            // its tokens of key `edge`
     __shared__ double slice_s[kMaxSlices];  // the slice's weights to the row's: exp((its max - max) / T)
     __shared__ float slice_d[kMaxSlices];   // the slice's bins to the row's
-    __shared__ uint8_t slice_in[kMaxSlices];
     __shared__ double powers[kPowers];
     __shared__ uint64_t red[kWaves][2];
     __shared__ int s_n;
@@ -396,7 +444,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
         slice_s[tid] = f;
         slice_d[tid] = top ? 0.0f : g.at - floorf(m.max * g.g);
         slice_w[tid] = S.filters ? 0 : f == 1.0 ? m.sum : (uint64_t)llrint((double)m.sum * f);
-        slice_n[tid] = 0, slice_in[tid] = 0;
+        slice_n[tid] = 0;
     }
     for (int i = tid; i < kDigits; i += kThreads) cnt[0][i] = cnt[1][i] = 0, wsum[0][i] = wsum[1][i] = 0;
     if (tid == 0) s_n = 0, s_lo = 0xffffffffu, s_hi = 0;
@@ -452,73 +500,66 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
         }
         const bool some = bin >= 0;
         const int cnt_bin = some ? (int)cnt[0][bin] : 0;
+        const bool light = some && cb && !wsum[0][bin];  // which of its tokens are kept changes nothing: none is
         const bool listed = cnt_bin <= kList;
         __syncthreads();
         for (int i = tid; i < kBins; i += kThreads) cnt[0][i] = 0, wsum[0][i] = 0;
-        // what each slice keeps above the bin, and which have tokens in it
+        // what each slice keeps above the bin
         entries([&](int e, uint32_t c, uint64_t w) {
             const int s = e / kBins, b = row_bin(s, e % kBins);
-            if (!some || b < bin)
-                atomicAdd(&slice_w[s], (unsigned long long)to_row(w, s));
-            else if (b == bin)
-                slice_in[s] = 1;
+            if (!some || b < bin) atomicAdd(&slice_w[s], (unsigned long long)to_row(w, s));
         });
         __syncthreads();
         if (some) {
-            // The slices that have tokens in the bin, kBatch of them on their way at a time: a thread's tokens
-            // of one slice, and the index of the first of each eight
-            auto read_slices = [&](auto&& look) {
-                int s = -1;
-                while (s < slices) {
-                    Eight<DT> x[kBatch][kPer / 8];
-                    int at[kBatch];
+            // A slice's list has the bin's tokens in a row, from `first`, n of them: a lane knows kLaneSlices slices,
+            // a wave reads every kWaves-th, with the `before` earlier slices' ones numbered first
+            int n[kLaneSlices], first[kLaneSlices], before;
+            {
+                uint64_t own = 0, unused;
 #pragma unroll
-                    for (int b = 0; b < kBatch; ++b) {
-                        do ++s;
-                        while (s < slices && !slice_in[s]);
-                        s = s < slices ? s : slices;
-                        at[b] = s;
-                    }
-                    // a short batch reads its first slice again
-                    bool whole = aligned && at[0] < slices;
-#pragma unroll
-                    for (int b = 0; b < kBatch; ++b) whole = whole && (at[b] >= slices || (at[b] + 1) * kSlice <= V);
-                    if (whole) {
-#pragma unroll
-                        for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-                            for (int j = 0; j < kPer / 8; ++j)
-                                x[b][j].load(A.logits,
-                                             row + (at[b] < slices ? at[b] : at[0]) * kSlice + (j * kThreads + tid) * 8);
-#pragma unroll
-                        for (int b = 0; b < kBatch; ++b)
-                            if (at[b] < slices) look(x[b], at[b] * kSlice + tid * 8);
-                    } else {
-#pragma unroll 1
-                        for (int b = 0; b < kBatch; ++b) {
-                            if (at[b] >= slices) break;
-                            load_slice<DT>(A, row, at[b], aligned, x[0]);
-                            look(x[0], at[b] * kSlice + tid * 8);
+                for (int i = 0; i < kLaneSlices; ++i) {
+                    const int s = lane * kLaneSlices + i;
+                    n[i] = first[i] = 0;
+                    if (s < slices) {
+                        const uint32_t* sc = hc + s * kBins;
+                        const uint16_t* so = (const uint16_t*)((uint8_t*)A.ws + o.off) + ((int64_t)r * slices + s) * kBins;
+                        const float b = (float)bin - slice_d[s];
+                        if (bin == kBins - 1) {  // all that lies that far
+                            first[i] = so[b > 0.0f ? (int)b : 0];
+                            n[i] = so[kBins - 1] + (int)sc[kBins - 1] - first[i];
+                        } else if (b >= 0.0f) {
+                            first[i] = so[(int)b];
+                            n[i] = (int)sc[(int)b];
                         }
                     }
+                    own += n[i];
                 }
-            };
-            auto place = [&](int i0, int j, int q) { return i0 + j * kThreads * 8 + q; };
-            // the bin's logits are those from xl to xh: the borders of its keys, by bisection near its place
-            auto first_key = [&](int b) {  // the least key of bin b or a nearer one
-                if (b >= kBins - 1) return key_of(-INFINITY) + 1;
-                if (b < 0) return key_of(mx) + 1;
-                return first_that(key_of((g.at - (float)b) / g.g), key_of(-INFINITY), key_of(mx),
-                                  [&](uint32_t k) { return g.bin(of_key(k)) <= b; });
-            };
-            const float xl = of_key(first_key(bin)), xh = of_key(first_key(bin - 1) - 1);
-            auto read_bin = [&](auto&& take) {  // the bin's tokens from memory
-                read_slices([&](const Eight<DT> (&x)[kPer / 8], int i0) {
-                    for (int j = 0; j < kPer / 8; ++j)
+                before = (int)wave_before(own, &unused);
+            }
+            auto read_bin = [&](auto&& take) {  // the bin's tokens from memory: number, key, index
+                for (int s = tid >> 6; s < slices; s += kWaves) {
+                    const int l = s / kLaneSlices;
+                    int at = __shfl(before, l), ns = 0, fs = 0;
 #pragma unroll
-                        for (int q = 0; q < 8; ++q)
-                            if (x[j][q] >= xl && x[j][q] <= xh) take(key_of(x[j][q]), place(i0, j, q));
-                });
+                    for (int i = 0; i < kLaneSlices; ++i) {
+                        const int ni = __shfl(n[i], l), fi = __shfl(first[i], l);
+                        at += i < s % kLaneSlices ? ni : 0;
+                        if (i == s % kLaneSlices) ns = ni, fs = fi;
+                    }
+                    const uint16_t* from = (const uint16_t*)((uint8_t*)A.ws + o.idx) + ((int64_t)r * slices + s) * kSlice + fs;
+                    constexpr int U = 8;  // of them on their way at a time
+                    for (int k = lane; k < ns; k += 64 * U) {
+                        int t[U];
+                        float y[U];
+#pragma unroll
+                        for (int q = 0; q < U; ++q) t[q] = s * kSlice + from[k + 64 * q < ns ? k + 64 * q : k];
+#pragma unroll
+                        for (int q = 0; q < U; ++q) y[q] = one_logit<DT>(A, row + t[q]);
+#pragma unroll
+                        for (int q = 0; q < U; ++q)
+                            if (k + 64 * q < ns) take(at + k + 64 * q, key_of(y[q]), t[q]);
+                    }
+                }
             };
             auto meet = [&](uint32_t l, uint32_t h) {  // the least and greatest key of the workgroup
                 for (int d = 32; d; d >>= 1) {
@@ -529,53 +570,11 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                 if (lane == 0 && l <= h) atomicMin(&s_lo, l), atomicMax(&s_hi, h);
             };
             uint32_t lo = 0xffffffffu, hi = 0;
-            if (listed) {  // their indexes, then their keys
-                read_slices([&](const Eight<DT> (&x)[kPer / 8], int i0) {
-                    uint32_t m = 0;
-#pragma unroll
-                    for (int j = 0; j < kPer / 8; ++j)
-#pragma unroll
-                        for (int q = 0; q < 8; ++q)
-                            m |= (uint32_t)(__builtin_amdgcn_fmed3f(x[j][q], xl, xh) == x[j][q]) << (8 * j + q);
-                    if (!__any(m != 0)) return;
-                    int n = __popc(m);  // room in the list: one request a wave and slice
-                    const int own = n;
-                    for (int d = 1; d < 64; d <<= 1) {
-                        const int p = __shfl_up(n, d);
-                        if (lane >= d) n += p;
-                    }
-                    int at = 0;
-                    if (lane == 63) at = atomicAdd(&s_n, n);
-                    at = __builtin_amdgcn_readlane(at, 63) + n - own;
-                    for (; m; m &= m - 1, ++at) {
-                        const int q = __builtin_ctz(m);
-                        if (at < kList) list[at].y = (uint32_t)place(i0, q >> 3, q & 7);
-                    }
-                });
-                __syncthreads();
-                constexpr int U = 8;  // keys on their way at a time
-                for (int i = tid; i < cnt_bin; i += U * kThreads) {
-                    float y[U];
-#pragma unroll
-                    for (int q = 0; q < U; ++q) {
-                        const int e = i + q * kThreads < cnt_bin ? i + q * kThreads : i;
-                        y[q] = one_logit<DT>(A, row + list[e].y);
-                    }
-#pragma unroll
-                    for (int q = 0; q < U; ++q)
-                        if (i + q * kThreads < cnt_bin) {
-                            const uint32_t k = key_of(y[q]);
-                            list[i + q * kThreads].x = k;
-                            lo = k < lo ? k : lo;
-                            hi = k > hi ? k : hi;
-                        }
-                }
-            } else {
-                read_bin([&](uint32_t k, int) {
-                    lo = k < lo ? k : lo;
-                    hi = k > hi ? k : hi;
-                });
-            }
+            read_bin([&](int i, uint32_t k, int t) {
+                if (listed) list[i] = make_uint2(k, (uint32_t)t);
+                lo = k < lo ? k : lo;
+                hi = k > hi ? k : hi;
+            });
             meet(lo, hi);
             __syncthreads();
             lo = s_lo, hi = s_hi;
@@ -583,7 +582,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
                 if (listed)
                     for (int i = tid; i < cnt_bin; i += kThreads) take(list[i].x, (int)list[i].y);
                 else
-                    read_bin(take);
+                    read_bin([&](int, uint32_t k, int t) { take(k, t); });
             };
             constexpr int N = kDigits / 64;
             int buf = 0;
@@ -644,7 +643,11 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs A
             };
             ties = cnt_bin;
             edge = lo - 1;
-            if (cnt_bin <= 64) {
+            if (light) {
+                edge = hi;
+                ties = 0;
+                settled = true;
+            } else if (cnt_bin <= 64) {
                 rank(lane < cnt_bin ? list[lane] : make_uint2(0u, 0u), cnt_bin);
             } else if (bin < kBins - 1 && lo < hi) {
                 scan([&](uint32_t u, int) {
