@@ -27,6 +27,7 @@ constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kPer = kSlice / kThreads;        // tokens of a thread
 constexpr int kBins = 256;                     // of the distance; the last holds all that lies further
+constexpr int kCopies = 4;                     // of a slice's histogram, by lane: equal bins of a wave meet less often
 constexpr float kPerNat = 8.0f;                // bins a unit of x / T
 constexpr int kDigitBits = 9;                  // of a level of the descent
 constexpr int kDigits = 1 << kDigitBits;
@@ -207,12 +208,13 @@ __device__ __forceinline__ uint64_t wave_before(uint64_t v, uint64_t* all) {
 template <int DT>
 __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs A) {
     constexpr int G = 8, N = kPer / G;  // groups of 8 tokens a thread
-    __shared__ uint32_t cnt[kBins];
-    __shared__ unsigned long long wgt[kBins];
+    __shared__ __attribute__((aligned(16))) uint32_t cnt[kBins * kCopies];
+    __shared__ unsigned long long wgt[kBins * kCopies];
     __shared__ double powers[kPowers];
     __shared__ float s_max[kWaves];
     __shared__ uint64_t s_sum[kWaves];
-    __shared__ uint16_t off[kBins];                              // where a bin's tokens begin in idx
+    __shared__ __attribute__((aligned(16))) uint16_t off[kBins * kCopies];  // where a bin's tokens begin in idx
+    __shared__ int s_all;
     __shared__ __attribute__((aligned(16))) uint16_t idx[kSlice];  // the tokens by bin
     __shared__ int s_first;
     const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, base = blockIdx.x * kSlice;
@@ -222,7 +224,7 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
     const Settings S(A, r);
     fill_powers(powers, tid);
     if (tid == 0) s_first = 0x7fffffff;
-    if (tid < kBins) cnt[tid] = 0, wgt[tid] = 0;
+    for (int i = tid; i < kBins * kCopies; i += kThreads) cnt[i] = 0, wgt[i] = 0;
     float mx = -INFINITY;
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
                 for (int e = 0; e < G; ++e) {
                     rank[j][e] = ~0u;
                     if (x[j][e] > -INFINITY) {
-                        const uint32_t b = g.bin(x[j][e]);
+                        const uint32_t b = g.bin(x[j][e]) * kCopies + lane % kCopies;
                         rank[j][e] = atomicAdd(&cnt[b], 1u) | b << 16;
                     }
                 }
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
         }
         if (S.filters) {
             if (tid < 64) {
-                constexpr int B = kBins / 64;
+                constexpr int B = kBins * kCopies / 64;
                 uint32_t n[B], own = 0;
 #pragma unroll
                 for (int i = 0; i < B; ++i) n[i] = cnt[lane * B + i], own += n[i];
@@ -294,6 +296,7 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
                     const uint32_t p = __shfl_up(at, d);
                     if (lane >= d) at += p;
                 }
+                if (lane == 63) s_all = (int)at;
                 at -= own;
 #pragma unroll
                 for (int i = 0; i < B; ++i) off[lane * B + i] = (uint16_t)at, at += n[i];
@@ -307,18 +310,22 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
                         idx[off[rank[j][e] >> 16] + (rank[j][e] & 0xffff)] = (uint16_t)((j * kThreads + tid) * G + e);
             __syncthreads();
             uint4* to = (uint4*)((uint16_t*)((uint8_t*)A.ws + o.idx) + at * kSlice);
-            for (int i = tid; i * 8 < off[kBins - 1] + (int)cnt[kBins - 1]; i += kThreads) to[i] = ((const uint4*)idx)[i];
+            for (int i = tid; i * 8 < s_all; i += kThreads) to[i] = ((const uint4*)idx)[i];
         }
     }
     if (S.filters) {
         if (mx == -INFINITY) {
-            if (tid < kBins) off[tid] = 0;
+            for (int i = tid; i < kBins * kCopies; i += kThreads) off[i] = 0;
             __syncthreads();
         }
         if (tid < kBins) {
-            ((uint32_t*)((uint8_t*)A.ws + o.cnt))[at * kBins + tid] = cnt[tid];
-            ((uint64_t*)((uint8_t*)A.ws + o.wgt))[at * kBins + tid] = wgt[tid];
-            ((uint16_t*)((uint8_t*)A.ws + o.off))[at * kBins + tid] = off[tid];
+            uint32_t c = 0;
+            uint64_t w = 0;
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) c += cnt[tid * kCopies + i], w += wgt[tid * kCopies + i];
+            ((uint32_t*)((uint8_t*)A.ws + o.cnt))[at * kBins + tid] = c;
+            ((uint64_t*)((uint8_t*)A.ws + o.wgt))[at * kBins + tid] = w;
+            ((uint16_t*)((uint8_t*)A.ws + o.off))[at * kBins + tid] = off[tid * kCopies];
         }
     }
 }
