@@ -145,7 +145,7 @@ struct Settings {
 };
 
 // w = exp((x - top) / T) = 2^(q / 256) e^g with |g| <= ln 2 / 512: a table of 256 powers and four terms of the
-// series, relative error 2^-50; fixed point by adding 2^52.
+// series, relative error 2^-50; fixed point by adding 2^52.  No branch: several tokens are under way at a time.
 constexpr int kPowers = 256;
 struct Weigh {
     const double* powers;  // 2^(i / 256), LDS
@@ -154,10 +154,9 @@ struct Weigh {
     int shift;
     __device__ __forceinline__ Weigh(const double* powers_, float top_, double inv_t, int shift_)
         : powers(powers_), top(top_), k(inv_t * 369.32993046757464), shift(shift_) {}
+    // 2^shift w; 2^(shift - 64) for less than that, -inf, NaN, and everything beside +inf
     __device__ __forceinline__ double scaled(float x, int shift_) const {
-        if (x == top) return __builtin_ldexp(1.0, shift_);
-        const double t = ((double)x - (double)top) * k;
-        if (!(t > -16384.0)) return 0.0;  // also -inf, NaN, and everything beside +inf; 2^-64
+        const double t = x == top ? 0.0 : __builtin_fmax(((double)x - (double)top) * k, -16384.0);
         const double q = __builtin_rint(t);
         const double g = (t - q) * 0.0027076061740622863;
         double p = __builtin_fma(g, 1.0 / 24.0, 1.0 / 6.0);
@@ -206,7 +205,7 @@ __device__ __forceinline__ uint64_t wave_before(uint64_t v, uint64_t* all) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs A) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8))) void sample_slice_kernel(const SampleArgs A) {
     constexpr int G = 8, N = kPer / G;  // groups of 8 tokens a thread
     __shared__ __attribute__((aligned(16))) uint32_t cnt[kBins * kCopies];
     __shared__ unsigned long long wgt[kBins * kCopies];
@@ -256,27 +255,33 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
         const Weigh W(powers, mx, S.inv_t, A.shift);
         const Grid g(mx, S.inv_t);
         uint64_t sum = 0;
-        uint32_t rank[N][G];  // of a token within its bin, in no order, beside the bin; none: no bin
+        uint32_t rank[N][G];  // of a token within its bin, in no order, beside the bin; 0xffff: no token
         if (S.filters) {
 #pragma unroll
-            for (int j = 0; j < N; ++j)
+            for (int j = 0; j < N; ++j) {
+                uint32_t b[G];
+#pragma unroll
+                for (int e = 0; e < G; ++e) b[e] = g.bin(x[j][e]) * kCopies + lane % kCopies;
 #pragma unroll
                 for (int e = 0; e < G; ++e) {
-                    rank[j][e] = ~0u;
-                    if (x[j][e] > -INFINITY) {
-                        const uint32_t b = g.bin(x[j][e]) * kCopies + lane % kCopies;
-                        rank[j][e] = atomicAdd(&cnt[b], 1u) | b << 16;
-                    }
+                    rank[j][e] = 0xffff;
+                    if (x[j][e] > -INFINITY) rank[j][e] = atomicAdd(&cnt[b[e]], 1u);
                 }
+#pragma unroll
+                for (int e = 0; e < G; ++e) rank[j][e] |= b[e] << 16;
+            }
         }
 #pragma unroll
-        for (int j = 0; j < N; ++j)
+        for (int j = 0; j < N; ++j) {
+            uint64_t f[G];
 #pragma unroll
-            for (int e = 0; e < G; ++e) {
-                const uint64_t f = W.fix(x[j][e]);
-                sum += f;
-                if (S.filters && f) atomicAdd(&wgt[rank[j][e] >> 16], (unsigned long long)f);
+            for (int e = 0; e < G; ++e) f[e] = W.fix(x[j][e]), sum += f[e];
+            if (S.filters) {
+#pragma unroll
+                for (int e = 0; e < G; ++e)
+                    if (f[e]) atomicAdd(&wgt[rank[j][e] >> 16], (unsigned long long)f[e]);
             }
+        }
         sum = wave_sum(sum);
         if (lane == 0) s_sum[tid >> 6] = sum;
         __syncthreads();
@@ -306,7 +311,7 @@ __global__ __launch_bounds__(kThreads) void sample_slice_kernel(const SampleArgs
             for (int j = 0; j < N; ++j)
 #pragma unroll
                 for (int e = 0; e < G; ++e)
-                    if (rank[j][e] != ~0u)
+                    if ((rank[j][e] & 0xffff) != 0xffff)
                         idx[off[rank[j][e] >> 16] + (rank[j][e] & 0xffff)] = (uint16_t)((j * kThreads + tid) * G + e);
             __syncthreads();
             uint4* to = (uint4*)((uint16_t*)((uint8_t*)A.ws + o.idx) + at * kSlice);
