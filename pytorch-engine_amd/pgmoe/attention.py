@@ -88,12 +88,12 @@ class HipRotary:
         self.attn_factor = float(attn_factor)
         if inv_freq is None:
             inv_freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
-        f = inv_freq.to(self.device, torch.float64)
+        f = inv_freq.to("cpu", torch.float64)
         if freq_factors is not None:
             if freq_factors.numel() != rotary_dim // 2:
                 raise ValueError("freq_factors holds one factor a pair (rotary_dim / 2)")
-            f = f / freq_factors.to(self.device, torch.float64).reshape(-1)
-        self.turns = f * (position_scale / (2.0 * math.pi))
+            f = f / freq_factors.to("cpu", torch.float64).reshape(-1)
+        self.turns = (f * (position_scale / (2.0 * math.pi))).to(self.device)
 
 
 class KVBatch:
@@ -171,6 +171,7 @@ class HipPagedKVCache:
         self._check(n_pages, page_size, n_kv_heads, head_dim, dtype)
         shape = (n_pages, n_kv_heads, page_size, head_dim)
         self._bind(torch.zeros(shape, dtype=dtype, device=dev), torch.zeros(shape, dtype=dtype, device=dev))
+        torch.cuda.current_stream(dev).synchronize()  # cleared before any other stream writes to them
 
     @classmethod
     def from_tensors(cls, k: torch.Tensor, v: torch.Tensor) -> "HipPagedKVCache":
