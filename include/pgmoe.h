@@ -351,7 +351,7 @@ typedef struct pgmoe_kv_batch {
  * multiple of 16 up to head_dim.  q_norm / k_norm: fp32 [head_dim] or NULL; x * (1 / sqrt(mean(x^2) + eps)) * w
  * in fp32.  Every value is rounded once, to the cache's type.  A token with a negative own index, or whose
  * page does not exist, gets its query and no cache row; rows of q_out behind the last sequence are left
- * alone.  Two tokens must not fall on one cache row. */
+ * alone.  Two tokens must not fall on one cache row.  n_tokens: below 2^24. */
 int pgmoe_rope_append(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, const void* q, int64_t q_token_stride,
                       int64_t q_head_stride, const void* k, int64_t k_token_stride, int64_t k_head_stride,
                       const void* v, int64_t v_token_stride, int64_t v_head_stride, int32_t src_dtype,
@@ -367,7 +367,10 @@ int pgmoe_rope_append(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, const vo
  * [n_tokens, n_q_heads, head_dim] in the cache's type (q with strides as above; out contiguous, not
  * overlapping q); lse fp32 [n_tokens, n_q_heads] or NULL.  A query that sees no key gets zeros and an lse
  * of -inf; one that sees a key on a page that does not exist gets NaN; what masked keys and unused rows of
- * pages hold is never seen, not even a NaN.  Rows behind the last sequence are left alone. */
+ * pages hold is never seen, not even a NaN.  Rows behind the last sequence are left alone.
+ * The workspace holds partial rows of this call and needs no clearing.  Limits (PGMOE_E_UNSUPPORTED beyond):
+ * with g query heads a KV head, n_tokens * g * g < 2^31, and (n_tokens * g / 128 + 1 + n_seqs) * n_kv_heads
+ * row tiles of (max_pages * page_size + prefix_len) / 32 + 16 key tiles number 2^30 at most. */
 size_t pgmoe_attend_workspace_bytes(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, int32_t n_tokens,
                                     int32_t n_q_heads);
 int pgmoe_attend(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, const void* q, int64_t q_token_stride,
@@ -393,9 +396,10 @@ typedef struct pgmoe_sampling {
  *   which the sum of w is below top_p times the sum of all; those with w >= min_p;
  *   token (int64 [rows]): the first in index order at which the sum of the kept w exceeds u times their
  *   total; logprob (fp32 [rows] or NULL): log(w_token / total).
- * Weights are summed in 64-bit fixed point, so no order of sums shows in the result.  NaN and -inf logits
+ * Weights are summed as multiples of 2^-s of the largest, s = min(51, 62 - ceil(log2 vocab)), so no order of sums
+ * shows in the result; a token of less than half of that has none and is not drawn.  NaN and -inf logits
  * have no weight; with +inf ones only those have.  A row without any logit above -inf gives token -1 and
- * logprob -inf.  vocab: 1 .. 2^20. */
+ * logprob -inf.  vocab: 1 .. 2^20; rows: up to 2^22.  The workspace is this call's and needs no clearing. */
 size_t pgmoe_sample_workspace_bytes(int32_t rows, int32_t vocab);
 int pgmoe_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab, const float* u,
                  const pgmoe_sampling* S, int64_t* token, float* logprob, void* ws, size_t ws_bytes, void* stream);

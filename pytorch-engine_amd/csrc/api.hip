@@ -778,6 +778,7 @@ int pgmoe_rope_append(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, const vo
     if (rot_dim < 0 || rot_dim > kc.dim || rot_dim % 16)
         return fail(PGMOE_E_INVALID, "rope_append: rot_dim %d (0 or a multiple of 16 up to head_dim %d)", rot_dim, kc.dim);
     if (!(eps >= 0.0f)) return fail(PGMOE_E_INVALID, "rope_append: negative eps");
+    if (n_tokens >= 1 << 24) return fail(PGMOE_E_UNSUPPORTED, "rope_append: %d tokens in one call", n_tokens);
     if (n_tokens == 0) return PGMOE_OK;
     if (!q || !k || !v || !q_out || (rot_dim && !turns)) return fail(PGMOE_E_INVALID, "rope_append: NULL pointer");
     const int64_t unit = src_dtype == PGMOE_DT_F32 ? 4 : 8;  // elements of 16 bytes
@@ -832,6 +833,7 @@ size_t pgmoe_sample_workspace_bytes(int32_t rows, int32_t vocab) {
 int pgmoe_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab, const float* u,
                  const pgmoe_sampling* S, int64_t* token, float* logprob, void* ws, size_t ws_bytes, void* stream) {
     if (rows < 0) return fail(PGMOE_E_INVALID, "sample: negative row count");
+    if (rows > (1 << 22)) return fail(PGMOE_E_UNSUPPORTED, "sample: %d rows in one call", rows);
     if (vocab < 1 || vocab > kMaxVocab) return fail(PGMOE_E_UNSUPPORTED, "sample: vocab %d (1 .. %d)", vocab, kMaxVocab);
     if (dtype != PGMOE_DT_F32 && dtype != PGMOE_DT_F16 && dtype != PGMOE_DT_BF16)
         return fail(PGMOE_E_UNSUPPORTED, "sample: logits dtype %d", dtype);

@@ -51,11 +51,12 @@ struct AttendArgs {
     float c;            // scale * log2(e)
     uint16_t* out;
     float* lse;
-    // partial rows [prefix, own][slot][T * hq][dim], their (max in log2 units, sum), and the slots a row has
+    // partial rows [prefix, if there is one, then own][slot][T * hq][dim], their (max in log2 units, sum), and
+    // the slots a row has
     float* part;
     float2* ml;
     int* slots;
-    int nslot;
+    int nslot, own;  // slots of a region; where the own keys' begin
 };
 
 template <int D>
@@ -561,7 +562,7 @@ __device__ __forceinline__ void put4(const AttendArgs& A, const Work& W, bool di
         *(uint2*)(A.out + row * D + d) = make_uint2(a, b);
     } else {
         const int64_t R = (int64_t)A.T * A.hq;
-        *(float4*)(A.part + (((W.prefix ? 0 : A.nslot) + W.slot) * R + row) * D + d) = v;
+        *(float4*)(A.part + (((W.prefix ? 0 : A.own) + W.slot) * R + row) * D + d) = v;
     }
 }
 // The row's statistics: lse of a finished row, (max, sum) of a partial one; slot 0 says how many there are.
@@ -571,7 +572,7 @@ __device__ __forceinline__ void put_row(const AttendArgs& A, const Work& W, bool
         if (A.lse) A.lse[row] = empty ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
     } else {
         const int64_t R = (int64_t)A.T * A.hq;
-        A.ml[((W.prefix ? 0 : A.nslot) + W.slot) * R + row] = make_float2(m, l);
+        A.ml[((W.prefix ? 0 : A.own) + W.slot) * R + row] = make_float2(m, l);
     }
     if (W.slot == 0) {
         A.slots[(W.prefix ? 0 : (int64_t)A.T * A.hq) + row] = empty ? 0 : W.nslots;
@@ -922,7 +923,7 @@ __global__ __launch_bounds__(kThreads) void combine_rows_kernel(const AttendArgs
     }
     const bool empty = !A.B.prefix && ns == 0;
     const int all = live ? np + ns : 0;
-    auto place = [&](int s) { return (s < np ? s : A.nslot + s - np) * R + row; };
+    auto place = [&](int s) { return (s < np ? s : A.own + s - np) * R + row; };
     float mx = -INFINITY;
     for (int s = c; s < all; s += LPR) mx = fmaxf(mx, A.ml[place(s)].x);
     for (int d = LPR < 64 ? LPR / 2 : 32; d; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
@@ -972,7 +973,7 @@ static AttendWs attend_ws(const KvCache& C, const KvBatch& B, int T, int hq) {
     const int64_t R = (int64_t)T * hq;
     AttendWs w;
     w.nslot = attend_slots(R, C.dim);
-    const int regions = 2;
+    const int regions = B.prefix ? 2 : 1;
     w.ml = R * w.nslot * regions * C.dim * 4;
     w.slots = w.ml + R * w.nslot * regions * 8;
     w.total = (w.slots + R * 2 * 4 + 255) / 256 * 256;
@@ -999,7 +1000,7 @@ int launch_attend(const KvCache& C, const KvBatch& B, const uint16_t* q, int64_t
     uint8_t* b = (uint8_t*)ws;
     const int group = hq / C.heads;
     const AttendArgs A{C,   B,         q,   q_tok, q_head, T, hq, group, (uint32_t)(0x100000000ull / group + (group > 1)),
-                       scale * 1.4426950408889634f, out, lse, (float*)b, (float2*)(b + w.ml), (int*)(b + w.slots), w.nslot};
+                       scale * 1.4426950408889634f, out, lse, (float*)b, (float2*)(b + w.ml), (int*)(b + w.slots), w.nslot, B.prefix ? w.nslot : 0};
     const int64_t R = (int64_t)T * hq;
     const dim3 block(kThreads);
     // few rows have many slots each: 1024 / D groups a row, one row a workgroup; many have few

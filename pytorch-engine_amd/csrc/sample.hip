@@ -216,10 +216,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8))) v
     __shared__ int s_all;
     __shared__ __attribute__((aligned(16))) uint16_t idx[kSlice];  // the tokens by bin
     __shared__ int s_first;
-    const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, base = blockIdx.x * kSlice;
+    const int r = blockIdx.x, slice = blockIdx.y, tid = threadIdx.x, lane = tid & 63, base = slice * kSlice;
     const int64_t row = (int64_t)r * A.row_stride;
     Eight<DT> x[N];
-    load_slice<DT>(A, row, blockIdx.x, row_aligned<DT>(A, row), x);
+    load_slice<DT>(A, row, slice, row_aligned<DT>(A, row), x);
     const Settings S(A, r);
     fill_powers(powers, tid);
     if (tid == 0) s_first = 0x7fffffff;
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8))) v
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) mx = fmaxf(mx, s_max[i]);
 
-    const int64_t at = (int64_t)r * gridDim.x + blockIdx.x;
+    const int64_t at = (int64_t)r * gridDim.y + slice;
     const Layout o = layout(A.rows, A.vocab);
     Slice* out = (Slice*)((uint8_t*)A.ws + o.slices) + at;
     if (S.greedy || mx == -INFINITY) {
@@ -836,7 +836,7 @@ size_t sample_ws_bytes(int rows, int vocab) { return (size_t)layout(rows, vocab)
 
 int launch_sample(const SampleArgs& A, hipStream_t st) {
     if (A.rows == 0) return PGMOE_OK;
-    const dim3 slices((A.vocab + kSlice - 1) / kSlice, A.rows), rows(A.rows), block(kThreads);
+    const dim3 slices(A.rows, (A.vocab + kSlice - 1) / kSlice), rows(A.rows), block(kThreads);
 #define SAMPLE(DT)                                                              \
     do {                                                                        \
         PG_LAUNCH((sample_slice_kernel<DT>), slices, block, 0, st, A);          \

@@ -43,7 +43,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Union[floa
     below top_p times the whole (1: off); those with w >= min_p (0: off); one at least.  The token is the
     first in index order at which the sum of the kept w exceeds u times their total, u in [0, 1).
     temperature 0: the largest logit.  Parameters: numbers, or a tensor of one value a row (float32;
-    top_k int32).  NaN and -inf logits are never drawn; a row that holds nothing else gives -1 and -inf."""
+    top_k int32).  w is held in multiples of 2^-s, s = min(51, 62 - ceil(log2(vocab))): a token with less than
+    half of that is not drawn, not even at u = 0.  NaN and -inf logits are never drawn; a row that holds nothing else gives -1 and -inf."""
     if logits.device.type != "cuda" or logits.dim() != 2:
         raise ValueError("logits: [rows, vocab] on a HIP device")
     if logits.dtype not in _DT:

@@ -126,3 +126,22 @@ def test_struct_sizes_follow_the_header():
     assert ctypes.sizeof(_lib.KVCache) == 2 * 8 + 3 * 8 + 5 * 4 + 4
     assert ctypes.sizeof(_lib.KVBatch) == 4 * 8 + 8 + 3 * 4 + 4
     assert ctypes.sizeof(_lib.Sampling) == 4 * 8 + 3 * 8 + 4 + 4
+
+
+def test_sizes_that_no_launch_holds():
+    L = _lib.lib()
+    C, B = _cache(), _batch(q_start=0x50000)
+    assert _append(L, C, B, T=1 << 24) == -2 and "tokens" in L.pgmoe_last_error().decode()
+    S = _lib.Sampling(None, None, None, None, 1.0, 1.0, 0.0, 0)
+    assert L.pgmoe_sample(0x1000, 0, 2, (1 << 22) + 1, 2, 0x2000, S, 0x3000, None, 0x100, 1 << 60, None) == -2
+    assert "rows" in L.pgmoe_last_error().decode()
+
+
+def test_attend_workspace_without_a_prefix_is_half():
+    L = _lib.lib()
+    C, B = _cache(), _batch(q_start=0x50000)
+    plain = L.pgmoe_attend_workspace_bytes(C, B, 3, 32)
+    B.prefix_pages, B.prefix_len = 0x60000, 100
+    both = L.pgmoe_attend_workspace_bytes(C, B, 3, 32)
+    rows = 3 * 32 * 2 * 4  # both count the slots of both parts
+    assert 2 * (plain - rows - 256) <= both - rows <= 2 * (plain - rows + 256)

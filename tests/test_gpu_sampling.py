@@ -200,3 +200,42 @@ def test_layouts_graphs_and_refusals(dev):
     with pytest.raises(ValueError):
         sample_tokens(x, u.double())
     assert sample_tokens(x[:0], u[:0])[0].shape == (0,)
+
+
+def test_borders_far_from_the_maximum(dev):
+    """The last kept token lies so far below the maximum that its weight is some units of the fixed point, or
+    none: 200 logits 0.4 apart, and one row of a large vocabulary at a low temperature.
+
+    u = 0 draws the first token that has a weight: one of half a unit, 2^-52 for 200 tokens, at least.  (Weights
+    0.4 apart in logarithm: the nearest to 2^-52 = e^-36.04 is e^-36, 4 % above, far from the 2^-50 that the
+    kernel's are off by.  Together the tokens without weight have at most 200 * 2^-52 of the probability, and u
+    in (0, 2^-24) is not drawn by any generator of 24 bits.)"""
+    from pgmoe import sample_tokens
+    log("sample far borders")
+    g = torch.Generator().manual_seed(12)
+    place = torch.randperm(200, generator=g)
+    x = (-0.4 * torch.arange(200.0))[place].expand(6, -1).contiguous()
+    u = torch.tensor([0.0, 0.2, 0.5, 0.9, 0.99, 1 - 2.0 ** -24])
+    for top_k in (77, 79, 80, 81, 90, 150, 199):
+        for min_p, least in ((0.0, 2.0 ** -52), (1e-15, 1e-15)):
+            _check(dev, x[1:], u[1:], 1.0, top_k, 1.0, min_p)
+            tok, _ = sample_tokens(x[:1].to(dev), u[:1].to(dev), 1.0, top_k, 1.0, min_p)
+            drawn = (place < top_k) & (torch.exp(x[0].double()) >= least)
+            assert int(tok) == int(drawn.nonzero()[0])
+    for vocab in (9000, 131072):
+        x, u = _logits(3, vocab, 31)
+        _check(dev, x, u, 0.02, 2000)
+        _check(dev, x, u, 0.05, vocab - 5, 0.999)
+
+
+def test_more_rows_than_a_grid_axis(dev):
+    """70000 rows: the same tokens as in two calls of half as many."""
+    log("sample many rows")
+    from pgmoe import sample_tokens
+    x, u = _logits(70000, 5, 77)
+    x, u = x.to(dev), u.to(dev)
+    tok, lp = sample_tokens(x, u, 0.9, 3, 0.9)
+    for a in (0, 35000):
+        t, p = sample_tokens(x[a:a + 35000], u[a:a + 35000], 0.9, 3, 0.9)
+        assert torch.equal(tok[a:a + 35000], t) and torch.equal(lp[a:a + 35000], p)
+    _check(dev, x[69990:].cpu(), u[69990:].cpu(), 0.9, 3, 0.9)
