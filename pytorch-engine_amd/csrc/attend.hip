@@ -310,6 +310,19 @@ struct Core {
             return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), acc,
                                                           0, 0, 0);
     }
+    // Queries in ordinary registers, arrived before the loops.  256-wide heads take more than 256 registers: the
+    // sums lie in accumulation registers throughout, and are moved only where they are rescaled.
+    __device__ __forceinline__ void hold() {
+#pragma unroll
+        for (int i = 0; i < NK; ++i) asm volatile("" : "+v"(q[i]));
+        hold_sums();
+    }
+    __device__ __forceinline__ void hold_sums() {
+        if constexpr (D == 256) {
+#pragma unroll
+            for (int i = 0; i < ND; ++i) asm volatile("" : "+a"(o[i]));
+        }
+    }
     __device__ __forceinline__ static float swap32(float v) { return xor_lane<32>(v); }
 
     __device__ __forceinline__ void begin(int lane_) {
@@ -783,9 +796,9 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             R.load_q(A, W, core);
             if (key < stop) bring_k(key), bring_v();
             const int jf = plain_tiles(A, pages, W.j0, W.j1, kSplitKeys, W.keys, uni(R.seen), lane);
-#pragma unroll
-            for (int i = 0; i < K::NK; ++i) asm volatile("" : "+v"(core.q[i]));  // arrived before the loops
+            core.hold();  // arrived before the loops
             for (int j = W.j0; j < jf; ++j) {
+                core.hold_sums();
                 const int next = key + kSplitKeys;
                 f32x16 s[1];
                 u16x8 p[2];
@@ -806,6 +819,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             }
             for (; key < stop; key += kSplitKeys) {
                 vm_wait<0>();
+                core.hold_sums();
                 core.checked(kp, vp, R.seen - key, bad_blocks(A, pages, key, W.keys, 2));
                 lds_wait();
                 if (key + kSplitKeys < stop) bring_k(key + kSplitKeys), bring_v();
@@ -858,8 +872,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                     least = s.seen(group_of(A, W.row0));
                 }
                 const int jf = from + plain_tiles(A, where, j - from, to - from, kSharedKeys, keys, least, lane);
-#pragma unroll
-                for (int i = 0; i < K::NK; ++i) asm volatile("" : "+v"(core.q[i]));  // arrived before the loops
+                core.hold();  // arrived before the loops
                 for (; j < jf; ++j) {
                     vm_wait<0>();
                     lds_barrier();
@@ -869,6 +882,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                         constexpr int NG = D == 256 ? 1 : 2;  // groups of 32 keys at a time; at 256 the registers hold one
 #pragma unroll 1
                         for (int half = 0; half < 2; half += NG) {
+                            core.hold_sums();
                             f32x16 s[NG];
                             u16x8 p[2 * NG];
                             core.template scores<NG>(buf + half * 64 * D, s);
@@ -887,6 +901,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                     for (int half = 0; half < 2 && works; ++half) {
                         const int key = (j - from) * kSharedKeys + 32 * half;
                         if (key >= seen1) break;
+                        core.hold_sums();
                         core.checked(buf + half * 64 * D, buf + 128 * D + half * 64 * D, seen - key,
                                      bad_blocks(A, where, key, keys, 2));
                     }
