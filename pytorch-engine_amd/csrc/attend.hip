@@ -34,7 +34,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 256;
-constexpr int kValu = 0x2, kMfma = 0x8, kDs = 0x100;  // instruction classes of sched_group_barrier
+constexpr int kValu = 0x2, kSalu = 0x4, kMfma = 0x8, kDs = 0x100;  // instruction classes of the sched_ barriers
 constexpr int kSplitKeys = 32, kSharedKeys = 64;  // keys of a tile, by kind of segment
 constexpr int kSplitRows = 32, kSharedRows = 128;
 constexpr int kAlone = 16;  // row tiles that a lane sums by itself
@@ -418,20 +418,17 @@ struct Core {
     }
     template <int N2>
     __device__ __forceinline__ void values(const uint8_t* V, const u16x8 (&p)[2 * N2]) {
+        // four reads ahead of the products, in this order; only arithmetic may move between them
+        constexpr int AHEAD = 4, ALL = 2 * N2 * ND;
+        u16x8 f[AHEAD];
 #pragma unroll
-        for (int st = 0; st < 2 * N2; ++st)
+        for (int i = 0; i < AHEAD; ++i) f[i] = vfrag(V, i / ND, i % ND);
 #pragma unroll
-            for (int d = 0; d < ND; ++d) o[d] = mfma(vfrag(V, st, d), p[st], o[d]);
-        // the first 16 keys' V and probabilities, then the products with the next 16 keys' beside them
-        __builtin_amdgcn_sched_group_barrier(kDs, 2 * ND, 0);
-        __builtin_amdgcn_sched_group_barrier(kValu, 28, 0);
-#pragma unroll
-        for (int i = 0; i < (2 * N2 - 1) * ND; ++i) {
-            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(kDs, 2, 0);
-            __builtin_amdgcn_sched_group_barrier(kValu, 28 / ND, 0);
+        for (int i = 0; i < ALL; ++i) {
+            __builtin_amdgcn_sched_barrier(kValu | kSalu);
+            o[i % ND] = mfma(f[i % AHEAD], p[i / ND], o[i % ND]);
+            if (i + AHEAD < ALL) f[i % AHEAD] = vfrag(V, (i + AHEAD) / ND, (i + AHEAD) % ND);
         }
-        __builtin_amdgcn_sched_group_barrier(kMfma, ND, 0);
     }
     __device__ __forceinline__ static bool odd(uint16_t v) {  // infinite or NaN
         constexpr uint16_t e = BF16 ? 0x7f80 : 0x7c00;
