@@ -391,6 +391,7 @@ struct Core {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
             m = mn;
+            hold_sums();
         }
     }
     // p = 2^(c (s - m)) rounded, l += sum p
@@ -497,10 +498,12 @@ struct Core {
         mask(s[0], left, bad);
         grow<1>(s);
         weigh<1>(s, p);
-        if (__builtin_expect(any_odd(V), 0))
+        if (__builtin_expect(any_odd(V), 0)) {
             values_odd(V, p, left);
-        else
+            hold_sums();
+        } else {
             values<1>(V, p);
+        }
     }
 };
 
