@@ -924,11 +924,7 @@ __global__ __launch_bounds__(kThreads) void combine_rows_kernel(const AttendArgs
     const int64_t R = (int64_t)A.T * A.hq;
     const int64_t row = (int64_t)blockIdx.x * RPB + tid / (LPR * GROUPS);
     int ns = 0, np = 0;
-    bool live = row < R;
-    if (live) {
-        const int64_t t = row / A.hq;
-        live = t < (A.B.q_start ? A.B.q_start[A.B.seqs] : A.B.seqs);
-    }
+    bool live = row < R && row < (int64_t)(A.B.q_start ? A.B.q_start[A.B.seqs] : A.B.seqs) * A.hq;
     if (live) {
         ns = A.slots[R + row];
         np = A.B.prefix ? A.slots[row] : 0;
