@@ -9,8 +9,9 @@
 //
 // A workgroup takes one token and up to 4 waves' worth of head rows: a row is D / 8 lanes of 8 values
 // (16-byte loads and stores of 16-bit types), so a wave holds 4 rows of 128.  The cosines of the token are
-// computed once a workgroup into LDS.  HBM-bound from some thousand tokens on, a chain of latencies
-// (sequence, page id, row) below.
+// computed once a workgroup into LDS.  HBM-bound from some thousand tokens on (4300 tokens of 48 rows of 128,
+// fp16: 26 us, 4.0 TB/s), a chain of latencies (sequence, page id, row) below (64 tokens: 3.4 us).  Three rows a
+// thread, all on their way at once, measured the same there and slower for 640 tokens (8.4 us against 6.8).
 #include "kv.h"
 #include "launch.h"
 

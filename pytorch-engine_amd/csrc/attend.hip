@@ -15,8 +15,15 @@
 // The products run on 32x32x16 MFMA, scores transposed: S^T = K Q^T has a query row per lane column, so the
 // maximum and sum of a row are sums over a lane's registers and one swap of wave halves, and the rounded
 // probabilities are already the B operand of O^T = V^T P^T (whose k index may be permuted as long as V's
-// rows are too).  K and V go from memory to LDS without registers, rows swizzled so that the 16-byte reads
-// of K and the transposing 8-byte reads of V meet no bank twice.
+// rows are too).  K and V go from memory to LDS without registers, rows swizzled so that the lanes of a 16-byte
+// read of K and of a transposing 8-byte read of V spread evenly over the banks.
+//
+// What bounds it (whole calls): a few rows a chain of latencies, lens to pages to keys to partial rows, and the
+// second launch (one sequence of 5003 keys: 11 + 5 us); long caches of few rows HBM (32 sequences of up to
+// 16000 keys, 8 KV heads of 128: 212 us, 5.4 TB/s); prompts and long prefixes the power of the matrix units (six
+// prompts behind 4097 keys: 394 us, 790 TFLOP/s, the clock at 1.7 GHz; giving half the waves a higher
+// priority, or the products alone, moves it by 1 to 2 % at most).  Heads of 256: the same 32
+// sequences on 4 KV heads 224 us, a prompt of 1024 behind 4096 keys 138 us, 560 TFLOP/s on one wave a SIMD.
 //
 // Masked keys: a tile with a key that some row does not see takes the checked path: scores of masked keys
 // become -inf, and V values that are not finite reach only the rows that see them.  Rows past the last
@@ -38,8 +45,12 @@ constexpr int kValu = 0x2, kSalu = 0x4, kMfma = 0x8, kDs = 0x100;  // instructio
 constexpr int kSplitKeys = 32, kSharedKeys = 64;  // keys of a tile, by kind of segment
 constexpr int kSplitRows = 32, kSharedRows = 128;
 constexpr int kAlone = 16;  // row tiles that a lane sums by itself
-constexpr int kSplitLeast = 2;  // tiles of a wave's run at least
-constexpr int kSplitHead = 3, kSharedHead = 5;  // what a segment costs beside its tiles, in tiles
+// Tiles of a wave's run at least: one sequence of 5003 keys takes 16.4 us at 1 and 2 (and half the partial
+// rows at 2), 16.7 at 4.
+constexpr int kSplitLeast = 2;
+// What a segment costs beside its tiles, in tiles.  64 rows of one token behind 8192 shared keys: 40.8 us;
+// split heads of 1 and 6 42.4 and 42.2, shared ones of 2 and 10 43.7 and 41.8.
+constexpr int kSplitHead = 3, kSharedHead = 5;
 
 struct AttendArgs {
     KvCache C;
@@ -1014,7 +1025,9 @@ int launch_attend(const KvCache& C, const KvBatch& B, const uint16_t* q, int64_t
                        scale * 1.4426950408889634f, out, lse, (float*)b, (float2*)(b + w.ml), (int*)(b + w.slots), w.nslot, B.prefix ? w.nslot : 0};
     const int64_t R = (int64_t)T * hq;
     const dim3 block(kThreads);
-    // few rows have many slots each: 1024 / D groups a row, one row a workgroup; many have few
+    // Few rows have many slots each: 1024 / D groups a row, one row a workgroup; many have few.  One sequence of
+    // 5003 keys (32 rows) 16.4 us, 25.3 with one group a row; 200 sequences of 1 to 60 keys (6400 rows) 17.1 with
+    // one, 20.6 with eight.
     const bool few = R <= 2048;
 #define COMBINE(D, BF)                                                                                           \
     do {                                                                                                         \

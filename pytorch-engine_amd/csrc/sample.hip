@@ -12,18 +12,18 @@
 // stay equal weights), the bin of the last kept token, its tokens by the slices' lists into LDS, the border among
 // them, and the sums along the index down to the token.
 //
-// Bound: the slices by the bytes of the logits where a row is not filtered (256 rows of 131072 in fp32: 41 us for
-// 134 MB), by the shared-memory atomics of the histogram where it is (64 us); the rows by a chain of some twelve
-// steps that wait for each other (15 to 40 us, whatever the rows).  The lists cost the slices 2 bytes a token and
-// save the rows a second look at their logits: 48 rows with all filters 69 -> 57 us, 64 rows whose bin holds more
-// than LDS does 186 -> 84, 256 rows 107 -> 104.
+// Bound: the slices by the bytes of the logits where a row is not filtered (256 rows of 131072 in fp32: 36 us for
+// 134 MB), by fp64 arithmetic, the histogram's atomics and the lists' stores side by side where it is (65 us); the
+// rows by a chain of some twelve steps that wait for each other (16 to 38 us, whatever the rows).  The lists
+// cost the slices 2 bytes a token and save the rows a second look at their logits: 48 rows with all filters 69
+// -> 57 us, 64 rows whose bin holds more than LDS does 186 -> 84, 256 rows 107 -> 104.
 #include "launch.h"
 #include "sample.h"
 
 namespace pgmoe {
 
-constexpr int kSlice = 8192;                   // tokens of a slice
-constexpr int kThreads = 512;
+constexpr int kSlice = 8192;                   // tokens of a slice: 16 a thread, four workgroups a CU
+constexpr int kThreads = 512;                  // 1024 for a row: 26.0 us for one row (25.1 with 512), 256 rows 106 (104)
 constexpr int kWaves = kThreads / 64;
 constexpr int kPer = kSlice / kThreads;        // tokens of a thread
 constexpr int kBins = 256;                     // of the distance; the last holds all that lies further
@@ -31,8 +31,8 @@ constexpr int kCopies = 4;                     // of a slice's histogram, by lan
 constexpr float kPerNat = 8.0f;                // bins a unit of x / T
 constexpr int kDigitBits = 9;                  // of a level of the descent
 constexpr int kDigits = 1 << kDigitBits;
-constexpr int kList = 7168;                    // tokens of one bin that fit LDS
-constexpr int kHeld = 12;                      // histogram entries that a thread keeps in registers
+constexpr int kList = 7168;                    // tokens of one bin that fit LDS, two workgroups a CU
+constexpr int kHeld = 12;                      // histogram entries that a thread keeps: 24 slices
 constexpr int kMaxSlices = kMaxVocab / kSlice;
 
 struct Slice {
