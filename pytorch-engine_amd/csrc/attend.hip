@@ -23,7 +23,7 @@
 // 16000 keys, 8 KV heads of 128: 212 us, 5.4 TB/s); prompts and long prefixes the power of the matrix units (six
 // prompts behind 4097 keys: 394 us, 790 TFLOP/s, the clock at 1.7 GHz; giving half the waves a higher
 // priority, or the products alone, moves it by 1 to 2 % at most).  Heads of 256: the same 32
-// sequences on 4 KV heads 224 us, a prompt of 1024 behind 4096 keys 138 us, 560 TFLOP/s on one wave a SIMD.
+// sequences on 4 KV heads 224 us, a prompt of 1024 behind 4096 keys 134 us, 580 TFLOP/s on one wave a SIMD.
 //
 // Masked keys: a tile with a key that some row does not see takes the checked path: scores of masked keys
 // become -inf, and V values that are not finite reach only the rows that see them.  Rows past the last
@@ -890,17 +890,13 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                     if (j + 1 < stop) bring(j + 1);
                     const uint8_t* buf = smem + (j & 1) * 256 * D;
                     if (works) {
-                        constexpr int NG = D == 256 ? 1 : 2;  // groups of 32 keys at a time; at 256 the registers hold one
-#pragma unroll 1
-                        for (int half = 0; half < 2; half += NG) {
-                            core.hold_sums();
-                            f32x16 s[NG];
-                            u16x8 p[2 * NG];
-                            core.template scores<NG>(buf + half * 64 * D, s);
-                            core.template grow<NG>(s);
-                            core.template weigh<NG>(s, p);
-                            core.template values<NG>(buf + 128 * D + half * 64 * D, p);
-                        }
+                        core.hold_sums();
+                        f32x16 s[2];
+                        u16x8 p[4];
+                        core.template scores<2>(buf, s);
+                        core.template grow<2>(s);
+                        core.template weigh<2>(s, p);
+                        core.template values<2>(buf + 128 * D, p);
                     }
                 }
                 for (; j < to; ++j) {
