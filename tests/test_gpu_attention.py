@@ -346,6 +346,72 @@ def test_repeats_are_the_same_bits(dev):
         assert torch.equal(a, o) and torch.equal(la, lo)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q_lens,lens,prefix", [([1, 1], [700, 90], 0), ([2, 1], [300, 40], 700), ([70], [400], 0),
+                                                ([40] * 4, [60, 50, 40, 45], 600)])
+def test_scores_that_grow_along_the_keys(dev, dim, q_lens, lens, prefix):
+    """Every key's scores are larger than those before it, by up to 60 in all: the running maximum moves
+    throughout, and the sums are rescaled."""
+    log(f"attend growing scores dim={dim} q={q_lens} prefix={prefix}")
+    s = Step(q_lens, lens, 8, 2, dim, 16, prefix, dtype=torch.float16, seed=dim + prefix)
+    k, v = s.pages()
+    c = 60.0 / (0.64 * dim ** 0.5)
+    for j in range(prefix):
+        at = int(s.prefix_pages[j // 16]), slice(None), j % 16
+        k[at] = (k[at].float().abs() * (c * j / (prefix + max(lens)))).half()
+    for b, n in enumerate(lens):
+        for j in range(n):
+            at = int(s.table[b, j // 16]), slice(None), j % 16
+            k[at] = (k[at].float().abs() * (c * (prefix + j) / (prefix + max(lens)))).half()
+    q = s.q().abs()
+    got, lse = _cache(dev, k, v).attend(q.to(dev), s.batch(dev), return_lse=True)
+    check_attend(s, got, attend_reference(s, q, k, v), lse)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,prefix", [(1, 0), (1, 40), (6, 0), (60, 0), (60, 40), (200, 17)])
+def test_values_that_are_not_finite(dev, dim, n, prefix):
+    """Infinite and NaN values of keys that some or all queries see show in their column of the rows that see
+    them; every other value is as if they were not there."""
+    log(f"attend bad values dim={dim} n={n} prefix={prefix}")
+    ln = n + 37
+    s = Step([n], [ln], 4, 1, dim, 16, prefix, dtype=torch.bfloat16, seed=n + dim)
+    k, v = s.pages()
+    q = s.q()
+    clean = v.clone()
+    seen = torch.zeros(n, dim, dtype=torch.bool)
+    for j, col, x in ((ln - 1, 3, math.inf), (ln - 2, 7, math.nan), (5, 11, -math.inf), (ln - 1 - n // 2, 60, math.nan)):
+        at = int(s.table[0, j // 16]), 0, j % 16, col
+        clean[at], v[at] = 0, x
+        seen[max(0, j - (ln - n)):, col] = True
+    out, _, tol, _ = attend_reference(s, q, k, clean)
+    got = _cache(dev, k, v).attend(q.to(dev), s.batch(dev)).cpu().double()
+    bad = seen[:, None].expand(n, 4, dim)
+    assert not bool(torch.isfinite(got[bad]).any())
+    assert bool(((got - out).abs() <= tol)[~bad].all())
+
+
+def test_two_streams_at_once(dev):
+    """Calls on two streams side by side, 256-wide heads and 128-wide ones: the bits of calls one by one."""
+    log("attend two streams")
+    made = []
+    for dim, seed in ((256, 3), (128, 4)):
+        s = Step([1] * 12 + [50], [(67 * i) % 500 for i in range(12)] + [300], 8, 2, dim, 16, 300, dtype=torch.bfloat16, seed=seed)
+        k, v = s.pages()
+        made.append((_cache(dev, k, v), s.q().to(dev), s.batch(dev)))
+    want = [c.attend(q, b) for c, q, b in made]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(8):
+        for st, (c, q, b) in zip(streams, made):
+            with torch.cuda.stream(st):
+                outs.append(c.attend(q, b))
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        assert torch.equal(o, want[i % 2]), i
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.parametrize("src", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("dt", ["f16", "bf16"])

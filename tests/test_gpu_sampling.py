@@ -239,3 +239,21 @@ def test_more_rows_than_a_grid_axis(dev):
         t, p = sample_tokens(x[a:a + 35000], u[a:a + 35000], 0.9, 3, 0.9)
         assert torch.equal(tok[a:a + 35000], t) and torch.equal(lp[a:a + 35000], p)
     _check(dev, x[69990:].cpu(), u[69990:].cpu(), 0.9, 3, 0.9)
+
+
+def test_two_streams_at_once(dev):
+    log("sample two streams")
+    from pgmoe import sample_tokens
+    a, b = [(x.to(dev), u.to(dev)) for x, u in (_logits(40, 60000, 1), _logits(7, 131072, 2, torch.float16))]
+    kw = dict(temperature=0.9, top_k=300, top_p=0.95)
+    want = [sample_tokens(*a, **kw), sample_tokens(*b, **kw)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(8):
+        for st, x in zip(streams, (a, b)):
+            with torch.cuda.stream(st):
+                outs.append(sample_tokens(*x, **kw))
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        assert torch.equal(o[0], want[i % 2][0]) and torch.equal(o[1], want[i % 2][1]), i
