@@ -169,6 +169,8 @@ class HipPagedKVCache:
                  dtype: torch.dtype = torch.float16, device: Optional[Union[torch.device, str]] = None) -> None:
         dev = _cuda_device(device)
         self._check(n_pages, page_size, n_kv_heads, head_dim, dtype)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a KV cache is made before a graph is captured: each replay would clear its pages")
         shape = (n_pages, n_kv_heads, page_size, head_dim)
         self._bind(torch.zeros(shape, dtype=dtype, device=dev), torch.zeros(shape, dtype=dtype, device=dev))
         torch.cuda.current_stream(dev).synchronize()  # cleared before any other stream writes to them

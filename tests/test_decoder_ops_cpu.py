@@ -145,3 +145,11 @@ def test_attend_workspace_without_a_prefix_is_half():
     both = L.pgmoe_attend_workspace_bytes(C, B, 3, 32)
     rows = 3 * 32 * 2 * 4  # both count the slots of both parts
     assert 2 * (plain - rows - 256) <= both - rows <= 2 * (plain - rows + 256)
+
+
+def test_no_cache_is_made_while_a_graph_is_captured(monkeypatch):
+    import torch
+    from pgmoe import HipPagedKVCache
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        HipPagedKVCache(4, 16, 1, 64, device="cuda:0")
