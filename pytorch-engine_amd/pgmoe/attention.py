@@ -11,8 +11,8 @@ The step between a layer's Q/K/V projections (FusedLinearPack) and its output pr
 Every sequence sees the ``prefix_len`` keys of ``prefix_pages`` (a system prompt, a document) and then
 its own keys; the prefix's keys and values are read once for the whole batch.  The batch's tensors
 live on the device and are read when the kernels run: a program updates them in place between steps
-(``lens.add_(1)``), and a captured graph replays on what they then hold.  Nothing synchronises with
-the host.  There is no CPU path: CPU tensors, and types, widths and page sizes without a kernel,
+(``lens.add_(1)``), and a captured graph replays on what they then hold (keep cache, batch, rotary and
+norm weights as long as the graph).  Nothing synchronises with the host but the constructors.  There is no CPU path: CPU tensors, and types, widths and page sizes without a kernel,
 raise.
 """
 
