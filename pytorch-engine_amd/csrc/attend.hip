@@ -84,10 +84,11 @@ struct Geo {
 };
 
 // 1 KB from memory to LDS, lane l's 16 bytes to lds + 16 l; waited for with vm_wait (copies are not in the
-// compiler's own count of loads, which only makes its waits longer).
+// compiler's own count of loads, which only makes its waits longer).  A copy reads m0 one wait state after a
+// scalar write of it at the earliest: s_nop, as nothing looks into inline assembly for it.
 __device__ __forceinline__ void copy_lds(const void* base, uint32_t off, uint32_t lds) {
     uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep)
                  : "v"(off), "s"(base), "s"(lds)
                  : "memory");
@@ -97,7 +98,7 @@ __device__ __forceinline__ void copy_lds4(const void* base, uint32_t o0, uint32_
                                           uint32_t lds) {
     uint32_t keep;
     asm volatile(
-        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\t"
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\ts_nop 0\n\t"
         "global_load_lds_dwordx4 %1, %5\n\t"
         "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
         "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
@@ -110,7 +111,7 @@ __device__ __forceinline__ void copy_lds4(const void* base, uint32_t o0, uint32_
 __device__ __forceinline__ void copy_lds2(const void* base, uint32_t o0, uint32_t o1, uint32_t lds) {
     uint32_t keep;
     asm volatile(
-        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\t"
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\t"
         "global_load_lds_dwordx4 %1, %3\n\t"
         "global_load_lds_dwordx4 %2, %3 offset:1024\n\t"
         "s_mov_b32 m0, %0"

@@ -121,10 +121,11 @@ struct GLay {
 // HBM -> LDS copy of 16 bytes per lane (lane l to lds + 16 l), written as inline asm so
 // the compiler neither adds waits for it before unrelated LDS reads nor counts it in its
 // own vmcnt bookkeeping; the kernel waits for the copies itself (vm_wait) before the
-// barrier that publishes a stage.  lds is the wave-uniform LDS byte address.
+// barrier that publishes a stage.  lds is the wave-uniform LDS byte address.  The copy reads m0
+// one wait state after a scalar write of it at the earliest: s_nop.
 __device__ __forceinline__ void g2l(const void* g, uint32_t lds) {
     uint32_t keep;  // m0 is reserved to the compiler: restore it around the copy
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep)
                  : "v"(g), "s"(lds)
                  : "memory");
