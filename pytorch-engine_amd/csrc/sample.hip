@@ -1,9 +1,11 @@
 // Token sampling: temperature, top-k, top-p, min-p and a given uniform number a row.
 //
 // Weights w = exp((x - max) / T) are held as 64-bit fixed point (2^-44 for vocabularies of 2^18, finer for
-// smaller ones: a sum stays below 2^63): integer sums have no order, and a row's result is the same bits however
-// it is cut.  No row is sorted: the last kept token is found from a histogram over the distance to the maximum,
-// then from the tokens of the one bin that holds it.
+// smaller ones: a sum stays below 2^63): integer sums have no order, and a row's result is the same bits on every
+// run.  A slice's sums are taken against its own maximum, to 2^-51 of it, and brought to the row's as a whole, which
+// rounds them to half a unit; a slice whose largest token rounds to nothing has none.  No row is sorted: the last
+// kept token is found from a histogram over the distance to the maximum, then from the tokens of the one bin that
+// holds it.
 //
 // sample_slice_kernel, a workgroup for 8192 tokens of a row, reads the logits once into registers: the slice's
 // maximum, and against it the tokens' weights, their sum, the histogram (256 bins of 1/8 in x / T on a grid that
@@ -450,17 +452,20 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
     const Weigh W(powers, mx, S.inv_t, A.shift);
     const Grid g(mx, S.inv_t);
     auto to_row = [&](uint64_t w, int s) { return slice_s[s] == 1.0 ? w : (uint64_t)llrint((double)w * slice_s[s]); };
+    for (int i = tid; i < kDigits; i += kThreads) cnt[0][i] = cnt[1][i] = 0, wsum[0][i] = wsum[1][i] = 0;
+    if (tid == 0) s_n = 0, s_lo = 0xffffffffu, s_hi = 0;
+    __syncthreads();  // the powers
     if (tid < slices) {
         const Slice m = sl[tid];
         const bool top = m.max == mx;
-        const double f = top ? 1.0 : m.max == -INFINITY || mx == INFINITY ? 0.0 : exp(((double)m.max - (double)mx) * S.inv_t);
+        // A slice whose largest logit has no weight has none, whatever its tokens' small ones add up to: where a slice
+        // has a sum, one token of it at least can be drawn.
+        const double f = top ? 1.0 : W.fix(m.max) ? W.w(m.max) : 0.0;
         slice_s[tid] = f;
         slice_d[tid] = top ? 0.0f : g.at - floorf(m.max * g.g);
         slice_w[tid] = S.filters ? 0 : f == 1.0 ? m.sum : (uint64_t)llrint((double)m.sum * f);
         slice_n[tid] = 0;
     }
-    for (int i = tid; i < kDigits; i += kThreads) cnt[0][i] = cnt[1][i] = 0, wsum[0][i] = wsum[1][i] = 0;
-    if (tid == 0) s_n = 0, s_lo = 0xffffffffu, s_hi = 0;
     __syncthreads();
 
     // The last kept token: key `edge`, of which the first `ties` in index order are kept; every greater key is.
@@ -809,21 +814,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
     // the slice's sum was rounded apart from its tokens', by some units of 2^-shift
     goal = goal < all ? goal : all - 1;
     uint64_t at = w0 + kept(n0);
-    if (all ? at <= goal && goal < w0 + w + kept(n0 + n) : tid == 0) {
+    if (at <= goal && goal < w0 + w + kept(n0 + n)) {
         int tok = -1;
         float xt = 0.0f;
-        if (all) {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                at += f[e];
-                if (x[e] > -INFINITY && key_of(x[e]) == edge) at += n0++ < ties ? fe : 0;
-                if (tok < 0 && at > goal) tok = i0 + e, xt = x[e];
-            }
-        } else {  // every weight of the slice rounds to nothing: its largest logit
-            for (int i = slice * kSlice; i < (slice + 1) * kSlice && i < V; ++i) {
-                const float y = one_logit<DT>(A, row + i);
-                if (y > -INFINITY && (tok < 0 || y > xt)) tok = i, xt = y;
-            }
+        for (int e = 0; e < kPer; ++e) {
+            at += f[e];
+            if (x[e] > -INFINITY && key_of(x[e]) == edge) at += n0++ < ties ? fe : 0;
+            if (tok < 0 && at > goal) tok = i0 + e, xt = x[e];
         }
         A.token[r] = tok;
         if (A.logprob) {
