@@ -310,7 +310,7 @@ struct Core {
     static constexpr int NK = D / 16, ND = D / 32;
     u16x8 q[NK];
     f32x16 o[ND];
-    float m, l, c;  // reference maximum (raw score), sum over this lane's keys, scale * log2(e)
+    float m, l, c;  // reference maximum (raw score), sum over this lane's keys times 2^kUp, scale * log2(e)
     int lane, n, h;
     uint32_t koff, voff[ND];  // LDS byte offsets of this lane's reads
 
@@ -383,9 +383,8 @@ struct Core {
             if (key_of(i, 0) >= left) s[i] = -INFINITY;
         }
     }
-    // The reference m follows the running maximum only when that has grown by 2^8: p = 2^(c (s - m)) stays
-    // within fp16's range and its relative precision, and the rescaling of o (64 products a lane) all but
-    // vanishes.
+    // The reference m follows the running maximum only when that has grown by 2^8, and the rescaling of o (64
+    // products a lane) all but vanishes: p = 2^(c (s - m) + kUp) is 2^(8 + kUp) at most.
     template <int N2>
     __device__ __forceinline__ void grow(const f32x16 (&s)[N2]) {
         float mx = s[0][0];
@@ -406,18 +405,25 @@ struct Core {
             hold_sums();
         }
     }
-    // p = 2^(c (s - m)) rounded, l += sum p
+    // p = 2^(c (s - m) + kUp) rounded, l += sum p.  The product with V takes 16-bit probabilities (that is what the
+    // matrix units multiply at full rate; each is off by half a step of the cache's type, as V itself is), the
+    // sum l takes them as they are.  fp16 holds them from 2^-14 on: moved up by kUp, they keep their precision down
+    // to 2^-21 of the reference, and those that vanish, below 2^-32 of it, add up to 2^-12 where 2^20 keys
+    // are (without kUp 2^17 keys of 2^-26 each were 2^-9 of l and nothing of o).  bf16 holds any.
+    static constexpr float kUp = BF16 ? 0.0f : 7.0f;
     template <int N2>
     __device__ __forceinline__ void weigh(const f32x16 (&s)[N2], u16x8 (&p)[2 * N2]) {
-        const float mc = m == -INFINITY ? 0.0f : m * c;
+        const float mc = m == -INFINITY ? 0.0f : m * c - kUp;
+        float sum = 0.0f;  // the tile's by itself, so that light keys are not lost one by one beside l
 #pragma unroll
         for (int g = 0; g < N2; ++g)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][i], c, -mc));
-                l += e;
+                sum = i + g ? sum + e : e;
                 p[2 * g + (i >> 3)][i & 7] = to16<BF16>(e);
             }
+        l += sum;
     }
     __device__ __forceinline__ u16x8 vfrag(const uint8_t* V, int st, int d) const {
         typedef __attribute__((address_space(3))) s16x4* lp;
@@ -645,7 +651,7 @@ struct Rows {
                               make_float4(core.o[d][4 * i], core.o[d][4 * i + 1], core.o[d][4 * i + 2],
                                           core.o[d][4 * i + 3]),
                               inv);
-        if (core.h == 0) put_row(A, W, direct, orow, core.m * A.c, l, empty);
+        if (core.h == 0) put_row(A, W, direct, orow, core.m * A.c - core.kUp, l, empty);
     }
 };
 
