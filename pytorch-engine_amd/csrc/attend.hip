@@ -311,6 +311,7 @@ struct Core {
     u16x8 q[NK];
     f32x16 o[ND];
     float m, l, c;  // reference maximum (raw score), sum over this lane's keys times 2^kUp, scale * log2(e)
+    bool far;       // a row's |m c| passes 2^23: see grow
     int lane, n, h;
     uint32_t koff, voff[ND];  // LDS byte offsets of this lane's reads
 
@@ -339,7 +340,7 @@ struct Core {
 
     __device__ __forceinline__ void begin(int lane_) {
         lane = lane_, n = lane & 31, h = lane >> 5;
-        m = -INFINITY, l = 0.0f;
+        m = -INFINITY, l = 0.0f, far = false;
 #pragma unroll
         for (int i = 0; i < ND; ++i) o[i] = f32x16{};
         koff = n * G::RB + ((h ^ (n & G::KM)) << 4);
@@ -384,16 +385,18 @@ struct Core {
         }
     }
     // The reference m follows the running maximum only when that has grown by 2^8, and the rescaling of o (64
-    // products a lane) all but vanishes: p = 2^(c (s - m) + kUp) is 2^(8 + kUp) at most.
+    // products a lane) all but vanishes: p = 2^(c (s - m) + kUp) is 2^(8 + kUp) at most.  weigh forms its exponent as
+    // fma(s, c, -round(m c)), which is off by half a step of m c: the same factor of all of a row's p, until it
+    // takes them out of fp16's range.  Rows with |m c| above 2^23, of which a step is 1, go on with s - m.
     template <int N2>
-    __device__ __forceinline__ void grow(const f32x16 (&s)[N2]) {
+    __device__ __forceinline__ void grow(f32x16 (&s)[N2]) {
         float mx = s[0][0];
 #pragma unroll
         for (int g = 0; g < N2; ++g)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[g][i]);
         mx = fmaxf(mx, swap32(mx));
-        if (__builtin_expect(__any((mx - m) * c > 8.0f), 0)) {
+        if (__builtin_expect(__any((mx - m) * c > 8.0f) || far, 0)) {
             const float mn = fmaxf(m, mx);
             const float f = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * c);
             l *= f;
@@ -402,6 +405,14 @@ struct Core {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
             m = mn;
+            far = __any(m > -INFINITY && fabsf(m) * c > 8388608.0f);
+            if (far) {
+                const float r = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int g = 0; g < N2; ++g)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[g][i] -= r;
+            }
             hold_sums();
         }
     }
@@ -413,7 +424,7 @@ struct Core {
     static constexpr float kUp = BF16 ? 0.0f : 7.0f;
     template <int N2>
     __device__ __forceinline__ void weigh(const f32x16 (&s)[N2], u16x8 (&p)[2 * N2]) {
-        const float mc = m == -INFINITY ? 0.0f : m * c - kUp;
+        const float mc = (m == -INFINITY || far ? 0.0f : m * c) - kUp;
         float sum = 0.0f;  // the tile's by itself, so that light keys are not lost one by one beside l
 #pragma unroll
         for (int g = 0; g < N2; ++g)

@@ -79,3 +79,38 @@ def test_light_keys_count_together(dev, kind, dim, dt):
         assert off <= tol, (col, want, off, tol)
     assert float(got[..., 2:].abs().max()) == 0.0
     assert float((lse - 8.0 - math.log(total)).abs().max()) <= in_l + 2.0 ** -20
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("dt,big,scale", [(torch.float16, 60000.0, 8.0), (torch.float16, 30000.0, 0.25), (torch.float16, 4096.0, 0.7),
+                                          (torch.bfloat16, 2.0 ** 50, 1.0), (torch.bfloat16, 2.0 ** 18, 0.3)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q_lens,lens,prefix", [([1, 1], [700, 33], 0), ([1], [5000], 300), ([60], [500], 0), ([100, 50], [120, 90], 400)])
+def test_scores_of_any_finite_size(dev, q_lens, lens, prefix, dim, dt, big, scale, sign):
+    """Scores of 10^7 to 10^30 that differ by a step of their type and more: each row is the average of the values of
+    its largest scores, as the formula has it, and nothing overflows.  Ordinary queries of other rows stay as they are.
+
+    The products of one column are exact in fp32 (11 bits by 11), scores next to each other differ by 2^-11 of `big`
+    times big * scale, more than 800 units: no other key has a weight.  The average: half a step of the cache's type, V and
+    the equal probabilities rounded once each."""
+    from kv_helpers import Step, attend_reference
+    log(f"attend far scores {q_lens} {prefix} {dim} {dt} {big} {scale} {sign}")
+    s = Step(q_lens, lens, 4, 1, dim, 16, prefix, dtype=dt, seed=dim)
+    k, v = s.pages()
+    step = 2.0 ** -10 if dt is torch.float16 else 2.0 ** -7
+    level = torch.randint(0, 9, k[..., 0].shape, generator=s.gen).double()
+    kk = torch.where(torch.isnan(k), k, torch.zeros_like(k))
+    kk[..., 0] = torch.where(torch.isnan(k[..., 0]), k[..., 0], (sign * big * (1 - 8 * step + level * step) * 0.5).to(dt))
+    q = torch.zeros(s.T, 4, dim, dtype=dt)
+    q[..., 0] = big
+    q[::3, 1] = 0.0  # a row whose scores are all 0: an average of every value
+    from pgmoe import HipPagedKVCache
+    got, lse = HipPagedKVCache.from_tensors(kk.to(dev), v.to(dev)).attend(q.to(dev), s.batch(dev), scale=scale, return_lse=True)
+    assert bool(torch.isfinite(got).all())
+    out, top, _, _ = attend_reference(s, q, kk, v, scale)
+    mag = v[~torch.isnan(v)].double().abs().max()
+    half = HALF_STEP[dt]
+    n = prefix + max(lens)
+    assert float((got.double().cpu() - out).abs().max()) <= half * (2.01 * mag) + 2 * (n + 64) * 2.0 ** -24 * mag + 2.0 ** -25
+    # m scale log2(e) + log2(l), times ln 2: eight roundings of 2^-24, and the sum's
+    assert float(((lse.double().cpu() - top).abs() / (1 + top.abs())).max()) <= 2.0 ** -21 + (n + 64) * 2.0 ** -24
