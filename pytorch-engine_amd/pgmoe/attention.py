@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Dict, Optional, Sequence, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -118,6 +118,8 @@ class KVBatch:
             raise NotImplementedError(f"{n} sequences (1 .. {_MAX_SEQS})")
         if self._table.shape[1] < 1 or self._lens.shape[0] != n:
             raise ValueError(f"page_table {tuple(self._table.shape)} and lens {tuple(self._lens.shape)} of {n} sequences")
+        if n > 1 and self._table.stride(0) < self._table.shape[1]:
+            raise ValueError("the rows of page_table overlap")
         self._q_start = None
         if q_start is not None:
             self._q_start = self._int32("q_start", q_start, 1, 0)
@@ -215,7 +217,6 @@ class HipPagedKVCache:
         self._c = _KVCache(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], self.n_pages, self.page_size,
                            self.n_kv_heads, self.head_dim, _DT[k.dtype])
         self._ref = ctypes.byref(self._c)
-        self._ws_bytes: Dict[Tuple[int, ...], int] = {}
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
@@ -330,10 +331,8 @@ class HipPagedKVCache:
         if out is not None:
             self._apart(out, q, self._k, self._v)
         lse = torch.empty((T, hq), dtype=torch.float32, device=self.device) if return_lse else None
-        key = (T, hq, batch.n_seqs, batch.max_pages, batch.prefix_len, batch._q_start is None)
-        n = self._ws_bytes.get(key)
-        if n is None:
-            n = self._ws_bytes[key] = int(lib().pgmoe_attend_workspace_bytes(self._ref, batch._ref, T, hq))
+        # 0 for what pgmoe_attend refuses, which then says why
+        n = int(lib().pgmoe_attend_workspace_bytes(self._ref, batch._ref, T, hq))
         # scratch of this call alone, from the stream's allocator: calls on other streams, and graphs that
         # replay side by side, each have their own
         ws = torch.empty(n, dtype=torch.uint8, device=self.device)

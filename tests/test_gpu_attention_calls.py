@@ -1,0 +1,63 @@
+"""What HipPagedKVCache, KVBatch and HipRotary accept, refuse and keep from call to call."""
+
+import pytest
+
+from gpu_helpers import log
+from kv_helpers import Step, attend_reference, check_attend
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch.device("cuda", 0)
+
+
+def _made(dev, **kw):
+    from pgmoe import HipPagedKVCache
+    s = Step([1, 1], [40, 70], 8, 2, 128, 16, seed=1, **kw)
+    k, v = s.pages()
+    q = s.q()
+    return s, HipPagedKVCache.from_tensors(k.to(dev), v.to(dev)), q.to(dev), attend_reference(s, q, k, v)
+
+
+def test_page_tables_whose_rows_overlap_are_refused(dev):
+    from pgmoe import KVBatch
+    log("page table rows that overlap")
+    row = torch.zeros(1, 4, dtype=torch.int32, device=dev)
+    with pytest.raises(ValueError, match="overlap"):
+        KVBatch(row.expand(2, 4), [4, 5])
+    with pytest.raises(ValueError, match="overlap"):
+        KVBatch(torch.zeros(9, dtype=torch.int32, device=dev).as_strided((2, 4), (3, 1)), [4, 5])
+    KVBatch(row.expand(1, 4), [4])  # a single row overlaps nothing
+
+
+def test_a_refused_call_leaves_the_next_ones(dev):
+    """A batch that the library refuses, then a valid one of the same shape on the same cache."""
+    log("attend after a refusal")
+    s, c, q, ref = _made(dev)
+    b = s.batch(dev)
+    stride, b._c.table_stride = b._c.table_stride, 0
+    with pytest.raises(RuntimeError, match="overlap"):
+        c.attend(q, b)
+    b._c.table_stride = stride
+    check_attend(s, c.attend(q, b), ref)
+
+
+def test_nothing_is_kept_for_a_call_s_sizes(dev):
+    """Calls of ever new sizes leave the cache object as it was."""
+    from pgmoe import KVBatch
+    log("attend of many sizes")
+    s, c, q, _ = _made(dev)
+
+    def held():
+        return {n: len(x) for n, x in vars(c).items() if hasattr(x, "__len__") and not isinstance(x, torch.Tensor)}
+
+    before = held()
+    for T in range(1, 20):
+        c.attend(torch.zeros(T, 8, 128, dtype=s.dtype, device=dev),
+                 KVBatch(s.table.to(dev), s.lens, q_start=[0, T, T], prefix_pages=[0, 1], prefix_len=T))
+    assert held() == before
