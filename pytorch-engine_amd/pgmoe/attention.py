@@ -12,8 +12,8 @@ Every sequence sees the ``prefix_len`` keys of ``prefix_pages`` (a system prompt
 its own keys; the prefix's keys and values are read once for the whole batch.  The batch's tensors
 live on the device and are read when the kernels run: a program updates them in place between steps
 (``lens.add_(1)``), and a captured graph replays on what they then hold (keep cache, batch, rotary and
-norm weights as long as the graph).  Nothing synchronises with the host but the constructors.  There is no CPU path: CPU tensors, and types, widths and page sizes without a kernel,
-raise.
+norm weights as long as the graph).  Nothing synchronises with the host but the constructors.  There is
+no CPU path: CPU tensors, and types, widths and page sizes without a kernel, raise.
 """
 
 from __future__ import annotations
@@ -83,9 +83,9 @@ class HipRotary:
             raise ValueError(f"rotary_dim {rotary_dim}: a multiple of 16 up to head_dim {head_dim}")
         if not (math.isfinite(position_scale) and math.isfinite(attn_factor) and base > 0):
             raise ValueError("base must be positive, position_scale and attn_factor finite")
-        self.device = _cuda_device(device)
-        self.head_dim, self.rotary_dim, self.interleaved = int(head_dim), rotary_dim, bool(interleaved)
-        self.attn_factor = float(attn_factor)
+        self._device = _cuda_device(device)
+        self._head_dim, self._rotary_dim, self._interleaved = int(head_dim), rotary_dim, bool(interleaved)
+        self._attn_factor = float(attn_factor)
         if inv_freq is None:
             inv_freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
         f = inv_freq.to("cpu", torch.float64)
@@ -93,7 +93,15 @@ class HipRotary:
             if freq_factors.numel() != rotary_dim // 2:
                 raise ValueError("freq_factors holds one factor a pair (rotary_dim / 2)")
             f = f / freq_factors.to("cpu", torch.float64).reshape(-1)
-        self.turns = (f * (position_scale / (2.0 * math.pi))).to(self.device)
+        self._turns = (f * (position_scale / (2.0 * math.pi))).to(self._device)
+
+    # as they were given: the kernel reads rotary_dim / 2 turns
+    device = property(lambda self: self._device)
+    head_dim = property(lambda self: self._head_dim)
+    rotary_dim = property(lambda self: self._rotary_dim)
+    interleaved = property(lambda self: self._interleaved)
+    attn_factor = property(lambda self: self._attn_factor)
+    turns = property(lambda self: self._turns)
 
 
 class KVBatch:
@@ -103,14 +111,15 @@ class KVBatch:
     `prefix_len` (keys every sequence sees before its own).
 
     Tensors on the device are kept, not copied, and may be updated in place.  Lists and CPU tensors
-    are checked and copied to the device."""
+    are checked and copied to the device.  The numbers (n_seqs, max_pages, prefix_len) are the batch's for
+    good: a step behind another prefix takes another batch."""
 
     def __init__(self, page_table: _IntTensor, lens: _IntTensor, q_start: Optional[_IntTensor] = None,
                  prefix_pages: Optional[_IntTensor] = None, prefix_len: int = 0,
                  device: Optional[Union[torch.device, str]] = None) -> None:
         given = [t for t in (page_table, lens, q_start, prefix_pages)
                  if isinstance(t, torch.Tensor) and t.device.type == "cuda"]
-        self.device = given[0].device if given else _cuda_device(device)
+        self._device = given[0].device if given else _cuda_device(device)
         self._table = self._int32("page_table", page_table, 2, -1)
         self._lens = self._int32("lens", lens, 1, 0)
         n = self._table.shape[0]
@@ -128,17 +137,17 @@ class KVBatch:
             host = q_start if not isinstance(q_start, torch.Tensor) else q_start.tolist() if q_start.device.type == "cpu" else None
             if host is not None and (host[0] != 0 or any(a > b for a, b in zip(host, host[1:]))):
                 raise ValueError("q_start begins at 0 and does not decrease")
-        self.prefix_len = int(prefix_len)
-        if self.prefix_len < 0:
+        self._prefix_len = int(prefix_len)
+        if self._prefix_len < 0:
             raise ValueError("negative prefix_len")
         self._prefix = None if prefix_pages is None else self._int32("prefix_pages", prefix_pages, 1, -1)
-        if self.prefix_len and self._prefix is None:
+        if self._prefix_len and self._prefix is None:
             raise ValueError("prefix_len without prefix_pages")
-        self.n_seqs, self.max_pages = n, int(self._table.shape[1])
+        self._n_seqs, self._max_pages = n, int(self._table.shape[1])
         self._c = _KVBatch(self._table.data_ptr(), self._lens.data_ptr(),
                            None if self._q_start is None else self._q_start.data_ptr(),
                            None if self._prefix is None else self._prefix.data_ptr(),
-                           self._table.stride(0), n, self.max_pages, self.prefix_len)
+                           self._table.stride(0), n, self._max_pages, self._prefix_len)
         self._ref = ctypes.byref(self._c)
 
     def _int32(self, name: str, x: _IntTensor, dims: int, least: int) -> torch.Tensor:
@@ -148,11 +157,11 @@ class KVBatch:
         if t.device.type != "cuda":
             if t.is_floating_point() or (t.numel() and (int(t.min()) < least or int(t.max()) > 2 ** 31 - 1)):
                 raise ValueError(f"{name} holds int32 values from {least} on")
-            return t.to(self.device, torch.int32).contiguous()
+            return t.to(self._device, torch.int32).contiguous()
         if t.dtype != torch.int32:
             raise ValueError(f"{name} is an int32 tensor")
-        if t.device != self.device:
-            raise ValueError(f"{name} is on {t.device}, the batch on {self.device}")
+        if t.device != self._device:
+            raise ValueError(f"{name} is on {t.device}, the batch on {self._device}")
         if t.numel() and t.stride(-1) != 1:
             raise ValueError(f"{name} must be contiguous along its rows")
         return t
@@ -162,6 +171,11 @@ class KVBatch:
     lens = property(lambda self: self._lens)
     q_start = property(lambda self: self._q_start)
     prefix_pages = property(lambda self: self._prefix)
+    device = property(lambda self: self._device)
+    # numbers that calls and captured graphs hold as they were given: another value is another batch
+    n_seqs = property(lambda self: self._n_seqs)
+    max_pages = property(lambda self: self._max_pages)
+    prefix_len = property(lambda self: self._prefix_len)
 
 
 class HipPagedKVCache:
@@ -211,26 +225,32 @@ class HipPagedKVCache:
     def _bind(self, k: torch.Tensor, v: torch.Tensor) -> None:
         lib()
         self._k, self._v = k, v
-        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = (int(x) for x in k.shape)
-        self.dtype, self.device = k.dtype, k.device
+        self._n_pages, self._n_kv_heads, self._page_size, self._head_dim = (int(x) for x in k.shape)
+        self._dtype, self._device = k.dtype, k.device
         st = k.stride()
-        self._c = _KVCache(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], self.n_pages, self.page_size,
-                           self.n_kv_heads, self.head_dim, _DT[k.dtype])
+        self._c = _KVCache(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], self._n_pages, self._page_size,
+                           self._n_kv_heads, self._head_dim, _DT[k.dtype])
         self._ref = ctypes.byref(self._c)
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
+    n_pages = property(lambda self: self._n_pages)
+    n_kv_heads = property(lambda self: self._n_kv_heads)
+    page_size = property(lambda self: self._page_size)
+    head_dim = property(lambda self: self._head_dim)
+    dtype = property(lambda self: self._dtype)
+    device = property(lambda self: self._device)
 
     # ------------------------------------------------------------------ checks
     def _heads(self, name: str, x: torch.Tensor, dtypes, heads: Optional[int] = None) -> Tuple[torch.Tensor, int, int]:
         """x checked, and its token and head strides; copied where its rows cannot be read 16 bytes at a time."""
         shape, dtype = x.shape, x.dtype
-        if x.device != self.device:
-            raise ValueError(f"{name} is on {x.device}, the cache on {self.device}")
+        if x.device != self._device:
+            raise ValueError(f"{name} is on {x.device}, the cache on {self._device}")
         if dtype not in dtypes:
             raise NotImplementedError(f"{name} of dtype {dtype}")
-        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
-            raise ValueError(f"{name} {tuple(shape)}: [tokens, {'heads' if heads is None else heads}, {self.head_dim}]")
+        if len(shape) != 3 or shape[2] != self._head_dim or (heads is not None and shape[1] != heads):
+            raise ValueError(f"{name} {tuple(shape)}: [tokens, {'heads' if heads is None else heads}, {self._head_dim}]")
         a, b, c = x.stride()
         if c != 1 or (a | b) & (3 if dtype is torch.float32 else 7) or x.data_ptr() & 15:
             x = x.clone(memory_format=torch.contiguous_format)
@@ -239,21 +259,21 @@ class HipPagedKVCache:
 
     def _tokens(self, q: torch.Tensor, batch: KVBatch) -> Tuple[int, int]:
         T, hq, _ = q.shape
-        if hq < 1 or hq % self.n_kv_heads:
-            raise ValueError(f"{hq} query heads on {self.n_kv_heads} KV heads")
-        if batch.device != self.device:
-            raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
-        if batch._q_start is None and T != batch.n_seqs:
+        if hq < 1 or hq % self._n_kv_heads:
+            raise ValueError(f"{hq} query heads on {self._n_kv_heads} KV heads")
+        if batch._device != self._device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {self._device}")
+        if batch._q_start is None and T != batch._n_seqs:
             raise ValueError(f"{T} tokens of {batch.n_seqs} sequences: q_start says which are whose")
-        if batch.prefix_len > (0 if batch._prefix is None else batch._prefix.shape[0]) * self.page_size:
-            raise ValueError(f"a prefix of {batch.prefix_len} keys on {batch._prefix.shape[0]} pages of {self.page_size}")
+        if batch._prefix_len > (0 if batch._prefix is None else batch._prefix.shape[0]) * self._page_size:
+            raise ValueError(f"a prefix of {batch.prefix_len} keys on {batch._prefix.shape[0]} pages of {self._page_size}")
         return T, hq
 
     def _out(self, out: Optional[torch.Tensor], T: int, hq: int) -> torch.Tensor:
         if out is None:
-            return torch.empty((T, hq, self.head_dim), dtype=self.dtype, device=self.device)
-        if out.shape != (T, hq, self.head_dim) or out.dtype != self.dtype or out.device != self.device:
-            raise ValueError(f"out: [{T}, {hq}, {self.head_dim}] of {self.dtype} on {self.device}")
+            return torch.empty((T, hq, self._head_dim), dtype=self._dtype, device=self._device)
+        if out.shape != (T, hq, self._head_dim) or out.dtype != self._dtype or out.device != self._device:
+            raise ValueError(f"out: [{T}, {hq}, {self._head_dim}] of {self._dtype} on {self._device}")
         if not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("out must be contiguous and 16-byte aligned")
         return out
@@ -286,28 +306,28 @@ class HipPagedKVCache:
             raise ValueError(f"q, k and v of one dtype, not {q.dtype}, {k.dtype}, {v.dtype}")
         q, qt, qh = self._heads("q", q, _DT)
         T, hq = self._tokens(q, batch)
-        k, kt, kh = self._heads("k", k, _DT, self.n_kv_heads)
-        v, vt, vh = self._heads("v", v, _DT, self.n_kv_heads)
+        k, kt, kh = self._heads("k", k, _DT, self._n_kv_heads)
+        v, vt, vh = self._heads("v", v, _DT, self._n_kv_heads)
         if k.shape[0] != T or v.shape[0] != T:
             raise ValueError(f"{T} queries, {k.shape[0]} keys, {v.shape[0]} values")
         turns, rot, inter, factor = None, 0, 0, 1.0
         if rope is not None:
-            if rope.head_dim != self.head_dim or rope.device != self.device:
-                raise ValueError(f"rotary of head_dim {rope.head_dim} on {rope.device}, cache of {self.head_dim} on {self.device}")
-            turns, rot, inter, factor = rope.turns.data_ptr(), rope.rotary_dim, rope.interleaved, rope.attn_factor
+            if rope._head_dim != self._head_dim or rope._device != self._device:
+                raise ValueError(f"rotary of head_dim {rope.head_dim} on {rope.device}, cache of {self._head_dim} on {self._device}")
+            turns, rot, inter, factor = rope._turns.data_ptr(), rope._rotary_dim, rope._interleaved, rope._attn_factor
         qn = None if q_norm is None else self._norm("q_norm", q_norm)
         kn = None if k_norm is None else self._norm("k_norm", k_norm)
         res = self._out(out, T, hq)
         if out is not None:
             self._apart(out, q, k, v, self._k, self._v)
-        launch(self.device, "pgmoe_rope_append", lib().pgmoe_rope_append, self._ref, batch._ref, q.data_ptr(), qt, qh,
+        launch(self._device, "pgmoe_rope_append", lib().pgmoe_rope_append, self._ref, batch._ref, q.data_ptr(), qt, qh,
                k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DT[q.dtype], T, hq, turns, rot, inter, factor,
                None if qn is None else qn.data_ptr(), None if kn is None else kn.data_ptr(), eps, res.data_ptr())
         return res
 
     def _norm(self, name: str, w: torch.Tensor) -> torch.Tensor:
-        if w.numel() != self.head_dim or w.device != self.device:
-            raise ValueError(f"{name}: {self.head_dim} weights on {self.device}")
+        if w.numel() != self._head_dim or w.device != self._device:
+            raise ValueError(f"{name}: {self._head_dim} weights on {self._device}")
         if w.dtype is not torch.float32 or not w.is_contiguous():
             w = w.to(torch.float32).contiguous()
         return w.clone() if w.data_ptr() & 15 else w
@@ -322,20 +342,20 @@ class HipPagedKVCache:
         A query that sees no key gets zeros and -inf; one that sees a key on a page that does not exist
         gets NaN.  Masked keys and unused page rows may hold anything.  Rows of `out` behind the last
         sequence are left alone."""
-        q, qt, qh = self._heads("q", q, (self.dtype,))
+        q, qt, qh = self._heads("q", q, (self._dtype,))
         T, hq = self._tokens(q, batch)
-        scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        scale = self._head_dim ** -0.5 if scale is None else float(scale)
         if not (0.0 < scale < 3e38):
             raise ValueError("scale must be positive and finite")
         res = self._out(out, T, hq)
         if out is not None:
             self._apart(out, q, self._k, self._v)
-        lse = torch.empty((T, hq), dtype=torch.float32, device=self.device) if return_lse else None
+        lse = torch.empty((T, hq), dtype=torch.float32, device=self._device) if return_lse else None
         # 0 for what pgmoe_attend refuses, which then says why
         n = int(lib().pgmoe_attend_workspace_bytes(self._ref, batch._ref, T, hq))
         # scratch of this call alone, from the stream's allocator: calls on other streams, and graphs that
         # replay side by side, each have their own
-        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
-        launch(self.device, "pgmoe_attend", lib().pgmoe_attend, self._ref, batch._ref, q.data_ptr(), qt, qh, T, hq, scale,
+        ws = torch.empty(n, dtype=torch.uint8, device=self._device)
+        launch(self._device, "pgmoe_attend", lib().pgmoe_attend, self._ref, batch._ref, q.data_ptr(), qt, qh, T, hq, scale,
                res.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), n)
         return res if lse is None else (res, lse)

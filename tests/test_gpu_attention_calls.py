@@ -61,3 +61,24 @@ def test_nothing_is_kept_for_a_call_s_sizes(dev):
         c.attend(torch.zeros(T, 8, 128, dtype=s.dtype, device=dev),
                  KVBatch(s.table.to(dev), s.lens, q_start=[0, T, T], prefix_pages=[0, 1], prefix_len=T))
     assert held() == before
+
+
+def test_what_a_call_holds_as_it_was_given_is_read_only(dev):
+    """The kernels read the numbers a batch, a cache and a rotary were made with: another value is refused, and the
+    next call computes what it did before."""
+    from pgmoe import HipRotary
+    log("read-only numbers")
+    s, c, q, ref = _made(dev, prefix=20)
+    b, rope = s.batch(dev), HipRotary(128, rotary_dim=64, device=dev)
+    for x, names in ((b, ("n_seqs", "max_pages", "prefix_len", "device")),
+                     (c, ("n_pages", "n_kv_heads", "page_size", "head_dim", "dtype", "device")),
+                     (rope, ("head_dim", "rotary_dim", "interleaved", "attn_factor", "turns", "device"))):
+        for n in names:
+            was = getattr(x, n)
+            with pytest.raises(AttributeError):
+                setattr(x, n, was)
+            assert getattr(x, n) is was or getattr(x, n) == was
+    assert (b.n_seqs, b.max_pages, b.prefix_len) == (2, 5, 20)
+    assert (c.n_pages, c.n_kv_heads, c.page_size, c.head_dim, c.dtype) == (s.n_pages, 2, 16, 128, s.dtype)
+    assert (rope.head_dim, rope.rotary_dim, rope.interleaved, rope.attn_factor) == (128, 64, False, 1.0)
+    check_attend(s, c.attend(q, b), ref)
