@@ -326,9 +326,10 @@ typedef struct pgmoe_kv_cache {
  * the last of its lens[b] own keys, so token i of n has own index lens[b] - n + i.  Own key j lies in row
  * j % page_size of page page_table[b * table_stride + j / page_size].  prefix_len keys before them (in the
  * pages prefix_pages, which need not be full) are shared by every sequence.  The positions of the own keys
- * follow the prefix: prefix_len + j.  All arrays are int32 on the device and are read when the kernels run:
- * a captured graph replays on their present contents.  Nothing is read or written through a page id
- * outside [0, n_pages) or past max_pages pages of a table row. */
+ * follow the prefix: prefix_len + j.  All arrays are int32 on the device and are read when the kernels run
+ * (and not to be changed meanwhile): a captured graph replays on their present contents.  Nothing is read or written through a page id
+ * outside [0, n_pages) or past max_pages pages of a table row, nor are rows past the call's tokens, whatever
+ * q_start holds; where it decreases, the call's rows of the outputs hold anything. */
 typedef struct pgmoe_kv_batch {
     const int32_t* page_table;   /* [n_seqs][max_pages], rows table_stride apart */
     const int32_t* lens;         /* [n_seqs]; negative counts as 0 */

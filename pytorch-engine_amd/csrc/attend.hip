@@ -687,7 +687,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
     __shared__ __attribute__((aligned(1024))) uint8_t smem[G::LDS];
     __shared__ int s_base[2][kThreads];
     __shared__ int s_seq[kThreads][3];
-    __shared__ int s_red[4][5];
+    __shared__ int s_red[4][6];
     const int tid = threadIdx.x, lane = tid & 63, wv = uni(tid >> 6);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem;
 
@@ -697,10 +697,12 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
     ax0.pre = ax1.pre = 0;
     const int per = (A.B.seqs + kThreads - 1) / kThreads;
     int mine[5] = {0, 0, 0, 0, 0};  // split and shared cost, shared row tiles; the longest segment of each kind
+    bool down = false;              // q_start decreases
     for (int i = 0; i < per; ++i) {
         const int b = tid * per + i;
         const bool in = b < A.B.seqs;
         const Seq s = load_seq(A, in ? b : A.B.seqs - 1);
+        if (in && A.B.q_start) down = down || A.B.q_start[b + 1] < A.B.q_start[b];
         if (per == 1) s_seq[tid][0] = s.lo, s_seq[tid][1] = s.n, s_seq[tid][2] = s.len;
         mine[0] += ax0.cost(A, s, in, lane) * A.C.heads;
         mine[1] += ax1.cost(A, s, in, lane) * A.C.heads;
@@ -723,12 +725,16 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             mine[k] = x > mine[k] ? x : mine[k];
         }
     }
+    down = __any(down);
     if (lane == 63) {
 #pragma unroll
         for (int k = 0; k < 3; ++k) s_red[wv][k] = inc[k];
-        s_red[wv][3] = mine[3], s_red[wv][4] = mine[4];
+        s_red[wv][3] = mine[3], s_red[wv][4] = mine[4], s_red[wv][5] = down;
     }
     __syncthreads();
+    // Sequences of a q_start that decreases hold more rows together than the call, and the axis could leave 32 bits:
+    // nothing is computed.
+    if (uni(s_red[0][5] | s_red[1][5] | s_red[2][5] | s_red[3][5])) return;
     int before[3] = {inc[0] - mine[0], inc[1] - mine[1], inc[2] - mine[2]}, own[3] = {0, 0, 0}, most[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

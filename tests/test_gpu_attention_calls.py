@@ -82,3 +82,23 @@ def test_what_a_call_holds_as_it_was_given_is_read_only(dev):
     assert (c.n_pages, c.n_kv_heads, c.page_size, c.head_dim, c.dtype) == (s.n_pages, 2, 16, 128, s.dtype)
     assert (rope.head_dim, rope.rotary_dim, rope.interleaved, rope.attn_factor) == (128, 64, False, 1.0)
     check_attend(s, c.attend(q, b), ref)
+
+
+@pytest.mark.parametrize("seqs,tokens,prefix", [(3, 40, 0), (300, 64, 20), (2048, 4096, 0)])
+def test_a_q_start_that_decreases_stays_inside(dev, seqs, tokens, prefix):
+    """Sequences that all claim every token, on the device where the host does not see it (together they are more work than
+    32 bits count): nothing behind the call's rows changes, and the next call is as ever."""
+    from pgmoe import HipPagedKVCache, KVBatch
+    log(f"attend q_start up and down, {seqs} sequences of {tokens} tokens, prefix {prefix}")
+    c = HipPagedKVCache(40, 256, 8, 64, device=dev)
+    up_down = torch.tensor([tokens * (i % 2) for i in range(seqs + 1)], dtype=torch.int32, device=dev)
+    table = torch.zeros(seqs, 256, dtype=torch.int32, device=dev)
+    b = KVBatch(table, torch.full((seqs,), 65536, dtype=torch.int32, device=dev), q_start=up_down,
+                prefix_pages=torch.zeros(1, dtype=torch.int32, device=dev), prefix_len=prefix)
+    buf = torch.full((tokens + 8, 64, 64), 3.0, dtype=torch.float16, device=dev)
+    k = c.k.clone()
+    c.attend(torch.zeros(tokens, 64, 64, dtype=torch.float16, device=dev), b, out=buf[:tokens])
+    torch.cuda.synchronize()
+    assert bool((buf[tokens:] == 3.0).all()) and torch.equal(c.k, k)
+    s, c, q, ref = _made(dev, prefix=20)
+    check_attend(s, c.attend(q, s.batch(dev)), ref)
