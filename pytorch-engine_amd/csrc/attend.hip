@@ -311,7 +311,7 @@ struct Core {
     u16x8 q[NK];
     f32x16 o[ND];
     float m, l, c;  // reference maximum (raw score), sum over this lane's keys times 2^kUp, scale * log2(e)
-    bool far;       // a row's |m c| passes 2^23: see grow
+    bool far;       // a row is out of step: see grow
     int lane, n, h;
     uint32_t koff, voff[ND];  // LDS byte offsets of this lane's reads
 
@@ -385,18 +385,16 @@ struct Core {
         }
     }
     // The reference m follows the running maximum only when that has grown by 2^8, and the rescaling of o (64
-    // products a lane) all but vanishes: p = 2^(c (s - m) + kUp) is 2^(8 + kUp) at most.  weigh forms its exponent as
-    // fma(s, c, -round(m c)), which is off by half a step of m c: the same factor of all of a row's p, until it
-    // takes them out of fp16's range.  Rows with |m c| above 2^23, of which a step is 1, go on with s - m.
+    // products a lane) all but vanishes: p = 2^(c (s - m) + kUp) is 2^(8 + kUp) at most.
     template <int N2>
-    __device__ __forceinline__ void grow(f32x16 (&s)[N2]) {
+    __device__ __forceinline__ void grow(const f32x16 (&s)[N2]) {
         float mx = s[0][0];
 #pragma unroll
         for (int g = 0; g < N2; ++g)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[g][i]);
         mx = fmaxf(mx, swap32(mx));
-        if (__builtin_expect(__any((mx - m) * c > 8.0f) || far, 0)) {
+        if (__builtin_expect(__any((mx - m) * c > 8.0f), 0)) {
             const float mn = fmaxf(m, mx);
             const float f = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * c);
             l *= f;
@@ -405,17 +403,16 @@ struct Core {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
             m = mn;
-            far = __any(m > -INFINITY && fabsf(m) * c > 8388608.0f);
-            if (far) {
-                const float r = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                for (int g = 0; g < N2; ++g)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[g][i] -= r;
-            }
+            far = far || __any(out_of_step());
             hold_sums();
         }
     }
+    // weigh forms c (s - m) as fma(s, c, -round(m c)), which is off by half a step of m c: the same factor of all of a
+    // row's p, until that takes them out of fp16's range.  A row with |m c| above 2^23, of which a step is 1, is out of
+    // step: the run is computed again on checked tiles, with s - m in such rows.  (s - m at once, where the maximum
+    // grows, kept the scores from staying where the matrix units put them: heads of 256, 4 prompts of 100 to
+    // 900 tokens 74 us, 69 so, 67 without either.)
+    __device__ __forceinline__ bool out_of_step() const { return fabsf(m * c) > 8388608.0f && fabsf(m * c) < INFINITY; }
     // p = 2^(c (s - m) + kUp) rounded, l += sum p.  The product with V takes 16-bit probabilities (that is what the
     // matrix units multiply at full rate; each is off by half a step of the cache's type, as V itself is), the
     // sum l takes them as they are.  fp16 holds them from 2^-14 on: moved up by kUp, they keep their precision down
@@ -423,14 +420,15 @@ struct Core {
     // are (without kUp 2^17 keys of 2^-26 each were 2^-9 of l and nothing of o).  bf16 holds any.
     static constexpr float kUp = BF16 ? 0.0f : 7.0f;
     template <int N2>
-    __device__ __forceinline__ void weigh(const f32x16 (&s)[N2], u16x8 (&p)[2 * N2]) {
-        const float mc = (m == -INFINITY || far ? 0.0f : m * c) - kUp;
+    __device__ __forceinline__ void weigh(const f32x16 (&s)[N2], u16x8 (&p)[2 * N2], bool again = false) {
+        float mc = (m == -INFINITY ? 0.0f : m * c) - kUp, r = 0.0f;
+        if (again && out_of_step()) mc = -kUp, r = m;
         float sum = 0.0f;  // the tile's by itself, so that light keys are not lost one by one beside l
 #pragma unroll
         for (int g = 0; g < N2; ++g)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][i], c, -mc));
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(again ? s[g][i] - r : s[g][i], c, -mc));
                 sum = i + g ? sum + e : e;
                 p[2 * g + (i >> 3)][i & 7] = to16<BF16>(e);
             }
@@ -519,14 +517,17 @@ struct Core {
             }
         }
     }
-    // 32 keys with masks
-    __device__ __forceinline__ void checked(const uint8_t* K, const uint8_t* V, int left, int bad) {
+    // 32 keys with masks; again: the second time of a run that had a row out of step
+    __device__ __forceinline__ void checked(const uint8_t* K, const uint8_t* V, int left, int bad, bool again) {
         f32x16 s[1];
         u16x8 p[2];
         scores<1>(K, s);
         mask(s[0], left, bad);
         grow<1>(s);
-        weigh<1>(s, p);
+        if (__builtin_expect(again, 0))
+            weigh<1>(s, p, true);
+        else
+            weigh<1>(s, p);
         if (__builtin_expect(any_odd(V), 0)) {
             values_odd(V, p, left);
             hold_sums();
@@ -688,6 +689,7 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
     __shared__ int s_base[2][kThreads];
     __shared__ int s_seq[kThreads][3];
     __shared__ int s_red[4][6];
+    __shared__ int s_far[4];
     const int tid = threadIdx.x, lane = tid & 63, wv = uni(tid >> 6);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)smem;
 
@@ -822,43 +824,47 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
                 copy_block<D, true>(A, A.C.v, b0, lane, vb);
                 copy_block<D, true>(A, A.C.v, b1, lane, vb + 32 * D);
             };
-            int key = W.j0 * kSplitKeys;
             const int stop = W.j1 * kSplitKeys < W.keys ? W.j1 * kSplitKeys : W.keys;
             K core;
-            core.begin(lane);
             core.c = A.c;
-            const Rows<D, BF16> R(A, W, core.n);
-            R.load_q(A, W, core);
-            if (key < stop) bring_k(key), bring_v();
-            const int jf = plain_tiles(A, pages, W.j0, W.j1, kSplitKeys, W.keys, uni(R.seen), lane);
-            core.hold();  // arrived before the loops
-            for (int j = W.j0; j < jf; ++j) {
-                core.hold_sums();
-                const int next = key + kSplitKeys;
-                f32x16 s[1];
-                u16x8 p[2];
-                vm_wait<D / 16>();
-                core.template scores<1>(kp, s);
-                lds_wait();
-                if (next < stop) bring_k(next);
-                core.template grow<1>(s);
-                core.template weigh<1>(s, p);
-                if (next < stop)
+            const Rows<D, BF16> R(A, W, lane & 31);
+            bool again = false;
+            do {
+                int key = W.j0 * kSplitKeys;
+                core.begin(lane);
+                R.load_q(A, W, core);
+                if (key < stop) bring_k(key), bring_v();
+                const int jf = again ? W.j0 : plain_tiles(A, pages, W.j0, W.j1, kSplitKeys, W.keys, uni(R.seen), lane);
+                core.hold();  // arrived before the loops
+                for (int j = W.j0; j < jf; ++j) {
+                    core.hold_sums();
+                    const int next = key + kSplitKeys;
+                    f32x16 s[1];
+                    u16x8 p[2];
                     vm_wait<D / 16>();
-                else
+                    core.template scores<1>(kp, s);
+                    lds_wait();
+                    if (next < stop) bring_k(next);
+                    core.template grow<1>(s);
+                    core.template weigh<1>(s, p);
+                    if (next < stop)
+                        vm_wait<D / 16>();
+                    else
+                        vm_wait<0>();
+                    core.template values<1>(vp, p);
+                    lds_wait();
+                    if (next < stop) bring_v();
+                    key = next;
+                }
+                for (; key < stop; key += kSplitKeys) {
                     vm_wait<0>();
-                core.template values<1>(vp, p);
-                lds_wait();
-                if (next < stop) bring_v();
-                key = next;
-            }
-            for (; key < stop; key += kSplitKeys) {
-                vm_wait<0>();
-                core.hold_sums();
-                core.checked(kp, vp, R.seen - key, bad_blocks(A, pages, key, W.keys, 2));
-                lds_wait();
-                if (key + kSplitKeys < stop) bring_k(key + kSplitKeys), bring_v();
-            }
+                    core.hold_sums();
+                    core.checked(kp, vp, R.seen - key, bad_blocks(A, pages, key, W.keys, 2), again);
+                    lds_wait();
+                    if (key + kSplitKeys < stop) bring_k(key + kSplitKeys), bring_v();
+                }
+                again = !again && core.far;
+            } while (__builtin_expect(again, 0));
             R.store(A, W, core);
         }
     } else {
@@ -885,59 +891,67 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
             const int last = W.keys > 0 ? W.j1 : W.pre < W.j1 ? W.pre : W.j1;
             const int stop = last > W.j0 ? last : W.j0;
             K core;
-            core.begin(lane);
             core.c = A.c;
-            const Rows<D, BF16> R(A, W, W.row0 + 32 * wv + core.n);
-            R.load_q(A, W, core);
-            lds_barrier();  // every wave is done with the last segment's buffers
-            if (W.j0 < stop) bring(W.j0);
-            int j = W.j0;
+            const Rows<D, BF16> R(A, W, W.row0 + 32 * wv + (lane & 31));
+            bool again = false;
+            do {
+                core.begin(lane);
+                R.load_q(A, W, core);
+                lds_barrier();  // every wave is done with the last segment's buffers
+                if (W.j0 < stop) bring(W.j0);
+                int j = W.j0;
 #pragma unroll 1
-            for (int part = 0; part < 2; ++part) {  // the prefix's tiles, which every row sees, then the own keys'
-                const int from = part ? W.pre : 0, to = part || stop < W.pre ? stop : W.pre;
-                if (j >= to) continue;
-                const int32_t* where = part ? pages : A.B.prefix_pages;
-                const int keys = part ? W.keys : A.B.prefix;
-                const int seen = part ? R.seen : keys;
-                const int seen1 = __builtin_amdgcn_readlane(seen, 31);  // the wave's last row sees most
-                int least = keys;
-                if (part && !W.prefix) {  // the first row of the whole tile sees least
-                    Seq s;
-                    s.len = W.len, s.n = W.n, s.cap = W.cap;
-                    least = s.seen(group_of(A, W.row0));
-                }
-                const int jf = from + plain_tiles(A, where, j - from, to - from, kSharedKeys, keys, least, lane);
-                core.hold();  // arrived before the loops
-                for (; j < jf; ++j) {
-                    vm_wait<0>();
-                    lds_barrier();
-                    if (j + 1 < stop) bring(j + 1);
-                    const uint8_t* buf = smem + (j & 1) * 256 * D;
-                    if (works) {
-                        core.hold_sums();
-                        f32x16 s[2];
-                        u16x8 p[4];
-                        core.template scores<2>(buf, s);
-                        core.template grow<2>(s);
-                        core.template weigh<2>(s, p);
-                        core.template values<2>(buf + 128 * D, p);
+                for (int part = 0; part < 2; ++part) {  // the prefix's tiles, which every row sees, then the own keys'
+                    const int from = part ? W.pre : 0, to = part || stop < W.pre ? stop : W.pre;
+                    if (j >= to) continue;
+                    const int32_t* where = part ? pages : A.B.prefix_pages;
+                    const int keys = part ? W.keys : A.B.prefix;
+                    const int seen = part ? R.seen : keys;
+                    const int seen1 = __builtin_amdgcn_readlane(seen, 31);  // the wave's last row sees most
+                    int least = keys;
+                    if (part && !W.prefix) {  // the first row of the whole tile sees least
+                        Seq s;
+                        s.len = W.len, s.n = W.n, s.cap = W.cap;
+                        least = s.seen(group_of(A, W.row0));
+                    }
+                    const int jf =
+                        again ? j : from + plain_tiles(A, where, j - from, to - from, kSharedKeys, keys, least, lane);
+                    core.hold();  // arrived before the loops
+                    for (; j < jf; ++j) {
+                        vm_wait<0>();
+                        lds_barrier();
+                        if (j + 1 < stop) bring(j + 1);
+                        const uint8_t* buf = smem + (j & 1) * 256 * D;
+                        if (works) {
+                            core.hold_sums();
+                            f32x16 s[2];
+                            u16x8 p[4];
+                            core.template scores<2>(buf, s);
+                            core.template grow<2>(s);
+                            core.template weigh<2>(s, p);
+                            core.template values<2>(buf + 128 * D, p);
+                        }
+                    }
+                    for (; j < to; ++j) {
+                        vm_wait<0>();
+                        lds_barrier();
+                        if (j + 1 < stop) bring(j + 1);
+                        const uint8_t* buf = smem + (j & 1) * 256 * D;
+#pragma unroll 1
+                        for (int half = 0; half < 2 && works; ++half) {
+                            const int key = (j - from) * kSharedKeys + 32 * half;
+                            if (key >= seen1) break;
+                            core.hold_sums();
+                            core.checked(buf + half * 64 * D, buf + 128 * D + half * 64 * D, seen - key,
+                                         bad_blocks(A, where, key, keys, 2), again);
+                        }
                     }
                 }
-                for (; j < to; ++j) {
-                    vm_wait<0>();
-                    lds_barrier();
-                    if (j + 1 < stop) bring(j + 1);
-                    const uint8_t* buf = smem + (j & 1) * 256 * D;
-#pragma unroll 1
-                    for (int half = 0; half < 2 && works; ++half) {
-                        const int key = (j - from) * kSharedKeys + 32 * half;
-                        if (key >= seen1) break;
-                        core.hold_sums();
-                        core.checked(buf + half * 64 * D, buf + 128 * D + half * 64 * D, seen - key,
-                                     bad_blocks(A, where, key, keys, 2));
-                    }
-                }
-            }
+                if (again) break;
+                if (lane == 0) s_far[wv] = core.far;  // the waves share the tiles
+                lds_barrier();
+                again = uni(s_far[0] | s_far[1] | s_far[2] | s_far[3]);
+            } while (__builtin_expect(again, 0));
             R.store(A, W, core);
         }
     }
