@@ -327,9 +327,9 @@ typedef struct pgmoe_kv_cache {
  * j % page_size of page page_table[b * table_stride + j / page_size].  prefix_len keys before them (in the
  * pages prefix_pages, which need not be full) are shared by every sequence.  The positions of the own keys
  * follow the prefix: prefix_len + j.  All arrays are int32 on the device and are read when the kernels run
- * (and not to be changed meanwhile): a captured graph replays on their present contents.  Nothing is read or written through a page id
- * outside [0, n_pages) or past max_pages pages of a table row, nor are rows past the call's tokens, whatever
- * q_start holds; where it decreases, the call's rows of the outputs hold anything. */
+ * (and are not to change meanwhile): a captured graph replays on their present contents.  Nothing is read or
+ * written through a page id outside [0, n_pages) or past max_pages pages of a table row, nor are rows past the
+ * call's tokens, whatever q_start holds; where it decreases, the call's rows of the outputs hold anything. */
 typedef struct pgmoe_kv_batch {
     const int32_t* page_table;   /* [n_seqs][max_pages], rows table_stride apart */
     const int32_t* lens;         /* [n_seqs]; negative counts as 0 */
@@ -369,7 +369,13 @@ int pgmoe_rope_append(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, const vo
  * overlapping q); lse fp32 [n_tokens, n_q_heads] or NULL.  A query that sees no key gets zeros and an lse
  * of -inf; one that sees a key on a page that does not exist gets NaN; what masked keys and unused rows of
  * pages hold is never seen, not even a NaN.  Rows behind the last sequence are left alone.
- * The workspace holds partial rows of this call and needs no clearing.  Limits (PGMOE_E_UNSUPPORTED beyond):
+ * Any finite scores do: probabilities are held times 2^7 in fp16, and rows whose scores reach some 10^6 are
+ * computed from differences of scores.
+ * The workspace holds partial rows of this call and needs no clearing: for R = n_tokens * n_q_heads rows, s * R *
+ * (4 * head_dim + 8) bytes and some, twice that behind a prefix, s = 2^26 / (R * head_dim) between 4 and 130 (32
+ * heads of 128: 132 MiB for 64 tokens, 261 for 4096, 1044 for 16384; behind a prefix twice that).  s also bounds how
+ * finely a long sequence is cut: single tokens behind very long ones of their own are faster in a call apart from
+ * prompts of thousands of tokens.  Limits (PGMOE_E_UNSUPPORTED beyond):
  * with g query heads a KV head, n_tokens * g * g < 2^31, and (n_tokens * g / 128 + 1 + n_seqs) * n_kv_heads
  * row tiles of (max_pages * page_size + prefix_len) / 32 + 16 key tiles number 2^30 at most. */
 size_t pgmoe_attend_workspace_bytes(const pgmoe_kv_cache* C, const pgmoe_kv_batch* B, int32_t n_tokens,
@@ -394,11 +400,13 @@ typedef struct pgmoe_sampling {
  * given uniform numbers u [rows] (fp32, [0, 1)):
  *   w_i = exp((x_i - max x) / temperature); tokens ordered by logit, equal ones by index;
  *   kept: the shortest of three prefixes of that order, one token at least: the first top_k; those before
- *   which the sum of w is below top_p times the sum of all; those with w >= min_p;
+ *   which the sum of w is below top_p times the sum of all (of the whole row, also where top_k is on: samplers that
+ *   take the share of the first top_k tokens keep fewer); those with w >= min_p;
  *   token (int64 [rows]): the first in index order at which the sum of the kept w exceeds u times their
  *   total; logprob (fp32 [rows] or NULL): log(w_token / total).
  * Weights are summed as multiples of 2^-s of the largest, s = min(51, 62 - ceil(log2 vocab)), so no order of sums
- * shows in the result; a token of less than half of that has none and is not drawn.  NaN and -inf logits
+ * shows in the result; a token of less than half of that has none and is not drawn.  (Sums of 8192 tokens at a
+ * time are rounded once each, not token by token.)  NaN and -inf logits
  * have no weight; with +inf ones only those have.  A row without any logit above -inf gives token -1 and
  * logprob -inf.  vocab: 1 .. 2^20; rows: up to 2^22.  The workspace is this call's and needs no clearing. */
 size_t pgmoe_sample_workspace_bytes(int32_t rows, int32_t vocab);

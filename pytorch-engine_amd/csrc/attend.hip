@@ -15,15 +15,18 @@
 // The products run on 32x32x16 MFMA, scores transposed: S^T = K Q^T has a query row per lane column, so the
 // maximum and sum of a row are sums over a lane's registers and one swap of wave halves, and the rounded
 // probabilities are already the B operand of O^T = V^T P^T (whose k index may be permuted as long as V's
-// rows are too).  K and V go from memory to LDS without registers, rows swizzled so that the lanes of a 16-byte
-// read of K and of a transposing 8-byte read of V spread evenly over the banks.
+// rows are too).  K and V go from memory to LDS without registers, rows swizzled over the banks for the 16-byte
+// reads of K and the transposing 8-byte reads of V (of the prompts' LDS cycles a third are conflicts all the same).
 //
 // What bounds it (whole calls): a few rows a chain of latencies, lens to pages to keys to partial rows, and the
-// second launch (one sequence of 5003 keys: 11 + 5 us); long caches of few rows HBM (32 sequences of up to
-// 16000 keys, 8 KV heads of 128: 212 us, 5.4 TB/s); prompts and long prefixes the power of the matrix units (six
-// prompts behind 4097 keys: 394 us, 790 TFLOP/s, the clock at 1.7 GHz; giving half the waves a higher
-// priority, or the products alone, moves it by 1 to 2 % at most).  Heads of 256: the same 32
-// sequences on 4 KV heads 224 us, a prompt of 1024 behind 4096 keys 134 us, 580 TFLOP/s on one wave a SIMD.
+// second launch (one sequence of 5003 keys: 12 + 5 us); long caches of few rows HBM (32 sequences of up to
+// 16000 keys, 8 KV heads of 128: 212 us, 5.4 TB/s); prompts and long prefixes reading K and V again for every row
+// tile as much as the matrix units: the row tiles of a KV head are dealt over all XCDs, each with an L2 of its own, and
+// stand at different keys.  Six prompts behind 4097 keys, 394 us, 790 TFLOP/s (414 on a slower card): 2.04 GB come from
+// behind the L2s, of 2.54 GB that tiles ask for and 0.03 that are there, 5.2 TB/s, while MFMA is busy 39 % of the
+// cycles; 256 rows behind 16000 shared keys, 125 us: 0.63 GB, for 0.19.  Giving half the waves a
+// higher priority, or the products alone, moves it by 1 to 2 % at most.  Heads of 256: the same 32
+// sequences on 4 KV heads 228 us, a prompt of 1024 behind 4096 keys 137 us, 565 TFLOP/s on one wave a SIMD.
 //
 // Masked keys: a tile with a key that some row does not see takes the checked path: scores of masked keys
 // become -inf, and V values that are not finite reach only the rows that see them.  Rows past the last
@@ -759,8 +762,10 @@ __global__ __launch_bounds__(kThreads, Geo<D>::OCC) void attend_kernel(const Att
         const bool sp = prows <= kSplitRows;
         const int tile = sp ? kSplitKeys : kSharedKeys, pt = (A.B.prefix + tile - 1) / tile;
         // Prompts: where every sequence fills row tiles of its own, the prefix has as few readers when each
-        // row tile goes through it on the way to its own keys, and no row is left in two parts (six prompts of
-        // 200 to 1201 tokens on a prefix of 4097 keys: 444 -> 409 us).
+        // row tile goes through it on the way to its own keys, and a row's parts are fewer (six prompts of
+        // 200 to 1201 tokens on a prefix of 4097 keys: 444 -> 409 us).  Up to 1.25 times the prefix's row tiles: 64 sequences
+        // of 16, 13, 11, 8 and 5 tokens (8 query heads on each of 4 KV heads) behind 4096 keys, 1, 1.23, 1.45, 2 and 3.2
+        // times, take 106, 103, 94, 78 and 77 us this way and 120, 102, 91, 72 and 54 apart.
         if (prows && !own[0] && own[2] * 8 <= (row_tiles(prows) * A.C.heads) * 10) {
             ax1.pre = pt;
             prows = 0;
@@ -1017,7 +1022,10 @@ __global__ __launch_bounds__(kThreads) void combine_rows_kernel(const AttendArgs
 }
 
 static int attend_slots(int64_t rows, int D) {
-    // partial rows of at most 256 MiB a region, 130 slots (a long sequence alone on the chip), at least 4
+    // Slots of every row, in each region: 130 (a long sequence alone on the chip), fewer where a region would pass 256
+    // MiB, 4 at least, which passes it from 65536 rows of 256 on (8192 tokens of 32 heads of 128: 522 MiB, 1042 behind
+    // a prefix).  A segment is cut into nslot - 2 runs at most: beside a prompt of 2048 tokens one sequence of
+    // 100000 keys runs on few waves (689 us the call; 79 and 87 each in a call of its own).
     int64_t n = ((int64_t)256 << 20) / (rows * D * 4);
     return (int)(n < 4 ? 4 : n > 130 ? 130 : n);
 }

@@ -9,11 +9,12 @@ The step between a layer's Q/K/V projections (FusedLinearPack) and its output pr
     o = cache.attend(q, batch)                                       # softmax(q K^T / sqrt(D)) V
 
 Every sequence sees the ``prefix_len`` keys of ``prefix_pages`` (a system prompt, a document) and then
-its own keys; the prefix's keys and values are read once for the whole batch.  The batch's tensors
-live on the device and are read when the kernels run: a program updates them in place between steps
-(``lens.add_(1)``), and a captured graph replays on what they then hold (keep cache, batch, rotary and
-norm weights as long as the graph).  Nothing synchronises with the host but the constructors.  There is
-no CPU path: CPU tensors, and types, widths and page sizes without a kernel, raise.
+its own keys; the prefix's keys and values are read for 128 query rows of a KV head at a time, whichever
+sequences they belong to.  The batch's tensors live on the device and are read when the kernels run: a
+program updates them in place between steps (``lens.add_(1)`` on the calls' stream, or ordered with it),
+and a captured graph replays on what they then hold (keep cache, batch, rotary and norm weights as long
+as the graph).  Nothing synchronises with the host but the constructors.  There is no CPU path: CPU
+tensors, and types, widths and page sizes without a kernel, raise.
 """
 
 from __future__ import annotations
@@ -341,7 +342,10 @@ class HipPagedKVCache:
         q [T, n_q_heads, D] in the cache's type; query head h reads KV head h // (n_q_heads / n_kv_heads).
         A query that sees no key gets zeros and -inf; one that sees a key on a page that does not exist
         gets NaN.  Masked keys and unused page rows may hold anything.  Rows of `out` behind the last
-        sequence are left alone."""
+        sequence are left alone.
+
+        Scratch is allocated at every call, for thousands of tokens some hundred MiB to GiB (pgmoe.h).  Single
+        tokens behind very long sequences of their own are faster in a call apart from such prompts."""
         q, qt, qh = self._heads("q", q, (self._dtype,))
         T, hq = self._tokens(q, batch)
         scale = self._head_dim ** -0.5 if scale is None else float(scale)

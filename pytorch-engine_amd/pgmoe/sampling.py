@@ -40,11 +40,13 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Union[floa
 
     With w_i = exp((x_i - max x) / temperature) and the tokens ordered by logit (equal ones by index),
     the kept tokens are the shortest of: the first top_k (0: off); those before which the sum of w is
-    below top_p times the whole (1: off); those with w >= min_p (0: off); one at least.  The token is the
-    first in index order at which the sum of the kept w exceeds u times their total, u in [0, 1).
-    temperature 0: the largest logit.  Parameters: numbers, or a tensor of one value a row (float32;
-    top_k int32).  w is held in multiples of 2^-s, s = min(51, 62 - ceil(log2(vocab))): a token with less than
-    half of that is not drawn, not even at u = 0.  NaN and -inf logits are never drawn; a row that holds nothing else gives -1 and -inf."""
+    below top_p times the whole (1: off); those with w >= min_p (0: off); one at least.  The whole is the
+    row's, also where top_k is on: samplers that apply top_k first and take top_p of what is left keep fewer
+    tokens at the same settings.  The token is the first in index order at which the sum of the kept w
+    exceeds u times their total, u in [0, 1).  temperature 0: the largest logit.  Parameters: numbers, or a
+    tensor of one value a row (float32; top_k int32).  w is held in multiples of 2^-s, s = min(51, 62 -
+    ceil(log2(vocab))): a token with less than half of that is not drawn, not even at u = 0.  NaN and -inf
+    logits are never drawn; a row that holds nothing else gives -1 and -inf."""
     if logits.device.type != "cuda" or logits.dim() != 2:
         raise ValueError("logits: [rows, vocab] on a HIP device")
     if logits.dtype not in _DT:
