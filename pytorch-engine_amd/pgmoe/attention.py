@@ -163,7 +163,7 @@ class KVBatch:
             raise ValueError(f"{name} is an int32 tensor")
         if t.device != self._device:
             raise ValueError(f"{name} is on {t.device}, the batch on {self._device}")
-        if t.numel() and t.stride(-1) != 1:
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
             raise ValueError(f"{name} must be contiguous along its rows")
         return t
 
@@ -198,19 +198,25 @@ class HipPagedKVCache:
         V interleaved): both [n_pages, n_kv_heads, page_size, head_dim] with the same strides, the last
         dimension contiguous, the others in multiples of 8 elements."""
         self = cls.__new__(cls)
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
+        same = k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device
+        if not same or cls._strides(k) != cls._strides(v):
             raise ValueError("k and v pages: [n_pages, n_kv_heads, page_size, head_dim] of one type, device and layout")
         if k.device.type != "cuda":
             raise ValueError("pgmoe attention runs on a HIP device tensor")
         n, h, ps, d = k.shape
         self._check(n, ps, h, d, k.dtype)
-        st = k.stride()
+        st = cls._strides(k)
         if st[3] != 1 or any(x % 8 for x in st[:3]) or k.data_ptr() % 16 or v.data_ptr() % 16:
             raise ValueError("pages need a contiguous head_dim, strides of whole 16 bytes and 16-byte alignment")
-        if st[2] < d or st[2] > 1 << 22 or any(s <= 0 and m > 1 for s, m in zip(st, k.shape)):
+        if st[2] < d or st[2] > 1 << 22 or any(s <= 0 for s, m in zip(st, k.shape) if m > 1):
             raise ValueError("the rows of a page overlap or lie too far apart")
         self._bind(k, v)
         return self
+
+    @staticmethod
+    def _strides(x: torch.Tensor) -> Tuple[int, ...]:
+        """x's strides; 0 of an axis of one element, whose stride means nothing."""
+        return tuple(s if m > 1 else 0 for s, m in zip(x.stride(), x.shape))
 
     @staticmethod
     def _check(n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype) -> None:
@@ -228,7 +234,7 @@ class HipPagedKVCache:
         self._k, self._v = k, v
         self._n_pages, self._n_kv_heads, self._page_size, self._head_dim = (int(x) for x in k.shape)
         self._dtype, self._device = k.dtype, k.device
-        st = k.stride()
+        st = self._strides(k)
         self._c = _KVCache(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], self._n_pages, self._page_size,
                            self._n_kv_heads, self._head_dim, _DT[k.dtype])
         self._ref = ctypes.byref(self._c)

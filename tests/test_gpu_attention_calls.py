@@ -102,3 +102,22 @@ def test_a_q_start_that_decreases_stays_inside(dev, seqs, tokens, prefix):
     assert bool((buf[tokens:] == 3.0).all()) and torch.equal(c.k, k)
     s, c, q, ref = _made(dev, prefix=20)
     check_attend(s, c.attend(q, s.batch(dev)), ref)
+
+
+def test_strides_of_axes_of_one_element_mean_nothing(dev):
+    """One page, one KV head, one sequence: views whose strides there are odd are as good as any."""
+    from pgmoe import HipPagedKVCache, KVBatch
+    log("strides of single elements")
+    g = torch.Generator(dev).manual_seed(1)
+    k, v = (torch.randn(1, 1, 16, 64, generator=g, device=dev).half() for _ in range(2))
+    q = torch.randn(1, 2, 64, generator=g, device=dev).half()
+    want = HipPagedKVCache.from_tensors(k, v).attend(q, KVBatch([[0]], [9], device=dev))
+    odd = k.as_strided(k.shape, (3, 5, 64, 1))
+    other = v.as_strided(v.shape, (1, 1, 64, 1))
+    c = HipPagedKVCache.from_tensors(odd, other)
+    table = torch.zeros(7, 3, dtype=torch.int32, device=dev)
+    lens = torch.full((7,), 9, dtype=torch.int32, device=dev)
+    assert torch.equal(c.attend(q, KVBatch(table[:1, :1], lens.as_strided((1,), (4,)))), want)
+    assert torch.equal(c.attend(q, KVBatch(table.t()[:1, :1], lens[:1])), want)
+    with pytest.raises(ValueError):
+        KVBatch(table.t()[:2], lens[:2])
