@@ -34,6 +34,7 @@ _CACHE_DT = (torch.float16, torch.bfloat16)
 _DIMS = (64, 128, 256)
 _PAGES = (16, 32, 64, 128, 256)
 _MAX_SEQS = 4096
+_MAX_KEYS = 1 << 30  # of a prefix, and of one sequence
 
 _IntTensor = Union[torch.Tensor, Sequence[int]]
 
@@ -141,6 +142,8 @@ class KVBatch:
         self._prefix_len = int(prefix_len)
         if self._prefix_len < 0:
             raise ValueError("negative prefix_len")
+        if self._prefix_len > _MAX_KEYS or self._table.shape[1] > _MAX_KEYS // _PAGES[0]:
+            raise NotImplementedError(f"prefix_len {prefix_len}, {self._table.shape[1]} pages a sequence (up to {_MAX_KEYS} keys)")
         self._prefix = None if prefix_pages is None else self._int32("prefix_pages", prefix_pages, 1, -1)
         if self._prefix_len and self._prefix is None:
             raise ValueError("prefix_len without prefix_pages")

@@ -20,6 +20,7 @@ from .attention import launch
 
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _MAX_VOCAB = 1 << 20
+_MAX_ROWS = 1 << 22
 
 
 def _param(name: str, v: Union[float, int, torch.Tensor], rows: int, dev: torch.device, dtype: torch.dtype):
@@ -54,6 +55,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Union[floa
     rows, vocab = logits.shape
     if not 1 <= vocab <= _MAX_VOCAB:
         raise NotImplementedError(f"vocabulary of {vocab} (1 .. {_MAX_VOCAB})")
+    if rows > _MAX_ROWS:
+        raise NotImplementedError(f"{rows} rows in one call (up to {_MAX_ROWS})")
     dev = logits.device
     if u.device != dev or u.dtype != torch.float32 or tuple(u.shape) != (rows,):
         raise ValueError(f"u: float32 [{rows}] on {dev}")

@@ -121,3 +121,17 @@ def test_strides_of_axes_of_one_element_mean_nothing(dev):
     assert torch.equal(c.attend(q, KVBatch(table.t()[:1, :1], lens[:1])), want)
     with pytest.raises(ValueError):
         KVBatch(table.t()[:2], lens[:2])
+
+
+def test_sizes_past_32_bits_are_refused(dev):
+    """Before they become another number on the way into the library."""
+    from pgmoe import KVBatch, sample_tokens
+    log("sizes past 32 bits")
+    one = torch.zeros(1, dtype=torch.int32, device=dev)
+    for n in (2 ** 30 + 1, 2 ** 32, 2 ** 32 + 5):
+        with pytest.raises(NotImplementedError, match="prefix_len"):
+            KVBatch([[0]], [1], prefix_pages=one, prefix_len=n, device=dev)
+    with pytest.raises(NotImplementedError, match="rows"):
+        sample_tokens(torch.zeros(1, 1, device=dev).expand(2 ** 32 + 2, 1), torch.zeros(1, device=dev).expand(2 ** 32 + 2))
+    with pytest.raises(NotImplementedError, match="rows"):
+        sample_tokens(torch.zeros(1, 1, device=dev).expand(2 ** 22 + 1, 1), torch.zeros(1, device=dev).expand(2 ** 22 + 1))
