@@ -413,6 +413,52 @@ size_t pgmoe_sample_workspace_bytes(int32_t rows, int32_t vocab);
 int pgmoe_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab, const float* u,
                  const pgmoe_sampling* S, int64_t* token, float* logprob, void* ws, size_t ws_bytes, void* stream);
 
+/* Microscaled blocks: rows of 32 values that share a power of two.  codes [rows, cols] (e4m3: one byte a value; e2m1:
+ * two values a byte, the even one in the low four bits), rows code_stride bytes apart (a multiple of 16, the
+ * pointer 16-byte aligned); scales [rows, cols / 32] bytes, E + 127 each, rows scale_stride bytes apart (a multiple
+ * of 4, the pointer 4-byte aligned).  A value is code * 2^E; byte 255 makes its block NaN.  cols: a multiple of 32, up
+ * to 2^24; rows below 2^24. */
+#define PGMOE_MX_E4M3 8 /* sign, 4 exponent bits, 3 of the mantissa: up to 448, no infinities */
+#define PGMOE_MX_E2M1 4 /* 0 0.5 1 1.5 2 3 4 6 and their negatives */
+typedef struct pgmoe_mx {
+    void* codes;
+    void* scales;
+    int64_t code_stride;
+    int64_t scale_stride;
+    int32_t rows;
+    int32_t cols;
+    int32_t fmt; /* PGMOE_MX_* */
+} pgmoe_mx;
+
+/* The blocks y of x [rows, cols] (PGMOE_DT_*, rows x_stride elements apart: 16-byte multiples, the pointer 16-byte
+ * aligned): E = max(-127, floor(log2 max|x|) - e), e = 8 (e4m3) or 2 (e2m1); codes x / 2^E to the nearest, ties to
+ * even, at most 448 or 6 in size.  A block that holds an infinity or NaN gets scale byte 255 and codes 0. */
+int pgmoe_mx_quantize(const void* x, int32_t dtype, int64_t x_stride, const pgmoe_mx* y, void* stream);
+
+/* out [rows, cols] (PGMOE_DT_*, contiguous, 16-byte aligned) = the values of x, rounded once. */
+int pgmoe_mx_dequantize(const pgmoe_mx* x, void* out, int32_t out_dtype, void* stream);
+
+/* pgmoe_add_rmsnorm (h_out as there, rows contiguous) with the blocks of the normalised rows as output: the fp32
+ * values are not rounded before. */
+int pgmoe_add_rmsnorm_mx(const void* x, int32_t x_dtype, const void* delta, int32_t delta_dtype, const float* weight,
+                         float eps, float* h_out, const pgmoe_mx* y, void* stream);
+
+/* The blocks of act(gate) * up (PGMOE_ACT_*), formed in fp32 and not rounded before; gate and up [rows, cols] of one
+ * type, strides as for pgmoe_mx_quantize (e.g. the halves of one product's output). */
+int pgmoe_mx_act_mul(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int32_t dtype, int32_t act,
+                     const pgmoe_mx* y, void* stream);
+
+/* Weights [rows, cols] in e2m1 blocks, laid out once for pgmoe_mx_linear: pgmoe_mx_packed_bytes bytes at dst (16-byte
+ * aligned; negative if the sizes are not taken). */
+int64_t pgmoe_mx_packed_bytes(int64_t rows, int64_t cols);
+int pgmoe_mx_pack(const pgmoe_mx* w, void* dst, void* stream);
+
+/* out [x.rows, out_features] (PGMOE_DT_*, contiguous, 16-byte aligned) = x . W^T (+ bias fp32 [out_features] or NULL):
+ * packed weights of out_features rows of x.cols, x in e4m3 or e2m1 blocks, products summed in fp32 in a fixed order
+ * and rounded once. */
+int pgmoe_mx_linear(const void* packed, int32_t out_features, const pgmoe_mx* x, const float* bias, void* out,
+                    int32_t out_dtype, void* stream);
+
 /* pgmoe_moe_forward with per-kernel timing.  No counterpart in the reference: it is for
  * benchmarks and profilers that want each kernel's duration from the caller's own stream.
  * The i-th kernel the call launches (i < n_events) records start_events[i] when it begins

@@ -8,6 +8,7 @@
 #include "common.h"
 #include "kv.h"
 #include "launch.h"
+#include "mx.h"
 #include "sample.h"
 
 namespace pgmoe {
@@ -853,6 +854,115 @@ int pgmoe_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t 
     while ((1 << bits) < vocab) ++bits;
     const SampleArgs A{logits, dtype, row_stride, rows, vocab, u, *S, token, logprob, bits < 11 ? 51 : 62 - bits, ws};
     return launch_sample(A, as_stream(stream));
+}
+
+static int check_mx(const char* what, const pgmoe_mx* T, MxRows* y) {
+    if (!T) return fail(PGMOE_E_INVALID, "%s: NULL blocks", what);
+    if (T->fmt != PGMOE_MX_E4M3 && T->fmt != PGMOE_MX_E2M1)
+        return fail(PGMOE_E_UNSUPPORTED, "%s: format %d (e4m3: 8, e2m1: 4)", what, T->fmt);
+    if (T->rows < 0 || T->rows >= (1 << 24) || T->cols < 32 || T->cols > (1 << 24) || T->cols % 32)
+        return fail(PGMOE_E_INVALID, "%s: %d rows of %d (a multiple of 32)", what, T->rows, T->cols);
+    const int64_t code = T->fmt == PGMOE_MX_E2M1 ? T->cols / 2 : T->cols;
+    if (T->rows > 1 && (T->code_stride < code || T->scale_stride < T->cols / 32))
+        return fail(PGMOE_E_INVALID, "%s: rows overlap", what);
+    if (T->rows > 1 && (T->code_stride % 16 || T->scale_stride % 4 || T->code_stride > (1ll << 31) || T->scale_stride > (1ll << 31)))
+        return fail(PGMOE_E_INVALID, "%s: rows of codes lie a multiple of 16 bytes apart, of scales one of 4", what);
+    if (T->rows && (!T->codes || !T->scales)) return fail(PGMOE_E_INVALID, "%s: NULL pointer", what);
+    if (((uintptr_t)T->codes & 15) || ((uintptr_t)T->scales & 3))
+        return fail(PGMOE_E_INVALID, "%s: codes must be 16-byte aligned, scales 4-byte aligned", what);
+    *y = MxRows{(uint8_t*)T->codes, (uint8_t*)T->scales, T->rows > 1 ? T->code_stride : 0, T->rows > 1 ? T->scale_stride : 0,
+                T->rows, T->cols, T->fmt == PGMOE_MX_E2M1};
+    return PGMOE_OK;
+}
+
+static bool float_type(int dt) { return dt == PGMOE_DT_F32 || dt == PGMOE_DT_F16 || dt == PGMOE_DT_BF16; }
+
+static int check_mx_floats(const char* what, const void* p, int dt, int64_t stride, const MxRows& y, MxFloats* x) {
+    if (!float_type(dt)) return fail(PGMOE_E_UNSUPPORTED, "%s: dtype %d", what, dt);
+    if (!p || ((uintptr_t)p & 15)) return fail(PGMOE_E_INVALID, "%s: rows must be a 16-byte aligned device pointer", what);
+    if (y.rows > 1 && (stride < y.cols || stride % (dt == PGMOE_DT_F32 ? 4 : 8) || stride > (1ll << 31)))
+        return fail(PGMOE_E_INVALID, "%s: rows lie a multiple of 16 bytes apart and do not overlap", what);
+    *x = MxFloats{p, y.rows > 1 ? stride : 0, dt};
+    return PGMOE_OK;
+}
+
+int pgmoe_mx_quantize(const void* x, int32_t dtype, int64_t x_stride, const pgmoe_mx* Y, void* stream) {
+    MxRows y;
+    MxFloats f;
+    int rc = check_mx("mx_quantize", Y, &y);
+    if (rc) return rc;
+    if (y.rows == 0) return PGMOE_OK;
+    rc = check_mx_floats("mx_quantize", x, dtype, x_stride, y, &f);
+    return rc ? rc : launch_mx_quantize(f, y, as_stream(stream));
+}
+
+int pgmoe_mx_dequantize(const pgmoe_mx* X, void* out, int32_t out_dtype, void* stream) {
+    MxRows x;
+    const int rc = check_mx("mx_dequantize", X, &x);
+    if (rc) return rc;
+    if (!float_type(out_dtype)) return fail(PGMOE_E_UNSUPPORTED, "mx_dequantize: dtype %d", out_dtype);
+    if (x.rows == 0) return PGMOE_OK;
+    if (!out || ((uintptr_t)out & 15)) return fail(PGMOE_E_INVALID, "mx_dequantize: out must be 16-byte aligned");
+    return launch_mx_dequantize(x, out, out_dtype, as_stream(stream));
+}
+
+int pgmoe_add_rmsnorm_mx(const void* x, int32_t x_dtype, const void* delta, int32_t delta_dtype, const float* weight,
+                         float eps, float* h_out, const pgmoe_mx* Y, void* stream) {
+    MxRows y;
+    int rc = check_mx("add_rmsnorm_mx", Y, &y);
+    if (rc) return rc;
+    if (!(eps >= 0.0f)) return fail(PGMOE_E_INVALID, "add_rmsnorm_mx: eps must be >= 0");
+    if (y.rows == 0) return PGMOE_OK;
+    MxFloats f;
+    if ((rc = check_mx_floats("add_rmsnorm_mx", x, x_dtype, y.cols, y, &f))) return rc;
+    if (delta && (rc = check_mx_floats("add_rmsnorm_mx", delta, delta_dtype, y.cols, y, &f))) return rc;
+    if (!weight || (((uintptr_t)weight | (uintptr_t)h_out) & 15))
+        return fail(PGMOE_E_INVALID, "add_rmsnorm_mx: weight and h_out must be 16-byte aligned");
+    return launch_add_rmsnorm_mx(x, x_dtype, delta, delta_dtype, weight, eps, h_out, y, as_stream(stream));
+}
+
+int pgmoe_mx_act_mul(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int32_t dtype, int32_t act,
+                     const pgmoe_mx* Y, void* stream) {
+    MxRows y;
+    MxFloats g, u;
+    int rc = check_mx("mx_act_mul", Y, &y);
+    if (rc) return rc;
+    if (act != PGMOE_ACT_SILU && act != PGMOE_ACT_GELU_TANH) return fail(PGMOE_E_UNSUPPORTED, "mx_act_mul: activation %d", act);
+    if (y.rows == 0) return PGMOE_OK;
+    if ((rc = check_mx_floats("mx_act_mul", gate, dtype, gate_stride, y, &g))) return rc;
+    if ((rc = check_mx_floats("mx_act_mul", up, dtype, up_stride, y, &u))) return rc;
+    return launch_mx_act_mul(g, u, act, y, as_stream(stream));
+}
+
+static bool mx_weight_sizes(int64_t rows, int64_t cols) {
+    return rows >= 1 && rows < (1 << 24) && cols >= 32 && cols <= (1 << 24) && cols % 32 == 0 && rows * cols <= (1ll << 40);
+}
+
+int64_t pgmoe_mx_packed_bytes(int64_t rows, int64_t cols) { return mx_weight_sizes(rows, cols) ? mx_packed_bytes(rows, cols) : -1; }
+
+int pgmoe_mx_pack(const pgmoe_mx* W, void* dst, void* stream) {
+    MxRows w;
+    const int rc = check_mx("mx_pack", W, &w);
+    if (rc) return rc;
+    if (!w.e2m1) return fail(PGMOE_E_UNSUPPORTED, "mx_pack: weights of format %d (e2m1)", W->fmt);
+    if (!mx_weight_sizes(w.rows, w.cols)) return fail(PGMOE_E_INVALID, "mx_pack: %d rows of %d", w.rows, w.cols);
+    if (!dst || ((uintptr_t)dst & 15)) return fail(PGMOE_E_INVALID, "mx_pack: dst must be 16-byte aligned");
+    return launch_mx_pack(w, (uint8_t*)dst, as_stream(stream));
+}
+
+int pgmoe_mx_linear(const void* packed, int32_t out_features, const pgmoe_mx* X, const float* bias, void* out,
+                    int32_t out_dtype, void* stream) {
+    MxRows x;
+    const int rc = check_mx("mx_linear", X, &x);
+    if (rc) return rc;
+    if (!mx_weight_sizes(out_features, x.cols)) return fail(PGMOE_E_INVALID, "mx_linear: %d outputs", out_features);
+    if (!float_type(out_dtype)) return fail(PGMOE_E_UNSUPPORTED, "mx_linear: output dtype %d", out_dtype);
+    if ((int64_t)x.rows * out_features > (1ll << 38)) return fail(PGMOE_E_UNSUPPORTED, "mx_linear: %d x %d outputs", x.rows, out_features);
+    if (x.rows == 0) return PGMOE_OK;
+    if (!packed || !out || (((uintptr_t)packed | (uintptr_t)out) & 15) || ((uintptr_t)bias & 3))
+        return fail(PGMOE_E_INVALID, "mx_linear: weights and out must be 16-byte aligned device pointers");
+    return launch_mx_linear(MxLinear{(const uint8_t*)packed, out_features, x.cols, x.rows, x, bias, out, out_dtype},
+                            as_stream(stream));
 }
 
 int pgmoe_moe_forward_timed(const pgmoe_layer* L, const uint16_t* x, int32_t M, float* out, void* ws,

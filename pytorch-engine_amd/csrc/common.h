@@ -309,7 +309,7 @@ template <> struct Fmt<PGMOE_Q6_K> {
 };
 
 // ---------------------------------------------------------------- launch helpers
-inline int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+__host__ __device__ inline int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 

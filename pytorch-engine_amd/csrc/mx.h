@@ -1,0 +1,96 @@
+// Microscaled blocks (mx.hip, mx_linear.hip): 32 values along a row share a power of two.
+#pragma once
+
+#include "kv.h"
+
+namespace pgmoe {
+
+struct MxRows {  // validated in api.hip
+    uint8_t* codes;
+    uint8_t* scales;
+    int64_t code_stride, scale_stride;  // bytes
+    int rows, cols;
+    int e2m1;
+};
+struct MxFloats {
+    const void* p;
+    int64_t stride;  // elements
+    int dt;
+};
+
+int launch_mx_quantize(const MxFloats& x, const MxRows& y, hipStream_t st);
+int launch_mx_dequantize(const MxRows& x, void* out, int odt, hipStream_t st);
+int launch_mx_act_mul(const MxFloats& gate, const MxFloats& up, int act, const MxRows& y, hipStream_t st);
+int launch_add_rmsnorm_mx(const void* x, int xdt, const void* delta, int ddt, const float* w, float eps, float* h_out,
+                          const MxRows& y, hipStream_t st);
+// The packed weights of a product: bytes, and their making from blocks of rows.
+int64_t mx_packed_bytes(int64_t rows, int64_t cols);
+int launch_mx_pack(const MxRows& w, uint8_t* dst, hipStream_t st);
+struct MxLinear {
+    const uint8_t* w;  // packed
+    int N, K, M;
+    MxRows x;          // activations in blocks
+    const float* bias;
+    void* out;
+    int odt;
+};
+int launch_mx_linear(const MxLinear& L, hipStream_t st);
+
+// ---------------------------------------------------------------- blocks in registers
+constexpr int kMxExpE4M3 = 8, kMxExpE2M1 = 2;  // exponents of the formats' largest powers of two
+
+// Rows of one launch are numbered chunk by chunk, below 2^31 of them; n / d for such n.
+struct FastDiv {
+    uint32_t d, m, s;
+    void set(uint32_t by) {
+        d = by;
+        uint32_t l = 0;
+        while ((1ull << l) < by) ++l;
+        m = (uint32_t)(((1ull << (31 + l)) + by - 1) / by);
+        s = 31 + l;
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (uint32_t)(((uint64_t)n * m) >> s); }
+};
+
+// The codes of N values of a lane, N * LPB = 32 in the LPB lanes of a block (aligned lanes, all of the wave
+// active), and the block's scale byte.  The scale is taken from the exponent bits of the largest magnitude, so
+// scaling is exact; a block with an infinity or NaN gets byte 255 (NaN) and codes 0.
+template <bool E2M1, int N>
+__device__ __forceinline__ void mx_encode(float (&v)[N], uint32_t (&code)[E2M1 ? (N + 7) / 8 : N / 4], int& scale) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+    if constexpr (N <= 16) m = max(m, xor_lane_u<1>(m));
+    if constexpr (N <= 8) m = max(m, xor_lane_u<2>(m));
+    if constexpr (N <= 4) m = max(m, xor_lane_u<4>(m));
+    const bool bad = m >= 0x7f800000u;
+    const int e = max((int)(m >> 23) - (E2M1 ? kMxExpE2M1 : kMxExpE4M3), 0);
+    const float inv = __builtin_bit_cast(float, (uint32_t)(254 - e) << 23);
+    if (__builtin_expect(bad, 0)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = 0.0f;
+    }
+    scale = bad ? 255 : e;
+    if constexpr (E2M1) {  // saturating, to nearest even
+#pragma unroll
+        for (int w = 0; w < (N + 7) / 8; ++w) {
+            uint32_t c = 0;
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w] * inv, v[8 * w + 1] * inv, 1.0f, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 2] * inv, v[8 * w + 3] * inv, 1.0f, 1);
+            if constexpr (N >= 8) {
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 4] * inv, v[8 * w + 5] * inv, 1.0f, 2);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 6] * inv, v[8 * w + 7] * inv, 1.0f, 3);
+            }
+            code[w] = c;
+        }
+    } else {  // to nearest even; past 464 the conversion gives NaN, so the values are held to 448 before it
+        auto at = [&](int i) { return __builtin_amdgcn_fmed3f(v[i] * inv, -448.0f, 448.0f); };
+#pragma unroll
+        for (int w = 0; w < N / 4; ++w) {
+            int c = __builtin_amdgcn_cvt_pk_fp8_f32(at(4 * w), at(4 * w + 1), 0, false);
+            code[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(at(4 * w + 2), at(4 * w + 3), c, true);
+        }
+    }
+}
+
+}  // namespace pgmoe

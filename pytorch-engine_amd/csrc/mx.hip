@@ -1,0 +1,342 @@
+// Rows to microscaled blocks and back: mx_quantize, the gated activation and the norm with blocks as output.
+//
+// Block of 32 along a row: E = max(-127, floor(log2 max|x|) - e), e = 8 (e4m3) or 2 (e2m1), held as the byte
+// E + 127; codes x / 2^E to the nearest, ties to even, at most 448 or 6 in size.  x / 2^E is exact, so the codes are
+// those of the definition whatever the order of the maximum.
+// Reference: nothing of this form; the norm is exec_fused_add_rmsnorm (pygguf_engine/quant_kernels.py:1552-1597), the
+// activation exec_fused_act_mul_rowscale (:1423-1475), whose output is fp16 with one scale a row.
+//
+// HBM-bound: values are read once, 16 bytes a lane, codes and scale bytes written once.
+#include "launch.h"
+#include "mx.h"
+
+namespace pgmoe {
+
+constexpr int kMxThreads = 256;
+
+template <int DT>
+struct Chunk {  // what one lane loads at once
+    static constexpr int N = DT == PGMOE_DT_F32 ? 4 : 8;
+};
+template <int DT>
+__device__ __forceinline__ void widen(const uint4& u, float (&v)[Chunk<DT>::N]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == PGMOE_DT_F32) {
+            v[i] = __builtin_bit_cast(float, w[i]);
+        } else if constexpr (DT == PGMOE_DT_F16) {
+            v[2 * i] = lo_half(w[i]);
+            v[2 * i + 1] = hi_half(w[i]);
+        } else {
+            v[2 * i] = __builtin_bit_cast(float, w[i] << 16);
+            v[2 * i + 1] = __builtin_bit_cast(float, w[i] & 0xffff0000u);
+        }
+    }
+}
+
+// Codes and scale byte of chunk c of a row (N values a chunk).
+template <bool E2M1, int N>
+__device__ __forceinline__ void put_codes(const MxRows& y, int64_t row, int c, const uint32_t (&code)[E2M1 ? (N + 7) / 8 : N / 4],
+                                          int scale) {
+    uint8_t* p = y.codes + row * y.code_stride + (int64_t)c * (E2M1 ? N / 2 : N);
+    if constexpr (E2M1 && N == 4)
+        *(uint16_t*)p = (uint16_t)code[0];
+    else if constexpr ((E2M1 && N == 8) || (!E2M1 && N == 4))
+        *(uint32_t*)p = code[0];
+    else
+        *(uint2*)p = make_uint2(code[0], code[1]);
+    constexpr int LPB = 32 / N;
+    if (c % LPB == 0) y.scales[row * y.scale_stride + c / LPB] = (uint8_t)scale;
+}
+
+// silu(g) = g / (1 + e^-g), gelu(g) = g / (1 + e^-2z) with z = sqrt(2 / pi) (g + 0.044715 g^3): no difference of near
+// values for negative g.  The hardware's power of two and reciprocal are good to 2^-23 each, where codes hold 4 bits.
+template <int ACT>
+__device__ __forceinline__ float gated(float g) {
+    constexpr float kLog2e = 1.44269504088896f;
+    const float z = ACT ? (2.0f * 0.7978845608028654f * kLog2e) * (g + 0.044715f * g * g * g) : kLog2e * g;
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-z));
+}
+
+// ACT < 0: the blocks of x; 0: of silu(x) u; 1: of gelu(x) u (tanh form).
+// U chunks a thread, all of their loads on the way before the first is used.
+template <int DT, bool E2M1, int ACT, int U>
+__global__ __launch_bounds__(kMxThreads) void mx_rows_kernel(const void* __restrict__ x, int64_t xs, const void* __restrict__ u,
+                                                            int64_t us, FastDiv cpr, uint32_t chunks, MxRows y) {
+    constexpr int N = Chunk<DT>::N;
+    constexpr int B = DT == PGMOE_DT_F32 ? 4 : 2;
+    const uint32_t first = blockIdx.x * (uint32_t)(kMxThreads * U) + threadIdx.x;
+    uint4 a[U], b[ACT >= 0 ? U : 1];
+    uint32_t row[U], col[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {  // lanes past the end repeat the last chunk: whole waves meet in mx_encode
+        const uint32_t n = min(first + j * kMxThreads, chunks - 1);
+        row[j] = cpr.div(n);
+        col[j] = n - row[j] * cpr.d;
+        a[j] = *(const uint4*)((const uint8_t*)x + ((int64_t)row[j] * xs + (int64_t)col[j] * N) * B);
+        if constexpr (ACT >= 0) b[j] = *(const uint4*)((const uint8_t*)u + ((int64_t)row[j] * us + (int64_t)col[j] * N) * B);
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        float v[N];
+        widen<DT>(a[j], v);
+        if constexpr (ACT >= 0) {
+            float w[N];
+            widen<DT>(b[j], w);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = gated<ACT>(v[i]) * w[i];
+        }
+        uint32_t code[E2M1 ? (N + 7) / 8 : N / 4];
+        int scale;
+        mx_encode<E2M1, N>(v, code, scale);
+        if (first + j * kMxThreads < chunks) put_codes<E2M1, N>(y, row[j], (int)col[j], code, scale);
+    }
+}
+
+template <bool E2M1>
+__global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(MxRows x, FastDiv cpr, uint32_t chunks, void* __restrict__ out,
+                                                                  int odt) {
+    const uint32_t n = blockIdx.x * (uint32_t)kMxThreads + threadIdx.x;
+    if (n >= chunks) return;
+    const int64_t row = cpr.div(n);
+    const int c = (int)(n - (uint32_t)row * cpr.d);  // chunk of 8 values
+    const int e = x.scales[row * x.scale_stride + c / 4];
+    const uint8_t* p = x.codes + row * x.code_stride + (int64_t)c * (E2M1 ? 4 : 8);
+    float v[8];
+    if constexpr (E2M1) {
+        const uint32_t w = *(const uint32_t*)p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // sign, two exponent bits, one of the mantissa
+            const uint32_t k = (w >> (4 * i)) & 15, m = k & 7;
+            const float a = m < 2 ? 0.5f * (float)m : __builtin_bit_cast(float, (((m >> 1) + 126u) << 23) | ((m & 1) << 22));
+            v[i] = k & 8 ? -a : a;
+        }
+    } else {
+        const uint2 w = *(const uint2*)p;
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, true);
+        const auto d = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, false), f = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, true);
+        v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = d[0], v[5] = d[1], v[6] = f[0], v[7] = f[1];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = e == 255 ? __builtin_nanf("") : ldexpf(v[i], e - 127);
+    const int64_t at = row * x.cols + 8 * (int64_t)c;
+    if (odt == PGMOE_DT_F32) {
+        float4* o = (float4*)((float*)out + at);
+        o[0] = make_float4(v[0], v[1], v[2], v[3]);
+        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] = odt == PGMOE_DT_F16 ? (uint32_t)to16<false>(v[2 * i]) | (uint32_t)to16<false>(v[2 * i + 1]) << 16
+                                       : (uint32_t)to16<true>(v[2 * i]) | (uint32_t)to16<true>(v[2 * i + 1]) << 16;
+        *(uint4*)((uint16_t*)out + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// ---------------------------------------------------------------- the norm
+// h = f32(x) + f32(delta), y = (h * r) * w, r = 1 / sqrt(sum(h^2) / D + eps), as add_rmsnorm_kernel, the rows of y to
+// blocks in the same registers.  A row takes T threads of a workgroup of max(T, 256); thread t owns the 4-value chunks
+// t, t + T, ...: eight neighbouring lanes hold a block.  VPT > 0: the row stays in registers (D <= 4 T VPT), its
+// loads all on the way before the first is used; VPT == 0: it is read twice.
+template <int T, int VPT, bool E2M1>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void add_rmsnorm_mx_kernel(const void* __restrict__ x, int xdt,
+                                                                          const void* __restrict__ delta, int ddt,
+                                                                          const float* __restrict__ w, float eps,
+                                                                          float* __restrict__ h_out, MxRows y) {
+    constexpr int RPB = T < 256 ? 256 / T : 1, W = T / 64;  // rows a workgroup, waves a row
+    __shared__ float wsum[W > 1 ? W : 1];
+    const int t = threadIdx.x % T, n4 = y.cols >> 2;
+    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / T;
+    if (row >= y.rows) return;  // whole waves; with one row a workgroup none
+    const int64_t row4 = row * n4;
+    auto load = [&](const void* p, int dt, int64_t i4) {
+        if (dt == PGMOE_DT_F32) return ((const uint4*)p)[i4];
+        const uint2 u = ((const uint2*)p)[i4];
+        return make_uint4(u.x, u.y, 0, 0);
+    };
+    auto widen4 = [&](const uint4& u, int dt) {
+        auto f = [](uint32_t v) { return __builtin_bit_cast(float, v); };
+        if (dt == PGMOE_DT_F32) return make_float4(f(u.x), f(u.y), f(u.z), f(u.w));
+        if (dt == PGMOE_DT_F16) return make_float4(lo_half(u.x), hi_half(u.x), lo_half(u.y), hi_half(u.y));
+        return make_float4(f(u.x << 16), f(u.x & 0xffff0000u), f(u.y << 16), f(u.y & 0xffff0000u));
+    };
+    auto add = [](float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); };
+    auto squares = [](float acc, float4 h) { return acc + h.x * h.x + h.y * h.y + h.z * h.z + h.w * h.w; };
+    auto total = [&](float acc) {
+        acc = group_sum<64>(acc);
+        if constexpr (W > 1) {
+            if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = acc;
+            __syncthreads();
+            acc = wsum[0];
+#pragma unroll
+            for (int i = 1; i < W; ++i) acc = acc + wsum[i];
+        }
+        return 1.0f / sqrtf(acc / (float)y.cols + eps);
+    };
+    auto put = [&](int c, float4 h, float4 g, float r) {
+        float v[4] = {(h.x * r) * g.x, (h.y * r) * g.y, (h.z * r) * g.z, (h.w * r) * g.w};
+        uint32_t code[1];
+        int scale;
+        mx_encode<E2M1, 4>(v, code, scale);
+        if (c < n4) put_codes<E2M1, 4>(y, row, c, code, scale);
+    };
+    if constexpr (VPT > 0) {
+        auto at = [&](int j) { return min(t + T * j, n4 - 1); };  // chunks past the row repeat its last one
+        uint4 xr[VPT], dr[VPT];
+        float4 g[VPT];
+        if (xdt == PGMOE_DT_F32) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) xr[j] = load(x, PGMOE_DT_F32, row4 + at(j));
+        } else {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) xr[j] = load(x, PGMOE_DT_F16, row4 + at(j));
+        }
+        if (delta) {
+            if (ddt == PGMOE_DT_F32) {
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) dr[j] = load(delta, PGMOE_DT_F32, row4 + at(j));
+            } else {
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) dr[j] = load(delta, PGMOE_DT_F16, row4 + at(j));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) g[j] = ((const float4*)w)[at(j)];
+        __builtin_amdgcn_sched_barrier(0);
+        float acc = 0.0f;
+        float4 h[VPT];
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            h[j] = widen4(xr[j], xdt);
+            if (delta) h[j] = add(h[j], widen4(dr[j], ddt));
+            if (t + T * j < n4) acc = squares(acc, h[j]);
+        }
+        const float r = total(acc);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int c = t + T * j;
+            if (h_out && c < n4) ((float4*)h_out)[row4 + c] = h[j];
+            put(c, h[j], g[j], r);
+        }
+    } else {
+        auto h_at = [&](int c) {
+            float4 h = widen4(load(x, xdt, row4 + c), xdt);
+            return delta ? add(h, widen4(load(delta, ddt, row4 + c), ddt)) : h;
+        };
+        float acc = 0.0f;
+        for (int c = t; c < n4; c += T) acc = squares(acc, h_at(c));
+        const float r = total(acc);
+        for (int c0 = 0; c0 < n4; c0 += T) {  // every lane, as blocks meet across lanes
+            const int c = c0 + t, k = min(c, n4 - 1);
+            const float4 h = h_at(k);
+            if (h_out && c < n4) ((float4*)h_out)[row4 + c] = h;
+            put(c, h, ((const float4*)w)[k], r);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- launches
+// One launch numbers fewer than 2^31 chunks: calls of more rows are cut into several.
+template <class F>
+static int by_rows(int64_t rows, int cpr, F launch) {
+    const int64_t most = std::max<int64_t>(1, 0x7fffffff / cpr);
+    for (int64_t r = 0; r < rows; r += most) {
+        const int rc = launch(r, std::min(most, rows - r));
+        if (rc) return rc;
+    }
+    return PGMOE_OK;
+}
+
+static MxRows rows_from(const MxRows& y, int64_t r, int64_t n) {
+    MxRows z = y;
+    z.codes += r * y.code_stride;
+    z.scales += r * y.scale_stride;
+    z.rows = (int)n;
+    return z;
+}
+
+template <int DT, bool E2M1, int ACT>
+static int rows_launch(const MxFloats& x, const MxFloats& u, const MxRows& y, hipStream_t st) {
+    constexpr int N = Chunk<DT>::N, B = DT == PGMOE_DT_F32 ? 4 : 2;
+    FastDiv cpr;
+    cpr.set(y.cols / N);
+    return by_rows(y.rows, y.cols / N, [&](int64_t r, int64_t n) {
+        const uint32_t chunks = (uint32_t)(n * (y.cols / N));
+        const void* xp = (const uint8_t*)x.p + r * x.stride * B;
+        const void* up = u.p ? (const uint8_t*)u.p + r * u.stride * B : nullptr;
+        const MxRows z = rows_from(y, r, n);
+        if (chunks >= 4 * 256 * kMxThreads)
+            PG_LAUNCH((mx_rows_kernel<DT, E2M1, ACT, 4>), dim3(div_up(chunks, 4 * kMxThreads)), dim3(kMxThreads), 0, st, xp,
+                      x.stride, up, u.stride, cpr, chunks, z);
+        else
+            PG_LAUNCH((mx_rows_kernel<DT, E2M1, ACT, 1>), dim3(div_up(chunks, kMxThreads)), dim3(kMxThreads), 0, st, xp,
+                      x.stride, up, u.stride, cpr, chunks, z);
+        return check_launch("mx_rows");
+    });
+}
+
+template <int ACT>
+static int rows_by_type(const MxFloats& x, const MxFloats& u, const MxRows& y, hipStream_t st) {
+#define ROWS(DT) return y.e2m1 ? rows_launch<DT, true, ACT>(x, u, y, st) : rows_launch<DT, false, ACT>(x, u, y, st)
+    if (x.dt == PGMOE_DT_F32) ROWS(PGMOE_DT_F32);
+    if (x.dt == PGMOE_DT_F16) ROWS(PGMOE_DT_F16);
+    ROWS(PGMOE_DT_BF16);
+#undef ROWS
+}
+
+int launch_mx_quantize(const MxFloats& x, const MxRows& y, hipStream_t st) {
+    return rows_by_type<-1>(x, MxFloats{nullptr, 0, 0}, y, st);
+}
+
+int launch_mx_act_mul(const MxFloats& gate, const MxFloats& up, int act, const MxRows& y, hipStream_t st) {
+    return act == PGMOE_ACT_SILU ? rows_by_type<0>(gate, up, y, st) : rows_by_type<1>(gate, up, y, st);
+}
+
+int launch_mx_dequantize(const MxRows& x, void* out, int odt, hipStream_t st) {
+    FastDiv cpr;
+    cpr.set(x.cols / 8);
+    return by_rows(x.rows, x.cols / 8, [&](int64_t r, int64_t n) {
+        const uint32_t chunks = (uint32_t)(n * (x.cols / 8));
+        const MxRows z = rows_from(x, r, n);
+        void* o = (uint8_t*)out + r * x.cols * (odt == PGMOE_DT_F32 ? 4 : 2);
+        const dim3 grid(div_up(chunks, kMxThreads)), block(kMxThreads);
+        if (x.e2m1)
+            PG_LAUNCH((mx_dequantize_kernel<true>), grid, block, 0, st, z, cpr, chunks, o, odt);
+        else
+            PG_LAUNCH((mx_dequantize_kernel<false>), grid, block, 0, st, z, cpr, chunks, o, odt);
+        return check_launch("mx_dequantize");
+    });
+}
+
+int launch_add_rmsnorm_mx(const void* x, int xdt, const void* delta, int ddt, const float* w, float eps, float* h_out,
+                          const MxRows& y, hipStream_t st) {
+    const int n4 = y.cols >> 2;
+#define NORM(T, V)                                                                                                         \
+    do {                                                                                                                   \
+        const dim3 grid(T < 256 ? div_up(y.rows, 256 / T) : y.rows), block(T < 256 ? 256 : T);                             \
+        if (y.e2m1)                                                                                                        \
+            PG_LAUNCH((add_rmsnorm_mx_kernel<T, V, true>), grid, block, 0, st, x, xdt, delta, ddt, w, eps, h_out, y);      \
+        else                                                                                                               \
+            PG_LAUNCH((add_rmsnorm_mx_kernel<T, V, false>), grid, block, 0, st, x, xdt, delta, ddt, w, eps, h_out, y);     \
+    } while (0)
+    if (n4 <= 64)
+        NORM(64, 1);
+    else if (n4 <= 128)
+        NORM(64, 2);
+    else if (n4 <= 256)
+        NORM(256, 1);
+    else if (n4 <= 512)
+        NORM(256, 2);
+    else if (n4 <= 1024)
+        NORM(256, 4);
+    else if (n4 <= 4096)
+        NORM(1024, 4);
+    else
+        NORM(1024, 0);
+#undef NORM
+    return check_launch("add_rmsnorm_mx");
+}
+
+}  // namespace pgmoe

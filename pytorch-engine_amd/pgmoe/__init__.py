@@ -10,6 +10,8 @@ from .gguf import GGMLType, GGUFFile, GGUFWriter, InMemoryGGUF, MoEConfig
 from .dense import HipDenseMLP
 from .linear import FusedLinearPack, GGUFQuantLinear, HipQuantLinear
 from .moe import HipSparseMoEMLP
+from .mx import (HipMXLinear, MXTensor, exec_fused_act_mul_mx, exec_fused_add_rmsnorm_mx, exec_fused_rmsnorm_mx,
+                 mx_quantize)
 from .norm import GGUFRMSNorm, HipRMSNorm, exec_fused_add_rmsnorm, exec_fused_rmsnorm
 from .sampling import sample_tokens
 
@@ -20,4 +22,5 @@ GGUFDenseMLP = HipDenseMLP
 __all__ = ["GGMLType", "GGUFFile", "GGUFWriter", "InMemoryGGUF", "MoEConfig", "HipSparseMoEMLP",
            "GGUFSparseMoEMLP", "HipDenseMLP", "GGUFDenseMLP", "GGUFRMSNorm", "HipRMSNorm",
            "exec_fused_add_rmsnorm", "exec_fused_rmsnorm", "GGUFQuantLinear", "HipQuantLinear",
-           "FusedLinearPack", "HipPagedKVCache", "HipRotary", "KVBatch", "sample_tokens"]
+           "FusedLinearPack", "HipPagedKVCache", "HipRotary", "KVBatch", "sample_tokens", "MXTensor",
+           "mx_quantize", "exec_fused_rmsnorm_mx", "exec_fused_add_rmsnorm_mx", "exec_fused_act_mul_mx", "HipMXLinear"]

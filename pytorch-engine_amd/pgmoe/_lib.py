@@ -115,6 +115,18 @@ class Sampling(ctypes.Structure):
     ]
 
 
+class Mx(ctypes.Structure):
+    _fields_ = [
+        ("codes", _P),
+        ("scales", _P),
+        ("code_stride", _I64),
+        ("scale_stride", _I64),
+        ("rows", _I32),
+        ("cols", _I32),
+        ("fmt", _I32),
+    ]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -179,13 +191,24 @@ def lib() -> ctypes.CDLL:
     L.pgmoe_sample_workspace_bytes.restype = ctypes.c_size_t
     L.pgmoe_sample_workspace_bytes.argtypes = [_I32, _I32]
     L.pgmoe_sample.argtypes = [_P, _I32, _I64, _I32, _I32, _P, ctypes.POINTER(Sampling), _P, _P, _P, ctypes.c_size_t, _P]
+    mx = ctypes.POINTER(Mx)
+    L.pgmoe_mx_quantize.argtypes = [_P, _I32, _I64, mx, _P]
+    L.pgmoe_mx_dequantize.argtypes = [mx, _P, _I32, _P]
+    L.pgmoe_add_rmsnorm_mx.argtypes = [_P, _I32, _P, _I32, _P, ctypes.c_float, _P, mx, _P]
+    L.pgmoe_mx_act_mul.argtypes = [_P, _I64, _P, _I64, _I32, _I32, mx, _P]
+    L.pgmoe_mx_packed_bytes.restype = _I64
+    L.pgmoe_mx_packed_bytes.argtypes = [_I64, _I64]
+    L.pgmoe_mx_pack.argtypes = [mx, _P, _P]
+    L.pgmoe_mx_linear.argtypes = [_P, _I32, mx, _P, _P, _I32, _P]
     for fn in ("pgmoe_moe_forward", "pgmoe_moe_forward_timed", "pgmoe_router_topk", "pgmoe_dispatch",
                "pgmoe_dispatch_ws", "pgmoe_expert_gateup",
                "pgmoe_expert_down", "pgmoe_combine", "pgmoe_relayout_weights", "pgmoe_relayout_weights_padded",
                "pgmoe_build_scale_plane",
                "pgmoe_dense_forward", "pgmoe_moe_routing", "pgmoe_moe_status", "pgmoe_moe_forward_noalloc",
                "pgmoe_add_rmsnorm", "pgmoe_linear_forward", "pgmoe_linear_forward_packed", "pgmoe_dequant_rows",
-               "pgmoe_requant_w4", "pgmoe_requant_w8_f16", "pgmoe_rope_append", "pgmoe_attend", "pgmoe_sample"):
+               "pgmoe_requant_w4", "pgmoe_requant_w8_f16", "pgmoe_rope_append", "pgmoe_attend", "pgmoe_sample",
+               "pgmoe_mx_quantize", "pgmoe_mx_dequantize", "pgmoe_add_rmsnorm_mx", "pgmoe_mx_act_mul", "pgmoe_mx_pack",
+               "pgmoe_mx_linear"):
         getattr(L, fn).restype = ctypes.c_int
     ver = L.pgmoe_abi_version()
     if ver != ABI_VERSION:
@@ -210,7 +233,8 @@ EXPORTS = (
     "pgmoe_moe_forward_noalloc", "pgmoe_add_rmsnorm", "pgmoe_linear_workspace_bytes", "pgmoe_linear_forward",
     "pgmoe_dequant_rows", "pgmoe_relayout_weights_padded", "pgmoe_requant_w4", "pgmoe_requant_w8_f16",
     "pgmoe_linear_forward_packed", "pgmoe_rope_append", "pgmoe_attend_workspace_bytes", "pgmoe_attend",
-    "pgmoe_sample_workspace_bytes", "pgmoe_sample",
+    "pgmoe_sample_workspace_bytes", "pgmoe_sample", "pgmoe_mx_quantize", "pgmoe_mx_dequantize",
+    "pgmoe_add_rmsnorm_mx", "pgmoe_mx_act_mul", "pgmoe_mx_packed_bytes", "pgmoe_mx_pack", "pgmoe_mx_linear",
 )
 
 STATUS_SPIN_TIMEOUT = 1  # PGMOE_STATUS_SPIN_TIMEOUT

@@ -1,0 +1,300 @@
+"""Microscaled blocks: 8-bit activations and 4-bit weights in blocks of 32 that share a power of two.
+
+    h, x = exec_fused_add_rmsnorm_mx(x, delta, norm_weight)        # the block's input, as 8-bit blocks
+    gu = gate_up(x, out_dtype=torch.float16)                       # HipMXLinear on 4-bit weights
+    a = exec_fused_act_mul_mx(gu[:, :I], gu[:, I:])                # silu(gate) * up, as 8-bit blocks
+    delta = down(a, out_dtype=torch.float32)
+
+A block of 32 values along a row is held as 2^E (a byte, E + 127) and codes: e4m3 (a byte each) or e2m1 (4 bits):
+E = max(-127, floor(log2 max|x|) - e), e = 8 (e4m3) or 2 (e2m1); codes x / 2^E to the nearest, ties to even, at
+most 448 or 6 in size.  Byte 255 makes a block NaN; blocks that hold an infinity or NaN become such ones.
+e2m1 is what GGUF files hold as MXFP4 (ggml type 39): HipMXLinear.from_gguf keeps those values exactly, where
+GGUFQuantLinear re-quantises them as the reference does (pygguf_engine/quant_kernels.py:906-942).
+
+Products run on the matrix cores' own scaled form: blocks are multiplied by their powers of two in the product.
+Nothing synchronises with the host but the layers' constructors.  There is no CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Any, Optional, Sequence, Tuple, Union
+
+import numpy as np
+import torch
+import torch.nn as nn
+
+from ._lib import ACT_GELU_TANH, ACT_SILU, BF16, F16, F32, MXFP4, Mx, lib
+from .attention import launch
+from .moe import _load_lock, load_float_tensor
+
+_DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+_FMT = {"e4m3": 8, "e2m1": 4}  # bits a value
+_ACT = {"silu": ACT_SILU, "gelu": ACT_GELU_TANH}
+_MAX = 1 << 24  # rows below, columns up to
+
+
+def _bits(fmt: str) -> int:
+    if fmt not in _FMT:
+        raise NotImplementedError(f"block format {fmt!r} (e4m3 or e2m1)")
+    return _FMT[fmt]
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements from one row of t [..., n] to the next as one matrix of rows; -1 if there is no such number."""
+    if t.dim() == 1 or t.numel() == 0:
+        return t.shape[-1]
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        return -1
+    step, rows = None, 1  # innermost first; an axis of one has no stride of its own
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if step is None:
+            step = s
+        elif s != step * rows:
+            return -1
+        rows *= n
+    return t.shape[-1] if step is None else step
+
+
+def _placed(t: torch.Tensor, align: int) -> torch.Tensor:
+    """t, or a contiguous copy, with rows that begin at multiples of `align` bytes and do not overlap."""
+    s = _row_stride(t)
+    if s < t.shape[-1] or s * t.element_size() % align or t.data_ptr() % align:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _empty_scales(lead: Sequence[int], blocks: int, device: torch.device) -> torch.Tensor:
+    """uint8 [..., blocks] whose rows begin at multiples of 4 bytes, as the kernels read four at once."""
+    return torch.empty(*lead, (blocks + 3) // 4 * 4, dtype=torch.uint8, device=device)[..., :blocks]
+
+
+class MXTensor:
+    """Rows in microscaled blocks: `codes` uint8 (or float8_e4m3fn) [..., cols], for e2m1 [..., cols / 2] with the even
+    value of a pair in the low four bits; `scales` uint8 (or float8_e8m0fnu) [..., cols / 32], E + 127 each; `fmt`
+    "e4m3" or "e2m1".  Tensors whose rows the kernels can read where they are are kept, not copied."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str = "e4m3") -> None:
+        per = 8 // _bits(fmt)
+        if codes.dtype not in (torch.uint8, torch.float8_e4m3fn) or (per == 2 and codes.dtype != torch.uint8):
+            raise ValueError(f"codes of dtype {codes.dtype} (uint8, for e4m3 also float8_e4m3fn)")
+        if scales.dtype not in (torch.uint8, torch.float8_e8m0fnu):
+            raise ValueError(f"scales of dtype {scales.dtype} (uint8 or float8_e8m0fnu)")
+        if codes.device.type != "cuda" or scales.device != codes.device:
+            raise ValueError("pgmoe blocks: codes and scales on one HIP device")
+        if codes.dim() < 1:
+            raise ValueError("codes: [..., cols]")
+        cols = codes.shape[-1] * per
+        if cols % 32 or not 32 <= cols <= _MAX:
+            raise ValueError(f"{cols} columns: a multiple of 32 up to {_MAX}")
+        if tuple(scales.shape) != (*codes.shape[:-1], cols // 32):
+            raise ValueError(f"scales {tuple(scales.shape)} of codes {tuple(codes.shape)} ({fmt})")
+        rows = codes.numel() // codes.shape[-1]
+        if rows >= _MAX:
+            raise NotImplementedError(f"{rows} rows (below {_MAX})")
+        codes = _placed(codes.view(torch.uint8), 16)
+        scales = scales.view(torch.uint8)
+        s = _row_stride(scales)
+        if s < scales.shape[-1] or s % 4 or scales.data_ptr() % 4:
+            scales = _empty_scales(scales.shape[:-1], scales.shape[-1], scales.device).copy_(scales)
+        self._set(codes, scales, fmt, rows, cols)
+
+    def _set(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, rows: int, cols: int) -> None:
+        self._codes, self._scales, self._fmt = codes, scales, fmt
+        self._c = Mx(codes.data_ptr(), scales.data_ptr(), _row_stride(codes), _row_stride(scales), rows, cols, _FMT[fmt])
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, shape: Sequence[int], fmt: str, device: torch.device) -> "MXTensor":
+        """Blocks of a tensor of this shape, not yet written."""
+        bits = _bits(fmt)
+        *lead, cols = shape
+        if cols % 32 or not 32 <= cols <= _MAX:
+            raise ValueError(f"{cols} columns: a multiple of 32 up to {_MAX}")
+        rows = 1
+        for n in lead:
+            rows *= n
+        if rows >= _MAX:
+            raise NotImplementedError(f"{rows} rows (below {_MAX})")
+        t = cls.__new__(cls)
+        t._set(torch.empty(*lead, cols * bits // 8, dtype=torch.uint8, device=device),
+               _empty_scales(lead, cols // 32, device), fmt, rows, cols)
+        return t
+
+    # as they were given: the kernels read what the struct of them says
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    fmt = property(lambda self: self._fmt)
+    device = property(lambda self: self._codes.device)
+
+    @property
+    def shape(self) -> Tuple[int, ...]:
+        return (*self._codes.shape[:-1], self._c.cols)
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values code * 2^E, each rounded once to `dtype` (fp32, fp16, bf16)."""
+        if dtype not in _DT:
+            raise NotImplementedError(f"values of dtype {dtype} (fp32, fp16 or bf16)")
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        if out.numel():
+            launch(self.device, "pgmoe_mx_dequantize", lib().pgmoe_mx_dequantize, self._ref, out.data_ptr(), _DT[dtype])
+        return out
+
+
+def _floats(name: str, x: torch.Tensor) -> torch.Tensor:
+    if x.device.type != "cuda":
+        raise ValueError(f"{name}: a tensor on a HIP device")
+    if x.dtype not in _DT:
+        raise NotImplementedError(f"{name} of dtype {x.dtype} (fp32, fp16 or bf16)")
+    if x.dim() < 1:
+        raise ValueError(f"{name}: [..., cols]")
+    return _placed(x, 16)
+
+
+def mx_quantize(x: torch.Tensor, fmt: str = "e4m3") -> MXTensor:
+    """x [..., cols] (fp32, fp16, bf16) in blocks of 32 along its rows."""
+    x = _floats("x", x)
+    y = MXTensor.empty(x.shape, fmt, x.device)
+    if x.numel():
+        launch(x.device, "pgmoe_mx_quantize", lib().pgmoe_mx_quantize, x.data_ptr(), _DT[x.dtype], _row_stride(x), y._ref)
+    return y
+
+
+def exec_fused_act_mul_mx(gate: torch.Tensor, up: torch.Tensor, act: str = "silu", fmt: str = "e4m3") -> MXTensor:
+    """act(gate) * up in blocks, act "silu" or "gelu" (tanh form), formed in fp32 from two tensors of one shape and type
+    (the halves of a fused projection's output are taken as they are)."""
+    if act not in _ACT:
+        raise NotImplementedError(f"activation {act!r} (silu or gelu)")
+    if up.shape != gate.shape or up.dtype != gate.dtype or up.device != gate.device:
+        raise ValueError(f"up {tuple(up.shape)} {up.dtype} beside gate {tuple(gate.shape)} {gate.dtype}: one shape, type and device")
+    gate, up = _floats("gate", gate), _floats("up", up)
+    y = MXTensor.empty(gate.shape, fmt, gate.device)
+    if gate.numel():
+        launch(gate.device, "pgmoe_mx_act_mul", lib().pgmoe_mx_act_mul, gate.data_ptr(), _row_stride(gate), up.data_ptr(),
+               _row_stride(up), _DT[gate.dtype], _ACT[act], y._ref)
+    return y
+
+
+def _norm(x: torch.Tensor, delta: Optional[torch.Tensor], norm_weight: torch.Tensor, eps: float, fmt: str):
+    x = _floats("x", x)
+    if not x.is_contiguous():
+        x = x.contiguous()
+    if delta is not None:
+        if delta.shape != x.shape or delta.device != x.device:
+            raise ValueError(f"delta {tuple(delta.shape)} on {delta.device} beside x {tuple(x.shape)} on {x.device}")
+        delta = _floats("delta", delta)
+        if not delta.is_contiguous():
+            delta = delta.contiguous()
+    if norm_weight.numel() != x.shape[-1]:
+        raise ValueError(f"norm weight has {norm_weight.numel()} elements, rows have {x.shape[-1]}")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    w = _placed(norm_weight.to(device=x.device, dtype=torch.float32).reshape(-1).contiguous(), 16)
+    y = MXTensor.empty(x.shape, fmt, x.device)
+    h = torch.empty(x.shape, dtype=torch.float32, device=x.device) if delta is not None else None
+    if x.numel():
+        launch(x.device, "pgmoe_add_rmsnorm_mx", lib().pgmoe_add_rmsnorm_mx, x.data_ptr(), _DT[x.dtype],
+               None if delta is None else delta.data_ptr(), 0 if delta is None else _DT[delta.dtype], w.data_ptr(),
+               float(eps), None if h is None else h.data_ptr(), y._ref)
+    return h, y
+
+
+def exec_fused_rmsnorm_mx(x: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6, fmt: str = "e4m3") -> MXTensor:
+    """exec_fused_rmsnorm with its output in blocks; the fp32 values are not rounded before."""
+    return _norm(x, None, norm_weight, eps, fmt)[1]
+
+
+def exec_fused_add_rmsnorm_mx(x: torch.Tensor, delta: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6,
+                              fmt: str = "e4m3") -> Tuple[torch.Tensor, MXTensor]:
+    """exec_fused_add_rmsnorm with its second output in blocks: (h = x.float() + delta.float(), RMSNorm(h) * w)."""
+    return _norm(x, delta, norm_weight, eps, fmt)
+
+
+def _gguf_blocks(raw: np.ndarray, rows: int, cols: int, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of GGUF MXFP4 bytes: 17 a block, the scale's and 16 of codes, byte j holding values j (low) and
+    j + 16 (high)."""
+    b = torch.from_numpy(np.ascontiguousarray(raw)).to(device).reshape(rows, cols // 32, 17)
+    v = torch.cat((b[..., 1:] & 15, b[..., 1:] >> 4), -1)
+    return (v[..., 0::2] | v[..., 1::2] << 4).reshape(rows, cols // 2), b[..., 0].contiguous()
+
+
+class HipMXLinear(nn.Module):
+    """y = x . W^T (+ bias) with W [out_features, in_features] in e2m1 blocks, laid out once for the matrix cores.
+
+    forward(x, out_dtype=None): x an MXTensor [..., in_features] (either format), or fp32 / fp16 / bf16 values, which
+    are brought to blocks of `act_fmt` first.  Products are summed in fp32 in a fixed order and rounded once, to
+    out_dtype (fp32, fp16, bf16; by default x's, fp16 for an MXTensor)."""
+
+    def __init__(self, weight: MXTensor, bias: Optional[torch.Tensor] = None, act_fmt: str = "e4m3") -> None:
+        super().__init__()
+        _bits(act_fmt)
+        if weight.fmt != "e2m1" or len(weight.shape) != 2 or weight.shape[0] < 1:
+            raise ValueError(f"weight: e2m1 blocks [out_features, in_features], not {weight.fmt} {tuple(weight.shape)}")
+        self.out_features, self.in_features = weight.shape
+        self.device = weight.device
+        self.act_fmt = act_fmt
+        if bias is not None and tuple(bias.shape) != (self.out_features,):
+            raise ValueError(f"bias {tuple(bias.shape)} of {self.out_features} outputs")
+        n = int(lib().pgmoe_mx_packed_bytes(self.out_features, self.in_features))
+        if n < 0:
+            raise NotImplementedError(f"weights of {self.out_features} x {self.in_features}")
+        # no buffers of the module: its to() and half() would move or round what the kernel reads as given
+        self._packed = torch.empty(n, dtype=torch.uint8, device=self.device)
+        self._bias = None if bias is None else bias.detach().to(self.device, torch.float32, copy=True).contiguous()
+        launch(self.device, "pgmoe_mx_pack", lib().pgmoe_mx_pack, weight._ref, self._packed.data_ptr())
+        torch.cuda.current_stream(self.device).synchronize()  # from here on any stream may use them
+
+    bias = property(lambda self: self._bias)
+
+    @classmethod
+    def from_gguf(cls, gguf_file: Any, weight_name: Union[str, Sequence[str]], bias_name: Optional[str] = None,
+                  device: Union[torch.device, str] = "cuda", act_fmt: str = "e4m3") -> "HipMXLinear":
+        """The named matrix; several names are one layer whose outputs follow each other.  MXFP4 tensors are kept
+        exactly, F32 / F16 / BF16 ones are brought to e2m1 blocks."""
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("HipMXLinear runs on a HIP device (torch.device('cuda', i))")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        codes, scales = [], []
+        with _load_lock, torch.cuda.device(device):
+            for name in [weight_name] if isinstance(weight_name, str) else weight_name:
+                info = gguf_file.tensors[name]
+                rows, cols, qt = int(info.shape[0]), int(info.shape[1]), int(info.qtype)
+                if cols % 32:
+                    raise ValueError(f"{name}: {cols} input features (a multiple of 32)")
+                if qt == MXFP4:
+                    c, s = _gguf_blocks(np.asarray(gguf_file.get_tensor_bytes(name)), rows, cols, device)
+                elif qt in (F32, F16, BF16):
+                    w = load_float_tensor(gguf_file, name, torch.device("cpu")).reshape(rows, cols)
+                    t = mx_quantize(w.to(device, torch.float32), "e2m1")
+                    c, s = t.codes, t.scales
+                else:
+                    raise NotImplementedError(f"{name}: ggml type {qt} (MXFP4, F32, F16 or BF16; GGUFQuantLinear takes the others)")
+                codes.append(c)
+                scales.append(s)
+            bias = None
+            if bias_name and bias_name in gguf_file.tensors:
+                bias = load_float_tensor(gguf_file, bias_name, torch.device("cpu"))
+            if len({c.shape[1] for c in codes}) != 1:
+                raise ValueError("matrices of one layer have the same number of input features")
+            return cls(MXTensor(torch.cat(codes), torch.cat(scales), "e2m1"), bias=bias, act_fmt=act_fmt)
+
+    def forward(self, x: Union[torch.Tensor, MXTensor], out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        given = isinstance(x, MXTensor)
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"{x.shape[-1]} input features, the layer has {self.in_features}")
+        if x.device != self.device:
+            raise ValueError(f"input on {x.device}, the layer is on {self.device}")
+        odt = out_dtype if out_dtype is not None else torch.float16 if given else x.dtype
+        if odt not in _DT:
+            raise NotImplementedError(f"outputs of dtype {odt} (fp32, fp16 or bf16)")
+        if not given:
+            x = mx_quantize(x, self.act_fmt)
+        out = torch.empty(*x.shape[:-1], self.out_features, dtype=odt, device=self.device)
+        if out.numel():
+            launch(self.device, "pgmoe_mx_linear", lib().pgmoe_mx_linear, self._packed.data_ptr(), self.out_features, x._ref,
+                   None if self._bias is None else self._bias.data_ptr(), out.data_ptr(), _DT[odt])
+        return out
