@@ -414,10 +414,11 @@ int pgmoe_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t 
                  const pgmoe_sampling* S, int64_t* token, float* logprob, void* ws, size_t ws_bytes, void* stream);
 
 /* Microscaled blocks: rows of 32 values that share a power of two.  codes [rows, cols] (e4m3: one byte a value; e2m1:
- * two values a byte, the even one in the low four bits), rows code_stride bytes apart (a multiple of 16, the
- * pointer 16-byte aligned); scales [rows, cols / 32] bytes, E + 127 each, rows scale_stride bytes apart (a multiple
- * of 4, the pointer 4-byte aligned).  A value is code * 2^E; byte 255 makes its block NaN.  cols: a multiple of 32, up
- * to 2^24; rows below 2^24. */
+ * two values a byte, the even one in the low four bits), rows code_stride bytes apart; scales
+ * [rows, cols / 32] bytes, E + 127 each, rows scale_stride bytes apart.  Both strides are multiples of 16, up to 2^23,
+ * both pointers 16-byte aligned; the scales of a row are read (never written) up to the next multiple of 16 bytes,
+ * whatever lies there.  A value is code * 2^E; byte 255 makes its block NaN.  cols: a multiple of 32, up to 2^22; rows
+ * below 2^24. */
 #define PGMOE_MX_E4M3 8 /* sign, 4 exponent bits, 3 of the mantissa: up to 448, no infinities */
 #define PGMOE_MX_E2M1 4 /* 0 0.5 1 1.5 2 3 4 6 and their negatives */
 typedef struct pgmoe_mx {
@@ -454,10 +455,19 @@ int64_t pgmoe_mx_packed_bytes(int64_t rows, int64_t cols);
 int pgmoe_mx_pack(const pgmoe_mx* w, void* dst, void* stream);
 
 /* out [x.rows, out_features] (PGMOE_DT_*, contiguous, 16-byte aligned) = x . W^T (+ bias fp32 [out_features] or NULL):
- * packed weights of out_features rows of x.cols, x in e4m3 or e2m1 blocks, products summed in fp32 in a fixed order
- * and rounded once. */
+ * packed weights of out_features rows of x.cols, x in e4m3 or e2m1 blocks; products summed in fp32 in a fixed order
+ * and rounded once.  16-bit outputs of more than 16 rows of e4m3 blocks take the matrix cores' 8-bit form, which cuts
+ * the products of 8 neighbouring inputs below 2^-13 of the largest of them (2e-5 of the outputs' 2-norm); fp32 outputs
+ * and up to 16 rows do not, and take an activation beyond fp32's range as an infinity. */
 int pgmoe_mx_linear(const void* packed, int32_t out_features, const pgmoe_mx* x, const float* bias, void* out,
                     int32_t out_dtype, void* stream);
+
+/* pgmoe_mx_linear of the blocks of x [rows, cols] (as pgmoe_mx_quantize makes them, in format fmt).  The workspace (16-byte
+ * aligned; none for up to 16 rows) holds them during the call and needs no clearing. */
+size_t pgmoe_mx_linear_values_workspace_bytes(int32_t rows, int32_t cols, int32_t fmt);
+int pgmoe_mx_linear_values(const void* packed, int32_t out_features, const void* x, int32_t dtype, int64_t x_stride,
+                           int32_t rows, int32_t cols, int32_t fmt, const float* bias, void* out, int32_t out_dtype,
+                           void* ws, size_t ws_bytes, void* stream);
 
 /* pgmoe_moe_forward with per-kernel timing.  No counterpart in the reference: it is for
  * benchmarks and profilers that want each kernel's duration from the caller's own stream.

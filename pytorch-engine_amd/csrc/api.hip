@@ -860,16 +860,16 @@ static int check_mx(const char* what, const pgmoe_mx* T, MxRows* y) {
     if (!T) return fail(PGMOE_E_INVALID, "%s: NULL blocks", what);
     if (T->fmt != PGMOE_MX_E4M3 && T->fmt != PGMOE_MX_E2M1)
         return fail(PGMOE_E_UNSUPPORTED, "%s: format %d (e4m3: 8, e2m1: 4)", what, T->fmt);
-    if (T->rows < 0 || T->rows >= (1 << 24) || T->cols < 32 || T->cols > (1 << 24) || T->cols % 32)
+    if (T->rows < 0 || T->rows >= (1 << 24) || T->cols < 32 || T->cols > (1 << 22) || T->cols % 32)
         return fail(PGMOE_E_INVALID, "%s: %d rows of %d (a multiple of 32)", what, T->rows, T->cols);
     const int64_t code = T->fmt == PGMOE_MX_E2M1 ? T->cols / 2 : T->cols;
     if (T->rows > 1 && (T->code_stride < code || T->scale_stride < T->cols / 32))
         return fail(PGMOE_E_INVALID, "%s: rows overlap", what);
-    if (T->rows > 1 && (T->code_stride % 16 || T->scale_stride % 4 || T->code_stride > (1ll << 31) || T->scale_stride > (1ll << 31)))
-        return fail(PGMOE_E_INVALID, "%s: rows of codes lie a multiple of 16 bytes apart, of scales one of 4", what);
+    if (T->rows > 1 && (T->code_stride % 16 || T->scale_stride % 16 || T->code_stride > (1 << 23) || T->scale_stride > (1 << 23)))
+        return fail(PGMOE_E_INVALID, "%s: rows of codes and of scales lie a multiple of 16 bytes apart, 2^23 at most", what);
     if (T->rows && (!T->codes || !T->scales)) return fail(PGMOE_E_INVALID, "%s: NULL pointer", what);
-    if (((uintptr_t)T->codes & 15) || ((uintptr_t)T->scales & 3))
-        return fail(PGMOE_E_INVALID, "%s: codes must be 16-byte aligned, scales 4-byte aligned", what);
+    if (((uintptr_t)T->codes | (uintptr_t)T->scales) & 15)
+        return fail(PGMOE_E_INVALID, "%s: codes and scales must be 16-byte aligned", what);
     *y = MxRows{(uint8_t*)T->codes, (uint8_t*)T->scales, T->rows > 1 ? T->code_stride : 0, T->rows > 1 ? T->scale_stride : 0,
                 T->rows, T->cols, T->fmt == PGMOE_MX_E2M1};
     return PGMOE_OK;
@@ -935,7 +935,7 @@ int pgmoe_mx_act_mul(const void* gate, int64_t gate_stride, const void* up, int6
 }
 
 static bool mx_weight_sizes(int64_t rows, int64_t cols) {
-    return rows >= 1 && rows < (1 << 24) && cols >= 32 && cols <= (1 << 24) && cols % 32 == 0 && rows * cols <= (1ll << 40);
+    return rows >= 1 && rows < (1 << 24) && cols >= 32 && cols <= (1 << 22) && cols % 32 == 0 && rows * cols <= (1ll << 40);
 }
 
 int64_t pgmoe_mx_packed_bytes(int64_t rows, int64_t cols) { return mx_weight_sizes(rows, cols) ? mx_packed_bytes(rows, cols) : -1; }
@@ -950,19 +950,54 @@ int pgmoe_mx_pack(const pgmoe_mx* W, void* dst, void* stream) {
     return launch_mx_pack(w, (uint8_t*)dst, as_stream(stream));
 }
 
-int pgmoe_mx_linear(const void* packed, int32_t out_features, const pgmoe_mx* X, const float* bias, void* out,
-                    int32_t out_dtype, void* stream) {
-    MxRows x;
-    const int rc = check_mx("mx_linear", X, &x);
-    if (rc) return rc;
+static int check_mx_product(int out_features, const MxRows& x, const void* packed, const float* bias, const void* out, int out_dtype) {
     if (!mx_weight_sizes(out_features, x.cols)) return fail(PGMOE_E_INVALID, "mx_linear: %d outputs", out_features);
     if (!float_type(out_dtype)) return fail(PGMOE_E_UNSUPPORTED, "mx_linear: output dtype %d", out_dtype);
     if ((int64_t)x.rows * out_features > (1ll << 38)) return fail(PGMOE_E_UNSUPPORTED, "mx_linear: %d x %d outputs", x.rows, out_features);
-    if (x.rows == 0) return PGMOE_OK;
-    if (!packed || !out || (((uintptr_t)packed | (uintptr_t)out) & 15) || ((uintptr_t)bias & 3))
+    if (x.rows && (!packed || !out || (((uintptr_t)packed | (uintptr_t)out) & 15) || ((uintptr_t)bias & 3)))
         return fail(PGMOE_E_INVALID, "mx_linear: weights and out must be 16-byte aligned device pointers");
+    return PGMOE_OK;
+}
+
+int pgmoe_mx_linear(const void* packed, int32_t out_features, const pgmoe_mx* X, const float* bias, void* out,
+                    int32_t out_dtype, void* stream) {
+    MxRows x;
+    int rc = check_mx("mx_linear", X, &x);
+    if (rc || (rc = check_mx_product(out_features, x, packed, bias, out, out_dtype))) return rc;
+    if (x.rows == 0) return PGMOE_OK;
     return launch_mx_linear(MxLinear{(const uint8_t*)packed, out_features, x.cols, x.rows, x, bias, out, out_dtype},
                             as_stream(stream));
+}
+
+static size_t mx_scratch(int64_t rows, int64_t cols, int fmt, int64_t* code_stride, int64_t* scale_stride) {
+    *code_stride = fmt == PGMOE_MX_E2M1 ? cols / 2 : cols;
+    *scale_stride = (cols / 32 + 15) / 16 * 16;
+    return rows <= kMxFewRows ? 0 : (size_t)(rows * (*code_stride + *scale_stride));
+}
+
+size_t pgmoe_mx_linear_values_workspace_bytes(int32_t rows, int32_t cols, int32_t fmt) {
+    int64_t c, s;
+    return rows <= 0 || cols <= 0 ? 0 : mx_scratch(rows, cols, fmt, &c, &s);
+}
+
+int pgmoe_mx_linear_values(const void* packed, int32_t out_features, const void* x, int32_t dtype, int64_t x_stride, int32_t rows,
+                           int32_t cols, int32_t fmt, const float* bias, void* out, int32_t out_dtype, void* ws, size_t ws_bytes,
+                           void* stream) {
+    int64_t cs, ss;
+    const size_t need = rows > 0 && cols > 0 ? mx_scratch(rows, cols, fmt, &cs, &ss) : 0;
+    if (need && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
+        return fail(PGMOE_E_WORKSPACE, "mx_linear_values: workspace %zu bytes, need %zu, 16-byte aligned", ws_bytes, need);
+    // (few rows need no blocks: an address that is not read or written)
+    const pgmoe_mx B = {need ? ws : (void*)x, need ? (uint8_t*)ws + rows * cs : (void*)x, need ? cs : cols, need ? ss : cols, rows, cols, fmt};
+    MxRows y;
+    MxFloats f;
+    int rc = check_mx("mx_linear_values", &B, &y);
+    if (rc) return rc;
+    if ((rc = check_mx_product(out_features, y, packed, bias, out, out_dtype))) return rc;
+    if (rows == 0) return PGMOE_OK;
+    if ((rc = check_mx_floats("mx_linear_values", x, dtype, x_stride, y, &f))) return rc;
+    return launch_mx_linear_values(MxLinear{(const uint8_t*)packed, out_features, cols, rows, y, bias, out, out_dtype}, f,
+                                   as_stream(stream));
 }
 
 int pgmoe_moe_forward_timed(const pgmoe_layer* L, const uint16_t* x, int32_t M, float* out, void* ws,

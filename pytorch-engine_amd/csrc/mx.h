@@ -34,7 +34,10 @@ struct MxLinear {
     void* out;
     int odt;
 };
+constexpr int kMxFewRows = 16;  // values of up to so many rows become blocks inside the product
 int launch_mx_linear(const MxLinear& L, hipStream_t st);
+// L.x: where the blocks of more rows go.
+int launch_mx_linear_values(const MxLinear& L, const MxFloats& F, hipStream_t st);
 
 // ---------------------------------------------------------------- blocks in registers
 constexpr int kMxExpE4M3 = 8, kMxExpE2M1 = 2;  // exponents of the formats' largest powers of two

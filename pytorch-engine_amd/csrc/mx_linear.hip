@@ -24,6 +24,9 @@
 
 namespace pgmoe {
 
+#define PG_INLINE __attribute__((always_inline))
+
+constexpr int kCUs = 256;
 typedef int intx8 __attribute__((ext_vector_type(8)));
 
 __host__ __device__ inline int mx_groups(int N) { return (N + 15) >> 4; }
@@ -65,19 +68,19 @@ enum MxMode { kS4, kS8, kB8 };  // scaled instruction on 4- or 8-bit activations
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// A lane's activations at step s of its row (kept inside the row).
 template <MxMode MODE>
-__device__ __forceinline__ intx8 x_frag(const uint8_t* row, int s, int g, int K) {
-    const int k = 128 * s + (MODE == kS8 ? 16 : 32) * g;
-    const int64_t at = k < K ? k : 0, next = MODE == kB8 ? at + 16 : k + 64 < K ? k + 64 : 0;
-    const int4 a = *(const int4*)(row + (MODE == kS4 ? at >> 1 : at));
-    intx8 f = {a.x, a.y, a.z, a.w, 0, 0, 0, 0};
-    if constexpr (MODE != kS4) {
-        const int4 b = *(const int4*)(row + next);
-        f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+struct XFrag {  // a lane's activations of one step
+    int4 a, b;
+    __device__ __forceinline__ intx8 operand() const { return intx8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}; }
+    __device__ __forceinline__ uint32_t word(int i) const {
+        return (uint32_t)(i == 0 ? a.x : i == 1 ? a.y : i == 2 ? a.z : i == 3 ? a.w : i == 4 ? b.x : i == 5 ? b.y : i == 6 ? b.z : b.w);
     }
-    return f;
-}
+};
+template <>
+struct XFrag<kS4> {
+    int4 a;
+    __device__ __forceinline__ intx8 operand() const { return intx8{a.x, a.y, a.z, a.w, 0, 0, 0, 0}; }
+};
 
 // 2^(b - 127) as the conversions take it: 0 for 2^-127, 255 for NaN.
 __device__ __forceinline__ float scale_of(uint32_t b) { return __builtin_bit_cast(float, b << 23); }
@@ -99,35 +102,49 @@ __device__ __forceinline__ bf16x8 bf16_of_e4m3(uint32_t lo, uint32_t hi, float s
     return __builtin_bit_cast(bf16x8, o);
 }
 
-// acc[b][t] += w[b] . x[t] over one step of 128 inputs; ws[b]'s byte S and xs[t]'s lowest are the scales.
-template <MxMode MODE, int S, int NB, int MT>
-__device__ __forceinline__ void mx_step(const int4 (&w)[NB], const int (&ws)[NB], const intx8 (&x)[MT], const int (&xs)[MT],
-                                        floatx4 (&acc)[NB][MT]) {
-    if constexpr (MODE == kB8) {
-        float wf[NB];
+// The weights of one step as the instructions take them; byte S of ws[b] is their scale.
+template <MxMode MODE, int NB>
+struct WOps {
+    int4 w[NB];
+    template <int S>
+    __device__ __forceinline__ void set(const int4 (&from)[NB], const int (&)[NB]) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) wf[b] = scale_of(((uint32_t)ws[b] >> (8 * S)) & 255u);
+        for (int b = 0; b < NB; ++b) w[b] = from[b];
+    }
+};
+template <int NB>
+struct WOps<kB8, NB> {
+    bf16x8 v[4][NB];
+    template <int S>
+    __device__ __forceinline__ void set(const int4 (&from)[NB], const int (&ws)[NB]) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float sw = scale_of(((uint32_t)ws[b] >> (8 * S)) & 255u);
+            v[0][b] = bf16_of_e2m1((uint32_t)from[b].x, sw);
+            v[1][b] = bf16_of_e2m1((uint32_t)from[b].y, sw);
+            v[2][b] = bf16_of_e2m1((uint32_t)from[b].z, sw);
+            v[3][b] = bf16_of_e2m1((uint32_t)from[b].w, sw);
+        }
+    }
+};
+// acc[b][t] += w[b] . f over one step of 128 inputs; byte S of ws[b] and byte SX of xs are the scales.
+template <MxMode MODE, int S, int SX, int NB, int MT>
+__device__ __forceinline__ void mx_products(const WOps<MODE, NB>& w, const int (&ws)[NB], int xs, const XFrag<MODE>& f, int t,
+                                            floatx4 (&acc)[NB][MT]) {
+    if constexpr (MODE == kB8) {
+        const float sx = scale_of(((uint32_t)xs >> (8 * SX)) & 255u);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            bf16x8 v[NB];
+            const bf16x8 u = bf16_of_e4m3(f.word(2 * j), f.word(2 * j + 1), sx);
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-                v[b] = bf16_of_e2m1((uint32_t)(j == 0 ? w[b].x : j == 1 ? w[b].y : j == 2 ? w[b].z : w[b].w), wf[b]);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const bf16x8 u = bf16_of_e4m3((uint32_t)x[t][2 * j], (uint32_t)x[t][2 * j + 1], scale_of((uint32_t)xs[t]));
-#pragma unroll
-                for (int b = 0; b < NB; ++b) acc[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[b], u, acc[b][t], 0, 0, 0);
-            }
+            for (int b = 0; b < NB; ++b) acc[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[j][b], u, acc[b][t], 0, 0, 0);
         }
     } else {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const intx8 a = {w[b].x, w[b].y, w[b].z, w[b].w, 0, 0, 0, 0};
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-                acc[b][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x[t], acc[b][t], 4, MODE == kS4 ? 4 : 0, S, ws[b],
-                                                                             0, xs[t]);
+            const intx8 a = {w.w[b].x, w.w[b].y, w.w[b].z, w.w[b].w, 0, 0, 0, 0};
+            acc[b][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, f.operand(), acc[b][t], 4, MODE == kS4 ? 4 : 0, S, ws[b],
+                                                                         SX, xs);
         }
     }
 }
@@ -165,31 +182,75 @@ __device__ __forceinline__ void put4(const MxLinear& L, int m, int n, float4 v) 
     }
 }
 
-// ---------------------------------------------------------------- few rows
-// A workgroup forms NB row groups of weights for 16 MT activation rows; its W waves take every W-th quad of steps,
-// weights and activations straight to registers, and their sums meet in LDS in wave order.
-template <MxMode MODE, int MT, int NB, int W>
-__global__ __launch_bounds__(64 * W) void mx_thin_kernel(const MxLinear L) {
-    __shared__ float4 part[W][NB * MT][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int G = mx_groups(L.N), Q = mx_quads(L.K), blocks = L.K >> 5;
-    const int across = div_up(G, NB);
-    const int g0 = (blockIdx.x % across) * NB, m0 = (blockIdx.x / across) * (16 * MT);
-    const uint8_t* xr[MT];
-    const uint8_t* xsr[MT];
+// ---------------------------------------------------------------- up to 16 rows
+// A workgroup forms 16 NB outputs of all rows; its W waves take every W-th quad of steps, weights and activations straight
+// to registers (all of a quad's on their way at once), and their sums meet in LDS in wave order.  Bound by the weights'
+// arrival and, from few of them, by the latencies of one load, one sum and the launch.
+// SRC: the rows come in blocks (-1), or as values of a PGMOE_DT_* that become blocks here: a lane holds the 32 values of
+// a block, so its largest magnitude needs no other lane.
+template <MxMode MODE, int SRC>
+struct ThinX {  // one step of a lane's row
+    static constexpr int N = SRC == PGMOE_DT_F32 ? 8 : 4;
+    uint4 v[N];
+    __device__ __forceinline__ void load(const uint8_t* row, int block) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = min(m0 + 16 * t + r, L.M - 1);
-        xr[t] = L.x.codes + m * L.x.code_stride;
-        xsr[t] = L.x.scales + m * L.x.scale_stride;
+        for (int i = 0; i < N; ++i) v[i] = ((const uint4*)(row + (int64_t)block * (16 * N)))[i];
     }
-    floatx4 acc[NB][MT];
+    __device__ __forceinline__ XFrag<MODE> blocks(int& scale) const {
+        float f[32];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+        for (int i = 0; i < N; ++i) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[b][t] = floatx4{0, 0, 0, 0};
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (SRC == PGMOE_DT_F32) {
+                    f[4 * i + k] = __builtin_bit_cast(float, w[k]);
+                } else if constexpr (SRC == PGMOE_DT_F16) {
+                    f[8 * i + 2 * k] = lo_half(w[k]);
+                    f[8 * i + 2 * k + 1] = hi_half(w[k]);
+                } else {
+                    f[8 * i + 2 * k] = __builtin_bit_cast(float, w[k] << 16);
+                    f[8 * i + 2 * k + 1] = __builtin_bit_cast(float, w[k] & 0xffff0000u);
+                }
+            }
+        }
+        uint32_t c[MODE == kS4 ? 4 : 8];
+        mx_encode<MODE == kS4, 32>(f, c, scale);
+        XFrag<MODE> x;
+        x.a = make_int4((int)c[0], (int)c[1], (int)c[2], (int)c[3]);
+        if constexpr (MODE != kS4) x.b = make_int4((int)c[4], (int)c[5], (int)c[6], (int)c[7]);
+        return x;
+    }
+};
+
+template <MxMode MODE, int SRC, int NB, int W>
+__global__ __launch_bounds__(64 * W, 4) void mx_thin_kernel(const MxLinear L, const MxFloats F) {
+    __shared__ float4 part[W][NB][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int G = mx_groups(L.N), Q = mx_quads(L.K), last = (L.K >> 5) - 1, g0 = blockIdx.x * NB;
+    const int m = min(r, L.M - 1);  // rows past the last repeat it, blocks past the row's last too: their weights are 0
+    const uint8_t* xr = SRC < 0 ? L.x.codes + m * L.x.code_stride : (const uint8_t*)F.p + m * F.stride * (SRC == PGMOE_DT_F32 ? 4 : 2);
+    const uint8_t* xsr = L.x.scales + m * L.x.scale_stride;
     const uint8_t* scales = L.w + (int64_t)G * Q * 4096;
+    floatx4 acc[NB][1];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b][0] = floatx4{0, 0, 0, 0};
     for (int q = wave; q < Q; q += W) {
+        XFrag<MODE> f[4];
+        int xs[4];
+        constexpr int AHEAD = SRC == PGMOE_DT_F32 ? 2 : 3;  // steps of values in registers
+        ThinX<MODE, SRC < 0 ? PGMOE_DT_F16 : SRC> raw[AHEAD];
+        auto block = [&](int s) { return min(16 * q + 4 * s + g, last); };
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if constexpr (SRC < 0) {
+                f[s].a = *(const int4*)(xr + (int64_t)block(s) * (MODE == kS4 ? 16 : 32));
+                if constexpr (MODE != kS4) f[s].b = *(const int4*)(xr + (int64_t)block(s) * 32 + 16);
+                xs[s] = xsr[block(s)];
+            } else if (s < AHEAD) {
+                raw[s].load(xr, block(s));
+            }
+        }
         int4 w[4][NB];
         int ws[NB];
 #pragma unroll
@@ -199,16 +260,16 @@ __global__ __launch_bounds__(64 * W) void mx_thin_kernel(const MxLinear L) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) w[s][b] = *(const int4*)(L.w + at * 4096 + s * 1024 + lane * 16);
         }
+        __builtin_amdgcn_sched_barrier(0);
         auto step = [&](auto sc) {
             constexpr int s = decltype(sc)::value;
-            intx8 x[MT];
-            int xs[MT];
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                x[t] = x_frag<MODE>(xr[t], 4 * q + s, g, L.K);
-                xs[t] = xsr[t][min(16 * q + 4 * s + g, blocks - 1)];
+            if constexpr (SRC >= 0) {
+                f[s] = raw[s % AHEAD].blocks(xs[s]);
+                if constexpr (s + AHEAD < 4) raw[s % AHEAD].load(xr, block(s + AHEAD));
             }
-            mx_step<MODE, s>(w[s], ws, x, xs, acc);
+            WOps<MODE, NB> ops;
+            ops.template set<s>(w[s], ws);
+            mx_products<MODE, s, 0>(ops, ws, xs[s], f[s], 0, acc);
         };
         step(std::integral_constant<int, 0>());
         step(std::integral_constant<int, 1>());
@@ -216,41 +277,381 @@ __global__ __launch_bounds__(64 * W) void mx_thin_kernel(const MxLinear L) {
         step(std::integral_constant<int, 3>());
     }
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) part[wave][b * MT + t][lane] = make_float4(acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]);
+    for (int b = 0; b < NB; ++b) part[wave][b][lane] = make_float4(acc[b][0][0], acc[b][0][1], acc[b][0][2], acc[b][0][3]);
     __syncthreads();
-    for (int i = threadIdx.x; i < NB * MT * 64; i += 64 * W) {
-        const int bt = i >> 6, l = i & 63;
-        float4 v = part[0][bt][l];
+    for (int i = threadIdx.x; i < NB * 64; i += 64 * W) {
+        const int b = i >> 6, l = i & 63;
+        float4 v = part[0][b][l];
 #pragma unroll
         for (int k = 1; k < W; ++k) {
-            const float4 p = part[k][bt][l];
+            const float4 p = part[k][b][l];
             v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
         }
-        const int m = m0 + 16 * (bt % MT) + (l & 15), n = 16 * (g0 + bt / MT) + 4 * (l >> 4);
-        if (m < L.M && n < L.N) put4(L, m, n, v);
+        const int n = 16 * (g0 + b) + 4 * (l >> 4);
+        if ((l & 15) < L.M && n < L.N) put4(L, l & 15, n, v);
     }
 }
 
-template <MxMode MODE>
-static int thin_launch(const MxLinear& L, hipStream_t st) {
-    const int G = mx_groups(L.N);
-#define THIN(MT, NB, W) \
-    PG_LAUNCH((mx_thin_kernel<MODE, MT, NB, W>), dim3(div_up(G, NB) * div_up(L.M, 16 * MT)), dim3(64 * W), 0, st, L)
-    if (L.M <= 16)
-        THIN(1, 2, 8);
-    else if (L.M <= 32)
-        THIN(2, 2, 8);
-    else
-        THIN(4, 2, 8);
-#undef THIN
+template <MxMode MODE, int SRC>
+static int thin_launch(const MxLinear& L, const MxFloats& F, hipStream_t st) {
+    PG_LAUNCH((mx_thin_kernel<MODE, SRC, 2, 8>), dim3(div_up(mx_groups(L.N), 2)), dim3(64 * 8), 0, st, L, F);
     return check_launch("mx_thin");
 }
 
+// ---------------------------------------------------------------- many rows
+// A workgroup forms BM x BN outputs in WM x WN waves of 16 MT x 16 NT.  Activations and weights come through a ring of
+// RING stages in LDS (128 bytes an activation row: 128 inputs in 8 bits, 256 in 4), copied straight from memory RING - 1
+// stages ahead, so that a chain of stages runs at the rate of the products and not at a memory latency each.  At the top of stage
+// s a wave waits until its copies of stage s + 1 have landed, and the barrier makes all waves' visible: the first
+// fragments of s + 1 are then read under the last products of s.  Chunk c (16 bytes) of activation row r lies at
+// c ^ (r / 2 & 7): the 16 rows of a fragment fall on different banks.  Weights lie as they are packed.  Scales of 512 inputs
+// come with the first of their stages: 16 bytes an activation row, which become a word a lane and row, a byte a step.
+// Copies of 1 KB from memory to LDS, lane l's 16 bytes at base + off to lds + 16 l, each STEP behind the one before.  By
+// hand, so that the compiler counts no loads and adds no waits; a copy reads m0 one wait state after its write.
+#define PG_COPY(off, base) "s_nop 0\n\tglobal_load_lds_dwordx4 " off ", " base "\n\t"
+template <int STEP>
+__device__ __forceinline__ void copy_lds(uint32_t lds, const uint8_t* b0, uint32_t o0) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\t" PG_COPY("%2", "%3") "s_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(o0), "s"(b0)
+                 : "memory");
+}
+template <int STEP>
+__device__ __forceinline__ void copy_lds(uint32_t lds, const uint8_t* b0, uint32_t o0, const uint8_t* b1, uint32_t o1) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\t" PG_COPY("%2", "%3") "s_add_u32 m0, m0, %6\n\t" PG_COPY("%4", "%5")
+                 "s_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(o0), "s"(b0), "v"(o1), "s"(b1), "n"(STEP)
+                 : "memory", "scc");
+}
+template <int STEP>
+__device__ __forceinline__ void copy_lds(uint32_t lds, const uint8_t* b0, uint32_t o0, const uint8_t* b1, uint32_t o1, const uint8_t* b2,
+                                         uint32_t o2, const uint8_t* b3, uint32_t o3) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\t" PG_COPY("%2", "%3") "s_add_u32 m0, m0, %10\n\t" PG_COPY("%4", "%5")
+                 "s_add_u32 m0, m0, %10\n\t" PG_COPY("%6", "%7") "s_add_u32 m0, m0, %10\n\t" PG_COPY("%8", "%9") "s_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(o0), "s"(b0), "v"(o1), "s"(b1), "v"(o2), "s"(b2), "v"(o3), "s"(b3), "n"(STEP)
+                 : "memory", "scc");
+}
+#undef PG_COPY
+// N of them, base(j) and off(j).
+template <int STEP, int N, int J = 0, class B, class O>
+__device__ __forceinline__ void copies_lds(uint32_t lds, B base, O off) {
+    if constexpr (N - J >= 4) {
+        copy_lds<STEP>(lds + J * STEP, base(J), off(J), base(J + 1), off(J + 1), base(J + 2), off(J + 2), base(J + 3), off(J + 3));
+        copies_lds<STEP, N, J + 4>(lds, base, off);
+    } else if constexpr (N - J >= 2) {
+        copy_lds<STEP>(lds + J * STEP, base(J), off(J), base(J + 1), off(J + 1));
+        copies_lds<STEP, N, J + 2>(lds, base, off);
+    } else if constexpr (N - J == 1) {
+        copy_lds<STEP>(lds + J * STEP, base(J), off(J));
+    }
+}
+// All but the last N of this wave's copies have landed and its reads of LDS are done; then every wave's.
+template <int N>
+__device__ __forceinline__ void stage_ready() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+template <MxMode MODE, int MT, int NT, int WM, int WN, int RING, bool EARLY>
+struct MxTile {
+    static constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN, NW = WM * WN;
+    static constexpr int SPS = MODE == kS4 ? 2 : 1;            // steps a stage
+    static constexpr int SPQ = 4 / SPS;                        // stages a quad
+    static constexpr int XB = BM * 128, WB = BN / 16 * SPS * 1024, STAGE = XB + WB;
+    static constexpr int XC = BM / 8 / NW, WC = WB / 1024 / NW;  // copies of a stage a wave
+    static constexpr int SROWS = BM < 64 ? 64 : BM, SCOLS = BN < 64 ? 64 : BN;
+    static constexpr int SPARTS = SROWS / 64 + SCOLS / 64, SC = (SPARTS + NW - 1) / NW;  // copies of scales: in all, a wave
+    static constexpr int SB = (SROWS + SCOLS) * 16;
+    static constexpr int NS = (RING - 1) / SPQ + 1;            // quads whose scales are held
+    static constexpr int LDS = RING * STAGE + NS * SB;
+    static_assert(XC * 8 * NW == BM && WC * NW * 1024 == WB, "copies of a stage over the waves");
+    // fragments read ahead: a step's, where registers hold two steps of them
+    static constexpr bool WHOLE = EARLY && MT * NT <= 8;
+    static constexpr int AHEAD = WHOLE ? MT : 1;
+    static_assert(RING >= (EARLY ? 3 : 2), "stages under way");
+    static_assert(LDS <= 160 * 1024, "LDS of a CU");
+    // copies of a wave that may be under way at the top of stage s = J of a quad: those behind stage s + EARLY
+    static constexpr int under_way(int j) {
+        int n = 0;
+        for (int k = EARLY ? 2 : 1; k <= RING - 2; ++k) n += XC + WC + ((j + k) % SPQ == 0 ? SC : 0);
+        return n;
+    }
+    static_assert(under_way(0) <= 63, "the counter's range");
+};
+
+// Tile of a workgroup.  Workgroups go to the 8 XCDs in turn: each XCD takes one run of the tiles, in bands of 8
+// row tiles at most, so that what it works on at a time shares rows and weights in its L2.
+__device__ __forceinline__ void mx_tile_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int n = tiles_m * tiles_n, per = n >> 3, rest = n & 7, x = id & 7;
+    id = x * per + min(x, rest) + (id >> 3);
+    const int band = id / (8 * tiles_n), in = id - band * 8 * tiles_n, high = min(8, tiles_m - 8 * band);
+    tm = 8 * band + in % high;
+    tn = in / high;
+}
+
+template <MxMode MODE, int MT, int NT, int WM, int WN, int RING, bool EARLY, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void mx_gemm_kernel(const MxLinear L, const int tiles_m, const int tiles_n) {
+    using T = MxTile<MODE, MT, NT, WM, WN, RING, EARLY>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[T::LDS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    int tm, tn;
+    mx_tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * T::BM, g0 = tn * (T::BN / 16);
+    const int wm = wave % WM, wn = wave / WM;
+    const int G = mx_groups(L.N), Q = mx_quads(L.K), blocks = L.K >> 5, stages = Q * T::SPQ;
+    const uint32_t row_bytes = MODE == kS4 ? L.K >> 1 : L.K;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+
+    // Copies: rows past the last repeat it, groups past the last too, inputs past the row its last ones (their weights are
+    // 0), stages behind the last the last one's (nothing reads them).
+    const uint8_t* xb = L.x.codes + (int64_t)m0 * L.x.code_stride;
+    const uint8_t* sb = L.x.scales + (int64_t)m0 * L.x.scale_stride;
+    const uint32_t stride = (uint32_t)L.x.code_stride;
+    const int rows = min(L.M - m0, T::BM) - 1;
+    uint32_t x_off[T::XC];
+#pragma unroll
+    for (int j = 0; j < T::XC; ++j) x_off[j] = (uint32_t)min((wave + T::NW * j) * 8 + (lane >> 3), rows) * stride;
+    const uint32_t chunk = 16u * (uint32_t)((lane ^ ((wave * 8 + (lane >> 3)) >> 1)) & 7);
+    const uint8_t* wb[T::WC];  // copy j of the weights: this group and step of a stage
+#pragma unroll
+    for (int j = 0; j < T::WC; ++j) {
+        const int c = wave + T::NW * j;
+        wb[j] = L.w + ((int64_t)min(g0 + c / T::SPS, G - 1) * (4 * Q) + c % T::SPS) * 1024;
+    }
+    auto copy_stage = [&](int s, int slot) PG_INLINE {
+        const uint32_t to = lds0 + (uint32_t)(slot * T::STAGE + wave * 1024);
+        const uint32_t x_at = min(128u * (uint32_t)s + chunk, row_bytes - 16u);
+        const uint32_t w_at = (uint32_t)(s * (T::SPS * 1024) + lane * 16);
+        copies_lds<T::NW * 1024, T::XC>(to, [&](int) PG_INLINE { return xb; }, [&](int j) PG_INLINE { return x_off[j] + x_at; });
+        copies_lds<T::NW * 1024, T::WC>(to + T::XB, [&](int j) PG_INLINE { return wb[j]; }, [&](int) PG_INLINE { return w_at; });
+    };
+    const uint8_t* wsb = L.w + ((int64_t)G * Q * 4096 + (int64_t)g0 * Q * 256);
+    auto copy_scales = [&](int q) PG_INLINE {
+        const uint32_t to = lds0 + RING * T::STAGE + (uint32_t)(q % T::NS) * T::SB;
+        q = min(q, Q - 1);
+#pragma unroll
+        for (int j = 0; j < T::SC; ++j) {
+            const int p = (wave + T::NW * j) % T::SPARTS;  // several waves may copy the same
+            const bool x = p < T::SROWS / 64;
+            const int c = x ? p : p - T::SROWS / 64;
+            const uint32_t x_at = (uint32_t)min(c * 64 + lane, rows) * (uint32_t)L.x.scale_stride + 16u * (uint32_t)q;
+            const uint32_t w_at = (uint32_t)min(c * 4 + (lane >> 4), G - 1 - g0) * (uint32_t)(Q * 256) + (uint32_t)(q * 256 + (lane & 15) * 16);
+            copy_lds<0>(to + p * 1024, x ? sb : wsb, x ? x_at : w_at);
+        }
+    };
+
+    floatx4 acc[NT][MT];
+#pragma unroll
+    for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[b][t] = floatx4{0, 0, 0, 0};
+    int4 w[2][NT];
+    int ws[NT], xs[MT];
+    constexpr int GR = MT / T::AHEAD;  // groups of fragments a step
+    XFrag<MODE> f[2][T::AHEAD];
+    // this lane's places: weights, and the chunks of its activation rows (4 bits: of the stage's two steps)
+    const int w_lane = lane * 16 + T::XB + wn * NT * T::SPS * 1024;
+    const int x_row = (wm * MT * 16 + r) * 128, c0 = MODE == kB8 ? 2 * g : g, c1 = MODE == kB8 ? c0 + 1 : c0 + 4;
+    const int x_lane[2] = {x_row + 16 * (c0 ^ (r >> 1)), x_row + 16 * (c1 ^ (r >> 1))};
+    auto get_w = [&](int4 (&to)[NT], int base, int u) PG_INLINE {
+        const uint8_t* from = smem + (w_lane + base);
+#pragma unroll
+        for (int b = 0; b < NT; ++b) to[b] = *(const int4*)(from + (b * T::SPS + u) * 1024);
+    };
+    auto get_x = [&](int base, int u, int t) PG_INLINE {
+        XFrag<MODE> v;
+        v.a = *(const int4*)(smem + (x_lane[MODE == kS4 ? u : 0] + base) + t * 2048);
+        if constexpr (MODE != kS4) v.b = *(const int4*)(smem + (x_lane[1] + base) + t * 2048);
+        return v;
+    };
+    const uint32_t pick = (uint32_t)(g | (4 + g) << 8);
+    uint4 sv[MT];
+    int wsv[NT];
+    auto read_scales = [&](int q) PG_INLINE {
+        const uint8_t* from = smem + RING * T::STAGE + (q % T::NS) * T::SB;
+#pragma unroll
+        for (int b = 0; b < NT; ++b) wsv[b] = *(const int*)(from + T::SROWS * 16 + (wn * NT + b) * 256 + lane * 4);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) sv[t] = *(const uint4*)(from + ((wm * MT + t) * 16 + r) * 16);
+    };
+    auto set_scales = [&](int q) PG_INLINE {
+#pragma unroll
+        for (int b = 0; b < NT; ++b) ws[b] = wsv[b];
+        // blocks past the row's last: 1, whatever lies there
+        const int have = min(max((blocks - 16 * q - g + 3) >> 2, 0), 4);
+        const uint32_t keep = have == 4 ? 0xffffffffu : (1u << (8 * have)) - 1u;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const uint32_t a = __builtin_amdgcn_perm(sv[t].y, sv[t].x, pick), b = __builtin_amdgcn_perm(sv[t].w, sv[t].z, pick);
+            xs[t] = (int)((__builtin_amdgcn_perm(b, a, 0x05040100u) & keep) | (0x7f7f7f7fu & ~keep));
+        }
+    };
+    // Step S of a quad, its weights and first AHEAD fragments in registers: the products of a group of fragments run while the
+    // next group, or the next step's first and its weights, are read.  x(t), t past MT: the next step's.
+    auto step = [&](auto sc, auto follows, int w_base, int w_u, auto x) PG_INLINE {
+        constexpr int S = decltype(sc)::value;
+        constexpr bool NEXT = decltype(follows)::value;  // the next step can be read already
+        if constexpr (NEXT) get_w(w[(S + 1) & 1], w_base, w_u);
+        WOps<MODE, NT> ops;
+        ops.template set<S>(w[S & 1], ws);
+#pragma unroll
+        for (int i = 0; i < GR; ++i) {
+            const int p = (S * GR + i) & 1;
+#pragma unroll
+            for (int k = 0; k < T::AHEAD; ++k)
+                if (NEXT || i + 1 < GR) f[p ^ 1][k] = x((i + 1) * T::AHEAD + k);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < T::AHEAD; ++k) mx_products<MODE, S, S>(ops, ws, xs[i * T::AHEAD + k], f[p][k], i * T::AHEAD + k, acc);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    copy_scales(0);
+#pragma unroll
+    for (int s = 0; s < RING - 1; ++s) {
+        if (s && s % T::SPQ == 0) copy_scales(s / T::SPQ);
+        copy_stage(min(s, stages - 1), s);
+    }
+    int slot = 0;
+    if constexpr (EARLY) {
+        stage_ready<T::under_way(T::SPQ - 1)>();  // stage 0, as at the top of the stage before it
+#pragma unroll
+        for (int k = 0; k < T::AHEAD; ++k) f[0][k] = get_x(0, 0, k);
+        get_w(w[0], 0, 0);
+    }
+    if constexpr (T::WHOLE) read_scales(0);
+    // stage J of quad q
+    auto stage = [&](auto jc, int q) PG_INLINE {
+        constexpr int J = decltype(jc)::value;
+        const int s = q * T::SPQ + J, here = slot * T::STAGE;
+        const int over = slot == 0 ? RING - 1 : slot - 1, after = slot == RING - 1 ? 0 : slot + 1, then = after * T::STAGE;
+        stage_ready<T::under_way(J)>();
+        if constexpr ((J + RING - 1) % T::SPQ == 0) copy_scales((s + RING - 1) / T::SPQ);
+        copy_stage(min(s + RING - 1, stages - 1), over);
+        if constexpr (J == 0) {
+            if constexpr (!T::WHOLE) read_scales(q);
+            set_scales(q);
+        }
+        if constexpr (T::WHOLE && J == T::SPQ - 1) read_scales(q + 1);  // theirs came with the next stage's
+        constexpr int S = J * T::SPS;
+        if constexpr (!EARLY) {
+            get_w(w[S & 1], here, 0);
+#pragma unroll
+            for (int k = 0; k < T::AHEAD; ++k) f[(S * GR) & 1][k] = get_x(here, 0, k);
+        }
+        using Next = std::integral_constant<bool, EARLY>;
+        if constexpr (T::SPS == 2) {
+            step(std::integral_constant<int, S>(), std::true_type(), here, 1,
+                 [&](int t) PG_INLINE { return t < MT ? get_x(here, 0, t) : get_x(here, 1, t - MT); });
+            step(std::integral_constant<int, S + 1>(), Next(), then, 0,
+                 [&](int t) PG_INLINE { return t < MT ? get_x(here, 1, t) : get_x(then, 0, t - MT); });
+        } else {
+            step(std::integral_constant<int, S>(), Next(), then, 0,
+                 [&](int t) PG_INLINE { return t < MT ? get_x(here, 0, t) : get_x(then, 0, t - MT); });
+        }
+        slot = after;
+    };
+    for (int q = 0; q < Q; ++q) {
+        stage(std::integral_constant<int, 0>(), q);
+        stage(std::integral_constant<int, 1>(), q);
+        if constexpr (T::SPQ == 4) {
+            stage(std::integral_constant<int, 2>(), q);
+            stage(std::integral_constant<int, 3>(), q);
+        }
+    }
+    stage_ready<0>();  // copies that nothing reads, before the LDS is another workgroup's
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = m0 + (wm * MT + t) * 16 + r;
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            const int n = (g0 + wn * NT + b) * 16 + 4 * g;
+            if (m < L.M && n < L.N) put4(L, m, n, make_float4(acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]));
+        }
+    }
+}
+
+template <MxMode MODE, int MT, int NT, int WM, int WN, int RING, bool EARLY, int OCC>
+static int gemm_launch(const MxLinear& L, hipStream_t st) {
+    using T = MxTile<MODE, MT, NT, WM, WN, RING, EARLY>;
+    const int tm = div_up(L.M, T::BM), tn = div_up(L.N, T::BN);
+    PG_LAUNCH((mx_gemm_kernel<MODE, MT, NT, WM, WN, RING, EARLY, OCC>), dim3(tm * tn), dim3(64 * T::NW), 0, st, L, tm, tn);
+    return check_launch("mx_gemm");
+}
+
+// Which tile: the one whose fit a + b ceil(tiles / CUs) to the times measured is least.  us at K = 4096, where tiles a CU is
+// n (other K change both alike):
+//   8 bits  128 x 256 33 / 55 / 103 at n = 1 / 2 / 4, 128 x 128 22 / 35 / 61, 64 x 128 14 / 20 / 38, 32 x 128 12 / 14 / 25
+//   4 bits  256 x 256 41 / 77 at 1 / 2, 128 x 128 17 / 26 / 46 at 1 / 2 / 4, 64 x 128 13 / 16 / 30, 32 x 128 12 / 13 / 23
+//   fp32    128 x 128 36 / 57 / 108, 64 x 128 22 / 35 / 61, 32 x 128 15 / 23 / 39
+// e.g. 1024 rows, 8 bits: 4096 outputs 33.2 / 21.8 / 20.7 / 24.9 by tile from the largest, 8192 36.5 / 33.5 / 37.1 / 43.6.
+struct MxCost {
+    int bm, bn;
+    float a, b;
+};
+constexpr int kMxTiles = 4;
+static int pick_tile(const MxCost (&c)[kMxTiles], int M, int N) {
+    int best = kMxTiles - 1;
+    float least = 0.0f;
+    for (int i = kMxTiles - 1; i >= 0; --i) {
+        const int64_t tiles = (int64_t)div_up(M, c[i].bm) * div_up(N, c[i].bn);
+        const float t = c[i].a + c[i].b * (float)((tiles + kCUs - 1) / kCUs);
+        if (i == kMxTiles - 1 || t < least) best = i, least = t;
+    }
+    return best;
+}
+
+static int linear_s8(const MxLinear& L, hipStream_t st) {
+    static constexpr MxCost cost[kMxTiles] = {{128, 256, 9.6f, 23.4f}, {128, 128, 8.0f, 13.8f}, {64, 128, 5.0f, 8.3f}, {32, 128, 3.5f, 5.1f}};
+    switch (pick_tile(cost, L.M, L.N)) {
+        case 0: return gemm_launch<kS8, 4, 8, 2, 2, 2, false, 2>(L, st);
+        case 1: return gemm_launch<kS8, 4, 4, 2, 2, 3, false, 2>(L, st);
+        case 2: return gemm_launch<kS8, 4, 2, 1, 4, 4, true, 2>(L, st);
+        default: return gemm_launch<kS8, 2, 2, 1, 4, 4, true, 2>(L, st);
+    }
+}
+static int linear_s4(const MxLinear& L, hipStream_t st) {
+    static constexpr MxCost cost[kMxTiles] = {{256, 256, 5.0f, 35.8f}, {128, 128, 6.5f, 9.9f}, {64, 128, 4.0f, 6.1f}, {32, 128, 4.0f, 5.0f}};
+    switch (pick_tile(cost, L.M, L.N)) {
+        case 0: return gemm_launch<kS4, 8, 4, 2, 4, 2, false, 2>(L, st);
+        case 1: return gemm_launch<kS4, 4, 4, 2, 2, 2, false, 2>(L, st);
+        case 2: return gemm_launch<kS4, 4, 2, 1, 4, 2, false, 4>(L, st);
+        default: return gemm_launch<kS4, 2, 2, 1, 4, 3, true, 2>(L, st);
+    }
+}
+static int linear_b8(const MxLinear& L, hipStream_t st) {  // 128 x 128 twice: 64 x 256 measured the same (107 for 108 at n = 4)
+    static constexpr MxCost cost[kMxTiles] = {{128, 128, 10.0f, 24.5f}, {128, 128, 10.0f, 24.5f}, {64, 128, 8.0f, 13.8f}, {32, 128, 6.0f, 8.3f}};
+    switch (pick_tile(cost, L.M, L.N)) {
+        case 0:
+        case 1: return gemm_launch<kB8, 4, 4, 2, 2, 3, false, 2>(L, st);
+        case 2: return gemm_launch<kB8, 4, 2, 1, 4, 2, false, 4>(L, st);
+        default: return gemm_launch<kB8, 2, 2, 1, 4, 4, true, 2>(L, st);
+    }
+}
+
+// Up to 16 rows are read against weights that go straight to registers (17 of 12288 x 4096: 12.0 us in two such tiles, 9 in
+// one of 32 rows; 16: 8.7).  There the bf16 instruction costs nothing, as the weights' arrival bounds both.
 int launch_mx_linear(const MxLinear& L, hipStream_t st) {
-    if (L.x.e2m1) return thin_launch<kS4>(L, st);
-    return thin_launch<kB8>(L, st);
+    if (L.M <= kMxFewRows) return L.x.e2m1 ? thin_launch<kS4, -1>(L, MxFloats{}, st) : thin_launch<kB8, -1>(L, MxFloats{}, st);
+    if (L.x.e2m1) return linear_s4(L, st);
+    return L.odt == PGMOE_DT_F32 ? linear_b8(L, st) : linear_s8(L, st);
+}
+
+int launch_mx_linear_values(const MxLinear& L, const MxFloats& F, hipStream_t st) {
+    if (L.M <= kMxFewRows) {
+#define VALUES(DT) return L.x.e2m1 ? thin_launch<kS4, DT>(L, F, st) : thin_launch<kB8, DT>(L, F, st)
+        if (F.dt == PGMOE_DT_F32) VALUES(PGMOE_DT_F32);
+        if (F.dt == PGMOE_DT_F16) VALUES(PGMOE_DT_F16);
+        VALUES(PGMOE_DT_BF16);
+#undef VALUES
+    }
+    const int rc = launch_mx_quantize(F, L.x, st);
+    return rc ? rc : launch_mx_linear(L, st);
 }
 
 }  // namespace pgmoe

@@ -200,6 +200,9 @@ def lib() -> ctypes.CDLL:
     L.pgmoe_mx_packed_bytes.argtypes = [_I64, _I64]
     L.pgmoe_mx_pack.argtypes = [mx, _P, _P]
     L.pgmoe_mx_linear.argtypes = [_P, _I32, mx, _P, _P, _I32, _P]
+    L.pgmoe_mx_linear_values_workspace_bytes.restype = ctypes.c_size_t
+    L.pgmoe_mx_linear_values_workspace_bytes.argtypes = [_I32, _I32, _I32]
+    L.pgmoe_mx_linear_values.argtypes = [_P, _I32, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I32, _P, ctypes.c_size_t, _P]
     for fn in ("pgmoe_moe_forward", "pgmoe_moe_forward_timed", "pgmoe_router_topk", "pgmoe_dispatch",
                "pgmoe_dispatch_ws", "pgmoe_expert_gateup",
                "pgmoe_expert_down", "pgmoe_combine", "pgmoe_relayout_weights", "pgmoe_relayout_weights_padded",
@@ -208,7 +211,7 @@ def lib() -> ctypes.CDLL:
                "pgmoe_add_rmsnorm", "pgmoe_linear_forward", "pgmoe_linear_forward_packed", "pgmoe_dequant_rows",
                "pgmoe_requant_w4", "pgmoe_requant_w8_f16", "pgmoe_rope_append", "pgmoe_attend", "pgmoe_sample",
                "pgmoe_mx_quantize", "pgmoe_mx_dequantize", "pgmoe_add_rmsnorm_mx", "pgmoe_mx_act_mul", "pgmoe_mx_pack",
-               "pgmoe_mx_linear"):
+               "pgmoe_mx_linear", "pgmoe_mx_linear_values"):
         getattr(L, fn).restype = ctypes.c_int
     ver = L.pgmoe_abi_version()
     if ver != ABI_VERSION:
@@ -235,6 +238,7 @@ EXPORTS = (
     "pgmoe_linear_forward_packed", "pgmoe_rope_append", "pgmoe_attend_workspace_bytes", "pgmoe_attend",
     "pgmoe_sample_workspace_bytes", "pgmoe_sample", "pgmoe_mx_quantize", "pgmoe_mx_dequantize",
     "pgmoe_add_rmsnorm_mx", "pgmoe_mx_act_mul", "pgmoe_mx_packed_bytes", "pgmoe_mx_pack", "pgmoe_mx_linear",
+    "pgmoe_mx_linear_values_workspace_bytes", "pgmoe_mx_linear_values",
 )
 
 STATUS_SPIN_TIMEOUT = 1  # PGMOE_STATUS_SPIN_TIMEOUT

@@ -31,7 +31,9 @@ from .moe import _load_lock, load_float_tensor
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _FMT = {"e4m3": 8, "e2m1": 4}  # bits a value
 _ACT = {"silu": ACT_SILU, "gelu": ACT_GELU_TANH}
-_MAX = 1 << 24  # rows below, columns up to
+_ROWS, _COLS = 1 << 24, 1 << 22  # rows below, columns up to
+_STRIDE = 1 << 23  # bytes from row to row
+_FEW_ROWS = 16  # up to so many rows of values become blocks inside the product, without a workspace
 
 
 def _bits(fmt: str) -> int:
@@ -58,17 +60,26 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.shape[-1] if step is None else step
 
 
-def _placed(t: torch.Tensor, align: int) -> torch.Tensor:
-    """t, or a contiguous copy, with rows that begin at multiples of `align` bytes and do not overlap."""
-    s = _row_stride(t)
-    if s < t.shape[-1] or s * t.element_size() % align or t.data_ptr() % align:
+def _placed(t: torch.Tensor, align: int = 16) -> torch.Tensor:
+    """t, or a contiguous copy, with rows that begin at multiples of `align` bytes, do not overlap and lie within
+    2^23 bytes of each other."""
+    s = _row_stride(t) * t.element_size()
+    if s < t.shape[-1] * t.element_size() or s % align or s > _STRIDE or t.data_ptr() % align:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _empty_scales(lead: Sequence[int], blocks: int, device: torch.device) -> torch.Tensor:
-    """uint8 [..., blocks] whose rows begin at multiples of 4 bytes, as the kernels read four at once."""
-    return torch.empty(*lead, (blocks + 3) // 4 * 4, dtype=torch.uint8, device=device)[..., :blocks]
+    """uint8 [..., blocks] whose rows begin at multiples of 16 bytes, as the kernels read so many at once."""
+    return torch.empty(*lead, (blocks + 15) // 16 * 16, dtype=torch.uint8, device=device)[..., :blocks]
+
+
+def _scales_as_they_are(t: torch.Tensor, rows: int) -> bool:
+    """Whether the kernels can read these scale bytes in place: 16 at a time, each of them in memory of the tensor's."""
+    s, n = _row_stride(t), (t.shape[-1] + 15) // 16 * 16
+    if s < t.shape[-1] or s % 16 or s > _STRIDE or t.data_ptr() % 16:
+        return False
+    return t.storage_offset() + max(rows - 1, 0) * s + n <= t.untyped_storage().nbytes()
 
 
 class MXTensor:
@@ -87,17 +98,16 @@ class MXTensor:
         if codes.dim() < 1:
             raise ValueError("codes: [..., cols]")
         cols = codes.shape[-1] * per
-        if cols % 32 or not 32 <= cols <= _MAX:
-            raise ValueError(f"{cols} columns: a multiple of 32 up to {_MAX}")
+        if cols % 32 or not 32 <= cols <= _COLS:
+            raise ValueError(f"{cols} columns: a multiple of 32 up to {_COLS}")
         if tuple(scales.shape) != (*codes.shape[:-1], cols // 32):
             raise ValueError(f"scales {tuple(scales.shape)} of codes {tuple(codes.shape)} ({fmt})")
         rows = codes.numel() // codes.shape[-1]
-        if rows >= _MAX:
-            raise NotImplementedError(f"{rows} rows (below {_MAX})")
-        codes = _placed(codes.view(torch.uint8), 16)
+        if rows >= _ROWS:
+            raise NotImplementedError(f"{rows} rows (below {_ROWS})")
+        codes = _placed(codes.view(torch.uint8))
         scales = scales.view(torch.uint8)
-        s = _row_stride(scales)
-        if s < scales.shape[-1] or s % 4 or scales.data_ptr() % 4:
+        if not _scales_as_they_are(scales, rows):
             scales = _empty_scales(scales.shape[:-1], scales.shape[-1], scales.device).copy_(scales)
         self._set(codes, scales, fmt, rows, cols)
 
@@ -111,13 +121,13 @@ class MXTensor:
         """Blocks of a tensor of this shape, not yet written."""
         bits = _bits(fmt)
         *lead, cols = shape
-        if cols % 32 or not 32 <= cols <= _MAX:
-            raise ValueError(f"{cols} columns: a multiple of 32 up to {_MAX}")
+        if cols % 32 or not 32 <= cols <= _COLS:
+            raise ValueError(f"{cols} columns: a multiple of 32 up to {_COLS}")
         rows = 1
         for n in lead:
             rows *= n
-        if rows >= _MAX:
-            raise NotImplementedError(f"{rows} rows (below {_MAX})")
+        if rows >= _ROWS:
+            raise NotImplementedError(f"{rows} rows (below {_ROWS})")
         t = cls.__new__(cls)
         t._set(torch.empty(*lead, cols * bits // 8, dtype=torch.uint8, device=device),
                _empty_scales(lead, cols // 32, device), fmt, rows, cols)
@@ -150,7 +160,7 @@ def _floats(name: str, x: torch.Tensor) -> torch.Tensor:
         raise NotImplementedError(f"{name} of dtype {x.dtype} (fp32, fp16 or bf16)")
     if x.dim() < 1:
         raise ValueError(f"{name}: [..., cols]")
-    return _placed(x, 16)
+    return _placed(x)
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "e4m3") -> MXTensor:
@@ -191,7 +201,7 @@ def _norm(x: torch.Tensor, delta: Optional[torch.Tensor], norm_weight: torch.Ten
         raise ValueError(f"norm weight has {norm_weight.numel()} elements, rows have {x.shape[-1]}")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    w = _placed(norm_weight.to(device=x.device, dtype=torch.float32).reshape(-1).contiguous(), 16)
+    w = _placed(norm_weight.to(device=x.device, dtype=torch.float32).reshape(-1).contiguous())
     y = MXTensor.empty(x.shape, fmt, x.device)
     h = torch.empty(x.shape, dtype=torch.float32, device=x.device) if delta is not None else None
     if x.numel():
@@ -292,9 +302,21 @@ class HipMXLinear(nn.Module):
         if odt not in _DT:
             raise NotImplementedError(f"outputs of dtype {odt} (fp32, fp16 or bf16)")
         if not given:
-            x = mx_quantize(x, self.act_fmt)
+            x = _floats("x", x)
         out = torch.empty(*x.shape[:-1], self.out_features, dtype=odt, device=self.device)
-        if out.numel():
+        if not out.numel():
+            return out
+        bias = None if self._bias is None else self._bias.data_ptr()
+        if given:
             launch(self.device, "pgmoe_mx_linear", lib().pgmoe_mx_linear, self._packed.data_ptr(), self.out_features, x._ref,
-                   None if self._bias is None else self._bias.data_ptr(), out.data_ptr(), _DT[odt])
+                   bias, out.data_ptr(), _DT[odt])
+            return out
+        rows, bits = x.numel() // self.in_features, _FMT[self.act_fmt]
+        ws, n = None, 0
+        if rows > _FEW_ROWS:
+            n = int(lib().pgmoe_mx_linear_values_workspace_bytes(rows, self.in_features, bits))
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device)  # of this call alone
+        launch(self.device, "pgmoe_mx_linear_values", lib().pgmoe_mx_linear_values, self._packed.data_ptr(), self.out_features,
+               x.data_ptr(), _DT[x.dtype], _row_stride(x), rows, self.in_features, bits, bias, out.data_ptr(), _DT[odt],
+               None if ws is None else ws.data_ptr(), n)
         return out

@@ -182,7 +182,9 @@ def test_act_mul(dev, fmt, act, dtype, rows, cols):
 @pytest.mark.parametrize("M,N,K", [
     (1, 1, 32), (1, 16, 128), (2, 17, 64), (5, 30, 96), (15, 100, 160), (16, 64, 512), (17, 257, 544), (33, 130, 1440),
     (64, 96, 2048), (65, 33, 288), (77, 1001, 1440), (130, 515, 320), (200, 256, 4096), (257, 300, 640), (1, 4099, 4096),
-    (8, 2000, 8192), (300, 1030, 992), (520, 777, 1056), (1030, 513, 416)])
+    (8, 2000, 8192), (300, 1030, 992), (520, 777, 1056), (1030, 513, 416),
+    # enough outputs for the larger tiles, of 64, 128 and 256 rows
+    (700, 4099, 96), (2001, 6000, 160), (4100, 8195, 64), (2050, 8190, 544)])
 def test_product(dev, fmt, M, N, K):
     from pgmoe import HipMXLinear
     log(f"product {fmt} {M} x {N} x {K}")
@@ -199,7 +201,8 @@ def test_product(dev, fmt, M, N, K):
 
 @pytest.mark.parametrize("dtype", H.DTYPES)
 @pytest.mark.parametrize("act_fmt", FMTS)
-@pytest.mark.parametrize("M,N,K", [(1, 100, 4096), (3, 1000, 96), (8, 48, 2080), (16, 272, 512), (40, 33, 1440), (150, 300, 288)])
+@pytest.mark.parametrize("M,N,K", [(1, 100, 4096), (3, 1000, 96), (8, 48, 2080), (16, 272, 512), (17, 40, 672),
+                                   (40, 33, 1440), (150, 300, 288)])
 def test_product_of_values(dev, dtype, act_fmt, M, N, K):
     """Rows of floating-point values are brought to blocks first, whichever way the call does that."""
     from pgmoe import HipMXLinear, mx_quantize
@@ -211,8 +214,12 @@ def test_product_of_values(dev, dtype, act_fmt, M, N, K):
     out = layer((x * 0.01).to(dev), out_dtype=torch.float32)  # another call before, with other values
     out = layer(x.to(dev), out_dtype=torch.float32)
     H.check_product(out, y, s, K)
+    assert torch.equal(out, layer(mx_quantize(x.to(dev), act_fmt), out_dtype=torch.float32))
     out = layer(x.to(dev).view(M, 1, K))
     assert out.shape == (M, 1, N) and out.dtype == dtype
+    wide = torch.zeros(M, K + 64, dtype=dtype, device=dev)
+    wide[:, 32:-32] = x.to(dev)
+    assert torch.equal(layer(wide[:, 32:-32]).view(M, 1, N), out)
 
 
 def test_product_exact_sums(dev):

@@ -12,16 +12,16 @@ P = 0x10000  # an aligned address that no call reaches
 
 
 def _blocks(fmt=8, rows=4, cols=128, codes=P, scales=P, code_stride=None, scale_stride=None):
-    return _lib.Mx(codes, scales, cols if code_stride is None else code_stride, 4 if scale_stride is None else scale_stride,
+    return _lib.Mx(codes, scales, cols if code_stride is None else code_stride, 16 if scale_stride is None else scale_stride,
                    rows, cols, fmt)
 
 
 BAD_BLOCKS = [
     (dict(fmt=6), UNSUPPORTED), (dict(rows=-1), INVALID), (dict(rows=1 << 24), INVALID), (dict(cols=0), INVALID),
-    (dict(cols=48, code_stride=48), INVALID), (dict(cols=(1 << 24) + 32), INVALID), (dict(code_stride=112), INVALID),
-    (dict(code_stride=136), INVALID), (dict(scale_stride=3), INVALID), (dict(scale_stride=6), INVALID),
-    (dict(codes=None), INVALID), (dict(scales=None), INVALID), (dict(codes=P + 8), INVALID), (dict(scales=P + 2), INVALID),
-    (dict(code_stride=1 << 40), INVALID)]
+    (dict(cols=48, code_stride=48), INVALID), (dict(cols=(1 << 22) + 32, code_stride=1 << 23), INVALID), (dict(code_stride=112), INVALID),
+    (dict(code_stride=136), INVALID), (dict(scale_stride=3), INVALID), (dict(scale_stride=20), INVALID), (dict(scale_stride=1 << 24), INVALID),
+    (dict(codes=None), INVALID), (dict(scales=None), INVALID), (dict(codes=P + 8), INVALID), (dict(scales=P + 4), INVALID),
+    (dict(code_stride=1 << 40), INVALID), (dict(code_stride=(1 << 23) + 16), INVALID)]
 
 
 @pytest.mark.parametrize("kw,rc", BAD_BLOCKS)
@@ -69,6 +69,22 @@ def test_other_arguments_are_checked():
     assert L.pgmoe_mx_pack(t, P, None) == UNSUPPORTED  # weights are e2m1
     assert L.pgmoe_mx_pack(_blocks(fmt=4, code_stride=64), None, None) == INVALID
     assert L.pgmoe_mx_pack(_blocks(fmt=4, code_stride=64, rows=0), P, None) == INVALID
+
+
+def test_products_of_values():
+    """Their arguments, and the workspace of the blocks of more than 16 rows."""
+    L = _lib.lib()
+    f = L.pgmoe_mx_linear_values_workspace_bytes
+    assert f(16, 4096, 8) == f(0, 4096, 8) == 0 and f(17, 4096, 8) == 17 * (4096 + 128) and f(100, 96, 4) == 100 * (48 + 16)
+    args = dict(w=P, n=16, x=P, dt=0, stride=128, rows=4, cols=128, fmt=8, bias=None, out=P, odt=0, ws=None, bytes=0)
+    call = lambda **k: L.pgmoe_mx_linear_values(*dict(args, **k).values(), None)  # noqa: E731
+    assert call(rows=0, x=None, w=None, out=None) == OK
+    for k, rc in [(dict(x=None), INVALID), (dict(x=P + 8), INVALID), (dict(w=None), INVALID), (dict(out=None), INVALID),
+                  (dict(dt=7), UNSUPPORTED), (dict(odt=7), UNSUPPORTED), (dict(fmt=5), UNSUPPORTED), (dict(cols=100), INVALID),
+                  (dict(rows=-1), INVALID), (dict(rows=1 << 24), -3), (dict(stride=64), INVALID), (dict(stride=129), INVALID),
+                  (dict(n=0), INVALID), (dict(rows=17), -3), (dict(rows=17, ws=P, bytes=17 * 144 - 1), -3),
+                  (dict(rows=17, ws=P + 8, bytes=1 << 20), -3), (dict(bias=P + 1), INVALID)]:
+        assert call(**k) == rc, k
 
 
 def test_packed_bytes():
