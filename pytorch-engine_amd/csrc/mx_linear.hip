@@ -183,9 +183,10 @@ __device__ __forceinline__ void put4(const MxLinear& L, int m, int n, float4 v) 
 }
 
 // ---------------------------------------------------------------- up to 16 rows
-// A workgroup forms 16 NB outputs of all rows; its W waves take every W-th quad of steps, weights and activations straight
-// to registers (all of a quad's on their way at once), and their sums meet in LDS in wave order.  Bound by the weights'
-// arrival and, from few of them, by the latencies of one load, one sum and the launch.
+// A workgroup forms 16 outputs of all rows at a time; its W waves take every W-th quad of steps, weights and activations
+// straight to registers, and their sums meet in LDS in wave order.  ONE: a quad is all that a wave has (K <= 512 W): the
+// rows stay in registers, and the workgroup goes on to its next 16 outputs, whose weights are on their way meanwhile.
+// Bound by the weights' arrival and, where they are few, by the latencies of one load, one sum and the launch.
 // SRC: the rows come in blocks (-1), or as values of a PGMOE_DT_* that become blocks here: a lane holds the 32 values of
 // a block, so its largest magnitude needs no other lane.
 template <MxMode MODE, int SRC>
@@ -223,24 +224,31 @@ struct ThinX {  // one step of a lane's row
     }
 };
 
-template <MxMode MODE, int SRC, int NB, int W>
-__global__ __launch_bounds__(64 * W, 4) void mx_thin_kernel(const MxLinear L, const MxFloats F) {
-    __shared__ float4 part[W][NB][64];
+template <MxMode MODE, int SRC, int W, bool ONE>
+__global__ __launch_bounds__(64 * W, SRC >= 0 && !ONE ? 2 : 4) void mx_thin_kernel(const MxLinear L, const MxFloats F) {
+    __shared__ float4 part[2][W][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int G = mx_groups(L.N), Q = mx_quads(L.K), last = (L.K >> 5) - 1, g0 = blockIdx.x * NB;
+    const int G = mx_groups(L.N), Q = mx_quads(L.K), last = (L.K >> 5) - 1, waves = min(W, Q);
     const int m = min(r, L.M - 1);  // rows past the last repeat it, blocks past the row's last too: their weights are 0
     const uint8_t* xr = SRC < 0 ? L.x.codes + m * L.x.code_stride : (const uint8_t*)F.p + m * F.stride * (SRC == PGMOE_DT_F32 ? 4 : 2);
     const uint8_t* xsr = L.x.scales + m * L.x.scale_stride;
     const uint8_t* scales = L.w + (int64_t)G * Q * 4096;
-    floatx4 acc[NB][1];
+    struct Weights {
+        int4 w[4][1];
+        int s[1];
+    };
+    auto load_w = [&](Weights& to, int gb, int q) PG_INLINE {
+        const int64_t at = (int64_t)min(gb, G - 1) * Q + min(q, Q - 1);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) acc[b][0] = floatx4{0, 0, 0, 0};
-    for (int q = wave; q < Q; q += W) {
-        XFrag<MODE> f[4];
-        int xs[4];
-        constexpr int AHEAD = SRC == PGMOE_DT_F32 ? 2 : 3;  // steps of values in registers
+        for (int s = 0; s < 4; ++s) to.w[s][0] = *(const int4*)(L.w + at * 4096 + s * 1024 + lane * 16);
+        to.s[0] = *(const int*)(scales + at * 256 + lane * 4);
+    };
+    XFrag<MODE> f[4];
+    int xs[4];
+    auto load_x = [&](int q) PG_INLINE {
+        constexpr int AHEAD = SRC == PGMOE_DT_F32 ? 2 : 4;  // steps of values in registers
         ThinX<MODE, SRC < 0 ? PGMOE_DT_F16 : SRC> raw[AHEAD];
-        auto block = [&](int s) { return min(16 * q + 4 * s + g, last); };
+        auto block = [&](int s) PG_INLINE { return min(16 * q + 4 * s + g, last); };
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             if constexpr (SRC < 0) {
@@ -251,50 +259,76 @@ __global__ __launch_bounds__(64 * W, 4) void mx_thin_kernel(const MxLinear L, co
                 raw[s].load(xr, block(s));
             }
         }
-        int4 w[4][NB];
-        int ws[NB];
+        if constexpr (SRC >= 0) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int64_t at = (int64_t)min(g0 + b, G - 1) * Q + q;
-            ws[b] = *(const int*)(scales + at * 256 + lane * 4);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) w[s][b] = *(const int4*)(L.w + at * 4096 + s * 1024 + lane * 16);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        auto step = [&](auto sc) {
-            constexpr int s = decltype(sc)::value;
-            if constexpr (SRC >= 0) {
+            for (int s = 0; s < 4; ++s) {
                 f[s] = raw[s % AHEAD].blocks(xs[s]);
-                if constexpr (s + AHEAD < 4) raw[s % AHEAD].load(xr, block(s + AHEAD));
+                if (s + AHEAD < 4) raw[s % AHEAD].load(xr, block(s + AHEAD));
             }
-            WOps<MODE, NB> ops;
-            ops.template set<s>(w[s], ws);
-            mx_products<MODE, s, 0>(ops, ws, xs[s], f[s], 0, acc);
+        }
+    };
+    auto products = [&](const Weights& w, floatx4 (&acc)[1][1]) PG_INLINE {
+        auto step = [&](auto sc) PG_INLINE {
+            constexpr int s = decltype(sc)::value;
+            WOps<MODE, 1> ops;
+            ops.template set<s>(w.w[s], w.s);
+            mx_products<MODE, s, 0>(ops, w.s, xs[s], f[s], 0, acc);
         };
         step(std::integral_constant<int, 0>());
         step(std::integral_constant<int, 1>());
         step(std::integral_constant<int, 2>());
         step(std::integral_constant<int, 3>());
+    };
+    Weights w;
+    if (wave < waves) {
+        load_w(w, blockIdx.x, wave);
+        if constexpr (ONE) load_x(wave);
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) part[wave][b][lane] = make_float4(acc[b][0][0], acc[b][0][1], acc[b][0][2], acc[b][0][3]);
-    __syncthreads();
-    for (int i = threadIdx.x; i < NB * 64; i += 64 * W) {
-        const int b = i >> 6, l = i & 63;
-        float4 v = part[0][b][l];
-#pragma unroll
-        for (int k = 1; k < W; ++k) {
-            const float4 p = part[k][b][l];
-            v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
+    int turn = 0;
+    for (int gb = blockIdx.x; gb < G; gb += gridDim.x, ++turn) {
+        if (wave < waves) {
+            floatx4 acc[1][1] = {{floatx4{0, 0, 0, 0}}};
+            Weights next;
+            if constexpr (ONE) {
+                load_w(next, gb + gridDim.x, wave);
+                products(w, acc);
+            } else {
+#pragma unroll 1
+                for (int q = wave; q < Q; q += W) {
+                    load_w(next, q + W < Q ? gb : gb + gridDim.x, q + W < Q ? q + W : wave);
+                    load_x(q);
+                    products(w, acc);
+                    if (q + W < Q) w = next;
+                }
+            }
+            w = next;
+            part[turn & 1][wave][lane] = make_float4(acc[0][0][0], acc[0][0][1], acc[0][0][2], acc[0][0][3]);
         }
-        const int n = 16 * (g0 + b) + 4 * (l >> 4);
-        if ((l & 15) < L.M && n < L.N) put4(L, l & 15, n, v);
+        // (no wait for loads and stores; a buffer is written again behind the next barrier, which its reader passes too)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (wave == turn % W) {
+            float4 v = part[turn & 1][0][lane];
+            for (int k = 1; k < waves; ++k) {
+                const float4 p = part[turn & 1][k][lane];
+                v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
+            }
+            const int n = 16 * gb + 4 * g;
+            if (r < L.M && n < L.N) put4(L, r, n, v);
+        }
     }
 }
 
+// Workgroups: as many as stay on the card at once where each goes on to further outputs.  Four waves where K has no more
+// quads (8 rows of 2048 inputs, 151936 outputs: 60 us with eight waves, half of them idle).
 template <MxMode MODE, int SRC>
 static int thin_launch(const MxLinear& L, const MxFloats& F, hipStream_t st) {
-    PG_LAUNCH((mx_thin_kernel<MODE, SRC, 2, 8>), dim3(div_up(mx_groups(L.N), 2)), dim3(64 * 8), 0, st, L, F);
+    const int G = mx_groups(L.N), Q = mx_quads(L.K);
+    if (Q <= 4)
+        PG_LAUNCH((mx_thin_kernel<MODE, SRC, 4, true>), dim3(std::min(G, 4 * kCUs)), dim3(256), 0, st, L, F);
+    else if (Q <= 8)
+        PG_LAUNCH((mx_thin_kernel<MODE, SRC, 8, true>), dim3(std::min(G, 2 * kCUs)), dim3(512), 0, st, L, F);
+    else
+        PG_LAUNCH((mx_thin_kernel<MODE, SRC, 8, false>), dim3(std::min(G, 2 * kCUs)), dim3(512), 0, st, L, F);
     return check_launch("mx_thin");
 }
 

@@ -37,9 +37,10 @@ _FEW_ROWS = 16  # up to so many rows of values become blocks inside the product,
 
 
 def _bits(fmt: str) -> int:
-    if fmt not in _FMT:
+    bits = _FMT.get(fmt)
+    if bits is None:
         raise NotImplementedError(f"block format {fmt!r} (e4m3 or e2m1)")
-    return _FMT[fmt]
+    return bits
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -60,18 +61,14 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.shape[-1] if step is None else step
 
 
-def _placed(t: torch.Tensor, align: int = 16) -> torch.Tensor:
-    """t, or a contiguous copy, with rows that begin at multiples of `align` bytes, do not overlap and lie within
-    2^23 bytes of each other."""
-    s = _row_stride(t) * t.element_size()
-    if s < t.shape[-1] * t.element_size() or s % align or s > _STRIDE or t.data_ptr() % align:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _empty_scales(lead: Sequence[int], blocks: int, device: torch.device) -> torch.Tensor:
-    """uint8 [..., blocks] whose rows begin at multiples of 16 bytes, as the kernels read so many at once."""
-    return torch.empty(*lead, (blocks + 15) // 16 * 16, dtype=torch.uint8, device=device)[..., :blocks]
+def _placed(t: torch.Tensor, align: int = 16) -> Tuple[torch.Tensor, int]:
+    """t, or a contiguous copy, with rows that begin at multiples of `align` bytes, do not overlap and lie within 2^23
+    bytes of each other; and the elements from row to row."""
+    n, size = t.shape[-1], t.element_size()
+    s = n if t.is_contiguous() else _row_stride(t)
+    if s < n or s * size % align or s * size > _STRIDE or t.data_ptr() % align:
+        return t.clone(memory_format=torch.contiguous_format), n
+    return t, s
 
 
 def _scales_as_they_are(t: torch.Tensor, rows: int) -> bool:
@@ -82,132 +79,154 @@ def _scales_as_they_are(t: torch.Tensor, rows: int) -> bool:
     return t.storage_offset() + max(rows - 1, 0) * s + n <= t.untyped_storage().nbytes()
 
 
+def _sizes(rows: int, cols: int) -> None:
+    if cols % 32 or not 32 <= cols <= _COLS:
+        raise ValueError(f"{cols} columns: a multiple of 32 up to {_COLS}")
+    if rows >= _ROWS:
+        raise NotImplementedError(f"{rows} rows (below {_ROWS})")
+
+
 class MXTensor:
     """Rows in microscaled blocks: `codes` uint8 (or float8_e4m3fn) [..., cols], for e2m1 [..., cols / 2] with the even
     value of a pair in the low four bits; `scales` uint8 (or float8_e8m0fnu) [..., cols / 32], E + 127 each; `fmt`
     "e4m3" or "e2m1".  Tensors whose rows the kernels can read where they are are kept, not copied."""
 
+    __slots__ = ("_codes", "_scales", "_fmt", "_shape", "_device", "_buf", "_c", "_ref")
+
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str = "e4m3") -> None:
-        per = 8 // _bits(fmt)
-        if codes.dtype not in (torch.uint8, torch.float8_e4m3fn) or (per == 2 and codes.dtype != torch.uint8):
+        bits = _bits(fmt)
+        if codes.dtype != torch.uint8 and not (bits == 8 and codes.dtype == torch.float8_e4m3fn):
             raise ValueError(f"codes of dtype {codes.dtype} (uint8, for e4m3 also float8_e4m3fn)")
         if scales.dtype not in (torch.uint8, torch.float8_e8m0fnu):
             raise ValueError(f"scales of dtype {scales.dtype} (uint8 or float8_e8m0fnu)")
         if codes.device.type != "cuda" or scales.device != codes.device:
             raise ValueError("pgmoe blocks: codes and scales on one HIP device")
-        if codes.dim() < 1:
+        if codes.dim() < 1 or codes.shape[-1] < 1:
             raise ValueError("codes: [..., cols]")
-        cols = codes.shape[-1] * per
-        if cols % 32 or not 32 <= cols <= _COLS:
-            raise ValueError(f"{cols} columns: a multiple of 32 up to {_COLS}")
+        cols, rows = codes.shape[-1] * 8 // bits, codes.numel() // codes.shape[-1]
+        _sizes(rows, cols)
         if tuple(scales.shape) != (*codes.shape[:-1], cols // 32):
             raise ValueError(f"scales {tuple(scales.shape)} of codes {tuple(codes.shape)} ({fmt})")
-        rows = codes.numel() // codes.shape[-1]
-        if rows >= _ROWS:
-            raise NotImplementedError(f"{rows} rows (below {_ROWS})")
-        codes = _placed(codes.view(torch.uint8))
+        codes, stride = _placed(codes.view(torch.uint8))
         scales = scales.view(torch.uint8)
         if not _scales_as_they_are(scales, rows):
-            scales = _empty_scales(scales.shape[:-1], scales.shape[-1], scales.device).copy_(scales)
-        self._set(codes, scales, fmt, rows, cols)
+            held = torch.empty(*scales.shape[:-1], (cols // 32 + 15) // 16 * 16, dtype=torch.uint8, device=scales.device)
+            scales = held[..., :cols // 32].copy_(scales)
+        self._codes, self._scales, self._buf = codes, scales, None
+        self._set((*codes.shape[:-1], cols), fmt, codes.device,
+                  Mx(codes.data_ptr(), scales.data_ptr(), stride, _row_stride(scales), rows, cols, bits))
 
-    def _set(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, rows: int, cols: int) -> None:
-        self._codes, self._scales, self._fmt = codes, scales, fmt
-        self._c = Mx(codes.data_ptr(), scales.data_ptr(), _row_stride(codes), _row_stride(scales), rows, cols, _FMT[fmt])
-        self._ref = ctypes.byref(self._c)
+    def _set(self, shape: Tuple[int, ...], fmt: str, device: torch.device, c: Mx) -> None:
+        self._shape, self._fmt, self._device, self._c, self._ref = shape, fmt, device, c, ctypes.byref(c)
 
     @classmethod
-    def empty(cls, shape: Sequence[int], fmt: str, device: torch.device) -> "MXTensor":
-        """Blocks of a tensor of this shape, not yet written."""
-        bits = _bits(fmt)
-        *lead, cols = shape
-        if cols % 32 or not 32 <= cols <= _COLS:
-            raise ValueError(f"{cols} columns: a multiple of 32 up to {_COLS}")
-        rows = 1
-        for n in lead:
-            rows *= n
-        if rows >= _ROWS:
-            raise NotImplementedError(f"{rows} rows (below {_ROWS})")
+    def _new(cls, shape: Tuple[int, ...], rows: int, fmt: str, device: torch.device) -> "MXTensor":
+        """Blocks of a tensor of this shape, not yet written: one allocation, whose tensors are made when asked for."""
+        bits, cols = _bits(fmt), shape[-1]
+        _sizes(rows, cols)
+        cs, ss = cols * bits // 8, (cols // 32 + 15) // 16 * 16
         t = cls.__new__(cls)
-        t._set(torch.empty(*lead, cols * bits // 8, dtype=torch.uint8, device=device),
-               _empty_scales(lead, cols // 32, device), fmt, rows, cols)
+        t._codes = t._scales = None
+        t._buf = torch.empty(rows * (cs + ss), dtype=torch.uint8, device=device)
+        at = t._buf.data_ptr()
+        t._set(shape, fmt, device, Mx(at, at + rows * cs, cs, ss, rows, cols, bits))
         return t
 
-    # as they were given: the kernels read what the struct of them says
-    codes = property(lambda self: self._codes)
-    scales = property(lambda self: self._scales)
-    fmt = property(lambda self: self._fmt)
-    device = property(lambda self: self._codes.device)
+    def _rows_of(self, width: int, step: int, offset: int) -> torch.Tensor:
+        strides = [1]
+        for n in reversed(self._shape[:-1]):
+            strides.append(step)
+            step *= n
+        return self._buf.as_strided((*self._shape[:-1], width), strides[::-1], offset)
 
     @property
-    def shape(self) -> Tuple[int, ...]:
-        return (*self._codes.shape[:-1], self._c.cols)
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._rows_of(self._c.code_stride, self._c.code_stride, 0)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            c = self._c
+            self._scales = self._rows_of(c.cols // 32, c.scale_stride, c.rows * c.code_stride)
+        return self._scales
+
+    # as they were given: the kernels read what the struct of them says
+    fmt = property(lambda self: self._fmt)
+    shape = property(lambda self: self._shape)
+    device = property(lambda self: self._device)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values code * 2^E, each rounded once to `dtype` (fp32, fp16, bf16)."""
         if dtype not in _DT:
             raise NotImplementedError(f"values of dtype {dtype} (fp32, fp16 or bf16)")
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        if out.numel():
-            launch(self.device, "pgmoe_mx_dequantize", lib().pgmoe_mx_dequantize, self._ref, out.data_ptr(), _DT[dtype])
+        out = torch.empty(self._shape, dtype=dtype, device=self._device)
+        if self._c.rows:
+            launch(self._device, "pgmoe_mx_dequantize", lib().pgmoe_mx_dequantize, self._ref, out.data_ptr(), _DT[dtype])
         return out
 
 
-def _floats(name: str, x: torch.Tensor) -> torch.Tensor:
-    if x.device.type != "cuda":
+def _floats(name: str, x: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """(x or a copy that the kernels read, elements from row to row, rows)."""
+    if not x.is_cuda:
         raise ValueError(f"{name}: a tensor on a HIP device")
     if x.dtype not in _DT:
         raise NotImplementedError(f"{name} of dtype {x.dtype} (fp32, fp16 or bf16)")
-    if x.dim() < 1:
+    if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name}: [..., cols]")
-    return _placed(x)
+    x, stride = _placed(x)
+    return x, stride, x.numel() // x.shape[-1]
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "e4m3") -> MXTensor:
     """x [..., cols] (fp32, fp16, bf16) in blocks of 32 along its rows."""
-    x = _floats("x", x)
-    y = MXTensor.empty(x.shape, fmt, x.device)
-    if x.numel():
-        launch(x.device, "pgmoe_mx_quantize", lib().pgmoe_mx_quantize, x.data_ptr(), _DT[x.dtype], _row_stride(x), y._ref)
+    x, stride, rows = _floats("x", x)
+    dev = x.device
+    y = MXTensor._new(tuple(x.shape), rows, fmt, dev)
+    if rows:
+        launch(dev, "pgmoe_mx_quantize", lib().pgmoe_mx_quantize, x.data_ptr(), _DT[x.dtype], stride, y._ref)
     return y
 
 
 def exec_fused_act_mul_mx(gate: torch.Tensor, up: torch.Tensor, act: str = "silu", fmt: str = "e4m3") -> MXTensor:
     """act(gate) * up in blocks, act "silu" or "gelu" (tanh form), formed in fp32 from two tensors of one shape and type
     (the halves of a fused projection's output are taken as they are)."""
-    if act not in _ACT:
+    code = _ACT.get(act)
+    if code is None:
         raise NotImplementedError(f"activation {act!r} (silu or gelu)")
     if up.shape != gate.shape or up.dtype != gate.dtype or up.device != gate.device:
         raise ValueError(f"up {tuple(up.shape)} {up.dtype} beside gate {tuple(gate.shape)} {gate.dtype}: one shape, type and device")
-    gate, up = _floats("gate", gate), _floats("up", up)
-    y = MXTensor.empty(gate.shape, fmt, gate.device)
-    if gate.numel():
-        launch(gate.device, "pgmoe_mx_act_mul", lib().pgmoe_mx_act_mul, gate.data_ptr(), _row_stride(gate), up.data_ptr(),
-               _row_stride(up), _DT[gate.dtype], _ACT[act], y._ref)
+    gate, gs, rows = _floats("gate", gate)
+    up, us, _ = _floats("up", up)
+    dev = gate.device
+    y = MXTensor._new(tuple(gate.shape), rows, fmt, dev)
+    if rows:
+        launch(dev, "pgmoe_mx_act_mul", lib().pgmoe_mx_act_mul, gate.data_ptr(), gs, up.data_ptr(), us, _DT[gate.dtype], code,
+               y._ref)
     return y
 
 
 def _norm(x: torch.Tensor, delta: Optional[torch.Tensor], norm_weight: torch.Tensor, eps: float, fmt: str):
-    x = _floats("x", x)
-    if not x.is_contiguous():
-        x = x.contiguous()
+    x, _, rows = _floats("x", x.contiguous())
+    dev, cols = x.device, x.shape[-1]
     if delta is not None:
-        if delta.shape != x.shape or delta.device != x.device:
-            raise ValueError(f"delta {tuple(delta.shape)} on {delta.device} beside x {tuple(x.shape)} on {x.device}")
-        delta = _floats("delta", delta)
-        if not delta.is_contiguous():
-            delta = delta.contiguous()
-    if norm_weight.numel() != x.shape[-1]:
-        raise ValueError(f"norm weight has {norm_weight.numel()} elements, rows have {x.shape[-1]}")
+        if delta.shape != x.shape or delta.device != dev:
+            raise ValueError(f"delta {tuple(delta.shape)} on {delta.device} beside x {tuple(x.shape)} on {dev}")
+        delta, _, _ = _floats("delta", delta.contiguous())
+    if norm_weight.numel() != cols:
+        raise ValueError(f"norm weight has {norm_weight.numel()} elements, rows have {cols}")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    w = _placed(norm_weight.to(device=x.device, dtype=torch.float32).reshape(-1).contiguous())
-    y = MXTensor.empty(x.shape, fmt, x.device)
-    h = torch.empty(x.shape, dtype=torch.float32, device=x.device) if delta is not None else None
-    if x.numel():
-        launch(x.device, "pgmoe_add_rmsnorm_mx", lib().pgmoe_add_rmsnorm_mx, x.data_ptr(), _DT[x.dtype],
+    w = norm_weight
+    if w.dtype != torch.float32 or w.device != dev or not w.is_contiguous() or w.data_ptr() % 16:
+        w = norm_weight.to(device=dev, dtype=torch.float32, copy=True).reshape(-1).contiguous()
+    y = MXTensor._new(tuple(x.shape), rows, fmt, dev)
+    h = torch.empty(x.shape, dtype=torch.float32, device=dev) if delta is not None else None
+    if rows:
+        launch(dev, "pgmoe_add_rmsnorm_mx", lib().pgmoe_add_rmsnorm_mx, x.data_ptr(), _DT[x.dtype],
                None if delta is None else delta.data_ptr(), 0 if delta is None else _DT[delta.dtype], w.data_ptr(),
-               float(eps), None if h is None else h.data_ptr(), y._ref)
+               eps, None if h is None else h.data_ptr(), y._ref)
     return h, y
 
 
@@ -225,7 +244,7 @@ def exec_fused_add_rmsnorm_mx(x: torch.Tensor, delta: torch.Tensor, norm_weight:
 def _gguf_blocks(raw: np.ndarray, rows: int, cols: int, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of GGUF MXFP4 bytes: 17 a block, the scale's and 16 of codes, byte j holding values j (low) and
     j + 16 (high)."""
-    b = torch.from_numpy(np.ascontiguousarray(raw)).to(device).reshape(rows, cols // 32, 17)
+    b = torch.from_numpy(np.array(raw)).to(device).reshape(rows, cols // 32, 17)
     v = torch.cat((b[..., 1:] & 15, b[..., 1:] >> 4), -1)
     return (v[..., 0::2] | v[..., 1::2] << 4).reshape(rows, cols // 2), b[..., 0].contiguous()
 
@@ -293,30 +312,35 @@ class HipMXLinear(nn.Module):
             return cls(MXTensor(torch.cat(codes), torch.cat(scales), "e2m1"), bias=bias, act_fmt=act_fmt)
 
     def forward(self, x: Union[torch.Tensor, MXTensor], out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        shape, n = x.shape, self.in_features
+        if shape[-1] != n:
+            raise ValueError(f"{shape[-1]} input features, the layer has {n}")
+        dev = self.device
+        if x.device != dev:
+            raise ValueError(f"input on {x.device}, the layer is on {dev}")
         given = isinstance(x, MXTensor)
-        if x.shape[-1] != self.in_features:
-            raise ValueError(f"{x.shape[-1]} input features, the layer has {self.in_features}")
-        if x.device != self.device:
-            raise ValueError(f"input on {x.device}, the layer is on {self.device}")
         odt = out_dtype if out_dtype is not None else torch.float16 if given else x.dtype
-        if odt not in _DT:
+        code = _DT.get(odt)
+        if code is None:
             raise NotImplementedError(f"outputs of dtype {odt} (fp32, fp16 or bf16)")
         if not given:
-            x = _floats("x", x)
-        out = torch.empty(*x.shape[:-1], self.out_features, dtype=odt, device=self.device)
-        if not out.numel():
+            x, stride, rows = _floats("x", x)
+        else:
+            rows = x._c.rows
+        out = torch.empty((*shape[:-1], self.out_features), dtype=odt, device=dev)
+        if not rows:
             return out
         bias = None if self._bias is None else self._bias.data_ptr()
         if given:
-            launch(self.device, "pgmoe_mx_linear", lib().pgmoe_mx_linear, self._packed.data_ptr(), self.out_features, x._ref,
-                   bias, out.data_ptr(), _DT[odt])
+            launch(dev, "pgmoe_mx_linear", lib().pgmoe_mx_linear, self._packed.data_ptr(), self.out_features, x._ref, bias,
+                   out.data_ptr(), code)
             return out
-        rows, bits = x.numel() // self.in_features, _FMT[self.act_fmt]
-        ws, n = None, 0
+        bits = _FMT[self.act_fmt]
+        ws, nbytes = None, 0
         if rows > _FEW_ROWS:
-            n = int(lib().pgmoe_mx_linear_values_workspace_bytes(rows, self.in_features, bits))
-            ws = torch.empty(n, dtype=torch.uint8, device=self.device)  # of this call alone
-        launch(self.device, "pgmoe_mx_linear_values", lib().pgmoe_mx_linear_values, self._packed.data_ptr(), self.out_features,
-               x.data_ptr(), _DT[x.dtype], _row_stride(x), rows, self.in_features, bits, bias, out.data_ptr(), _DT[odt],
-               None if ws is None else ws.data_ptr(), n)
+            nbytes = rows * (n * bits // 8 + (n // 32 + 15) // 16 * 16)  # pgmoe_mx_linear_values_workspace_bytes
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # of this call alone
+        launch(dev, "pgmoe_mx_linear_values", lib().pgmoe_mx_linear_values, self._packed.data_ptr(), self.out_features,
+               x.data_ptr(), _DT[x.dtype], stride, rows, n, bits, bias, out.data_ptr(), code,
+               None if ws is None else ws.data_ptr(), nbytes)
         return out
