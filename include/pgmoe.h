@@ -458,7 +458,8 @@ int pgmoe_mx_pack(const pgmoe_mx* w, void* dst, void* stream);
  * packed weights of out_features rows of x.cols, x in e4m3 or e2m1 blocks; products summed in fp32 in a fixed order
  * and rounded once.  16-bit outputs of more than 16 rows of e4m3 blocks take the matrix cores' 8-bit form, which cuts
  * the products of 8 neighbouring inputs below 2^-13 of the largest of them (2e-5 of the outputs' 2-norm); fp32 outputs
- * and up to 16 rows do not, and take an activation beyond fp32's range as an infinity. */
+ * and up to 16 rows do not, and take a value beyond fp32's range as an infinity, one below 2^-126 to the nearest
+ * multiple of 2^-133. */
 int pgmoe_mx_linear(const void* packed, int32_t out_features, const pgmoe_mx* x, const float* bias, void* out,
                     int32_t out_dtype, void* stream);
 

@@ -45,7 +45,7 @@ def _bits(fmt: str) -> int:
 
 def _row_stride(t: torch.Tensor) -> int:
     """Elements from one row of t [..., n] to the next as one matrix of rows; -1 if there is no such number."""
-    if t.dim() == 1 or t.numel() == 0:
+    if t.numel() == 0:
         return t.shape[-1]
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         return -1

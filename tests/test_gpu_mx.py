@@ -122,6 +122,23 @@ def test_quantize_takes_views(dev, fmt):
 
 # ---------------------------------------------------------------- norm and activation
 @pytest.mark.parametrize("fmt", FMTS)
+def test_vectors_with_gaps(dev, fmt):
+    """A single row whose elements do not lie next to each other: of values, codes and scale bytes."""
+    from pgmoe import HipMXLinear, MXTensor, exec_fused_act_mul_mx, mx_quantize
+    x = _spread(1, 2048, 10).to(dev)[0, ::2]
+    t = mx_quantize(x, fmt)
+    codes, e = H.encode(x.cpu()[None], fmt)
+    assert torch.equal(H.scales(t), e) and torch.equal(H.unpack(t), codes)
+    gap = lambda v: torch.stack((v, torch.full_like(v, 3)), 1).flatten()[::2]  # noqa: E731
+    again = MXTensor(gap(t.codes), gap(t.scales), fmt)
+    assert torch.equal(again.dequantize(), t.dequantize())
+    for act in ("silu", "gelu"):
+        assert torch.equal(exec_fused_act_mul_mx(x, x, act, fmt).codes, exec_fused_act_mul_mx(x.contiguous(), x.contiguous(), act, fmt).codes)
+    layer = HipMXLinear(_random_blocks(40, 1024, "e2m1", 11)[0], act_fmt=fmt)
+    assert torch.equal(layer(x), layer(x.contiguous()))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("rows,cols,dt,ddt", [
     (1, 32, torch.float32, None), (1, 4096, torch.float32, torch.float32), (5, 160, torch.float16, torch.bfloat16),
     (9, 288, torch.bfloat16, torch.float32), (3, 1440, torch.float32, torch.float16), (2, 5120, torch.float16, None),
@@ -142,6 +159,24 @@ def test_norm(dev, fmt, rows, cols, dt, ddt):
         assert got.dtype == torch.float32 and torch.equal(got.cpu(), h)
     h = h.double()
     H.check_blocks(t, h / (h.square().mean(-1, keepdim=True) + 1e-5).sqrt() * w.double(), NORM_REL)
+
+
+def test_norm_of_very_many_wide_rows(dev):
+    """More rows of a width that takes a workgroup of 1024 threads each than one launch has threads for."""
+    from pgmoe import exec_fused_rmsnorm_mx
+    rows, cols = (1 << 22) + 5, 4128
+    if torch.cuda.mem_get_info(dev)[0] < (rows * cols * 4):
+        pytest.skip("needs 70 GB")
+    x = torch.zeros(rows, cols, dtype=torch.float16, device=dev)
+    at = torch.tensor([0, 1, (1 << 21) + 7, (1 << 22) - 2, (1 << 22) - 1, 1 << 22, rows - 1])
+    some = _spread(len(at), cols, 14, torch.float16)
+    x[at.to(dev)] = some.to(dev)
+    w = torch.randn(cols, generator=torch.Generator().manual_seed(15)).to(dev)
+    t = exec_fused_rmsnorm_mx(x, w)
+    few = exec_fused_rmsnorm_mx(some.to(dev), w)
+    assert torch.equal(t.codes[at.to(dev)], few.codes) and torch.equal(t.scales[at.to(dev)], few.scales)
+    # the other rows are 0 w: zeros of w's sign
+    assert not (t.codes[2:64] & 127).any() and not (t.codes[rows - 4:rows - 1] & 127).any()
 
 
 def test_norm_rows_of_zeros_and_not_finite_ones(dev):
@@ -254,6 +289,37 @@ def test_product_of_nan_blocks(dev, fmt, M):
     want = torch.zeros(M, N, dtype=torch.bool)
     want[M // 2], want[M - 1], want[:, 17] = True, True, True
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("M", [1, 16, 20, 70, 300])
+def test_product_of_nan_codes(dev, M):
+    """The e4m3 codes 0x7f and 0xff are NaN, whatever their block's scale."""
+    from pgmoe import HipMXLinear, MXTensor
+    N, K = 70, 416
+    w, _ = _random_blocks(N, K, "e2m1", 4)
+    x, _ = _random_blocks(M, K, "e4m3", 5)
+    c = x.codes.clone()
+    c[M // 2, 3], c[M - 1, K - 1] = 0x7f, 0xff
+    x = MXTensor(c, x.scales, "e4m3")
+    want = torch.zeros(M, dtype=torch.bool)
+    want[M // 2], want[M - 1] = True, True
+    assert torch.equal(torch.isnan(x.dequantize().cpu()).any(1), want)
+    for dt in H.DTYPES:
+        assert torch.equal(torch.isnan(HipMXLinear(w)(x, out_dtype=dt)).cpu(), want[:, None].expand(M, N)), dt
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M", [1, 16, 20, 70, 300])
+@pytest.mark.parametrize("xs,ws", [(3, 250), (10, 244), (30, 210), (130, 110), (240, 24), (246, 3)])
+def test_product_of_far_scales(dev, fmt, M, xs, ws):
+    """Rows near the ends of fp32's normal range against weights near the other end: nothing is lost on the way."""
+    from pgmoe import HipMXLinear
+    N, K = 90, 288
+    w, w64 = _random_blocks(N, K, "e2m1", 12, ws, ws + 1)
+    x, x64 = _random_blocks(M, K, fmt, 13, xs, xs + 1)
+    y, s = H.product(x64, w64)
+    for dt in (torch.float32, torch.bfloat16):
+        H.check_product(HipMXLinear(w)(x, out_dtype=dt), y, s, K, cut=fmt == "e4m3" and dt != torch.float32)
 
 
 def test_product_takes_views_of_blocks(dev):
