@@ -59,41 +59,35 @@ __device__ __forceinline__ float gated(float g) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-z));
 }
 
-// ACT < 0: the blocks of x; 0: of silu(x) u; 1: of gelu(x) u (tanh form).
-// U chunks a thread, all of their loads on the way before the first is used.
-template <int DT, bool E2M1, int ACT, int U>
+// ACT < 0: the blocks of x; 0: of silu(x) u; 1: of gelu(x) u (tanh form).  A chunk a thread: with four (their loads on the way
+// at once) 4096 x 12288 fp16 took as long, 28.8 us for 28.1 (5.4 TB/s) and 48.1 for 45.8 gated (5.5 TB/s), 64 x 4096 3.3 for 2.7.
+template <int DT, bool E2M1, int ACT>
 __global__ __launch_bounds__(kMxThreads) void mx_rows_kernel(const void* __restrict__ x, int64_t xs, const void* __restrict__ u,
                                                             int64_t us, FastDiv cpr, uint32_t chunks, MxRows y) {
     constexpr int N = Chunk<DT>::N;
     constexpr int B = DT == PGMOE_DT_F32 ? 4 : 2;
-    const uint32_t first = blockIdx.x * (uint32_t)(kMxThreads * U) + threadIdx.x;
-    uint4 a[U], b[ACT >= 0 ? U : 1];
-    uint32_t row[U], col[U];
+    const uint32_t own = blockIdx.x * (uint32_t)kMxThreads + threadIdx.x;
+    const uint32_t n = min(own, chunks - 1);  // lanes past the end repeat the last chunk: whole waves meet in mx_encode
+    const uint32_t row = cpr.div(n), col = n - row * cpr.d;
+    const uint4 a = *(const uint4*)((const uint8_t*)x + ((int64_t)row * xs + (int64_t)col * N) * B);
+    float v[N];
+    if constexpr (ACT >= 0) {
+        const uint4 b = *(const uint4*)((const uint8_t*)u + ((int64_t)row * us + (int64_t)col * N) * B);
+        float w[N];
+        widen<DT>(a, v);
+        widen<DT>(b, w);
 #pragma unroll
-    for (int j = 0; j < U; ++j) {  // lanes past the end repeat the last chunk: whole waves meet in mx_encode
-        const uint32_t n = min(first + j * kMxThreads, chunks - 1);
-        row[j] = cpr.div(n);
-        col[j] = n - row[j] * cpr.d;
-        a[j] = *(const uint4*)((const uint8_t*)x + ((int64_t)row[j] * xs + (int64_t)col[j] * N) * B);
-        if constexpr (ACT >= 0) b[j] = *(const uint4*)((const uint8_t*)u + ((int64_t)row[j] * us + (int64_t)col[j] * N) * B);
+        for (int i = 0; i < N; ++i) v[i] = gated<ACT>(v[i]) * w[i];
+    } else {
+        widen<DT>(a, v);
     }
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-        float v[N];
-        widen<DT>(a[j], v);
-        if constexpr (ACT >= 0) {
-            float w[N];
-            widen<DT>(b[j], w);
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = gated<ACT>(v[i]) * w[i];
-        }
-        uint32_t code[E2M1 ? (N + 7) / 8 : N / 4];
-        int scale;
-        mx_encode<E2M1, N>(v, code, scale);
-        if (first + j * kMxThreads < chunks) put_codes<E2M1, N>(y, row[j], (int)col[j], code, scale);
-    }
+    uint32_t code[E2M1 ? (N + 7) / 8 : N / 4];
+    int scale;
+    mx_encode<E2M1, N>(v, code, scale);
+    if (own < chunks) put_codes<E2M1, N>(y, row, (int)col, code, scale);
 }
 
+// 4096 x 4096 to fp16: 9.7 us (5.2 TB/s) from 8 bits, 8.9 (4.8) from 4; 12288 x 4096 of 4 bits to fp32 36.5 (6.2).
 template <bool E2M1>
 __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(MxRows x, FastDiv cpr, uint32_t chunks, void* __restrict__ out,
                                                                   int odt) {
@@ -106,12 +100,9 @@ __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(MxRows x, Fas
     float v[8];
     if constexpr (E2M1) {
         const uint32_t w = *(const uint32_t*)p;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {  // sign, two exponent bits, one of the mantissa
-            const uint32_t k = (w >> (4 * i)) & 15, m = k & 7;
-            const float a = m < 2 ? 0.5f * (float)m : __builtin_bit_cast(float, (((m >> 1) + 126u) << 23) | ((m & 1) << 22));
-            v[i] = k & 8 ? -a : a;
-        }
+        const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+        const auto d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+        v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = d[0], v[5] = d[1], v[6] = f[0], v[7] = f[1];
     } else {
         const uint2 w = *(const uint2*)p;
         const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, true);
@@ -267,12 +258,8 @@ static int rows_launch(const MxFloats& x, const MxFloats& u, const MxRows& y, hi
         const void* xp = (const uint8_t*)x.p + r * x.stride * B;
         const void* up = u.p ? (const uint8_t*)u.p + r * u.stride * B : nullptr;
         const MxRows z = rows_from(y, r, n);
-        if (chunks >= 4 * 256 * kMxThreads)
-            PG_LAUNCH((mx_rows_kernel<DT, E2M1, ACT, 4>), dim3(div_up(chunks, 4 * kMxThreads)), dim3(kMxThreads), 0, st, xp,
-                      x.stride, up, u.stride, cpr, chunks, z);
-        else
-            PG_LAUNCH((mx_rows_kernel<DT, E2M1, ACT, 1>), dim3(div_up(chunks, kMxThreads)), dim3(kMxThreads), 0, st, xp,
-                      x.stride, up, u.stride, cpr, chunks, z);
+        PG_LAUNCH((mx_rows_kernel<DT, E2M1, ACT>), dim3(div_up(chunks, kMxThreads)), dim3(kMxThreads), 0, st, xp, x.stride, up,
+                  u.stride, cpr, chunks, z);
         return check_launch("mx_rows");
     });
 }
@@ -310,8 +297,7 @@ int launch_mx_dequantize(const MxRows& x, void* out, int odt, hipStream_t st) {
     });
 }
 
-// Threads a row: 64 up to 512 columns and 256 up to 4096, where the row stays in registers, then 1024 (1 row of 4096, with
-// its launch: 3.8 us with 256 threads).  Rows of one launch: as many as 2^31 threads.
+// Rows of one launch: as many as 2^31 threads.
 template <int T, int VPT>
 static int norm_launch(const void* x, int xdt, const void* delta, int ddt, const float* w, float eps, float* h_out, const MxRows& y,
                        hipStream_t st) {
@@ -333,12 +319,18 @@ static int norm_launch(const void* x, int xdt, const void* delta, int ddt, const
 int launch_add_rmsnorm_mx(const void* x, int xdt, const void* delta, int ddt, const float* w, float eps, float* h_out,
                           const MxRows& y, hipStream_t st) {
     const int n4 = y.cols >> 2;
+    // 4 threads' work or less each while it fills workgroups of 256, more threads where a row is a CU's only one: 4096 columns,
+    // fp32 and fp32, with 256 / 1024 threads: 1 row 4.3 / 3.4 us, 256 6.4 / 5.2, 700 9.5 / 8.9, 1024 11.5 / 11.7, 4003 41.4
+    // (5.2 TB/s) / 44.3; 2048 columns, 1 row 3.2 / 3.1, 1024 7.4 / 8.4.  8192 columns in two chunks a thread or four of half the
+    // threads: 1 row 4.3 / 5.7, 4003 79.7 (5.4 TB/s) / 85.7; 16384 in registers 152, read twice 203.
 #define NORM(T, V) return norm_launch<T, V>(x, xdt, delta, ddt, w, eps, h_out, y, st)
     if (n4 <= 64) NORM(64, 1);
     if (n4 <= 128) NORM(64, 2);
     if (n4 <= 256) NORM(256, 1);
     if (n4 <= 512) NORM(256, 2);
-    if (n4 <= 1024) NORM(256, 4);
+    if (n4 <= 1024 && y.rows > 768) NORM(256, 4);
+    if (n4 <= 1024) NORM(1024, 1);
+    if (n4 <= 2048) NORM(1024, 2);
     if (n4 <= 4096) NORM(1024, 4);
     NORM(1024, 0);
 #undef NORM

@@ -628,20 +628,20 @@ struct MxCost {
     int bm, bn;
     float a, b;
 };
-constexpr int kMxTiles = 4;
-static int pick_tile(const MxCost (&c)[kMxTiles], int M, int N) {
-    int best = kMxTiles - 1;
+template <int TILES>
+static int pick_tile(const MxCost (&c)[TILES], int M, int N) {
+    int best = TILES - 1;
     float least = 0.0f;
-    for (int i = kMxTiles - 1; i >= 0; --i) {
+    for (int i = TILES - 1; i >= 0; --i) {
         const int64_t tiles = (int64_t)div_up(M, c[i].bm) * div_up(N, c[i].bn);
         const float t = c[i].a + c[i].b * (float)((tiles + kCUs - 1) / kCUs);
-        if (i == kMxTiles - 1 || t < least) best = i, least = t;
+        if (i == TILES - 1 || t < least) best = i, least = t;
     }
     return best;
 }
 
 static int linear_s8(const MxLinear& L, hipStream_t st) {
-    static constexpr MxCost cost[kMxTiles] = {{128, 256, 9.6f, 23.4f}, {128, 128, 8.0f, 13.8f}, {64, 128, 5.0f, 8.3f}, {32, 128, 3.5f, 5.1f}};
+    static constexpr MxCost cost[] = {{128, 256, 9.6f, 23.4f}, {128, 128, 8.0f, 13.8f}, {64, 128, 5.0f, 8.3f}, {32, 128, 3.5f, 5.1f}};
     switch (pick_tile(cost, L.M, L.N)) {
         case 0: return gemm_launch<kS8, 4, 8, 2, 2, 2, false, 2>(L, st);
         case 1: return gemm_launch<kS8, 4, 4, 2, 2, 3, false, 2>(L, st);
@@ -650,7 +650,7 @@ static int linear_s8(const MxLinear& L, hipStream_t st) {
     }
 }
 static int linear_s4(const MxLinear& L, hipStream_t st) {
-    static constexpr MxCost cost[kMxTiles] = {{256, 256, 5.0f, 35.8f}, {128, 128, 6.5f, 9.9f}, {64, 128, 4.0f, 6.1f}, {32, 128, 4.0f, 5.0f}};
+    static constexpr MxCost cost[] = {{256, 256, 5.0f, 35.8f}, {128, 128, 6.5f, 9.9f}, {64, 128, 4.0f, 6.1f}, {32, 128, 4.0f, 5.0f}};
     switch (pick_tile(cost, L.M, L.N)) {
         case 0: return gemm_launch<kS4, 8, 4, 2, 4, 2, false, 2>(L, st);
         case 1: return gemm_launch<kS4, 4, 4, 2, 2, 2, false, 2>(L, st);
@@ -658,12 +658,11 @@ static int linear_s4(const MxLinear& L, hipStream_t st) {
         default: return gemm_launch<kS4, 2, 2, 1, 4, 3, true, 2>(L, st);
     }
 }
-static int linear_b8(const MxLinear& L, hipStream_t st) {  // 128 x 128 twice: 64 x 256 measured the same (107 for 108 at n = 4)
-    static constexpr MxCost cost[kMxTiles] = {{128, 128, 10.0f, 24.5f}, {128, 128, 10.0f, 24.5f}, {64, 128, 8.0f, 13.8f}, {32, 128, 6.0f, 8.3f}};
+static int linear_b8(const MxLinear& L, hipStream_t st) {
+    static constexpr MxCost cost[] = {{64, 256, 10.0f, 24.5f}, {64, 128, 8.0f, 13.8f}, {32, 128, 6.0f, 8.3f}};
     switch (pick_tile(cost, L.M, L.N)) {
-        case 0:
-        case 1: return gemm_launch<kB8, 4, 4, 2, 2, 3, false, 2>(L, st);
-        case 2: return gemm_launch<kB8, 4, 2, 1, 4, 2, false, 4>(L, st);
+        case 0: return gemm_launch<kB8, 4, 4, 1, 4, 2, false, 2>(L, st);
+        case 1: return gemm_launch<kB8, 4, 2, 1, 4, 2, false, 4>(L, st);
         default: return gemm_launch<kB8, 2, 2, 1, 4, 4, true, 2>(L, st);
     }
 }

@@ -161,6 +161,18 @@ def test_norm(dev, fmt, rows, cols, dt, ddt):
     H.check_blocks(t, h / (h.square().mean(-1, keepdim=True) + 1e-5).sqrt() * w.double(), NORM_REL)
 
 
+@pytest.mark.parametrize("rows,cols", [(769, 4096), (900, 2080), (768, 4096)])
+def test_norm_of_many_rows(dev, rows, cols):
+    """Both divisions of a row among threads, beside each other's sizes."""
+    from pgmoe import exec_fused_add_rmsnorm_mx
+    x, d = _spread(rows, cols, 16, torch.bfloat16, 1.0), _spread(rows, cols, 17, torch.float32, 1.0)
+    w = torch.randn(cols, generator=torch.Generator().manual_seed(18))
+    h, t = exec_fused_add_rmsnorm_mx(x.to(dev), d.to(dev), w.to(dev))
+    assert torch.equal(h.cpu(), x.float() + d)
+    h64 = h.cpu().double()
+    H.check_blocks(t, h64 / torch.sqrt((h64 * h64).mean(-1, keepdim=True) + 1e-6) * w.double(), NORM_REL)
+
+
 def test_norm_of_very_many_wide_rows(dev):
     """More rows of a width that takes a workgroup of 1024 threads each than one launch has threads for."""
     from pgmoe import exec_fused_rmsnorm_mx
