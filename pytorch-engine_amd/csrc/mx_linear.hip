@@ -9,9 +9,9 @@
 // With 4-bit activations the instruction's sums are exact to fp32.  With 8-bit ones it cuts the products of 8 neighbouring
 // inputs below 2^-13 of the largest of them (2^10 + 2^-4 gives 2^10) before it adds them up: 1.6e-5 of the outputs'
 // 2-norm at 500 x 4096 x 4096, far below what a 16-bit output keeps, and above an fp32 one.  fp32 outputs of 8-bit
-// activations therefore take the bf16 instruction (16x16x32, cut at 2^-24): code times power of two is exact in bf16, and
-// v_cvt_scalef32_pk_bf16_fp4 / _fp8 makes two of them at once.  Lane l then holds inputs 32 g .. 32 g + 31 of both, eight to
-// each of four instructions.
+// activations, and up to 16 rows, where it costs nothing, therefore take the bf16 instruction (16x16x32, cut at 2^-24): code
+// times power of two is exact in bf16, and v_cvt_scalef32_pk_bf16_fp4 / _fp8 makes two of them at once.  Lane l then holds
+// inputs 32 g .. 32 g + 31 of both, eight to each of four instructions.
 //
 // Packed weights: (16 rows x 128 inputs) tiles of 1 KB, lane l's 16 bytes at 16 l, K / 128 steps rounded up to a multiple
 // of 4 a row group; behind all of them the scales, 256 bytes for 16 rows x 512 inputs: lane l's four bytes at 4 l,
@@ -186,7 +186,9 @@ __device__ __forceinline__ void put4(const MxLinear& L, int m, int n, float4 v) 
 // A workgroup forms 16 outputs of all rows at a time; its W waves take every W-th quad of steps, weights and activations
 // straight to registers, and their sums meet in LDS in wave order.  ONE: a quad is all that a wave has (K <= 512 W): the
 // rows stay in registers, and the workgroup goes on to its next 16 outputs, whose weights are on their way meanwhile.
-// Bound by the weights' arrival and, where they are few, by the latencies of one load, one sum and the launch.
+// Bound by the weights' arrival and, where they are few, by the latencies of one load, one sum and the launch: 1 x 4096 x 24576,
+// fp16 values, 11.5 us (4.7 TB/s), 8 x 2048 x 151936 35.2 (4.8), 16 x 4096 x 12288 8.7.  ONE, the weights of the next outputs under
+// way during the sum of these: 11.5 for 18.7 us; 35.2 for 44.
 // SRC: the rows come in blocks (-1), or as values of a PGMOE_DT_* that become blocks here: a lane holds the 32 values of
 // a block, so its largest magnitude needs no other lane.
 template <MxMode MODE, int SRC>
@@ -336,10 +338,19 @@ static int thin_launch(const MxLinear& L, const MxFloats& F, hipStream_t st) {
 // A workgroup forms BM x BN outputs in WM x WN waves of 16 MT x 16 NT.  Activations and weights come through a ring of
 // RING stages in LDS (128 bytes an activation row: 128 inputs in 8 bits, 256 in 4), copied straight from memory RING - 1
 // stages ahead, so that a chain of stages runs at the rate of the products and not at a memory latency each.  At the top of stage
-// s a wave waits until its copies of stage s + 1 have landed, and the barrier makes all waves' visible: the first
-// fragments of s + 1 are then read under the last products of s.  Chunk c (16 bytes) of activation row r lies at
+// s a wave waits until its copies of stage s have landed (EARLY: of s + 1), and the barrier makes all waves' visible; EARLY,
+// the first fragments of s + 1 are then read under the last products of s.  Chunk c (16 bytes) of activation row r lies at
 // c ^ (r / 2 & 7): the 16 rows of a fragment fall on different banks.  Weights lie as they are packed.  Scales of 512 inputs
 // come with the first of their stages: 16 bytes an activation row, which become a word a lane and row, a byte a step.
+//
+// WK parts of a workgroup, WM x WN waves and a ring each, share out the quads of the inputs, and their sums meet in LDS in
+// the parts' order.  They are for few tiles: a CU then has more waves to hide a wait with and more copies under way, and smaller
+// tiles spread the weights over more CUs (a CU takes in some 28 bytes a ns from memory, 110 from its L2).  77 x 4096 x 4096, 8
+// bits: 96 tiles of 32 x 128 10.2 us, 192 of 32 x 64 in two parts 7.9; fp32 15.6, in four parts 9.3; 4 bits 8.3, in four 6.6.
+//
+// What bounds it: many rows the instruction, whose rate the power budget sets (random codes in registers alone: 4.0 PFLOP/s with
+// 8-bit activations, 7.2 with 4-bit; 4096 x 24576 x 4096 runs at 2.6 and 4.4); fp32 outputs the conversions beside the products
+// (96 and 32 instructions a stage of a 64 x 128 tile: 1.3 of 2.0 PFLOP/s); few rows the weights' way to the CUs and the launch.
 // Copies of 1 KB from memory to LDS, lane l's 16 bytes at base + off to lds + 16 l, each STEP behind the one before.  By
 // hand, so that the compiler counts no loads and adds no waits; a copy reads m0 one wait state after its write.
 #define PG_COPY(off, base) "s_nop 0\n\tglobal_load_lds_dwordx4 " off ", " base "\n\t"
@@ -390,7 +401,7 @@ __device__ __forceinline__ void stage_ready() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <MxMode MODE, int MT, int NT, int WM, int WN, int RING, bool EARLY>
+template <MxMode MODE, int MT, int NT, int WM, int WN, int WK, int RING, bool EARLY>
 struct MxTile {
     static constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN, NW = WM * WN;
     static constexpr int SPS = MODE == kS4 ? 2 : 1;            // steps a stage
@@ -401,7 +412,8 @@ struct MxTile {
     static constexpr int SPARTS = SROWS / 64 + SCOLS / 64, SC = (SPARTS + NW - 1) / NW;  // copies of scales: in all, a wave
     static constexpr int SB = (SROWS + SCOLS) * 16;
     static constexpr int NS = (RING - 1) / SPQ + 1;            // quads whose scales are held
-    static constexpr int LDS = RING * STAGE + NS * SB;
+    static constexpr int PART = RING * STAGE + NS * SB, LDS = WK * PART;
+    static_assert(LDS >= (WK - 1) * BM * BN * 4, "sums of the other parts");
     static_assert(XC * 8 * NW == BM && WC * NW * 1024 == WB, "copies of a stage over the waves");
     // fragments read ahead: a step's, where registers hold two steps of them
     static constexpr bool WHOLE = EARLY && MT * NT <= 8;
@@ -427,16 +439,19 @@ __device__ __forceinline__ void mx_tile_of(int id, int tiles_m, int tiles_n, int
     tn = in / high;
 }
 
-template <MxMode MODE, int MT, int NT, int WM, int WN, int RING, bool EARLY, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void mx_gemm_kernel(const MxLinear L, const int tiles_m, const int tiles_n) {
-    using T = MxTile<MODE, MT, NT, WM, WN, RING, EARLY>;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[T::LDS];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+template <MxMode MODE, int MT, int NT, int WM, int WN, int WK, int RING, bool EARLY, int OCC>
+__global__ __launch_bounds__(64 * WM * WN * WK, OCC) void mx_gemm_kernel(const MxLinear L, const int tiles_m, const int tiles_n) {
+    using T = MxTile<MODE, MT, NT, WM, WN, WK, RING, EARLY>;
+    __shared__ __attribute__((aligned(1024))) uint8_t all[T::LDS];
+    const int lane = threadIdx.x & 63, own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int part = own / T::NW, wave = own % T::NW;
+    uint8_t* smem = all + part * T::PART;
     int tm, tn;
     mx_tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * T::BM, g0 = tn * (T::BN / 16);
     const int wm = wave % WM, wn = wave / WM;
     const int G = mx_groups(L.N), Q = mx_quads(L.K), blocks = L.K >> 5, stages = Q * T::SPQ;
+    const int each = (Q + WK - 1) / WK, first = part * each, end = min(first + each, Q);  // quads of a part
     const uint32_t row_bytes = MODE == kS4 ? L.K >> 1 : L.K;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
 
@@ -545,11 +560,11 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx_gemm_kernel(const MxLine
         }
     };
 
-    copy_scales(0);
+    copy_scales(first);
 #pragma unroll
     for (int s = 0; s < RING - 1; ++s) {
-        if (s && s % T::SPQ == 0) copy_scales(s / T::SPQ);
-        copy_stage(min(s, stages - 1), s);
+        if (s && s % T::SPQ == 0) copy_scales(first + s / T::SPQ);
+        copy_stage(min(first * T::SPQ + s, stages - 1), s);
     }
     int slot = 0;
     if constexpr (EARLY) {
@@ -558,7 +573,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx_gemm_kernel(const MxLine
         for (int k = 0; k < T::AHEAD; ++k) f[0][k] = get_x(0, 0, k);
         get_w(w[0], 0, 0);
     }
-    if constexpr (T::WHOLE) read_scales(0);
+    if constexpr (T::WHOLE) read_scales(first);
     // stage J of quad q
     auto stage = [&](auto jc, int q) PG_INLINE {
         constexpr int J = decltype(jc)::value;
@@ -590,7 +605,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx_gemm_kernel(const MxLine
         }
         slot = after;
     };
-    for (int q = 0; q < Q; ++q) {
+    for (int q = first; q < end; ++q) {
         stage(std::integral_constant<int, 0>(), q);
         stage(std::integral_constant<int, 1>(), q);
         if constexpr (T::SPQ == 4) {
@@ -598,7 +613,30 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx_gemm_kernel(const MxLine
             stage(std::integral_constant<int, 3>(), q);
         }
     }
+    if constexpr (WK > 1)
+        for (int n = (each - max(end - first, 0)) * T::SPQ; n > 0; --n) asm volatile("s_barrier" ::: "memory");  // a part with fewer
     stage_ready<0>();  // copies that nothing reads, before the LDS is another workgroup's
+    if constexpr (WK > 1) {  // the parts' sums, in their order
+        float4* sums = (float4*)all + wave * 64 + lane;
+        auto at = [&](int p, int b, int t) PG_INLINE { return (((p - 1) * NT + b) * MT + t) * T::NW * 64; };
+        if (part > 0) {
+#pragma unroll
+            for (int b = 0; b < NT; ++b)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) sums[at(part, b, t)] = make_float4(acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]);
+        }
+        __syncthreads();
+        if (part > 0) return;
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int p = 1; p < WK; ++p) {
+                    const float4 v = sums[at(p, b, t)];
+                    acc[b][t] += floatx4{v.x, v.y, v.z, v.w};
+                }
+    }
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int m = m0 + (wm * MT + t) * 16 + r;
@@ -610,20 +648,21 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx_gemm_kernel(const MxLine
     }
 }
 
-template <MxMode MODE, int MT, int NT, int WM, int WN, int RING, bool EARLY, int OCC>
+template <MxMode MODE, int MT, int NT, int WM, int WN, int WK, int RING, bool EARLY, int OCC>
 static int gemm_launch(const MxLinear& L, hipStream_t st) {
-    using T = MxTile<MODE, MT, NT, WM, WN, RING, EARLY>;
+    using T = MxTile<MODE, MT, NT, WM, WN, WK, RING, EARLY>;
     const int tm = div_up(L.M, T::BM), tn = div_up(L.N, T::BN);
-    PG_LAUNCH((mx_gemm_kernel<MODE, MT, NT, WM, WN, RING, EARLY, OCC>), dim3(tm * tn), dim3(64 * T::NW), 0, st, L, tm, tn);
+    PG_LAUNCH((mx_gemm_kernel<MODE, MT, NT, WM, WN, WK, RING, EARLY, OCC>), dim3(tm * tn), dim3(64 * T::NW * WK), 0, st, L, tm, tn);
     return check_launch("mx_gemm");
 }
 
-// Which tile: the one whose fit a + b ceil(tiles / CUs) to the times measured is least.  us at K = 4096, where tiles a CU is
-// n (other K change both alike):
-//   8 bits  128 x 256 33 / 55 / 103 at n = 1 / 2 / 4, 128 x 128 22 / 35 / 61, 64 x 128 14 / 20 / 38, 32 x 128 12 / 14 / 25
-//   4 bits  256 x 256 41 / 77 at 1 / 2, 128 x 128 17 / 26 / 46 at 1 / 2 / 4, 64 x 128 13 / 16 / 30, 32 x 128 12 / 13 / 23
-//   fp32    128 x 128 36 / 57 / 108, 64 x 128 22 / 35 / 61, 32 x 128 15 / 23 / 39
-// e.g. 1024 rows, 8 bits: 4096 outputs 33.2 / 21.8 / 20.7 / 24.9 by tile from the largest, 8192 36.5 / 33.5 / 37.1 / 43.6.
+// Which tile: the one whose fit a + b ceil(tiles / CUs) to the times measured is least.  us at K = 4096 (other K change all
+// alike) for n tiles a CU, n = 1 / 2 / 4:
+//   8 bits  128 x 256 33 / 52 / 100, 128 x 128 22 / 35 / 63, 64 x 128 14 / 22 / 39, 32 x 128 11 / 14 / 26, 32 x 64 8.2 / 11 / 19
+//   4 bits  256 x 256 41 / 77, 128 x 128 17 / 27 / 47, 64 x 64 9.5 / 12.7 / 22, 32 x 128 11.8 / 13 / 24, 32 x 64 7.4 / 13 / 24
+//   fp32    64 x 256 35 / 58 / 115, 64 x 128 21 / 34 / 62, 32 x 128 14 / 22 / 40, 32 x 64 9.8 / 14 / 25
+// The choice against the best of them, 8 bits, outputs x 4096: 128 rows, 4096: 8.2 (others 10.6 / 13 / 20 / 33); 500: 14.5 (14.1
+// to 33); 1024: 22.7 (22.2 to 34); 4096: 56.5 (57 to 122); fp32 500: 21.9 (21.2 to 35).
 struct MxCost {
     int bm, bn;
     float a, b;
@@ -641,34 +680,37 @@ static int pick_tile(const MxCost (&c)[TILES], int M, int N) {
 }
 
 static int linear_s8(const MxLinear& L, hipStream_t st) {
-    static constexpr MxCost cost[] = {{128, 256, 9.6f, 23.4f}, {128, 128, 8.0f, 13.8f}, {64, 128, 5.0f, 8.3f}, {32, 128, 3.5f, 5.1f}};
+    static constexpr MxCost cost[] = {{128, 256, 9.6f, 23.4f}, {128, 128, 8.0f, 13.8f}, {64, 128, 6.0f, 8.1f}, {32, 128, 5.5f, 5.1f}, {32, 64, 4.8f, 3.5f}};
     switch (pick_tile(cost, L.M, L.N)) {
-        case 0: return gemm_launch<kS8, 4, 8, 2, 2, 2, false, 2>(L, st);
-        case 1: return gemm_launch<kS8, 4, 4, 2, 2, 3, false, 2>(L, st);
-        case 2: return gemm_launch<kS8, 4, 2, 1, 4, 4, true, 2>(L, st);
-        default: return gemm_launch<kS8, 2, 2, 1, 4, 4, true, 2>(L, st);
+        case 0: return gemm_launch<kS8, 4, 8, 2, 2, 1, 2, false, 2>(L, st);
+        case 1: return gemm_launch<kS8, 4, 4, 2, 2, 1, 3, false, 2>(L, st);
+        case 2: return gemm_launch<kS8, 4, 2, 1, 4, 1, 4, true, 2>(L, st);
+        case 3: return gemm_launch<kS8, 2, 2, 1, 4, 1, 4, true, 2>(L, st);
+        default: return gemm_launch<kS8, 2, 2, 1, 2, 2, 4, true, 2>(L, st);
     }
 }
 static int linear_s4(const MxLinear& L, hipStream_t st) {
-    static constexpr MxCost cost[] = {{256, 256, 5.0f, 35.8f}, {128, 128, 6.5f, 9.9f}, {64, 128, 4.0f, 6.1f}, {32, 128, 4.0f, 5.0f}};
+    static constexpr MxCost cost[] = {{256, 256, 5.0f, 35.8f}, {128, 128, 6.5f, 9.9f}, {64, 64, 5.5f, 3.9f}, {32, 128, 6.5f, 4.5f}, {32, 64, 2.2f, 5.4f}};
     switch (pick_tile(cost, L.M, L.N)) {
-        case 0: return gemm_launch<kS4, 8, 4, 2, 4, 2, false, 2>(L, st);
-        case 1: return gemm_launch<kS4, 4, 4, 2, 2, 2, false, 2>(L, st);
-        case 2: return gemm_launch<kS4, 4, 2, 1, 4, 2, false, 4>(L, st);
-        default: return gemm_launch<kS4, 2, 2, 1, 4, 3, true, 2>(L, st);
+        case 0: return gemm_launch<kS4, 8, 4, 2, 4, 1, 2, false, 2>(L, st);
+        case 1: return gemm_launch<kS4, 4, 4, 2, 2, 1, 2, false, 2>(L, st);
+        case 2: return gemm_launch<kS4, 4, 1, 1, 4, 2, 2, false, 2>(L, st);
+        case 3: return gemm_launch<kS4, 2, 2, 1, 4, 1, 3, true, 2>(L, st);
+        default: return gemm_launch<kS4, 2, 1, 1, 4, 4, 2, false, 4>(L, st);
     }
 }
 static int linear_b8(const MxLinear& L, hipStream_t st) {
-    static constexpr MxCost cost[] = {{64, 256, 10.0f, 24.5f}, {64, 128, 8.0f, 13.8f}, {32, 128, 6.0f, 8.3f}};
+    static constexpr MxCost cost[] = {{64, 256, 10.0f, 24.5f}, {64, 128, 7.0f, 13.5f}, {32, 128, 5.5f, 8.3f}, {32, 64, 5.0f, 4.9f}};
     switch (pick_tile(cost, L.M, L.N)) {
-        case 0: return gemm_launch<kB8, 4, 4, 1, 4, 2, false, 2>(L, st);
-        case 1: return gemm_launch<kB8, 4, 2, 1, 4, 2, false, 4>(L, st);
-        default: return gemm_launch<kB8, 2, 2, 1, 4, 4, true, 2>(L, st);
+        case 0: return gemm_launch<kB8, 4, 4, 1, 4, 1, 2, false, 2>(L, st);
+        case 1: return gemm_launch<kB8, 4, 2, 1, 4, 2, 2, false, 2>(L, st);
+        case 2: return gemm_launch<kB8, 2, 2, 1, 4, 2, 2, false, 2>(L, st);
+        default: return gemm_launch<kB8, 2, 2, 1, 2, 4, 2, false, 4>(L, st);
     }
 }
 
-// Up to 16 rows are read against weights that go straight to registers (17 of 12288 x 4096: 12.0 us in two such tiles, 9 in
-// one of 32 rows; 16: 8.7).  There the bf16 instruction costs nothing, as the weights' arrival bounds both.
+// Up to 16 rows are read against weights that go straight to registers (17 of 12288 x 4096: 12.0 us in two such tiles, 8.6 in
+// tiles of 32 rows; 16: 8.7).  There the bf16 instruction costs nothing, as the weights' arrival bounds both.
 int launch_mx_linear(const MxLinear& L, hipStream_t st) {
     if (L.M <= kMxFewRows) return L.x.e2m1 ? thin_launch<kS4, -1>(L, MxFloats{}, st) : thin_launch<kB8, -1>(L, MxFloats{}, st);
     if (L.x.e2m1) return linear_s4(L, st);
