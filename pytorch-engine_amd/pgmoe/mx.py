@@ -61,14 +61,15 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.shape[-1] if step is None else step
 
 
-def _placed(t: torch.Tensor, align: int = 16) -> Tuple[torch.Tensor, int]:
-    """t, or a contiguous copy, with rows that begin at multiples of `align` bytes, do not overlap and lie within 2^23
-    bytes of each other; and the elements from row to row."""
-    n, size = t.shape[-1], t.element_size()
+def _placed(t: torch.Tensor, n: int, size: int) -> Tuple[torch.Tensor, int, int]:
+    """t [..., n] of `size` bytes an element, or a contiguous copy, with rows that begin at multiples of 16 bytes, do not
+    overlap and lie within 2^23 bytes of each other; the elements from row to row; its address."""
     s = n if t.is_contiguous() else _row_stride(t)
-    if s < n or s * size % align or s * size > _STRIDE or t.data_ptr() % align:
-        return t.clone(memory_format=torch.contiguous_format), n
-    return t, s
+    p = t.data_ptr()
+    if s < n or (s * size | p) & 15 or s * size > _STRIDE:
+        t = t.clone(memory_format=torch.contiguous_format)
+        return t, n, t.data_ptr()
+    return t, s, p
 
 
 def _scales_as_they_are(t: torch.Tensor, rows: int) -> bool:
@@ -107,14 +108,14 @@ class MXTensor:
         _sizes(rows, cols)
         if tuple(scales.shape) != (*codes.shape[:-1], cols // 32):
             raise ValueError(f"scales {tuple(scales.shape)} of codes {tuple(codes.shape)} ({fmt})")
-        codes, stride = _placed(codes.view(torch.uint8))
+        codes, stride, at = _placed(codes.view(torch.uint8), codes.shape[-1], 1)
         scales = scales.view(torch.uint8)
         if not _scales_as_they_are(scales, rows):
             held = torch.empty(*scales.shape[:-1], (cols // 32 + 15) // 16 * 16, dtype=torch.uint8, device=scales.device)
             scales = held[..., :cols // 32].copy_(scales)
         self._codes, self._scales, self._buf = codes, scales, None
         self._set((*codes.shape[:-1], cols), fmt, codes.device,
-                  Mx(codes.data_ptr(), scales.data_ptr(), stride, _row_stride(scales), rows, cols, bits))
+                  Mx(at, scales.data_ptr(), stride, _row_stride(scales), rows, cols, bits))
 
     def _set(self, shape: Tuple[int, ...], fmt: str, device: torch.device, c: Mx) -> None:
         self._shape, self._fmt, self._device, self._c, self._ref = shape, fmt, device, c, ctypes.byref(c)
@@ -124,7 +125,7 @@ class MXTensor:
         """Blocks of a tensor of this shape, not yet written: one allocation, whose tensors are made when asked for."""
         bits, cols = _bits(fmt), shape[-1]
         _sizes(rows, cols)
-        cs, ss = cols * bits // 8, (cols // 32 + 15) // 16 * 16
+        cs, ss = cols * bits >> 3, cols // 32 + 15 & -16
         t = cls.__new__(cls)
         t._codes = t._scales = None
         t._buf = torch.empty(rows * (cs + ss), dtype=torch.uint8, device=device)
@@ -133,6 +134,8 @@ class MXTensor:
         return t
 
     def _rows_of(self, width: int, step: int, offset: int) -> torch.Tensor:
+        if len(self._shape) == 2:
+            return self._buf.as_strided((self._shape[0], width), (step, 1), offset)
         strides = [1]
         for n in reversed(self._shape[:-1]):
             strides.append(step)
@@ -167,25 +170,27 @@ class MXTensor:
         return out
 
 
-def _floats(name: str, x: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
-    """(x or a copy that the kernels read, elements from row to row, rows)."""
+def _floats(name: str, x: torch.Tensor) -> Tuple[torch.Tensor, int, int, int, int]:
+    """(x or a copy that the kernels read, its type's code, its address, elements from row to row, rows)."""
     if not x.is_cuda:
         raise ValueError(f"{name}: a tensor on a HIP device")
-    if x.dtype not in _DT:
+    dt, shape = _DT.get(x.dtype), x.shape
+    if dt is None:
         raise NotImplementedError(f"{name} of dtype {x.dtype} (fp32, fp16 or bf16)")
-    if x.dim() < 1 or x.shape[-1] < 1:
+    if not shape or shape[-1] < 1:
         raise ValueError(f"{name}: [..., cols]")
-    x, stride = _placed(x)
-    return x, stride, x.numel() // x.shape[-1]
+    n = shape[-1]
+    x, stride, at = _placed(x, n, 4 if dt == 0 else 2)
+    return x, dt, at, stride, x.numel() // n
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "e4m3") -> MXTensor:
     """x [..., cols] (fp32, fp16, bf16) in blocks of 32 along its rows."""
-    x, stride, rows = _floats("x", x)
+    x, dt, at, stride, rows = _floats("x", x)
     dev = x.device
     y = MXTensor._new(tuple(x.shape), rows, fmt, dev)
     if rows:
-        launch(dev, "pgmoe_mx_quantize", lib().pgmoe_mx_quantize, x.data_ptr(), _DT[x.dtype], stride, y._ref)
+        launch(dev, "pgmoe_mx_quantize", lib().pgmoe_mx_quantize, at, dt, stride, y._ref)
     return y
 
 
@@ -197,36 +202,36 @@ def exec_fused_act_mul_mx(gate: torch.Tensor, up: torch.Tensor, act: str = "silu
         raise NotImplementedError(f"activation {act!r} (silu or gelu)")
     if up.shape != gate.shape or up.dtype != gate.dtype or up.device != gate.device:
         raise ValueError(f"up {tuple(up.shape)} {up.dtype} beside gate {tuple(gate.shape)} {gate.dtype}: one shape, type and device")
-    gate, gs, rows = _floats("gate", gate)
-    up, us, _ = _floats("up", up)
+    gate, dt, g, gs, rows = _floats("gate", gate)
+    up, _, u, us, _ = _floats("up", up)
     dev = gate.device
     y = MXTensor._new(tuple(gate.shape), rows, fmt, dev)
     if rows:
-        launch(dev, "pgmoe_mx_act_mul", lib().pgmoe_mx_act_mul, gate.data_ptr(), gs, up.data_ptr(), us, _DT[gate.dtype], code,
-               y._ref)
+        launch(dev, "pgmoe_mx_act_mul", lib().pgmoe_mx_act_mul, g, gs, u, us, dt, code, y._ref)
     return y
 
 
 def _norm(x: torch.Tensor, delta: Optional[torch.Tensor], norm_weight: torch.Tensor, eps: float, fmt: str):
-    x, _, rows = _floats("x", x.contiguous())
-    dev, cols = x.device, x.shape[-1]
+    x, dt, at, _, rows = _floats("x", x.contiguous())
+    dev, shape = x.device, x.shape
+    cols = shape[-1]
+    d, ddt = None, 0
     if delta is not None:
-        if delta.shape != x.shape or delta.device != dev:
-            raise ValueError(f"delta {tuple(delta.shape)} on {delta.device} beside x {tuple(x.shape)} on {dev}")
-        delta, _, _ = _floats("delta", delta.contiguous())
-    if norm_weight.numel() != cols:
-        raise ValueError(f"norm weight has {norm_weight.numel()} elements, rows have {cols}")
+        if delta.shape != shape or delta.device != dev:
+            raise ValueError(f"delta {tuple(delta.shape)} on {delta.device} beside x {tuple(shape)} on {dev}")
+        delta, ddt, d, _, _ = _floats("delta", delta.contiguous())
+    w = norm_weight
+    if w.numel() != cols:
+        raise ValueError(f"norm weight has {w.numel()} elements, rows have {cols}")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    w = norm_weight
     if w.dtype != torch.float32 or w.device != dev or not w.is_contiguous() or w.data_ptr() % 16:
         w = norm_weight.to(device=dev, dtype=torch.float32, copy=True).reshape(-1).contiguous()
-    y = MXTensor._new(tuple(x.shape), rows, fmt, dev)
-    h = torch.empty(x.shape, dtype=torch.float32, device=dev) if delta is not None else None
+    y = MXTensor._new(tuple(shape), rows, fmt, dev)
+    h = torch.empty(shape, dtype=torch.float32, device=dev) if delta is not None else None
     if rows:
-        launch(dev, "pgmoe_add_rmsnorm_mx", lib().pgmoe_add_rmsnorm_mx, x.data_ptr(), _DT[x.dtype],
-               None if delta is None else delta.data_ptr(), 0 if delta is None else _DT[delta.dtype], w.data_ptr(),
-               eps, None if h is None else h.data_ptr(), y._ref)
+        launch(dev, "pgmoe_add_rmsnorm_mx", lib().pgmoe_add_rmsnorm_mx, at, dt, d, ddt, w.data_ptr(), eps,
+               None if h is None else h.data_ptr(), y._ref)
     return h, y
 
 
@@ -324,7 +329,7 @@ class HipMXLinear(nn.Module):
         if code is None:
             raise NotImplementedError(f"outputs of dtype {odt} (fp32, fp16 or bf16)")
         if not given:
-            x, stride, rows = _floats("x", x)
+            x, dt, at, stride, rows = _floats("x", x)
         else:
             rows = x._c.rows
         out = torch.empty((*shape[:-1], self.out_features), dtype=odt, device=dev)
@@ -341,6 +346,6 @@ class HipMXLinear(nn.Module):
             nbytes = rows * (n * bits // 8 + (n // 32 + 15) // 16 * 16)  # pgmoe_mx_linear_values_workspace_bytes
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # of this call alone
         launch(dev, "pgmoe_mx_linear_values", lib().pgmoe_mx_linear_values, self._packed.data_ptr(), self.out_features,
-               x.data_ptr(), _DT[x.dtype], stride, rows, n, bits, bias, out.data_ptr(), code,
+               at, dt, stride, rows, n, bits, bias, out.data_ptr(), code,
                None if ws is None else ws.data_ptr(), nbytes)
         return out
