@@ -296,6 +296,8 @@ class HipMXLinear(nn.Module):
         with _load_lock, torch.cuda.device(device):
             for name in [weight_name] if isinstance(weight_name, str) else weight_name:
                 info = gguf_file.tensors[name]
+                if len(info.shape) != 2:
+                    raise ValueError(f"{name}: a matrix, not {tuple(info.shape)}")
                 rows, cols, qt = int(info.shape[0]), int(info.shape[1]), int(info.qtype)
                 if cols % 32:
                     raise ValueError(f"{name}: {cols} input features (a multiple of 32)")

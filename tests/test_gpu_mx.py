@@ -269,6 +269,28 @@ def test_product_of_values(dev, dtype, act_fmt, M, N, K):
     assert torch.equal(layer(wide[:, 32:-32]).view(M, 1, N), out)
 
 
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", torch.float32), ("e4m3", torch.float16), ("e2m1", torch.float32)])
+@pytest.mark.parametrize("K", [32, 512, 544, 1056, 1536, 2080, 4128])
+def test_product_of_few_tiles(dev, fmt, dtype, K):
+    """The inputs shared out among parts of a workgroup, some of which have fewer or none."""
+    from pgmoe import HipMXLinear
+    for M, N in [(17, 16), (40, 70), (65, 130), (90, 300), (260, 520)]:
+        w, w64 = _random_blocks(N, K, "e2m1", M + K)
+        x, x64 = _random_blocks(M, K, fmt, M)
+        layer = HipMXLinear(w, bias=torch.arange(N, dtype=torch.float32, device=dev))
+        y, s = H.product(x64, w64, torch.arange(N))
+        out = layer(x, out_dtype=dtype)
+        assert torch.equal(layer(x, out_dtype=dtype), out)
+        # sums of 65520 and more, half a step past the largest, are infinities in fp16: those within the sum's own error
+        # (as in check_product, before its rounding) of that may be
+        over = torch.isinf(out.cpu())
+        error = (K / 128 + 17) * 2.0 ** -21 * s[0] + 2.0 ** -10 * s[1]
+        assert not over.any() or dtype == torch.float16
+        assert (y.abs() + error)[over].ge(65520).all() and torch.equal(out.cpu()[over] > 0, y[over] > 0)
+        out, y = out.cpu().masked_fill(over, 0), y.masked_fill(over, 0)
+        H.check_product(out, y, s, K, cut=fmt == "e4m3" and dtype != torch.float32)
+
+
 def test_product_exact_sums(dev):
     """Small whole numbers: every order of the sum is exact, so every output is, in each way the work is laid out."""
     from pgmoe import HipMXLinear, MXTensor
@@ -348,6 +370,34 @@ def test_product_takes_views_of_blocks(dev):
     x, _ = _random_blocks(60, 128, "e4m3", 9)
     assert layer(MXTensor(x.codes.view(3, 4, 5, 128), x.scales.view(3, 4, 5, 4), "e4m3")).shape == (3, 4, 5, 40)
     assert layer(MXTensor(x.codes[:0], x.scales[:0], "e4m3")).shape == (0, 40)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_room_between_rows_is_left_alone(dev, fmt):
+    """Blocks written at strides of the caller's: nothing lands between the rows, before or behind them."""
+    import ctypes
+    from pgmoe import exec_fused_act_mul_mx, exec_fused_rmsnorm_mx, mx_quantize
+    from pgmoe._lib import Mx, check, lib
+    st = torch.cuda.current_stream().cuda_stream
+    for rows, cols in [(1, 32), (3, 96), (70, 544), (9, 4128)]:
+        n, bits = cols if fmt == "e4m3" else cols // 2, 8 if fmt == "e4m3" else 4
+        cs, ss = (n + 15) // 16 * 16 + 32, (cols // 32 + 15) // 16 * 16 + 16
+        x = _spread(rows, cols, 20, torch.float16).to(dev)
+        w = torch.randn(cols, generator=torch.Generator().manual_seed(21)).to(dev)
+        calls = [(mx_quantize(x, fmt), lambda y: lib().pgmoe_mx_quantize(x.data_ptr(), 1, cols, y, st)),
+                 (exec_fused_act_mul_mx(x, x, "gelu", fmt),
+                  lambda y: lib().pgmoe_mx_act_mul(x.data_ptr(), cols, x.data_ptr(), cols, 1, 1, y, st)),
+                 (exec_fused_rmsnorm_mx(x, w, 1e-6, fmt),
+                  lambda y: lib().pgmoe_add_rmsnorm_mx(x.data_ptr(), 1, None, 0, w.data_ptr(), 1e-6, None, y, st))]
+        for want, call in calls:
+            codes = torch.full((rows + 2, cs), 0x5a, dtype=torch.uint8, device=dev)
+            scales = torch.full((rows + 2, ss), 0x5a, dtype=torch.uint8, device=dev)
+            y = Mx(codes[1].data_ptr(), scales[1].data_ptr(), cs, ss, rows, cols, bits)
+            check(call(ctypes.byref(y)), "call")
+            torch.cuda.synchronize()
+            assert torch.equal(codes[1:-1, :n], want.codes) and torch.equal(scales[1:-1, :cols // 32], want.scales)
+            codes[1:-1, :n], scales[1:-1, :cols // 32] = 0x5a, 0x5a
+            assert (codes == 0x5a).all() and (scales == 0x5a).all()
 
 
 def test_outputs_past_the_end_are_left_alone(dev):
@@ -503,6 +553,9 @@ def test_refusals(dev):
             (ValueError, lambda: layer(x[:, :32])), (NotImplementedError, lambda: layer(x, out_dtype=torch.float64)),
             (ValueError, lambda: layer(x.cpu())), (NotImplementedError, lambda: layer(x.double(), out_dtype=torch.float32)),
             (NotImplementedError, lambda: HipMXLinear.from_gguf(_gguf({"a": (12, (4, 256), b"")}), "a", device=dev)),
-            (ValueError, lambda: HipMXLinear.from_gguf(_gguf({"a": (0, (4, 48), b"")}), "a", device=dev))]:
+            (ValueError, lambda: HipMXLinear.from_gguf(_gguf({"a": (0, (4, 48), b"")}), "a", device=dev)),
+            (ValueError, lambda: HipMXLinear.from_gguf(_gguf({"a": (39, (2, 4, 32), bytes(136))}), "a", device=dev)),
+            (ValueError, lambda: HipMXLinear.from_gguf(_gguf({"a": (0, (32,), bytes(128))}), "a", device=dev)),
+            (KeyError, lambda: HipMXLinear.from_gguf(_gguf({}), "a", device=dev))]:
         with pytest.raises(err):
             call()
