@@ -149,13 +149,23 @@ __device__ __forceinline__ void mx_products(const WOps<MODE, NB>& w, const int (
     }
 }
 
-// Outputs n .. n + 3 of row m.
-__device__ __forceinline__ void put4(const MxLinear& L, int m, int n, float4 v) {
-    float f[4] = {v.x, v.y, v.z, v.w};
+// Outputs n .. n + 3 of a row, with their bias; and as 16-bit values.
+__device__ __forceinline__ void add_bias(const MxLinear& L, int n, float (&f)[4]) {
     if (L.bias) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] += n + i < L.N ? L.bias[n + i] : 0.0f;
     }
+}
+__device__ __forceinline__ uint2 halves(const MxLinear& L, const float (&f)[4]) {
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = L.odt == PGMOE_DT_F16 ? to16<false>(f[i]) : to16<true>(f[i]);
+    return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+}
+// Outputs n .. n + 3 of row m.
+__device__ __forceinline__ void put4(const MxLinear& L, int m, int n, float4 v) {
+    float f[4] = {v.x, v.y, v.z, v.w};
+    add_bias(L, n, f);
     const int64_t at = (int64_t)m * L.N + n;
     const bool whole = n + 4 <= L.N && (L.N & 3) == 0;
     if (L.odt == PGMOE_DT_F32) {
@@ -168,18 +178,30 @@ __device__ __forceinline__ void put4(const MxLinear& L, int m, int n, float4 v) 
                 if (n + i < L.N) o[i] = f[i];
         }
     } else {
-        uint32_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = L.odt == PGMOE_DT_F16 ? to16<false>(f[i]) : to16<true>(f[i]);
+        const uint2 h = halves(L, f);
         uint16_t* o = (uint16_t*)L.out + at;
         if (whole) {
-            *(uint2*)o = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+            *(uint2*)o = h;
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (n + i < L.N) o[i] = (uint16_t)h[i];
+                if (n + i < L.N) o[i] = (uint16_t)((i < 2 ? h.x : h.y) >> (16 * (i & 1)));
         }
     }
+}
+// 16-bit outputs of row m of two fragments, n .. n + 15 and n + 16 .. n + 31, of a lane 16 g + r the four at 4 g: after the two
+// exchanges it has the eight at 8 g, and a row's 64 bytes go out at once.  N is a multiple of 8; all lanes take part.
+__device__ __forceinline__ void put_pair(const MxLinear& L, int m, int n, int g, floatx4 v0, floatx4 v1) {
+    float f0[4] = {v0[0], v0[1], v0[2], v0[3]}, f1[4] = {v1[0], v1[1], v1[2], v1[3]};
+    add_bias(L, n + 4 * g, f0);
+    add_bias(L, n + 16 + 4 * g, f1);
+    const uint2 h0 = halves(L, f0), h1 = halves(L, f1);
+    auto x = __builtin_amdgcn_permlane32_swap(h0.x, h1.x, false, false);
+    auto y = __builtin_amdgcn_permlane32_swap(h0.y, h1.y, false, false);
+    x = __builtin_amdgcn_permlane16_swap(x[0], x[1], false, false);
+    y = __builtin_amdgcn_permlane16_swap(y[0], y[1], false, false);
+    n += 8 * g;
+    if (m < L.M && n < L.N) *(uint4*)((uint16_t*)L.out + (int64_t)m * L.N + n) = make_uint4(x[0], y[0], x[1], y[1]);
 }
 
 // ---------------------------------------------------------------- up to 16 rows
@@ -636,6 +658,16 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void mx_gemm_kernel(const M
                     const float4 v = sums[at(p, b, t)];
                     acc[b][t] += floatx4{v.x, v.y, v.z, v.w};
                 }
+    }
+    if constexpr (NT % 2 == 0 && MODE != kB8) {  // kB8: fp32 outputs, 16 bytes a lane by themselves
+        if (L.odt != PGMOE_DT_F32 && (L.N & 7) == 0) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int b = 0; b < NT; b += 2)
+                    put_pair(L, m0 + (wm * MT + t) * 16 + r, (g0 + wn * NT + b) * 16, g, acc[b][t], acc[b + 1][t]);
+            return;
+        }
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
