@@ -190,7 +190,9 @@ __device__ __forceinline__ void put4(const MxLinear& L, int m, int n, float4 v) 
     }
 }
 // 16-bit outputs of row m of two fragments, n .. n + 15 and n + 16 .. n + 31, of a lane 16 g + r the four at 4 g: after the two
-// exchanges it has the eight at 8 g, and a row's 64 bytes go out at once.  N is a multiple of 8; all lanes take part.
+// exchanges it has the eight at 8 g, and a row's 64 bytes go out at once (4096 x 24576 x 4096: 317 us, as 32 bytes 327; 4 bits 230
+// and 242).  Stores past the caches made these products 4 % faster and what reads them slower (an FFN of 4096 rows 487 -> 505
+// us), so they are ordinary ones.  N is a multiple of 8; all lanes take part.
 __device__ __forceinline__ void put_pair(const MxLinear& L, int m, int n, int g, floatx4 v0, floatx4 v1) {
     float f0[4] = {v0[0], v0[1], v0[2], v0[3]}, f1[4] = {v1[0], v1[1], v1[2], v1[3]};
     add_bias(L, n + 4 * g, f0);
@@ -370,9 +372,10 @@ static int thin_launch(const MxLinear& L, const MxFloats& F, hipStream_t st) {
 // tiles spread the weights over more CUs (a CU takes in some 28 bytes a ns from memory, 110 from its L2).  77 x 4096 x 4096, 8
 // bits: 96 tiles of 32 x 128 10.2 us, 192 of 32 x 64 in two parts 7.9; fp32 15.6, in four parts 9.3; 4 bits 8.3, in four 6.6.
 //
-// What bounds it: many rows the instruction, whose rate the power budget sets (random codes in registers alone: 4.0 PFLOP/s with
-// 8-bit activations, 7.2 with 4-bit; 4096 x 24576 x 4096 runs at 2.6 and 4.4); fp32 outputs the conversions beside the products
-// (96 and 32 instructions a stage of a 64 x 128 tile: 1.3 of 2.0 PFLOP/s); few rows the weights' way to the CUs and the launch.
+// What bounds it: many rows the instruction, whose rate the power budget sets (random codes in registers alone: 4.0 PFLOP/s
+// with 8-bit activations, 7.2 with 4-bit; 4096 x 24576 x 4096 runs at 2.6 and 3.6, 4096 x 4096 x 12288 at 2.7 and 4.4); fp32
+// outputs the conversions beside the products (96 and 32 instructions a stage of a 64 x 128 tile: 1.3 of 2.0 PFLOP/s); few rows
+// the weights' way to the CUs and the launch.
 // Copies of 1 KB from memory to LDS, lane l's 16 bytes at base + off to lds + 16 l, each STEP behind the one before.  By
 // hand, so that the compiler counts no loads and adds no waits; a copy reads m0 one wait state after its write.
 #define PG_COPY(off, base) "s_nop 0\n\tglobal_load_lds_dwordx4 " off ", " base "\n\t"
