@@ -464,7 +464,7 @@ int pgmoe_mx_linear(const void* packed, int32_t out_features, const pgmoe_mx* x,
                     int32_t out_dtype, void* stream);
 
 /* pgmoe_mx_linear of the blocks of x [rows, cols] (as pgmoe_mx_quantize makes them, in format fmt).  The workspace (16-byte
- * aligned; none for up to 16 rows) holds them during the call and needs no clearing. */
+ * aligned; none for up to 16 rows of up to 4096) holds them during the call and needs no clearing. */
 size_t pgmoe_mx_linear_values_workspace_bytes(int32_t rows, int32_t cols, int32_t fmt);
 int pgmoe_mx_linear_values(const void* packed, int32_t out_features, const void* x, int32_t dtype, int64_t x_stride,
                            int32_t rows, int32_t cols, int32_t fmt, const float* bias, void* out, int32_t out_dtype,

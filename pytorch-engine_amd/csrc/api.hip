@@ -972,7 +972,7 @@ int pgmoe_mx_linear(const void* packed, int32_t out_features, const pgmoe_mx* X,
 static size_t mx_scratch(int64_t rows, int64_t cols, int fmt, int64_t* code_stride, int64_t* scale_stride) {
     *code_stride = fmt == PGMOE_MX_E2M1 ? cols / 2 : cols;
     *scale_stride = (cols / 32 + 15) / 16 * 16;
-    return rows <= kMxFewRows ? 0 : (size_t)(rows * (*code_stride + *scale_stride));
+    return mx_values_inside(rows, cols) ? 0 : (size_t)(rows * (*code_stride + *scale_stride));
 }
 
 size_t pgmoe_mx_linear_values_workspace_bytes(int32_t rows, int32_t cols, int32_t fmt) {

@@ -34,7 +34,10 @@ struct MxLinear {
     void* out;
     int odt;
 };
-constexpr int kMxFewRows = 16;  // values of up to so many rows become blocks inside the product
+constexpr int kMxFewRows = 16;  // up to so many rows are read against weights in registers
+// Values of them become blocks inside the product where a workgroup keeps its rows; longer ones would become them again for
+// every 16 outputs (1 x 12288 x 4096 16.1 us; in a launch of their own before, as more rows' are, 11).
+inline bool mx_values_inside(int64_t rows, int64_t cols) { return rows <= kMxFewRows && cols <= 4096; }
 int launch_mx_linear(const MxLinear& L, hipStream_t st);
 // L.x: where the blocks of more rows go.
 int launch_mx_linear_values(const MxLinear& L, const MxFloats& F, hipStream_t st);

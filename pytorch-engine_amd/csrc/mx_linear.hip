@@ -210,21 +210,21 @@ __device__ __forceinline__ void put_pair(const MxLinear& L, int m, int n, int g,
 // A workgroup forms 16 outputs of all rows at a time; its W waves take every W-th quad of steps, weights and activations
 // straight to registers, and their sums meet in LDS in wave order.  ONE: a quad is all that a wave has (K <= 512 W): the
 // rows stay in registers, and the workgroup goes on to its next 16 outputs, whose weights are on their way meanwhile.
-// Bound by the weights' arrival and, where they are few, by the latencies of one load, one sum and the launch: 1 x 4096 x 24576,
-// fp16 values, 11.5 us (4.7 TB/s), 8 x 2048 x 151936 35.2 (4.8), 16 x 4096 x 12288 8.7.  ONE, the weights of the next outputs under
-// way during the sum of these: 11.5 for 18.7 us; 35.2 for 44.
-// SRC: the rows come in blocks (-1), or as values of a PGMOE_DT_* that become blocks here: a lane holds the 32 values of
-// a block, so its largest magnitude needs no other lane.
-template <MxMode MODE, int SRC>
-struct ThinX {  // one step of a lane's row
-    static constexpr int N = SRC == PGMOE_DT_F32 ? 8 : 4;
+// Bound by the weights' arrival and, where they are few, by the latencies of one load, one sum and the launch: us for 1 / 16
+// rows of fp16 values to 8 bits, 4096 x 4096 4.3 / 9.0, 4096 x 24576 12.5 (4.3 TB/s) / 19, 2048 x 151936 31 (5.4) / 39, 12288 x 4096
+// 10.2 / 15.4 (2.6 of it the blocks' own launch).  ONE, the next outputs' weights under way during the sum of these, rows kept:
+// 2048 x 151936 35 for 44 us.
+// SRC: the rows come in blocks (-1), or (ONE) as values of a PGMOE_DT_* that become blocks here, in LDS, eight values a lane, a
+// wave its quad of every row: as much work as there are values.
+template <int SRC>
+struct ThinX {  // eight values of a row
+    static constexpr int N = SRC == PGMOE_DT_F32 ? 2 : 1;
     uint4 v[N];
-    __device__ __forceinline__ void load(const uint8_t* row, int block) {
+    __device__ __forceinline__ void load(const uint8_t* row, int chunk) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = ((const uint4*)(row + (int64_t)block * (16 * N)))[i];
+        for (int i = 0; i < N; ++i) v[i] = ((const uint4*)(row + (int64_t)chunk * (16 * N)))[i];
     }
-    __device__ __forceinline__ XFrag<MODE> blocks(int& scale) const {
-        float f[32];
+    __device__ __forceinline__ void widen(float (&f)[8]) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
@@ -233,30 +233,28 @@ struct ThinX {  // one step of a lane's row
                 if constexpr (SRC == PGMOE_DT_F32) {
                     f[4 * i + k] = __builtin_bit_cast(float, w[k]);
                 } else if constexpr (SRC == PGMOE_DT_F16) {
-                    f[8 * i + 2 * k] = lo_half(w[k]);
-                    f[8 * i + 2 * k + 1] = hi_half(w[k]);
+                    f[2 * k] = lo_half(w[k]);
+                    f[2 * k + 1] = hi_half(w[k]);
                 } else {
-                    f[8 * i + 2 * k] = __builtin_bit_cast(float, w[k] << 16);
-                    f[8 * i + 2 * k + 1] = __builtin_bit_cast(float, w[k] & 0xffff0000u);
+                    f[2 * k] = __builtin_bit_cast(float, w[k] << 16);
+                    f[2 * k + 1] = __builtin_bit_cast(float, w[k] & 0xffff0000u);
                 }
             }
         }
-        uint32_t c[MODE == kS4 ? 4 : 8];
-        mx_encode<MODE == kS4, 32>(f, c, scale);
-        XFrag<MODE> x;
-        x.a = make_int4((int)c[0], (int)c[1], (int)c[2], (int)c[3]);
-        if constexpr (MODE != kS4) x.b = make_int4((int)c[4], (int)c[5], (int)c[6], (int)c[7]);
-        return x;
     }
 };
 
 template <MxMode MODE, int SRC, int W, bool ONE>
-__global__ __launch_bounds__(64 * W, SRC >= 0 && !ONE ? 2 : 4) void mx_thin_kernel(const MxLinear L, const MxFloats F) {
-    __shared__ float4 part[2][W][64];
+__global__ __launch_bounds__(64 * W, 4) void mx_thin_kernel(const MxLinear L, const MxFloats F) {
+    static_assert(ONE || SRC < 0, "longer rows come in blocks");
+    constexpr int ROW = MODE == kS4 ? 256 : 512, WAVE = kMxFewRows * (ROW + 16);  // a quad of a row's codes; of all rows, with scales
+    constexpr int SUMS = 2 * W * 1024;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[SRC < 0 || SUMS > W * WAVE ? SUMS : W * WAVE];
+    auto part = (float4(*)[W][64])smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int G = mx_groups(L.N), Q = mx_quads(L.K), last = (L.K >> 5) - 1, waves = min(W, Q);
     const int m = min(r, L.M - 1);  // rows past the last repeat it, blocks past the row's last too: their weights are 0
-    const uint8_t* xr = SRC < 0 ? L.x.codes + m * L.x.code_stride : (const uint8_t*)F.p + m * F.stride * (SRC == PGMOE_DT_F32 ? 4 : 2);
+    const uint8_t* xr = L.x.codes + m * L.x.code_stride;
     const uint8_t* xsr = L.x.scales + m * L.x.scale_stride;
     const uint8_t* scales = L.w + (int64_t)G * Q * 4096;
     struct Weights {
@@ -272,25 +270,57 @@ __global__ __launch_bounds__(64 * W, SRC >= 0 && !ONE ? 2 : 4) void mx_thin_kern
     XFrag<MODE> f[4];
     int xs[4];
     auto load_x = [&](int q) PG_INLINE {
-        constexpr int AHEAD = SRC == PGMOE_DT_F32 ? 2 : 4;  // steps of values in registers
-        ThinX<MODE, SRC < 0 ? PGMOE_DT_F16 : SRC> raw[AHEAD];
         auto block = [&](int s) PG_INLINE { return min(16 * q + 4 * s + g, last); };
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            if constexpr (SRC < 0) {
-                f[s].a = *(const int4*)(xr + (int64_t)block(s) * (MODE == kS4 ? 16 : 32));
-                if constexpr (MODE != kS4) f[s].b = *(const int4*)(xr + (int64_t)block(s) * 32 + 16);
-                xs[s] = xsr[block(s)];
-            } else if (s < AHEAD) {
-                raw[s].load(xr, block(s));
+            f[s].a = *(const int4*)(xr + (int64_t)block(s) * (MODE == kS4 ? 16 : 32));
+            if constexpr (MODE != kS4) f[s].b = *(const int4*)(xr + (int64_t)block(s) * 32 + 16);
+            xs[s] = xsr[block(s)];
+        }
+    };
+    // The wave's quad of all rows, as values, to blocks; 16-byte chunk c of row i lies at c ^ i.
+    auto encode_x = [&](int q, auto meanwhile) PG_INLINE {
+        using X = ThinX<SRC < 0 ? PGMOE_DT_F16 : SRC>;
+        constexpr int AHEAD = 8 / X::N;  // rows of values in registers
+        X raw[AHEAD];
+        uint8_t* own = smem + wave * WAVE;
+        const int chunk = min(64 * q + lane, 4 * last + 3);  // past the row's last eight: them again
+        auto load_rows = [&](int i0) PG_INLINE {
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (i0 + k < L.M) raw[k].load((const uint8_t*)F.p + (i0 + k) * F.stride * (SRC == PGMOE_DT_F32 ? 4 : 2), chunk);
+        };
+        load_rows(0);
+        meanwhile();
+        for (int i0 = 0; i0 < L.M; i0 += AHEAD) {
+            if (i0) load_rows(i0);
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                if (i0 + k < L.M) {
+                    const int i = i0 + k;
+                    float v[8];
+                    raw[k].widen(v);
+                    uint32_t c[MODE == kS4 ? 1 : 2];
+                    int scale;
+                    mx_encode<MODE == kS4, 8>(v, c, scale);
+                    if constexpr (MODE == kS4)
+                        *(uint32_t*)(own + i * ROW + 16 * ((lane >> 2) ^ i) + 4 * (lane & 3)) = c[0];
+                    else
+                        *(uint2*)(own + i * ROW + 16 * ((lane >> 1) ^ i) + 8 * (lane & 1)) = make_uint2(c[0], c[1]);
+                    if ((lane & 3) == 0) own[kMxFewRows * ROW + i * 16 + (lane >> 2)] = (uint8_t)scale;
+                }
             }
         }
-        if constexpr (SRC >= 0) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                f[s] = raw[s % AHEAD].blocks(xs[s]);
-                if (s + AHEAD < 4) raw[s % AHEAD].load(xr, block(s + AHEAD));
+        for (int s = 0; s < 4; ++s) {
+            const int b = 4 * s + g;
+            if constexpr (MODE == kS4) {
+                f[s].a = *(const int4*)(own + m * ROW + 16 * (b ^ m));
+            } else {
+                f[s].a = *(const int4*)(own + m * ROW + 16 * ((2 * b) ^ m));
+                f[s].b = *(const int4*)(own + m * ROW + 16 * ((2 * b + 1) ^ m));
             }
+            xs[s] = own[kMxFewRows * ROW + m * 16 + b];
         }
     };
     auto products = [&](const Weights& w, floatx4 (&acc)[1][1]) PG_INLINE {
@@ -307,9 +337,14 @@ __global__ __launch_bounds__(64 * W, SRC >= 0 && !ONE ? 2 : 4) void mx_thin_kern
     };
     Weights w;
     if (wave < waves) {
-        load_w(w, blockIdx.x, wave);
-        if constexpr (ONE) load_x(wave);
+        if constexpr (SRC >= 0) {
+            encode_x(wave, [&]() PG_INLINE { load_w(w, blockIdx.x, wave); });
+        } else {
+            load_w(w, blockIdx.x, wave);
+            if constexpr (ONE) load_x(wave);
+        }
     }
+    if constexpr (SRC >= 0) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the sums go to the same places
     int turn = 0;
     for (int gb = blockIdx.x; gb < G; gb += gridDim.x, ++turn) {
         if (wave < waves) {
@@ -353,7 +388,7 @@ static int thin_launch(const MxLinear& L, const MxFloats& F, hipStream_t st) {
         PG_LAUNCH((mx_thin_kernel<MODE, SRC, 4, true>), dim3(std::min(G, 4 * kCUs)), dim3(256), 0, st, L, F);
     else if (Q <= 8)
         PG_LAUNCH((mx_thin_kernel<MODE, SRC, 8, true>), dim3(std::min(G, 2 * kCUs)), dim3(512), 0, st, L, F);
-    else
+    else if constexpr (SRC < 0)
         PG_LAUNCH((mx_thin_kernel<MODE, SRC, 8, false>), dim3(std::min(G, 2 * kCUs)), dim3(512), 0, st, L, F);
     return check_launch("mx_thin");
 }
@@ -753,7 +788,7 @@ int launch_mx_linear(const MxLinear& L, hipStream_t st) {
 }
 
 int launch_mx_linear_values(const MxLinear& L, const MxFloats& F, hipStream_t st) {
-    if (L.M <= kMxFewRows) {
+    if (mx_values_inside(L.M, L.K)) {
 #define VALUES(DT) return L.x.e2m1 ? thin_launch<kS4, DT>(L, F, st) : thin_launch<kB8, DT>(L, F, st)
         if (F.dt == PGMOE_DT_F32) VALUES(PGMOE_DT_F32);
         if (F.dt == PGMOE_DT_F16) VALUES(PGMOE_DT_F16);

@@ -33,7 +33,7 @@ _FMT = {"e4m3": 8, "e2m1": 4}  # bits a value
 _ACT = {"silu": ACT_SILU, "gelu": ACT_GELU_TANH}
 _ROWS, _COLS = 1 << 24, 1 << 22  # rows below, columns up to
 _STRIDE = 1 << 23  # bytes from row to row
-_FEW_ROWS = 16  # up to so many rows of values become blocks inside the product, without a workspace
+_INSIDE = (16, 4096)  # up to so many rows and columns of values become blocks inside the product, without a workspace
 
 
 def _bits(fmt: str) -> int:
@@ -344,7 +344,7 @@ class HipMXLinear(nn.Module):
             return out
         bits = _FMT[self.act_fmt]
         ws, nbytes = None, 0
-        if rows > _FEW_ROWS:
+        if rows > _INSIDE[0] or n > _INSIDE[1]:
             nbytes = rows * (n * bits // 8 + (n // 32 + 15) // 16 * 16)  # pgmoe_mx_linear_values_workspace_bytes
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # of this call alone
         launch(dev, "pgmoe_mx_linear_values", lib().pgmoe_mx_linear_values, self._packed.data_ptr(), self.out_features,

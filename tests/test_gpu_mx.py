@@ -269,6 +269,24 @@ def test_product_of_values(dev, dtype, act_fmt, M, N, K):
     assert torch.equal(layer(wide[:, 32:-32]).view(M, 1, N), out)
 
 
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("act_fmt", FMTS)
+@pytest.mark.parametrize("K", [32, 96, 512, 1440, 2048, 2080, 4064, 4096, 4128, 8224])
+def test_product_of_few_rows_of_values(dev, dtype, act_fmt, K):
+    """Every number of rows that become blocks inside the product, and rows too long for that: the same bits as by two calls;
+    one of them with a block that is not finite."""
+    from pgmoe import HipMXLinear, mx_quantize
+    w, _ = _random_blocks(70, K, "e2m1", K)
+    layer = HipMXLinear(w, act_fmt=act_fmt)
+    x = _spread(16, K, K + 1, dtype, span=1.0)
+    x[3, K - 1], x[9, 0] = float("inf"), float("nan")
+    x = x.to(dev)
+    for M in range(1, 17):
+        got, want = layer(x[:M], out_dtype=torch.float32), layer(mx_quantize(x[:M], act_fmt), out_dtype=torch.float32)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num()), M
+        assert torch.equal(got.isnan().all(1).cpu(), torch.arange(M).eq(3) | torch.arange(M).eq(9)) and not got[:3].isnan().any()
+
+
 @pytest.mark.parametrize("fmt,dtype", [("e4m3", torch.float32), ("e4m3", torch.float16), ("e2m1", torch.float32)])
 @pytest.mark.parametrize("K", [32, 512, 544, 1056, 1536, 2080, 4128])
 def test_product_of_few_tiles(dev, fmt, dtype, K):
