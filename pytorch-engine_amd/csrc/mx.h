@@ -71,30 +71,34 @@ __device__ __forceinline__ void mx_encode(float (&v)[N], uint32_t (&code)[E2M1 ?
     if constexpr (N <= 4) m = max(m, xor_lane_u<4>(m));
     const bool bad = m >= 0x7f800000u;
     const int e = max((int)(m >> 23) - (E2M1 ? kMxExpE2M1 : kMxExpE4M3), 0);
-    const float inv = __builtin_bit_cast(float, (uint32_t)(254 - e) << 23);
     if (__builtin_expect(bad, 0)) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = 0.0f;
     }
     scale = bad ? 255 : e;
-    if constexpr (E2M1) {  // saturating, to nearest even
+    const float by = __builtin_bit_cast(float, (uint32_t)e << 23);  // 2^E as the conversions take it, 0 for 2^-127
+    if constexpr (E2M1) {  // to nearest even, saturating
 #pragma unroll
         for (int w = 0; w < (N + 7) / 8; ++w) {
             uint32_t c = 0;
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w] * inv, v[8 * w + 1] * inv, 1.0f, 0);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 2] * inv, v[8 * w + 3] * inv, 1.0f, 1);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w], v[8 * w + 1], by, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 2], v[8 * w + 3], by, 1);
             if constexpr (N >= 8) {
-                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 4] * inv, v[8 * w + 5] * inv, 1.0f, 2);
-                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 6] * inv, v[8 * w + 7] * inv, 1.0f, 3);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 4], v[8 * w + 5], by, 2);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 6], v[8 * w + 7], by, 3);
             }
             code[w] = c;
         }
-    } else {  // to nearest even; past 464 the conversion gives NaN, so the values are held to 448 before it
-        auto at = [&](int i) { return __builtin_amdgcn_fmed3f(v[i] * inv, -448.0f, 448.0f); };
+    } else {  // to nearest even; past 464 2^E the conversion gives NaN, so the values are held to 448 2^E before it
+        const float top = ldexpf(448.0f, e - 127);
+        typedef short short2v __attribute__((ext_vector_type(2)));
+        auto at = [&](int i) { return __builtin_amdgcn_fmed3f(v[i], -top, top); };
 #pragma unroll
         for (int w = 0; w < N / 4; ++w) {
-            int c = __builtin_amdgcn_cvt_pk_fp8_f32(at(4 * w), at(4 * w + 1), 0, false);
-            code[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(at(4 * w + 2), at(4 * w + 3), c, true);
+            short2v c = {0, 0};
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, at(4 * w), at(4 * w + 1), by, false);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, at(4 * w + 2), at(4 * w + 3), by, true);
+            code[w] = __builtin_bit_cast(uint32_t, c);
         }
     }
 }
