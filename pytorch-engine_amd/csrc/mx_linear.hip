@@ -207,7 +207,7 @@ __device__ __forceinline__ void put_pair(const MxLinear& L, int m, int n, int g,
 }
 
 // ---------------------------------------------------------------- up to 16 rows
-// A workgroup forms 16 outputs of all rows at a time; its W waves take every W-th quad of steps, weights and activations
+// A workgroup forms NB times 16 outputs of all rows at a time; its W waves take every W-th quad of steps, weights and activations
 // straight to registers, and their sums meet in LDS in wave order.  ONE: a quad is all that a wave has (K <= 512 W): the
 // rows stay in registers, and the workgroup goes on to its next 16 outputs, whose weights are on their way meanwhile.
 // Bound by the weights' arrival and, where they are few, by the latencies of one load, one sum and the launch: us for 1 / 16
@@ -244,13 +244,13 @@ struct ThinX {  // eight values of a row
     }
 };
 
-template <MxMode MODE, int SRC, int W, bool ONE>
-__global__ __launch_bounds__(64 * W, 4) void mx_thin_kernel(const MxLinear L, const MxFloats F) {
+template <MxMode MODE, int SRC, int W, bool ONE, int NB>
+__global__ __launch_bounds__(64 * W, 4 / NB) void mx_thin_kernel(const MxLinear L, const MxFloats F) {
     static_assert(ONE || SRC < 0, "longer rows come in blocks");
     constexpr int ROW = MODE == kS4 ? 256 : 512, WAVE = kMxFewRows * (ROW + 16);  // a quad of a row's codes; of all rows, with scales
-    constexpr int SUMS = 2 * W * 1024;
+    constexpr int SUMS = 2 * W * NB * 1024;
     __shared__ __attribute__((aligned(16))) uint8_t smem[SRC < 0 || SUMS > W * WAVE ? SUMS : W * WAVE];
-    auto part = (float4(*)[W][64])smem;
+    auto part = (float4(*)[W][NB][64])smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int G = mx_groups(L.N), Q = mx_quads(L.K), last = (L.K >> 5) - 1, waves = min(W, Q);
     const int m = min(r, L.M - 1);  // rows past the last repeat it, blocks past the row's last too: their weights are 0
@@ -258,28 +258,33 @@ __global__ __launch_bounds__(64 * W, 4) void mx_thin_kernel(const MxLinear L, co
     const uint8_t* xsr = L.x.scales + m * L.x.scale_stride;
     const uint8_t* scales = L.w + (int64_t)G * Q * 4096;
     struct Weights {
-        int4 w[4][1];
-        int s[1];
+        int4 w[4][NB];
+        int s[NB];
     };
     auto load_w = [&](Weights& to, int gb, int q) PG_INLINE {
-        const int64_t at = (int64_t)min(gb, G - 1) * Q + min(q, Q - 1);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) to.w[s][0] = *(const int4*)(L.w + at * 4096 + s * 1024 + lane * 16);
-        to.s[0] = *(const int*)(scales + at * 256 + lane * 4);
+        for (int b = 0; b < NB; ++b) {
+            const int64_t at = (int64_t)min(gb * NB + b, G - 1) * Q + min(q, Q - 1);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) to.w[s][b] = *(const int4*)(L.w + at * 4096 + s * 1024 + lane * 16);
+            to.s[b] = *(const int*)(scales + at * 256 + lane * 4);
+        }
     };
-    XFrag<MODE> f[4];
-    int xs[4];
-    auto load_x = [&](int q) PG_INLINE {
+    struct Rows {
+        XFrag<MODE> f[4];
+        int s[4];
+    };
+    auto load_x = [&](Rows& to, int q) PG_INLINE {
         auto block = [&](int s) PG_INLINE { return min(16 * q + 4 * s + g, last); };
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            f[s].a = *(const int4*)(xr + (int64_t)block(s) * (MODE == kS4 ? 16 : 32));
-            if constexpr (MODE != kS4) f[s].b = *(const int4*)(xr + (int64_t)block(s) * 32 + 16);
-            xs[s] = xsr[block(s)];
+            to.f[s].a = *(const int4*)(xr + (int64_t)block(s) * (MODE == kS4 ? 16 : 32));
+            if constexpr (MODE != kS4) to.f[s].b = *(const int4*)(xr + (int64_t)block(s) * 32 + 16);
+            to.s[s] = xsr[block(s)];
         }
     };
     // The wave's quad of all rows, as values, to blocks; 16-byte chunk c of row i lies at c ^ i.
-    auto encode_x = [&](int q, auto meanwhile) PG_INLINE {
+    auto encode_x = [&](Rows& to, int q, auto meanwhile) PG_INLINE {
         using X = ThinX<SRC < 0 ? PGMOE_DT_F16 : SRC>;
         constexpr int AHEAD = 8 / X::N;  // rows of values in registers
         X raw[AHEAD];
@@ -315,20 +320,20 @@ __global__ __launch_bounds__(64 * W, 4) void mx_thin_kernel(const MxLinear L, co
         for (int s = 0; s < 4; ++s) {
             const int b = 4 * s + g;
             if constexpr (MODE == kS4) {
-                f[s].a = *(const int4*)(own + m * ROW + 16 * (b ^ m));
+                to.f[s].a = *(const int4*)(own + m * ROW + 16 * (b ^ m));
             } else {
-                f[s].a = *(const int4*)(own + m * ROW + 16 * ((2 * b) ^ m));
-                f[s].b = *(const int4*)(own + m * ROW + 16 * ((2 * b + 1) ^ m));
+                to.f[s].a = *(const int4*)(own + m * ROW + 16 * ((2 * b) ^ m));
+                to.f[s].b = *(const int4*)(own + m * ROW + 16 * ((2 * b + 1) ^ m));
             }
-            xs[s] = own[kMxFewRows * ROW + m * 16 + b];
+            to.s[s] = own[kMxFewRows * ROW + m * 16 + b];
         }
     };
-    auto products = [&](const Weights& w, floatx4 (&acc)[1][1]) PG_INLINE {
+    auto products = [&](const Weights& w, const Rows& x, floatx4 (&acc)[NB][1]) PG_INLINE {
         auto step = [&](auto sc) PG_INLINE {
             constexpr int s = decltype(sc)::value;
-            WOps<MODE, 1> ops;
+            WOps<MODE, NB> ops;
             ops.template set<s>(w.w[s], w.s);
-            mx_products<MODE, s, 0>(ops, w.s, xs[s], f[s], 0, acc);
+            mx_products<MODE, s, 0>(ops, w.s, x.s[s], x.f[s], 0, acc);
         };
         step(std::integral_constant<int, 0>());
         step(std::integral_constant<int, 1>());
@@ -336,60 +341,78 @@ __global__ __launch_bounds__(64 * W, 4) void mx_thin_kernel(const MxLinear L, co
         step(std::integral_constant<int, 3>());
     };
     Weights w;
+    Rows x;
     if (wave < waves) {
         if constexpr (SRC >= 0) {
-            encode_x(wave, [&]() PG_INLINE { load_w(w, blockIdx.x, wave); });
+            encode_x(x, wave, [&]() PG_INLINE { load_w(w, blockIdx.x, wave); });
         } else {
+            if constexpr (ONE || NB > 1) load_x(x, wave);
             load_w(w, blockIdx.x, wave);
-            if constexpr (ONE) load_x(wave);
         }
     }
     if constexpr (SRC >= 0) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the sums go to the same places
     int turn = 0;
-    for (int gb = blockIdx.x; gb < G; gb += gridDim.x, ++turn) {
+    for (int gb = blockIdx.x; gb * NB < G; gb += gridDim.x, ++turn) {
         if (wave < waves) {
-            floatx4 acc[1][1] = {{floatx4{0, 0, 0, 0}}};
-            Weights next;
+            floatx4 acc[NB][1];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[b][0] = floatx4{0, 0, 0, 0};
             if constexpr (ONE) {
+                Weights next;
                 load_w(next, gb + gridDim.x, wave);
-                products(w, acc);
+                products(w, x, acc);
+                w = next;
             } else {
 #pragma unroll 1
-                for (int q = wave; q < Q; q += W) {
-                    load_w(next, q + W < Q ? gb : gb + gridDim.x, q + W < Q ? q + W : wave);
-                    load_x(q);
-                    products(w, acc);
-                    if (q + W < Q) w = next;
+                for (int q = wave; q < Q; q += W) {  // the next quad's weights, or the next outputs' first, on their way
+                    Weights next;
+                    Rows then;
+                    const bool more = q + W < Q;
+                    if constexpr (NB > 1) load_x(then, more ? q + W : wave);
+                    load_w(next, more ? gb : gb + gridDim.x, more ? q + W : wave);
+                    if constexpr (NB == 1) load_x(x, q);
+                    products(w, x, acc);
+                    w = next;
+                    if constexpr (NB > 1) x = then;
                 }
             }
-            w = next;
-            part[turn & 1][wave][lane] = make_float4(acc[0][0][0], acc[0][0][1], acc[0][0][2], acc[0][0][3]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                part[turn & 1][wave][b][lane] = make_float4(acc[b][0][0], acc[b][0][1], acc[b][0][2], acc[b][0][3]);
         }
         // (no wait for loads and stores; a buffer is written again behind the next barrier, which its reader passes too)
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (wave == turn % W) {
-            float4 v = part[turn & 1][0][lane];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (wave != (turn * NB + b) % W) continue;
+            float4 v = part[turn & 1][0][b][lane];
             for (int k = 1; k < waves; ++k) {
-                const float4 p = part[turn & 1][k][lane];
+                const float4 p = part[turn & 1][k][b][lane];
                 v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
             }
-            const int n = 16 * gb + 4 * g;
+            const int n = 16 * (gb * NB + b) + 4 * g;
             if (r < L.M && n < L.N) put4(L, r, n, v);
         }
     }
 }
 
 // Workgroups: as many as stay on the card at once where each goes on to further outputs.  Four waves where K has no more
-// quads (8 rows of 2048 inputs, 151936 outputs: 60 us with eight waves, half of them idle).
+// quads (8 rows of 2048 inputs, 151936 outputs: 60 us with eight waves, half of them idle).  Longer rows: two groups of outputs at
+// a time, on rows that are read once for both, with the next quad's on their way, where that leaves a workgroup to every CU
+// (8 bits, 1 / 16 rows, 28672 x 8192 23.8 / 33 us for 28.7 / 50 one by one; 12288 x 4096 9.1 / 14.5 for 7.5 / 12.5).
 template <MxMode MODE, int SRC>
 static int thin_launch(const MxLinear& L, const MxFloats& F, hipStream_t st) {
     const int G = mx_groups(L.N), Q = mx_quads(L.K);
     if (Q <= 4)
-        PG_LAUNCH((mx_thin_kernel<MODE, SRC, 4, true>), dim3(std::min(G, 4 * kCUs)), dim3(256), 0, st, L, F);
+        PG_LAUNCH((mx_thin_kernel<MODE, SRC, 4, true, 1>), dim3(std::min(G, 4 * kCUs)), dim3(256), 0, st, L, F);
     else if (Q <= 8)
-        PG_LAUNCH((mx_thin_kernel<MODE, SRC, 8, true>), dim3(std::min(G, 2 * kCUs)), dim3(512), 0, st, L, F);
-    else if constexpr (SRC < 0)
-        PG_LAUNCH((mx_thin_kernel<MODE, SRC, 8, false>), dim3(std::min(G, 2 * kCUs)), dim3(512), 0, st, L, F);
+        PG_LAUNCH((mx_thin_kernel<MODE, SRC, 8, true, 1>), dim3(std::min(G, 2 * kCUs)), dim3(512), 0, st, L, F);
+    else if constexpr (SRC < 0) {
+        if (G < 2 * kCUs)
+            PG_LAUNCH((mx_thin_kernel<MODE, SRC, 8, false, 1>), dim3(G), dim3(512), 0, st, L, F);
+        else
+            PG_LAUNCH((mx_thin_kernel<MODE, SRC, 4, false, 2>), dim3(std::min((G + 1) / 2, 2 * kCUs)), dim3(256), 0, st, L, F);
+    }
     return check_launch("mx_thin");
 }
 

@@ -269,6 +269,18 @@ def test_product_of_values(dev, dtype, act_fmt, M, N, K):
     assert torch.equal(layer(wide[:, 32:-32]).view(M, 1, N), out)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("N", [8160, 8177, 8209])
+def test_product_of_few_long_rows(dev, fmt, N):
+    """Rows of more than 4096 against outputs that a workgroup takes 16 or 32 of at a time."""
+    from pgmoe import HipMXLinear
+    for M, K in [(1, 4128), (7, 6176), (16, 8192)]:
+        w, w64 = _random_blocks(N, K, "e2m1", N + M)
+        x, x64 = _random_blocks(M, K, fmt, M)
+        y, s = H.product(x64, w64)
+        H.check_product(HipMXLinear(w)(x, out_dtype=torch.float32), y, s, K)
+
+
 @pytest.mark.parametrize("dtype", H.DTYPES)
 @pytest.mark.parametrize("act_fmt", FMTS)
 @pytest.mark.parametrize("K", [32, 96, 512, 1440, 2048, 2080, 4064, 4096, 4128, 8224])
