@@ -149,6 +149,8 @@ __device__ __forceinline__ void mx_products(const WOps<MODE, NB>& w, const int (
     }
 }
 
+// Rows of outputs begin at any value, as N is any, and stores of several values take any place (2452 x 288 x 14951 to fp32: 51 us,
+// value by value 94; 3024 x 192 x 8131 to fp16 31 and 52; rows at multiples of 16 bytes as before).
 // Outputs n .. n + 3 of a row, with their bias; and as 16-bit values.
 __device__ __forceinline__ void add_bias(const MxLinear& L, int n, float (&f)[4]) {
     if (L.bias) {
@@ -162,29 +164,29 @@ __device__ __forceinline__ uint2 halves(const MxLinear& L, const float (&f)[4]) 
     for (int i = 0; i < 4; ++i) h[i] = L.odt == PGMOE_DT_F16 ? to16<false>(f[i]) : to16<true>(f[i]);
     return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
-// Outputs n .. n + 3 of row m.
+// Outputs n .. n + 3 of row m; WHOLE: all of them are the row's; BITS: of every output of the kernel's, 0: either.
+template <bool WHOLE, int BITS>
 __device__ __forceinline__ void put4(const MxLinear& L, int m, int n, float4 v) {
     float f[4] = {v.x, v.y, v.z, v.w};
     add_bias(L, n, f);
     const int64_t at = (int64_t)m * L.N + n;
-    const bool whole = n + 4 <= L.N && (L.N & 3) == 0;
-    if (L.odt == PGMOE_DT_F32) {
+    if (BITS == 32 || (BITS == 0 && L.odt == PGMOE_DT_F32)) {
         float* o = (float*)L.out + at;
-        if (whole) {
-            *(float4*)o = make_float4(f[0], f[1], f[2], f[3]);
+        if (WHOLE || n + 4 <= L.N) {
+            __builtin_memcpy(o, f, 16);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 3; ++i)
                 if (n + i < L.N) o[i] = f[i];
         }
     } else {
         const uint2 h = halves(L, f);
         uint16_t* o = (uint16_t*)L.out + at;
-        if (whole) {
-            *(uint2*)o = h;
+        if (WHOLE || n + 4 <= L.N) {
+            __builtin_memcpy(o, &h, 8);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 3; ++i)
                 if (n + i < L.N) o[i] = (uint16_t)((i < 2 ? h.x : h.y) >> (16 * (i & 1)));
         }
     }
@@ -192,7 +194,7 @@ __device__ __forceinline__ void put4(const MxLinear& L, int m, int n, float4 v) 
 // 16-bit outputs of row m of two fragments, n .. n + 15 and n + 16 .. n + 31, of a lane 16 g + r the four at 4 g: after the two
 // exchanges it has the eight at 8 g, and a row's 64 bytes go out at once (4096 x 24576 x 4096: 317 us, as 32 bytes 327; 4 bits 230
 // and 242).  Stores past the caches made these products 4 % faster and what reads them slower (an FFN of 4096 rows 487 -> 505
-// us), so they are ordinary ones.  N is a multiple of 8; all lanes take part.
+// us), so they are ordinary ones.  All lanes take part; all of the outputs are the row's.
 __device__ __forceinline__ void put_pair(const MxLinear& L, int m, int n, int g, floatx4 v0, floatx4 v1) {
     float f0[4] = {v0[0], v0[1], v0[2], v0[3]}, f1[4] = {v1[0], v1[1], v1[2], v1[3]};
     add_bias(L, n + 4 * g, f0);
@@ -202,8 +204,8 @@ __device__ __forceinline__ void put_pair(const MxLinear& L, int m, int n, int g,
     auto y = __builtin_amdgcn_permlane32_swap(h0.y, h1.y, false, false);
     x = __builtin_amdgcn_permlane16_swap(x[0], x[1], false, false);
     y = __builtin_amdgcn_permlane16_swap(y[0], y[1], false, false);
-    n += 8 * g;
-    if (m < L.M && n < L.N) *(uint4*)((uint16_t*)L.out + (int64_t)m * L.N + n) = make_uint4(x[0], y[0], x[1], y[1]);
+    const uint4 h = make_uint4(x[0], y[0], x[1], y[1]);
+    if (m < L.M) __builtin_memcpy((uint16_t*)L.out + (int64_t)m * L.N + n + 8 * g, &h, 16);
 }
 
 // ---------------------------------------------------------------- up to 16 rows
@@ -391,7 +393,7 @@ __global__ __launch_bounds__(64 * W, 4 / NB) void mx_thin_kernel(const MxLinear 
                 v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
             }
             const int n = 16 * (gb * NB + b) + 4 * g;
-            if (r < L.M && n < L.N) put4(L, r, n, v);
+            if (r < L.M && n < L.N) put4<false, 0>(L, r, n, v);
         }
     }
 }
@@ -720,25 +722,30 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void mx_gemm_kernel(const M
                     acc[b][t] += floatx4{v.x, v.y, v.z, v.w};
                 }
     }
-    if constexpr (NT % 2 == 0 && MODE != kB8) {  // kB8: fp32 outputs, 16 bytes a lane by themselves
-        if (L.odt != PGMOE_DT_F32 && (L.N & 7) == 0) {
+    constexpr int BITS = MODE == kB8 ? 32 : MODE == kS8 ? 16 : 0;
+    auto each_of = [&](auto put) PG_INLINE {
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int b = 0; b < NT; b += 2)
-                    put_pair(L, m0 + (wm * MT + t) * 16 + r, (g0 + wn * NT + b) * 16, g, acc[b][t], acc[b + 1][t]);
-            return;
+            for (int b = 0; b < NT; ++b) put(t, b, m0 + (wm * MT + t) * 16 + r, (g0 + wn * NT + b) * 16);
+    };
+    if (16 * g0 + T::BN <= L.N) {  // no row ends in this tile
+        if constexpr (NT % 2 == 0 && BITS != 32) {
+            if (BITS == 16 || L.odt != PGMOE_DT_F32) {
+                each_of([&](int t, int b, int m, int n) PG_INLINE {
+                    if (b % 2 == 0) put_pair(L, m, n, g, acc[b][t], acc[b + 1][t]);
+                });
+                return;
+            }
         }
+        each_of([&](int t, int b, int m, int n) PG_INLINE {
+            if (m < L.M) put4<true, BITS>(L, m, n + 4 * g, make_float4(acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]));
+        });
+        return;
     }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = m0 + (wm * MT + t) * 16 + r;
-#pragma unroll
-        for (int b = 0; b < NT; ++b) {
-            const int n = (g0 + wn * NT + b) * 16 + 4 * g;
-            if (m < L.M && n < L.N) put4(L, m, n, make_float4(acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]));
-        }
-    }
+    each_of([&](int t, int b, int m, int n) PG_INLINE {
+        if (m < L.M && n + 4 * g < L.N) put4<false, BITS>(L, m, n + 4 * g, make_float4(acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]));
+    });
 }
 
 template <MxMode MODE, int MT, int NT, int WM, int WN, int WK, int RING, bool EARLY, int OCC>
