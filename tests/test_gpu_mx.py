@@ -205,6 +205,27 @@ def test_norm_rows_of_zeros_and_not_finite_ones(dev):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+def test_more_chunks_than_one_launch_numbers(dev, fmt):
+    """To blocks, back and the gated activation over 2^31 pieces of 16 bytes and more: rows on both sides of where calls are cut."""
+    from pgmoe import exec_fused_act_mul_mx, mx_quantize
+    rows, cols = (1 << 22) + 5, 4128
+    if torch.cuda.mem_get_info(dev)[0] < rows * cols * 6:
+        pytest.skip("needs 104 GB")
+    cut = ((1 << 31) - 1) // (cols // 8)
+    at = torch.tensor([0, 1, cut - 2, cut - 1, cut, cut + 1, rows - 1])
+    x = torch.zeros(rows, cols, dtype=torch.float16, device=dev)
+    some = _spread(len(at), cols, 19, torch.float16).to(dev)
+    x[at.to(dev)] = some
+    t, few = mx_quantize(x, fmt), mx_quantize(some, fmt)
+    assert torch.equal(t.codes[at.to(dev)], few.codes) and torch.equal(t.scales[at.to(dev)], few.scales)
+    assert not t.codes[cut + 2:cut + 64].any() and not t.codes[2:64].any()
+    assert torch.equal(t.dequantize(torch.float16)[at.to(dev)], few.dequantize(torch.float16))
+    del t
+    t, few = exec_fused_act_mul_mx(x, x, "silu", fmt), exec_fused_act_mul_mx(some, some, "silu", fmt)
+    assert torch.equal(t.codes[at.to(dev)], few.codes) and torch.equal(t.scales[at.to(dev)], few.scales)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("dtype", H.DTYPES)
 @pytest.mark.parametrize("rows,cols", [(1, 32), (3, 1440), (61, 768), (300, 4096)])
