@@ -291,6 +291,34 @@ def test_product_of_values(dev, dtype, act_fmt, M, N, K):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,N,K,dtype", [((1 << 20) + 9, 48, 8224, torch.float32), ((1 << 20) + 9, 2100, 96, torch.float16),
+                                         (3, (1 << 21) + 7, 4128, torch.float16), (21, (1 << 21) + 7, 4128, torch.float32)])
+def test_product_of_far_offsets(dev, fmt, M, N, K, dtype):
+    """Blocks, weights and outputs whose bytes pass 2^32 and whose outputs pass 2^31."""
+    from pgmoe import HipMXLinear, MXTensor
+    if torch.cuda.mem_get_info(dev)[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    g = torch.Generator(device=dev).manual_seed(M + N)
+
+    def blocks(rows, f):
+        codes = torch.randint(0, 256, (rows, K if f == "e4m3" else K // 2), generator=g, device=dev, dtype=torch.uint8)
+        if f == "e4m3":
+            codes.masked_fill_(codes & 127 == 127, 0)
+        return MXTensor(codes, torch.randint(118, 124, (rows, K // 32), generator=g, device=dev, dtype=torch.uint8), f)
+
+    def some(t, at):
+        at = at.to(dev)
+        return H.values(MXTensor(t.codes[at], t.scales[at], t.fmt))
+
+    x, w = blocks(M, fmt), blocks(N, "e2m1")
+    out = HipMXLinear(w)(x, out_dtype=dtype)
+    pick = lambda n: torch.unique(torch.tensor([0, 1, n // 2, n - 9, n - 2, n - 1]).clamp(min=0))  # noqa: E731
+    m, n = pick(M), pick(N)
+    y, s = H.product(some(x, m), some(w, n))
+    H.check_product(out[m.to(dev)][:, n.to(dev)], y, s, K, cut=fmt == "e4m3" and dtype != torch.float32)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("N", [8160, 8177, 8209])
 def test_product_of_few_long_rows(dev, fmt, N):
     """Rows of more than 4096 against outputs that a workgroup takes 16 or 32 of at a time."""
