@@ -439,8 +439,8 @@ int pgmoe_mx_quantize(const void* x, int32_t dtype, int64_t x_stride, const pgmo
 /* out [rows, cols] (PGMOE_DT_*, contiguous, 16-byte aligned) = the values of x, rounded once. */
 int pgmoe_mx_dequantize(const pgmoe_mx* x, void* out, int32_t out_dtype, void* stream);
 
-/* pgmoe_add_rmsnorm (h_out as there, rows contiguous) with the blocks of the normalised rows as output: the fp32
- * values are not rounded before. */
+/* pgmoe_add_rmsnorm (h_out as there, rows contiguous) with the blocks of the normalised rows as output, formed in 64 bits from
+ * x + delta before its rounding to h_out's fp32. */
 int pgmoe_add_rmsnorm_mx(const void* x, int32_t x_dtype, const void* delta, int32_t delta_dtype, const float* weight,
                          float eps, float* h_out, const pgmoe_mx* y, void* stream);
 

@@ -127,17 +127,44 @@ __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(MxRows x, Fas
 }
 
 // ---------------------------------------------------------------- the norm
-// h = f32(x) + f32(delta), y = (h * r) * w, r = 1 / sqrt(sum(h^2) / D + eps), as add_rmsnorm_kernel, the rows of y to
-// blocks in the same registers.  A row takes T threads of a workgroup of max(T, 256); thread t owns the 4-value chunks
-// t, t + T, ...: eight neighbouring lanes hold a block.  VPT > 0: the row stays in registers (D <= 4 T VPT), its
-// loads all on the way before the first is used; VPT == 0: it is read twice.
+// h = x + delta, y = h * r * w, r = 1 / sqrt(sum(h^2) / D + eps), the rows of y to blocks in the same registers.  In 64 bits up
+// to the codes, whatever the order of the sum: a code is then that of the formula, where roundings to fp32 put one of a million on
+// the other side of a border, squares of no row pass the range, and the memory still bounds the time.  h_out is h, rounded once.
+// A row takes T threads of a workgroup of max(T, 256); thread t owns the 4-value chunks t, t + T, ...: eight
+// neighbouring lanes hold a block.  VPT > 0: the row stays in registers (D <= 4 T VPT), its loads all on the way before
+// the first is used; VPT == 0: it is read twice.
+struct Doubles {
+    double v[4];
+};
+__device__ __forceinline__ double wave_sum(double v) {
+    auto add = [&](auto sc) {
+        constexpr int S = decltype(sc)::value;
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        v += __builtin_bit_cast(double, (uint64_t)xor_lane_u<S>((uint32_t)(b >> 32)) << 32 | xor_lane_u<S>((uint32_t)b));
+    };
+    add(std::integral_constant<int, 32>());
+    add(std::integral_constant<int, 16>());
+    add(std::integral_constant<int, 8>());
+    add(std::integral_constant<int, 4>());
+    add(std::integral_constant<int, 2>());
+    add(std::integral_constant<int, 1>());
+    return v;
+}
+// d in fp32 for a further rounding to fewer bits: what does not fit sets the last bit (the other 29 of d's 52 are cut), so that
+// no value moves onto a border between codes.
+__device__ __forceinline__ float to_odd(double d) {
+    uint64_t b = __builtin_bit_cast(uint64_t, d);
+    if ((uint32_t)b & 0x1fffffffu) b = (b & ~(uint64_t)0x1fffffff) | 0x20000000u;
+    return (float)__builtin_bit_cast(double, b);
+}
+
 template <int T, int VPT, bool E2M1>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rmsnorm_mx_kernel(const void* __restrict__ x, int xdt,
                                                                           const void* __restrict__ delta, int ddt,
                                                                           const float* __restrict__ w, float eps,
                                                                           float* __restrict__ h_out, MxRows y) {
     constexpr int RPB = T < 256 ? 256 / T : 1, W = T / 64;  // rows a workgroup, waves a row
-    __shared__ float wsum[W > 1 ? W : 1];
+    __shared__ double wsum[W > 1 ? W : 1];
     const int t = threadIdx.x % T, n4 = y.cols >> 2;
     const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / T;
     if (row >= y.rows) return;  // whole waves; with one row a workgroup none
@@ -153,10 +180,15 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rmsnorm_mx_kernel(const
         if (dt == PGMOE_DT_F16) return make_float4(lo_half(u.x), hi_half(u.x), lo_half(u.y), hi_half(u.y));
         return make_float4(f(u.x << 16), f(u.x & 0xffff0000u), f(u.y << 16), f(u.y & 0xffff0000u));
     };
-    auto add = [](float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); };
-    auto squares = [](float acc, float4 h) { return acc + h.x * h.x + h.y * h.y + h.z * h.z + h.w * h.w; };
-    auto total = [&](float acc) {
-        acc = group_sum<64>(acc);
+    auto wide = [](float4 a) { return Doubles{{(double)a.x, (double)a.y, (double)a.z, (double)a.w}}; };
+    auto add = [](Doubles a, Doubles b) { return Doubles{{a.v[0] + b.v[0], a.v[1] + b.v[1], a.v[2] + b.v[2], a.v[3] + b.v[3]}}; };
+    auto squares = [](double acc, Doubles h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc = __builtin_fma(h.v[i], h.v[i], acc);
+        return acc;
+    };
+    auto total = [&](double acc) {
+        acc = wave_sum(acc);
         if constexpr (W > 1) {
             if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = acc;
             __syncthreads();
@@ -164,10 +196,15 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rmsnorm_mx_kernel(const
 #pragma unroll
             for (int i = 1; i < W; ++i) acc = acc + wsum[i];
         }
-        return 1.0f / sqrtf(acc / (float)y.cols + eps);
+        return 1.0 / sqrt(acc / (double)y.cols + (double)eps);
     };
-    auto put = [&](int c, float4 h, float4 g, float r) {
-        float v[4] = {(h.x * r) * g.x, (h.y * r) * g.y, (h.z * r) * g.z, (h.w * r) * g.w};
+    auto put_h = [&](int c, Doubles h) {
+        if (h_out && c < n4) ((float4*)h_out)[row4 + c] = make_float4((float)h.v[0], (float)h.v[1], (float)h.v[2], (float)h.v[3]);
+    };
+    auto put = [&](int c, Doubles h, Doubles g, double r) {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = to_odd((h.v[i] * r) * g.v[i]);
         uint32_t code[1];
         int scale;
         mx_encode<E2M1, 4>(v, code, scale);
@@ -196,34 +233,34 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rmsnorm_mx_kernel(const
 #pragma unroll
         for (int j = 0; j < VPT; ++j) g[j] = ((const float4*)w)[at(j)];
         __builtin_amdgcn_sched_barrier(0);
-        float acc = 0.0f;
-        float4 h[VPT];
+        double acc = 0.0;
+        Doubles h[VPT];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            h[j] = widen4(xr[j], xdt);
-            if (delta) h[j] = add(h[j], widen4(dr[j], ddt));
+            h[j] = wide(widen4(xr[j], xdt));
+            if (delta) h[j] = add(h[j], wide(widen4(dr[j], ddt)));
             if (t + T * j < n4) acc = squares(acc, h[j]);
         }
-        const float r = total(acc);
+        const double r = total(acc);
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int c = t + T * j;
-            if (h_out && c < n4) ((float4*)h_out)[row4 + c] = h[j];
-            put(c, h[j], g[j], r);
+            put_h(c, h[j]);
+            put(c, h[j], wide(g[j]), r);
         }
     } else {
         auto h_at = [&](int c) {
-            float4 h = widen4(load(x, xdt, row4 + c), xdt);
-            return delta ? add(h, widen4(load(delta, ddt, row4 + c), ddt)) : h;
+            const Doubles h = wide(widen4(load(x, xdt, row4 + c), xdt));
+            return delta ? add(h, wide(widen4(load(delta, ddt, row4 + c), ddt))) : h;
         };
-        float acc = 0.0f;
+        double acc = 0.0;
         for (int c = t; c < n4; c += T) acc = squares(acc, h_at(c));
-        const float r = total(acc);
+        const double r = total(acc);
         for (int c0 = 0; c0 < n4; c0 += T) {  // every lane, as blocks meet across lanes
             const int c = c0 + t, k = min(c, n4 - 1);
-            const float4 h = h_at(k);
-            if (h_out && c < n4) ((float4*)h_out)[row4 + c] = h;
-            put(c, h, ((const float4*)w)[k], r);
+            const Doubles h = h_at(k);
+            put_h(c, h);
+            put(c, h, wide(((const float4*)w)[k]), r);
         }
     }
 }

@@ -236,13 +236,14 @@ def _norm(x: torch.Tensor, delta: Optional[torch.Tensor], norm_weight: torch.Ten
 
 
 def exec_fused_rmsnorm_mx(x: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6, fmt: str = "e4m3") -> MXTensor:
-    """exec_fused_rmsnorm with its output in blocks; the fp32 values are not rounded before."""
+    """exec_fused_rmsnorm with its output in blocks; the values are formed in 64 bits and not rounded before."""
     return _norm(x, None, norm_weight, eps, fmt)[1]
 
 
 def exec_fused_add_rmsnorm_mx(x: torch.Tensor, delta: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6,
                               fmt: str = "e4m3") -> Tuple[torch.Tensor, MXTensor]:
-    """exec_fused_add_rmsnorm with its second output in blocks: (h = x.float() + delta.float(), RMSNorm(h) * w)."""
+    """exec_fused_add_rmsnorm with its second output in blocks: (h = x.float() + delta.float(), RMSNorm(x + delta) * w), the
+    second formed in 64 bits from the sum before its rounding to fp32."""
     return _norm(x, delta, norm_weight, eps, fmt)
 
 
