@@ -50,13 +50,36 @@ __device__ __forceinline__ void put_codes(const MxRows& y, int64_t row, int c, c
     if (c % LPB == 0) y.scales[row * y.scale_stride + c / LPB] = (uint8_t)scale;
 }
 
-// silu(g) = g / (1 + e^-g), gelu(g) = g / (1 + e^-2z) with z = sqrt(2 / pi) (g + 0.044715 g^3): no difference of near
-// values for negative g.  The hardware's power of two and reciprocal are good to 2^-23 each, where codes hold 4 bits.
+// silu(g) = g / (1 + 2^-z) with z = log2(e) g, gelu(g) the same with z = 2 log2(e) sqrt(2 / pi) (g + 0.044715 g^3): no
+// difference of near values for negative g.  The hardware's power of two and reciprocal are good to 2^-23 each, where codes
+// hold 4 bits; what rounding z leaves out of silu's (|z| 2^-24 of the value) is put back to first order.
+constexpr float kLog2e = 1.44269504088896f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.69314718f;
+constexpr float kFarGate = -120.0f;  // z below it: 2^-z nears the end of fp32's range
 template <int ACT>
-__device__ __forceinline__ float gated(float g) {
-    constexpr float kLog2e = 1.44269504088896f;
-    const float z = ACT ? (2.0f * 0.7978845608028654f * kLog2e) * (g + 0.044715f * g * g * g) : kLog2e * g;
-    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-z));
+__device__ __forceinline__ float gate_exponent(float g) {
+    return ACT ? (2.0f * 0.7978845608028654f * kLog2e) * (g + 0.044715f * g * g * g) : kLog2e * g;
+}
+template <int ACT>
+__device__ __forceinline__ float gated(float g, float z) {
+    float t;
+    if constexpr (ACT) {
+        t = __builtin_amdgcn_exp2f(-z);
+    } else {  // (past z = 120 and below -120 the sum below is 1, or another's work)
+        z = __builtin_amdgcn_fmed3f(z, kFarGate, -kFarGate);
+        const float c = __builtin_amdgcn_fmed3f(g, kFarGate / kLog2e, -kFarGate / kLog2e);
+        t = __builtin_amdgcn_exp2f(-z);
+        t = __builtin_fmaf(-kLn2 * t, __builtin_fmaf(c, kLog2eRest, __builtin_fmaf(c, kLog2e, -z)), t);
+    }
+    return g * __builtin_amdgcn_rcpf(1.0f + t);
+}
+// act(g) u for z below kFarGate, where 1 + 2^-z is 2^-z to fp32: g u 2^z, the power in parts so that none of them leaves the range
+// before the product does (g = -100 is worth 1e-3 beside u = 2e38).
+template <int ACT>
+__device__ __forceinline__ float gated_far(float g, float z, float u) {
+    z = fmaxf(z, -400.0f);
+    const float n = rintf(z), c = fmaxf(g, -400.0f / kLog2e);
+    const float f = ACT ? z - n : __builtin_fmaf(c, kLog2eRest, __builtin_fmaf(c, kLog2e, -n));
+    return g * ldexpf(__builtin_amdgcn_exp2f(f), -120) * ldexpf(u, (int)n + 120);
 }
 
 // ACT < 0: the blocks of x; 0: of silu(x) u; 1: of gelu(x) u (tanh form).  A chunk a thread: with four (their loads on the way
@@ -76,8 +99,23 @@ __global__ __launch_bounds__(kMxThreads) void mx_rows_kernel(const void* __restr
         float w[N];
         widen<DT>(a, v);
         widen<DT>(b, w);
+        bool far = false;
+        float gu[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = gated<ACT>(v[i]) * w[i];
+        for (int i = 0; i < N; ++i) {
+            const float z = gate_exponent<ACT>(v[i]);
+            far |= z < kFarGate;
+            gu[i] = gated<ACT>(v[i], z) * w[i];
+        }
+        if (__builtin_expect(far, 0)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float z = gate_exponent<ACT>(v[i]);
+                if (z < kFarGate) gu[i] = gated_far<ACT>(v[i], z, w[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = gu[i];
     } else {
         widen<DT>(a, v);
     }

@@ -61,3 +61,46 @@ def test_norm_of_far_rows(dev, fmt, cols):
         assert torch.equal(h.cpu(), x)
         for v in (t, u):
             assert torch.equal(H.scales(v), e) and torch.equal(H.unpack(v), codes)
+
+
+# ---------------------------------------------------------------- activation
+def _act64(act, g, u):
+    if act == "silu":
+        return g / (1 + torch.exp(-g)) * u
+    return g / (1 + torch.exp(-2 * (2 / torch.pi) ** 0.5 * (g + 0.044715 * g ** 3))) * u
+
+
+# what fp32 leaves of a product: 2^-23 each of a power of two and a reciprocal, four roundings and what the first order leaves
+# out; of gelu's exponent eight roundings of 2^-24, times its size, up to 400 ln 2
+_FAR_REL = {"silu": 2.0 ** -20, "gelu": 2.0 ** -12}
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("act,lo,hi,size", [
+    ("silu", -84, -60, 1.0), ("silu", -105, -82, 1e20), ("silu", -180, -90, 3e38), ("silu", -400, -170, 3e38), ("silu", -90, 90, 1e30),
+    ("gelu", -8, -5, 1.0), ("gelu", -10.5, -8, 1e20), ("gelu", -14, -9.5, 3e38), ("gelu", -30, -12, 3e38), ("gelu", -14, 14, 1e30)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_act_of_far_gates(dev, fmt, act, lo, hi, size, dtype):
+    """Negative gates whose activation is far below one, beside values that bring the product back."""
+    from pgmoe import exec_fused_act_mul_mx
+    gen = torch.Generator().manual_seed(int(-lo) + len(act))
+    g = (lo + (hi - lo) * torch.rand(130, 320, generator=gen)).to(dtype)
+    u = (size * (0.01 + 0.99 * torch.rand(130, 320, generator=gen))).clamp(max=3.3e38).to(dtype)
+    g[:3] = torch.tensor([lo, (lo + hi) / 2, hi]).to(dtype)[:, None]
+    t = exec_fused_act_mul_mx(g.to(dev), u.to(dev), act, fmt)
+    y = _act64(act, g.double(), u.double())
+    H.check_blocks(t, torch.where(y.abs() < 2.0 ** -140, torch.zeros_like(y), y), _FAR_REL[act])
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_act_of_the_largest_gates(dev, act):
+    """Gates at both ends of fp32's range: the gate itself, or nothing; not finite ones make NaN blocks."""
+    from pgmoe import exec_fused_act_mul_mx
+    top = torch.finfo(torch.float32).max
+    g = torch.tensor([top, -top, 1e30, -1e30, 1e10, -1e10, -1000.0, float("inf"), -float("inf"), float("nan")])[:, None].repeat(1, 32)
+    u = torch.full_like(g, 0.5)
+    t = exec_fused_act_mul_mx(g.to(dev), u.to(dev), act)
+    v = t.dequantize().cpu()
+    want, _ = H.encode(torch.where(g > 0, g * 0.5, torch.zeros_like(g))[:7], "e4m3")
+    assert torch.equal(H.unpack(t)[:7] & 127, want)
+    assert torch.isfinite(v[:7]).all() and torch.isnan(v[7:]).all()
