@@ -54,28 +54,22 @@ __device__ __forceinline__ void put_codes(const MxRows& y, int64_t row, int c, c
 // difference of near values for negative g.  The hardware's power of two and reciprocal are good to 2^-23 each, where codes
 // hold 4 bits; what rounding z leaves out of silu's (|z| 2^-24 of the value) is put back to first order.
 constexpr float kLog2e = 1.44269504088896f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.69314718f;
-constexpr float kFarGate = -120.0f;  // z below it: 2^-z nears the end of fp32's range
+constexpr float kFarGate = 120.0f;  // |z| past it: 2^-z nears the end of fp32's range
 template <int ACT>
 __device__ __forceinline__ float gate_exponent(float g) {
     return ACT ? (2.0f * 0.7978845608028654f * kLog2e) * (g + 0.044715f * g * g * g) : kLog2e * g;
 }
 template <int ACT>
 __device__ __forceinline__ float gated(float g, float z) {
-    float t;
-    if constexpr (ACT) {
-        t = __builtin_amdgcn_exp2f(-z);
-    } else {  // (past z = 120 and below -120 the sum below is 1, or another's work)
-        z = __builtin_amdgcn_fmed3f(z, kFarGate, -kFarGate);
-        const float c = __builtin_amdgcn_fmed3f(g, kFarGate / kLog2e, -kFarGate / kLog2e);
-        t = __builtin_amdgcn_exp2f(-z);
-        t = __builtin_fmaf(-kLn2 * t, __builtin_fmaf(c, kLog2eRest, __builtin_fmaf(c, kLog2e, -z)), t);
-    }
+    float t = __builtin_amdgcn_exp2f(-z);
+    if constexpr (ACT == 0) t = __builtin_fmaf(-kLn2 * t, __builtin_fmaf(g, kLog2eRest, __builtin_fmaf(g, kLog2e, -z)), t);
     return g * __builtin_amdgcn_rcpf(1.0f + t);
 }
-// act(g) u for z below kFarGate, where 1 + 2^-z is 2^-z to fp32: g u 2^z, the power in parts so that none of them leaves the range
-// before the product does (g = -100 is worth 1e-3 beside u = 2e38).
+// act(g) u for z past kFarGate, where 1 + 2^-z is 1 to fp32, or 2^-z: g u, or g u 2^z, the power in parts so that none of them
+// leaves the range before the product does (g = -100 is worth 7e-4 beside u = 2e38).
 template <int ACT>
 __device__ __forceinline__ float gated_far(float g, float z, float u) {
+    if (z > 0) return g * u;
     z = fmaxf(z, -400.0f);
     const float n = rintf(z), c = fmaxf(g, -400.0f / kLog2e);
     const float f = ACT ? z - n : __builtin_fmaf(c, kLog2eRest, __builtin_fmaf(c, kLog2e, -n));
@@ -83,7 +77,8 @@ __device__ __forceinline__ float gated_far(float g, float z, float u) {
 }
 
 // ACT < 0: the blocks of x; 0: of silu(x) u; 1: of gelu(x) u (tanh form).  A chunk a thread: with four (their loads on the way
-// at once) 4096 x 12288 fp16 took as long, 28.8 us for 28.1 (5.4 TB/s) and 48.1 for 45.8 gated (5.5 TB/s), 64 x 4096 3.3 for 2.7.
+// at once) 4096 x 12288 fp16 took as long, 28.8 us for 28.1 (5.4 TB/s) and 48.1 for 45.8 gated (41 to 42 alone, 6.1 TB/s), 64 x 4096
+// 3.3 for 2.7.  Far gates are looked for once a chunk, by the largest |z|: a flag a gate cost silu 3 us of 41.
 template <int DT, bool E2M1, int ACT>
 __global__ __launch_bounds__(kMxThreads) void mx_rows_kernel(const void* __restrict__ x, int64_t xs, const void* __restrict__ u,
                                                             int64_t us, FastDiv cpr, uint32_t chunks, MxRows y) {
@@ -99,19 +94,18 @@ __global__ __launch_bounds__(kMxThreads) void mx_rows_kernel(const void* __restr
         float w[N];
         widen<DT>(a, v);
         widen<DT>(b, w);
-        bool far = false;
-        float gu[N];
+        float gu[N], most = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float z = gate_exponent<ACT>(v[i]);
-            far |= z < kFarGate;
+            most = fmaxf(most, fabsf(z));
             gu[i] = gated<ACT>(v[i], z) * w[i];
         }
-        if (__builtin_expect(far, 0)) {
+        if (__builtin_expect(most > kFarGate, 0)) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float z = gate_exponent<ACT>(v[i]);
-                if (z < kFarGate) gu[i] = gated_far<ACT>(v[i], z, w[i]);
+                if (fabsf(z) > kFarGate) gu[i] = gated_far<ACT>(v[i], z, w[i]);
             }
         }
 #pragma unroll
