@@ -16,7 +16,7 @@
 // Packed weights: (16 rows x 128 inputs) tiles of 1 KB, lane l's 16 bytes at 16 l, K / 128 steps rounded up to a multiple
 // of 4 a row group; behind all of them the scales, 256 bytes for 16 rows x 512 inputs: lane l's four bytes at 4 l,
 // one a step.  Inputs past K have code 0 and scale 1 there, and activations past K are read from the same row's valid
-// blocks: they count nothing, and their row is NaN anyway where one of them is.
+// blocks with scale 1: they count nothing, and their row is NaN anyway where a code of them is.
 // Reference: the W4A16 product of GGUFQuantLinear (pygguf_engine/quant_kernels.py:1165-1293), whose weights are integers
 // with fp16 scales and whose activations stay fp16.
 #include "launch.h"
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * W, 4 / NB) void mx_thin_kernel(const MxLinear 
         for (int s = 0; s < 4; ++s) {
             to.f[s].a = *(const int4*)(xr + (int64_t)block(s) * (MODE == kS4 ? 16 : 32));
             if constexpr (MODE != kS4) to.f[s].b = *(const int4*)(xr + (int64_t)block(s) * 32 + 16);
-            to.s[s] = xsr[block(s)];
+            to.s[s] = 16 * q + 4 * s + g <= last ? xsr[block(s)] : 127;  // 1 past the row: the weights' 0 meets no infinity
         }
     };
     // The wave's quad of all rows, as values, to blocks; 16-byte chunk c of row i lies at c ^ i.

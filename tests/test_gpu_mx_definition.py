@@ -104,3 +104,34 @@ def test_act_of_the_largest_gates(dev, act):
     want, _ = H.encode(torch.where(g > 0, g * 0.5, torch.zeros_like(g))[:7], "e4m3")
     assert torch.equal(H.unpack(t)[:7] & 127, want)
     assert torch.isfinite(v[:7]).all() and torch.isnan(v[7:]).all()
+
+
+# ---------------------------------------------------------------- product
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M", [1, 5, 16, 20, 70])
+@pytest.mark.parametrize("K", [32, 288, 512, 544, 2080, 4128, 8224])
+def test_product_of_infinite_blocks(dev, fmt, M, K):
+    """Blocks beyond fp32's range, the row's last among them: sums of one sign are infinite, and other rows as they were."""
+    from pgmoe import HipMXLinear, MXTensor
+    N = 40
+    g = torch.Generator().manual_seed(K + M)
+    wc = torch.randint(1, 8, (N, K), generator=g)
+    top = 8 if fmt == "e2m1" else 127
+    xc = torch.randint(1, top, (M, K), generator=g)
+    ws, xs = torch.full((N, K // 32), 127), torch.full((M, K // 32), 120)
+    far = sorted({0, M // 2, M - 1})
+    if fmt == "e4m3":
+        xc[far, -32:] = torch.randint(80, top, (len(far), 32), generator=g)
+    for i, r in enumerate(far):
+        xs[r, -1 if i != 1 else 0] = 254
+        if i == 1:
+            xc[r, :32] = top - 1
+    w = MXTensor(H.pack(wc, "e2m1").to(dev), ws.to(torch.uint8).to(dev), "e2m1")
+    x = MXTensor(H.pack(xc, fmt).to(dev), xs.to(torch.uint8).to(dev), fmt)
+    y = H.decode(xc, xs, fmt) @ H.decode(wc, ws, "e2m1").T
+    assert (y[far] > 2.0 ** 129).all()
+    for dt in H.DTYPES:
+        out = HipMXLinear(w)(x, out_dtype=dt).cpu()
+        assert (out[far] == float("inf")).all(), dt
+        rest = [r for r in range(M) if r not in far]
+        torch.testing.assert_close(out[rest].double(), y[rest], rtol=2.0 ** -7, atol=0)
