@@ -318,6 +318,9 @@ __global__ __launch_bounds__(64 * W, 4 / NB) void mx_thin_kernel(const MxLinear 
                 }
             }
         }
+        // Lanes read what others of the wave wrote: its accesses to LDS run in their order, which the compiler has to keep.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const int b = 4 * s + g;

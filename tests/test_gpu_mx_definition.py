@@ -135,3 +135,33 @@ def test_product_of_infinite_blocks(dev, fmt, M, K):
         assert (out[far] == float("inf")).all(), dt
         rest = [r for r in range(M) if r not in far]
         torch.testing.assert_close(out[rest].double(), y[rest], rtol=2.0 ** -7, atol=0)
+
+
+def _random_blocks(rows, cols, fmt, seed, dev):
+    """Any codes but NaN, scales within 2^14 of each other."""
+    from pgmoe import MXTensor
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 256 if fmt == "e4m3" else 16, (rows, cols), generator=g)
+    if fmt == "e4m3":
+        codes = torch.where(codes % 128 == 127, torch.zeros_like(codes), codes)
+    e = torch.randint(117, 131, (rows, cols // 32), generator=g)
+    return MXTensor(H.pack(codes, fmt).to(dev), e.to(torch.uint8).to(dev), fmt), H.decode(codes, e, fmt)
+
+
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("act_fmt", FMTS)
+@pytest.mark.parametrize("M,K", [(2, 512), (5, 96), (8, 4096), (9, 1440), (16, 2080), (16, 4096), (50, 1440), (200, 544)])
+def test_rows_do_not_depend_on_the_others(dev, dtype, act_fmt, M, K):
+    """Rows of values in another order, and one row among others of other values: the same bits for each row."""
+    from pgmoe import HipMXLinear
+    layer = HipMXLinear(_random_blocks(300, K, "e2m1", K, dev)[0], act_fmt=act_fmt)
+    g = torch.Generator().manual_seed(M)
+    x = (torch.randn(M, K, generator=g) * torch.exp(torch.randn(M, 1, generator=g))).to(dtype).to(dev)
+    order = torch.randperm(M, generator=g).to(dev)
+    for dt in (torch.float32, torch.float16):
+        out = layer(x, out_dtype=dt)
+        assert torch.equal(layer(x[order], out_dtype=dt), out[order])
+        for i in (0, M // 2, M - 1):
+            other = torch.randn(M, K, generator=g).to(dtype).to(dev)
+            other[i] = x[i]
+            assert torch.equal(layer(other, out_dtype=dt)[i], out[i])
