@@ -165,3 +165,29 @@ def test_rows_do_not_depend_on_the_others(dev, dtype, act_fmt, M, K):
             other = torch.randn(M, K, generator=g).to(dtype).to(dev)
             other[i] = x[i]
             assert torch.equal(layer(other, out_dtype=dt)[i], out[i])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 32), (3, 5, 64), (16, 515, 96), (17, 33, 96), (70, 130, 160), (130, 257, 288), (300, 515, 512),
+                                   (700, 4099, 96), (2050, 8190, 64), (4100, 8195, 64), (3, 8209, 4128)])
+def test_outputs_past_the_end_are_left_alone(dev, fmt, dtype, M, N, K):
+    """Whole and ragged tiles of every size, written into the middle of a larger buffer through the C ABI."""
+    from pgmoe import HipMXLinear
+    from pgmoe._lib import check, lib
+    w, w64 = _random_blocks(N, K, "e2m1", 1, dev)
+    x, x64 = _random_blocks(M, K, fmt, 2, dev)
+    layer = HipMXLinear(w)
+    buf = torch.full((M * N + 1024,), 7.0, device=dev, dtype=dtype)
+    out = buf[512:512 + M * N]
+    check(lib().pgmoe_mx_linear(layer._packed.data_ptr(), N, x._ref, None, out.data_ptr(), {torch.float32: 0, torch.float16: 1}.get(dtype, 30),
+                                torch.cuda.current_stream().cuda_stream), "pgmoe_mx_linear")
+    torch.cuda.synchronize()
+    assert (buf[:512] == 7).all() and (buf[512 + M * N:] == 7).all()
+    at = torch.unique(torch.tensor([0, 1, M // 2, M - 2, M - 1]).clamp(0, M - 1))
+    got = out.view(M, N)[at.to(dev)]
+    y, s = H.product(x64[at], w64)
+    over = y.abs() > 6e4  # fp16 ends there
+    got = got.masked_fill(over.to(dev), 0) if dtype == torch.float16 else got
+    y = y.masked_fill(over, 0) if dtype == torch.float16 else y
+    H.check_product(got, y, s, K, cut=fmt == "e4m3" and dtype != torch.float32)
