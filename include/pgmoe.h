@@ -457,9 +457,10 @@ int pgmoe_mx_pack(const pgmoe_mx* w, void* dst, void* stream);
 /* out [x.rows, out_features] (PGMOE_DT_*, contiguous, 16-byte aligned) = x . W^T (+ bias fp32 [out_features] or NULL):
  * packed weights of out_features rows of x.cols, x in e4m3 or e2m1 blocks; products summed in fp32 in a fixed order
  * and rounded once.  16-bit outputs of more than 16 rows of e4m3 blocks take the matrix cores' 8-bit form, which cuts
- * the products of 8 neighbouring inputs below 2^-13 of the largest of them (2e-5 of the outputs' 2-norm); fp32 outputs
- * and up to 16 rows do not, and take a value beyond fp32's range as an infinity, one below 2^-126 to the nearest
- * multiple of 2^-133. */
+ * the products of 8 neighbouring inputs below 2^-13 of the largest of them (2e-5 of the outputs' 2-norm), unless
+ * PGMOE_MX_FP32_SUMS is added to out_dtype, at half the rate.  That form, fp32 outputs and up to 16 rows cut nothing above 2^-24,
+ * and take a value beyond fp32's range as an infinity, one below 2^-126 to the nearest multiple of 2^-133. */
+#define PGMOE_MX_FP32_SUMS 0x100
 int pgmoe_mx_linear(const void* packed, int32_t out_features, const pgmoe_mx* x, const float* bias, void* out,
                     int32_t out_dtype, void* stream);
 

@@ -950,6 +950,13 @@ int pgmoe_mx_pack(const pgmoe_mx* W, void* dst, void* stream) {
     return launch_mx_pack(w, (uint8_t*)dst, as_stream(stream));
 }
 
+// Whether the outputs' type asks for fp32 sums; the type by itself.
+static bool mx_wide(int32_t* out_dtype) {
+    const bool wide = *out_dtype >= 0 && (*out_dtype & PGMOE_MX_FP32_SUMS);
+    if (wide) *out_dtype &= ~PGMOE_MX_FP32_SUMS;
+    return wide;
+}
+
 static int check_mx_product(int out_features, const MxRows& x, const void* packed, const float* bias, const void* out, int out_dtype) {
     if (!mx_weight_sizes(out_features, x.cols)) return fail(PGMOE_E_INVALID, "mx_linear: %d outputs", out_features);
     if (!float_type(out_dtype)) return fail(PGMOE_E_UNSUPPORTED, "mx_linear: output dtype %d", out_dtype);
@@ -962,10 +969,11 @@ static int check_mx_product(int out_features, const MxRows& x, const void* packe
 int pgmoe_mx_linear(const void* packed, int32_t out_features, const pgmoe_mx* X, const float* bias, void* out,
                     int32_t out_dtype, void* stream) {
     MxRows x;
+    const bool wide = mx_wide(&out_dtype);
     int rc = check_mx("mx_linear", X, &x);
     if (rc || (rc = check_mx_product(out_features, x, packed, bias, out, out_dtype))) return rc;
     if (x.rows == 0) return PGMOE_OK;
-    return launch_mx_linear(MxLinear{(const uint8_t*)packed, out_features, x.cols, x.rows, x, bias, out, out_dtype},
+    return launch_mx_linear(MxLinear{(const uint8_t*)packed, out_features, x.cols, x.rows, x, bias, out, out_dtype, wide},
                             as_stream(stream));
 }
 
@@ -984,6 +992,7 @@ int pgmoe_mx_linear_values(const void* packed, int32_t out_features, const void*
                            int32_t cols, int32_t fmt, const float* bias, void* out, int32_t out_dtype, void* ws, size_t ws_bytes,
                            void* stream) {
     int64_t cs, ss;
+    const bool wide = mx_wide(&out_dtype);
     const size_t need = rows > 0 && cols > 0 ? mx_scratch(rows, cols, fmt, &cs, &ss) : 0;
     if (need && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need))
         return fail(PGMOE_E_WORKSPACE, "mx_linear_values: workspace %zu bytes, need %zu, 16-byte aligned", ws_bytes, need);
@@ -996,7 +1005,7 @@ int pgmoe_mx_linear_values(const void* packed, int32_t out_features, const void*
     if ((rc = check_mx_product(out_features, y, packed, bias, out, out_dtype))) return rc;
     if (rows == 0) return PGMOE_OK;
     if ((rc = check_mx_floats("mx_linear_values", x, dtype, x_stride, y, &f))) return rc;
-    return launch_mx_linear_values(MxLinear{(const uint8_t*)packed, out_features, cols, rows, y, bias, out, out_dtype}, f,
+    return launch_mx_linear_values(MxLinear{(const uint8_t*)packed, out_features, cols, rows, y, bias, out, out_dtype, wide}, f,
                                    as_stream(stream));
 }
 

@@ -33,6 +33,7 @@ struct MxLinear {
     const float* bias;
     void* out;
     int odt;
+    bool wide;  // no product of a sum is cut above 2^-24 of its neighbours
 };
 constexpr int kMxFewRows = 16;  // up to so many rows are read against weights in registers
 // Values of them become blocks inside the product where a workgroup keeps its rows; longer ones would become them again for

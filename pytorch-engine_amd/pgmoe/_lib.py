@@ -115,6 +115,9 @@ class Sampling(ctypes.Structure):
     ]
 
 
+MX_FP32_SUMS = 0x100  # PGMOE_MX_FP32_SUMS
+
+
 class Mx(ctypes.Structure):
     _fields_ = [
         ("codes", _P),

@@ -24,7 +24,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
-from ._lib import ACT_GELU_TANH, ACT_SILU, BF16, F16, F32, MXFP4, Mx, lib
+from ._lib import ACT_GELU_TANH, ACT_SILU, BF16, F16, F32, MX_FP32_SUMS, MXFP4, Mx, lib
 from .attention import launch
 from .moe import _load_lock, load_float_tensor
 
@@ -260,9 +260,16 @@ class HipMXLinear(nn.Module):
 
     forward(x, out_dtype=None): x an MXTensor [..., in_features] (either format), or fp32 / fp16 / bf16 values, which
     are brought to blocks of `act_fmt` first.  Products are summed in fp32 in a fixed order and rounded once, to
-    out_dtype (fp32, fp16, bf16; by default x's, fp16 for an MXTensor)."""
+    out_dtype (fp32, fp16, bf16; by default x's, fp16 for an MXTensor).
 
-    def __init__(self, weight: MXTensor, bias: Optional[torch.Tensor] = None, act_fmt: str = "e4m3") -> None:
+    What a sum keeps: with e2m1 activations, fp32 outputs or up to 16 rows, products down to 2^-24 of their largest neighbour.
+    16-bit outputs of more than 16 rows in e4m3 blocks are formed by the matrix cores' 8-bit products, which leave out what is
+    below 2^-13 of the largest of 8 neighbouring ones (some 2e-5 of the outputs' 2-norm, a tenth of fp16's rounding): a row then
+    differs by that from the same row in a call of up to 16.  fp32_sums=True takes the form of the few rows for all, at half
+    the rate where rows are many."""
+
+    def __init__(self, weight: MXTensor, bias: Optional[torch.Tensor] = None, act_fmt: str = "e4m3",
+                 fp32_sums: bool = False) -> None:
         super().__init__()
         _bits(act_fmt)
         if weight.fmt != "e2m1" or len(weight.shape) != 2 or weight.shape[0] < 1:
@@ -270,6 +277,7 @@ class HipMXLinear(nn.Module):
         self.out_features, self.in_features = weight.shape
         self.device = weight.device
         self.act_fmt = act_fmt
+        self.fp32_sums = bool(fp32_sums)
         if bias is not None and tuple(bias.shape) != (self.out_features,):
             raise ValueError(f"bias {tuple(bias.shape)} of {self.out_features} outputs")
         n = int(lib().pgmoe_mx_packed_bytes(self.out_features, self.in_features))
@@ -285,7 +293,7 @@ class HipMXLinear(nn.Module):
 
     @classmethod
     def from_gguf(cls, gguf_file: Any, weight_name: Union[str, Sequence[str]], bias_name: Optional[str] = None,
-                  device: Union[torch.device, str] = "cuda", act_fmt: str = "e4m3") -> "HipMXLinear":
+                  device: Union[torch.device, str] = "cuda", act_fmt: str = "e4m3", fp32_sums: bool = False) -> "HipMXLinear":
         """The named matrix; several names are one layer whose outputs follow each other.  MXFP4 tensors are kept
         exactly, F32 / F16 / BF16 ones are brought to e2m1 blocks."""
         device = torch.device(device)
@@ -317,7 +325,7 @@ class HipMXLinear(nn.Module):
                 bias = load_float_tensor(gguf_file, bias_name, torch.device("cpu"))
             if len({c.shape[1] for c in codes}) != 1:
                 raise ValueError("matrices of one layer have the same number of input features")
-            return cls(MXTensor(torch.cat(codes), torch.cat(scales), "e2m1"), bias=bias, act_fmt=act_fmt)
+            return cls(MXTensor(torch.cat(codes), torch.cat(scales), "e2m1"), bias=bias, act_fmt=act_fmt, fp32_sums=fp32_sums)
 
     def forward(self, x: Union[torch.Tensor, MXTensor], out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         shape, n = x.shape, self.in_features
@@ -331,6 +339,8 @@ class HipMXLinear(nn.Module):
         code = _DT.get(odt)
         if code is None:
             raise NotImplementedError(f"outputs of dtype {odt} (fp32, fp16 or bf16)")
+        if self.fp32_sums:
+            code += MX_FP32_SUMS
         if not given:
             x, dt, at, stride, rows = _floats("x", x)
         else:

@@ -191,3 +191,38 @@ def test_outputs_past_the_end_are_left_alone(dev, fmt, dtype, M, N, K):
     got = got.masked_fill(over.to(dev), 0) if dtype == torch.float16 else got
     y = y.masked_fill(over, 0) if dtype == torch.float16 else y
     H.check_product(got, y, s, K, cut=fmt == "e4m3" and dtype != torch.float32)
+
+
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("M,N,K", [(3, 100, 1440), (17, 33, 96), (70, 130, 4096), (300, 1030, 992), (700, 2050, 544), (2050, 4099, 160)])
+def test_product_of_fp32_sums(dev, dtype, M, N, K):
+    """Outputs of any type without the 8-bit products' cut, from blocks and from values, with a bias."""
+    from pgmoe import HipMXLinear, MXTensor
+    w, w64 = _random_blocks(N, K, "e2m1", N + K, dev)
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(1)) * 10
+    layer = HipMXLinear(w, bias=bias.to(dev), fp32_sums=True)
+    x, x64 = _random_blocks(M, K, "e4m3", M + K, dev)
+    y, s = H.product(x64 / 64, w64 / 64, bias)  # within fp16's range
+    layer_small = HipMXLinear(MXTensor(w.codes, w.scales - 6, "e2m1"), bias=bias.to(dev), fp32_sums=True)
+    H.check_product(layer_small(MXTensor(x.codes, x.scales - 6, "e4m3"), out_dtype=dtype), y, s, K)
+    v = torch.randn(M, K, generator=torch.Generator().manual_seed(2)).to(dtype)
+    codes, e = H.encode(v, "e4m3")
+    y, s = H.product(H.decode(codes, e, "e4m3"), w64, bias)
+    H.check_product(layer(v.to(dev), out_dtype=torch.float32), y, s, K)
+    assert torch.equal(layer(v.to(dev), out_dtype=torch.float32), HipMXLinear(w, bias=bias.to(dev))(v.to(dev), out_dtype=torch.float32))
+
+
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("M", [1, 16, 17, 80, 300, 2100])
+def test_fp32_sums_keep_small_products_beside_large_ones(dev, dtype, M):
+    """Two products that cancel out, 15 octaves above the others: in a call of any number of rows the others' sum is exact."""
+    from pgmoe import HipMXLinear, MXTensor
+    N, K = 130, 32
+    x, w = torch.full((M, K), 2.0 ** -4), torch.full((N, K), 2, dtype=torch.long)  # codes of 1
+    x[:, 0], x[:, 8] = 448, 448
+    w[:, 0], w[:, 8] = 7, 15  # 6 and -6
+    one = torch.full((1, 1), 127, dtype=torch.uint8, device=dev)
+    xt = MXTensor(x.to(torch.float8_e4m3fn).to(dev), one.expand(M, 1), "e4m3")
+    wt = MXTensor(H.pack(w, "e2m1").to(dev), one.expand(N, 1), "e2m1")
+    out = HipMXLinear(wt, fp32_sums=True)(xt, out_dtype=dtype)
+    assert torch.equal(out, torch.full((M, N), 30 * 2.0 ** -4, dtype=dtype, device=dev))
