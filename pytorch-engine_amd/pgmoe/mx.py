@@ -32,7 +32,8 @@ _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _FMT = {"e4m3": 8, "e2m1": 4}  # bits a value
 _ACT = {"silu": ACT_SILU, "gelu": ACT_GELU_TANH}
 _ROWS, _COLS = 1 << 24, 1 << 22  # rows below, columns up to
-_STRIDE = 1 << 23  # bytes from row to row
+_STRIDE = 1 << 23  # bytes from row to row of blocks
+_FLOAT_STRIDE = 1 << 31  # elements from row to row of values
 _INSIDE = (16, 4096)  # up to so many rows and columns of values become blocks inside the product, without a workspace
 
 
@@ -61,12 +62,12 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.shape[-1] if step is None else step
 
 
-def _placed(t: torch.Tensor, n: int, size: int) -> Tuple[torch.Tensor, int, int]:
+def _placed(t: torch.Tensor, n: int, size: int, most: int) -> Tuple[torch.Tensor, int, int]:
     """t [..., n] of `size` bytes an element, or a contiguous copy, with rows that begin at multiples of 16 bytes, do not
-    overlap and lie within 2^23 bytes of each other; the elements from row to row; its address."""
+    overlap and lie at most `most` elements from each other; the elements from row to row; its address."""
     s = n if t.is_contiguous() else _row_stride(t)
     p = t.data_ptr()
-    if s < n or (s * size | p) & 15 or s * size > _STRIDE:
+    if s < n or (s * size | p) & 15 or s > most:
         t = t.clone(memory_format=torch.contiguous_format)
         return t, n, t.data_ptr()
     return t, s, p
@@ -108,7 +109,7 @@ class MXTensor:
         _sizes(rows, cols)
         if tuple(scales.shape) != (*codes.shape[:-1], cols // 32):
             raise ValueError(f"scales {tuple(scales.shape)} of codes {tuple(codes.shape)} ({fmt})")
-        codes, stride, at = _placed(codes.view(torch.uint8), codes.shape[-1], 1)
+        codes, stride, at = _placed(codes.view(torch.uint8), codes.shape[-1], 1, _STRIDE)
         scales = scales.view(torch.uint8)
         if not _scales_as_they_are(scales, rows):
             held = torch.empty(*scales.shape[:-1], (cols // 32 + 15) // 16 * 16, dtype=torch.uint8, device=scales.device)
@@ -180,7 +181,7 @@ def _floats(name: str, x: torch.Tensor) -> Tuple[torch.Tensor, int, int, int, in
     if not shape or shape[-1] < 1:
         raise ValueError(f"{name}: [..., cols]")
     n = shape[-1]
-    x, stride, at = _placed(x, n, 4 if dt == 0 else 2)
+    x, stride, at = _placed(x, n, 4 if dt == 0 else 2, _FLOAT_STRIDE)
     return x, dt, at, stride, x.numel() // n
 
 

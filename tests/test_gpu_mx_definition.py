@@ -226,3 +226,28 @@ def test_fp32_sums_keep_small_products_beside_large_ones(dev, dtype, M):
     wt = MXTensor(H.pack(w, "e2m1").to(dev), one.expand(N, 1), "e2m1")
     out = HipMXLinear(wt, fp32_sums=True)(xt, out_dtype=dtype)
     assert torch.equal(out, torch.full((M, N), 30 * 2.0 ** -4, dtype=dtype, device=dev))
+
+
+# ---------------------------------------------------------------- calls
+def test_wide_rows_are_not_copied(dev):
+    """Rows of 16 MB, next to each other and of a wider matrix: read where they are, as narrow ones."""
+    from pgmoe import HipMXLinear, exec_fused_act_mul_mx, exec_fused_rmsnorm_mx, mx_quantize
+    base = torch.randn(5, 1 << 22, generator=torch.Generator().manual_seed(3)).to(dev)
+    w = torch.ones(1 << 22, device=dev)
+    part, few = base[:, 4096:8192], base[:, 4096:8192].contiguous()
+    layer = HipMXLinear(_random_blocks(70, 4096, "e2m1", 1, dev)[0])
+    for call in (lambda: mx_quantize(base), lambda: exec_fused_rmsnorm_mx(base, w), lambda: exec_fused_act_mul_mx(base, base)):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats(dev)
+        had = torch.cuda.memory_allocated(dev)
+        t = call()
+        assert torch.cuda.max_memory_allocated(dev) - had < base.numel() * 2  # the blocks, not the values
+        del t
+    codes, e = H.encode(base[:1].cpu(), "e4m3")
+    t = mx_quantize(base)
+    assert torch.equal(H.unpack(t)[:1], codes) and torch.equal(H.scales(t)[:1], e)
+    a, b = mx_quantize(part), mx_quantize(few)
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    a, b = exec_fused_act_mul_mx(part, base[:, :4096]), exec_fused_act_mul_mx(few, base[:, :4096].contiguous())
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    assert torch.equal(layer(part), layer(few))
