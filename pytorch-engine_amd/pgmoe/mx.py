@@ -181,8 +181,11 @@ def _floats(name: str, x: torch.Tensor) -> Tuple[torch.Tensor, int, int, int, in
     if not shape or shape[-1] < 1:
         raise ValueError(f"{name}: [..., cols]")
     n = shape[-1]
+    rows = x.numel() // n
+    if rows >= _ROWS:
+        raise NotImplementedError(f"{name}: {rows} rows (below {_ROWS})")
     x, stride, at = _placed(x, n, 4 if dt == 0 else 2, _FLOAT_STRIDE)
-    return x, dt, at, stride, x.numel() // n
+    return x, dt, at, stride, rows
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "e4m3") -> MXTensor:
@@ -330,8 +333,8 @@ class HipMXLinear(nn.Module):
 
     def forward(self, x: Union[torch.Tensor, MXTensor], out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         shape, n = x.shape, self.in_features
-        if shape[-1] != n:
-            raise ValueError(f"{shape[-1]} input features, the layer has {n}")
+        if not shape or shape[-1] != n:
+            raise ValueError(f"input of shape {tuple(shape)}, the layer has {n} input features")
         dev = self.device
         if x.device != dev:
             raise ValueError(f"input on {x.device}, the layer is on {dev}")

@@ -251,3 +251,22 @@ def test_wide_rows_are_not_copied(dev):
     a, b = exec_fused_act_mul_mx(part, base[:, :4096]), exec_fused_act_mul_mx(few, base[:, :4096].contiguous())
     assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
     assert torch.equal(layer(part), layer(few))
+
+
+def test_calls_that_are_refused(dev):
+    """More rows than a call takes (here of one row's memory), inputs of no dimension."""
+    from pgmoe import HipMXLinear, exec_fused_act_mul_mx, exec_fused_rmsnorm_mx, mx_quantize
+    layer = HipMXLinear(_random_blocks(8, 32, "e2m1", 1, dev)[0])
+    none = torch.ones((), device=dev)
+    had = torch.cuda.memory_allocated(dev)
+    torch.cuda.reset_peak_memory_stats(dev)
+    for rows in (1 << 24, 1 << 31, (1 << 32) + 3):
+        x = torch.ones(1, 32, device=dev).expand(rows, 32)
+        for call in (lambda: layer(x), lambda: mx_quantize(x), lambda: exec_fused_act_mul_mx(x, x)):
+            with pytest.raises(NotImplementedError, match="rows"):
+                call()
+    assert torch.cuda.max_memory_allocated(dev) - had < 1 << 20
+    for call in (lambda: layer(none), lambda: mx_quantize(none), lambda: exec_fused_act_mul_mx(none, none),
+                 lambda: exec_fused_rmsnorm_mx(none, none)):
+        with pytest.raises(ValueError):
+            call()
