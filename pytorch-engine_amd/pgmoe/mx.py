@@ -276,6 +276,7 @@ class HipMXLinear(nn.Module):
                  fp32_sums: bool = False) -> None:
         super().__init__()
         _bits(act_fmt)
+        self._not_while_captured()
         if weight.fmt != "e2m1" or len(weight.shape) != 2 or weight.shape[0] < 1:
             raise ValueError(f"weight: e2m1 blocks [out_features, in_features], not {weight.fmt} {tuple(weight.shape)}")
         self.out_features, self.in_features = weight.shape
@@ -295,6 +296,11 @@ class HipMXLinear(nn.Module):
 
     bias = property(lambda self: self._bias)
 
+    @staticmethod
+    def _not_while_captured() -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a layer is made before a graph is captured: its weights are laid out once, and waited for")
+
     @classmethod
     def from_gguf(cls, gguf_file: Any, weight_name: Union[str, Sequence[str]], bias_name: Optional[str] = None,
                   device: Union[torch.device, str] = "cuda", act_fmt: str = "e4m3", fp32_sums: bool = False) -> "HipMXLinear":
@@ -303,6 +309,7 @@ class HipMXLinear(nn.Module):
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError("HipMXLinear runs on a HIP device (torch.device('cuda', i))")
+        cls._not_while_captured()
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         codes, scales = [], []

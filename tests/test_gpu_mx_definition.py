@@ -270,3 +270,25 @@ def test_calls_that_are_refused(dev):
                  lambda: exec_fused_rmsnorm_mx(none, none)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_layers_are_not_made_while_a_graph_is_captured(dev):
+    """The refusal leaves the capture as it was: the graph holds the call before and the call behind it."""
+    from pgmoe import HipMXLinear
+    w, _ = _random_blocks(40, 128, "e2m1", 1, dev)
+    layer = HipMXLinear(w)
+    x = torch.randn(3, 128, generator=torch.Generator().manual_seed(1)).to(dev)
+    want = layer(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = layer(x)
+        with pytest.raises(RuntimeError, match="captured"):
+            HipMXLinear(w)
+        with pytest.raises(RuntimeError, match="captured"):
+            HipMXLinear.from_gguf(None, "a", device=dev)
+        last = layer(x)
+    for _ in range(3):
+        first.zero_(), last.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(last, want) and torch.equal(layer(x), want)
