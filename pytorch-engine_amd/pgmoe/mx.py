@@ -34,7 +34,6 @@ _ACT = {"silu": ACT_SILU, "gelu": ACT_GELU_TANH}
 _ROWS, _COLS = 1 << 24, 1 << 22  # rows below, columns up to
 _STRIDE = 1 << 23  # bytes from row to row of blocks
 _FLOAT_STRIDE = 1 << 31  # elements from row to row of values
-_INSIDE = (16, 4096)  # up to so many rows and columns of values become blocks inside the product, without a workspace
 
 
 def _bits(fmt: str) -> int:
@@ -365,11 +364,10 @@ class HipMXLinear(nn.Module):
                    out.data_ptr(), code)
             return out
         bits = _FMT[self.act_fmt]
-        ws, nbytes = None, 0
-        if rows > _INSIDE[0] or n > _INSIDE[1]:
-            nbytes = rows * (n * bits // 8 + (n // 32 + 15) // 16 * 16)  # pgmoe_mx_linear_values_workspace_bytes
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # of this call alone
-        launch(dev, "pgmoe_mx_linear_values", lib().pgmoe_mx_linear_values, self._packed.data_ptr(), self.out_features,
+        L = lib()
+        nbytes = L.pgmoe_mx_linear_values_workspace_bytes(rows, n, bits)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # of this call alone
+        launch(dev, "pgmoe_mx_linear_values", L.pgmoe_mx_linear_values, self._packed.data_ptr(), self.out_features,
                at, dt, stride, rows, n, bits, bias, out.data_ptr(), code,
                None if ws is None else ws.data_ptr(), nbytes)
         return out

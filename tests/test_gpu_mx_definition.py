@@ -292,3 +292,29 @@ def test_layers_are_not_made_while_a_graph_is_captured(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(first, want) and torch.equal(last, want) and torch.equal(layer(x), want)
+
+
+def test_the_library_says_how_much_scratch_a_product_needs(dev, monkeypatch):
+    """The layer asks at every call: a library that wants more gets more."""
+    from pgmoe import HipMXLinear, _lib, mx
+    real, asked = _lib.lib(), []
+
+    class More:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def pgmoe_mx_linear_values_workspace_bytes(self, rows, cols, fmt):
+            asked.append((rows, cols, fmt))
+            return real.pgmoe_mx_linear_values_workspace_bytes(rows, cols, fmt) + 4096
+
+        def pgmoe_mx_linear_values(self, *a):
+            assert a[-3] and a[-2] == real.pgmoe_mx_linear_values_workspace_bytes(*asked[-1]) + 4096
+            return real.pgmoe_mx_linear_values(*a)
+
+    layer = HipMXLinear(_random_blocks(70, 4128, "e2m1", 1, dev)[0], act_fmt="e2m1")
+    small = HipMXLinear(_random_blocks(70, 64, "e2m1", 1, dev)[0])
+    x = torch.randn(20, 4128, generator=torch.Generator().manual_seed(1)).to(dev)
+    want = layer(x), layer(x[:3]), small(x[:3, :64])
+    monkeypatch.setattr(mx, "lib", lambda: More())
+    assert all(torch.equal(a, b) for a, b in zip((layer(x), layer(x[:3]), small(x[:3, :64])), want))
+    assert asked == [(20, 4128, 4), (3, 4128, 4), (3, 64, 8)]
