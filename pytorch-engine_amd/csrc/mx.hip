@@ -52,27 +52,35 @@ __device__ __forceinline__ void put_codes(const MxRows& y, int64_t row, int c, c
 
 // silu(g) = g / (1 + 2^-z) with z = log2(e) g, gelu(g) the same with z = 2 log2(e) sqrt(2 / pi) (g + 0.044715 g^3): no
 // difference of near values for negative g.  The hardware's power of two and reciprocal are good to 2^-23 each, where codes
-// hold 4 bits; what rounding z leaves out of silu's (|z| 2^-24 of the value) is put back to first order.
-constexpr float kLog2e = 1.44269504088896f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.69314718f;
+// hold 4 bits; what rounding z = g slope leaves out (|z| 2^-24 of the value) is put back to first order.
 constexpr float kFarGate = 120.0f;  // |z| past it: 2^-z nears the end of fp32's range
+constexpr float kLn2 = 0.69314718f;
 template <int ACT>
-__device__ __forceinline__ float gate_exponent(float g) {
-    return ACT ? (2.0f * 0.7978845608028654f * kLog2e) * (g + 0.044715f * g * g * g) : kLog2e * g;
-}
-template <int ACT>
-__device__ __forceinline__ float gated(float g, float z) {
-    float t = __builtin_amdgcn_exp2f(-z);
-    if constexpr (ACT == 0) t = __builtin_fmaf(-kLn2 * t, __builtin_fmaf(g, kLog2eRest, __builtin_fmaf(g, kLog2e, -z)), t);
-    return g * __builtin_amdgcn_rcpf(1.0f + t);
-}
+struct Gate {
+    static constexpr float kSlope = ACT ? 2.30220819813f : 1.44269504089f;   // z / g at 0, as fp32
+    static constexpr float kRest = ACT ? 1.29484e-8f : 1.92596e-8f;          // and what is left
+    float slope, z;
+    __device__ __forceinline__ explicit Gate(float g) {
+        slope = ACT ? __builtin_fmaf(0.102943239579f, g * g, kSlope) : kSlope;
+        z = g * slope;
+    }
+    // z - from, to more bits than z has
+    __device__ __forceinline__ float beyond(float g, float from) const {
+        return __builtin_fmaf(g, kRest, __builtin_fmaf(g, slope, -from));
+    }
+    __device__ __forceinline__ float act(float g) const {
+        float t = __builtin_amdgcn_exp2f(-z);
+        t = __builtin_fmaf(-kLn2 * t, beyond(g, z), t);
+        return g * __builtin_amdgcn_rcpf(1.0f + t);
+    }
+};
 // act(g) u for z past kFarGate, where 1 + 2^-z is 1 to fp32, or 2^-z: g u, or g u 2^z, the power in parts so that none of them
 // leaves the range before the product does (g = -100 is worth 7e-4 beside u = 2e38).
 template <int ACT>
-__device__ __forceinline__ float gated_far(float g, float z, float u) {
-    if (z > 0) return g * u;
-    z = fmaxf(z, -400.0f);
-    const float n = rintf(z), c = fmaxf(g, -400.0f / kLog2e);
-    const float f = ACT ? z - n : __builtin_fmaf(c, kLog2eRest, __builtin_fmaf(c, kLog2e, -n));
+__device__ __forceinline__ float gated_far(float g, const Gate<ACT>& a, float u) {
+    if (a.z > 0) return g * u;
+    const bool gone = a.z < -400.0f;  // of any u
+    const float n = gone ? -400.0f : rintf(a.z), f = gone ? 0.0f : a.beyond(g, n);
     return g * ldexpf(__builtin_amdgcn_exp2f(f), -120) * ldexpf(u, (int)n + 120);
 }
 
@@ -97,15 +105,15 @@ __global__ __launch_bounds__(kMxThreads) void mx_rows_kernel(const void* __restr
         float gu[N], most = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float z = gate_exponent<ACT>(v[i]);
-            most = fmaxf(most, fabsf(z));
-            gu[i] = gated<ACT>(v[i], z) * w[i];
+            const Gate<ACT> gate(v[i]);
+            most = fmaxf(most, fabsf(gate.z));
+            gu[i] = gate.act(v[i]) * w[i];
         }
         if (__builtin_expect(most > kFarGate, 0)) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float z = gate_exponent<ACT>(v[i]);
-                if (fabsf(z) > kFarGate) gu[i] = gated_far<ACT>(v[i], z, w[i]);
+                const Gate<ACT> gate(v[i]);
+                if (fabsf(gate.z) > kFarGate) gu[i] = gated_far<ACT>(v[i], gate, w[i]);
             }
         }
 #pragma unroll
