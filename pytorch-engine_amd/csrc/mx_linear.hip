@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * W, 4 / NB) void mx_thin_kernel(const MxLinear 
         for (int s = 0; s < 4; ++s) {
             to.f[s].a = *(const int4*)(xr + (int64_t)block(s) * (MODE == kS4 ? 16 : 32));
             if constexpr (MODE != kS4) to.f[s].b = *(const int4*)(xr + (int64_t)block(s) * 32 + 16);
-            to.s[s] = 16 * q + 4 * s + g <= last ? xsr[block(s)] : 127;  // 1 past the row: the weights' 0 meets no infinity
+            to.s[s] = xsr[block(s)];
         }
     };
     // The wave's quad of all rows, as values, to blocks; 16-byte chunk c of row i lies at c ^ i.
@@ -333,12 +333,14 @@ __global__ __launch_bounds__(64 * W, 4 / NB) void mx_thin_kernel(const MxLinear 
             to.s[s] = own[kMxFewRows * ROW + m * 16 + b];
         }
     };
-    auto products = [&](const Weights& w, const Rows& x, floatx4 (&acc)[NB][1]) PG_INLINE {
+    auto products = [&](const Weights& w, const Rows& x, int q, floatx4 (&acc)[NB][1]) PG_INLINE {
         auto step = [&](auto sc) PG_INLINE {
             constexpr int s = decltype(sc)::value;
             WOps<MODE, NB> ops;
             ops.template set<s>(w.w[s], w.s);
-            mx_products<MODE, s, 0>(ops, w.s, x.s[s], x.f[s], 0, acc);
+            // 1 past the row, where the weights' 0 is to meet no infinity (chosen here, so that no load waits for it)
+            const int xs = 16 * q + 4 * s + g <= last ? x.s[s] : 127;
+            mx_products<MODE, s, 0>(ops, w.s, xs, x.f[s], 0, acc);
         };
         step(std::integral_constant<int, 0>());
         step(std::integral_constant<int, 1>());
@@ -365,7 +367,7 @@ __global__ __launch_bounds__(64 * W, 4 / NB) void mx_thin_kernel(const MxLinear 
             if constexpr (ONE) {
                 Weights next;
                 load_w(next, gb + gridDim.x, wave);
-                products(w, x, acc);
+                products(w, x, wave, acc);
                 w = next;
             } else {
 #pragma unroll 1
@@ -376,7 +378,7 @@ __global__ __launch_bounds__(64 * W, 4 / NB) void mx_thin_kernel(const MxLinear 
                     if constexpr (NB > 1) load_x(then, more ? q + W : wave);
                     load_w(next, more ? gb : gb + gridDim.x, more ? q + W : wave);
                     if constexpr (NB == 1) load_x(x, q);
-                    products(w, x, acc);
+                    products(w, x, q, acc);
                     w = next;
                     if constexpr (NB > 1) x = then;
                 }
