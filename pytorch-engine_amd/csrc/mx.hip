@@ -176,18 +176,14 @@ __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(MxRows x, Fas
 struct Doubles {
     double v[4];
 };
-__device__ __forceinline__ double wave_sum(double v) {
-    auto add = [&](auto sc) {
-        constexpr int S = decltype(sc)::value;
+// group_sum in 64 bits: over G aligned lanes, each with the sum.
+template <int G>
+__device__ __forceinline__ double lanes_sum(double v) {
+    if constexpr (G > 1) {
         const uint64_t b = __builtin_bit_cast(uint64_t, v);
-        v += __builtin_bit_cast(double, (uint64_t)xor_lane_u<S>((uint32_t)(b >> 32)) << 32 | xor_lane_u<S>((uint32_t)b));
-    };
-    add(std::integral_constant<int, 32>());
-    add(std::integral_constant<int, 16>());
-    add(std::integral_constant<int, 8>());
-    add(std::integral_constant<int, 4>());
-    add(std::integral_constant<int, 2>());
-    add(std::integral_constant<int, 1>());
+        v += __builtin_bit_cast(double, (uint64_t)xor_lane_u<G / 2>((uint32_t)(b >> 32)) << 32 | xor_lane_u<G / 2>((uint32_t)b));
+        return lanes_sum<G / 2>(v);
+    }
     return v;
 }
 // d in fp32 for a further rounding to fewer bits: what does not fit sets the last bit (the other 29 of d's 52 are cut), so that
@@ -199,9 +195,9 @@ __device__ __forceinline__ float to_odd(double d) {
 }
 
 template <int T, int VPT, bool E2M1>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void add_rmsnorm_mx_kernel(const void* __restrict__ x, int xdt,
+__global__ __launch_bounds__(T < 256 ? 256 : T, T == 1024 ? 8 : 1) void add_rmsnorm_mx_kernel(const void* __restrict__ x, int xdt,
                                                                           const void* __restrict__ delta, int ddt,
-                                                                          const float* __restrict__ w, float eps,
+                                                                          const float* __restrict__ w, float eps, double inv_cols,
                                                                           float* __restrict__ h_out, MxRows y) {
     constexpr int RPB = T < 256 ? 256 / T : 1, W = T / 64;  // rows a workgroup, waves a row
     __shared__ double wsum[W > 1 ? W : 1];
@@ -228,15 +224,15 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rmsnorm_mx_kernel(const
         return acc;
     };
     auto total = [&](double acc) {
-        acc = wave_sum(acc);
+        acc = lanes_sum<64>(acc);
         if constexpr (W > 1) {
             if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = acc;
             __syncthreads();
-            acc = wsum[0];
-#pragma unroll
-            for (int i = 1; i < W; ++i) acc = acc + wsum[i];
+            acc = lanes_sum<W>(wsum[threadIdx.x % W]);
         }
-        return 1.0 / sqrt(acc / (double)y.cols + (double)eps);
+        // the hardware's 1 / sqrt is good to 2^-24 or better, one step of Newton's to 2^-47; 0 and infinity stand
+        const double m = __builtin_fma(acc, inv_cols, (double)eps), r = __builtin_amdgcn_rsq(m);
+        return m > 0.0 && m < (double)__builtin_inff() ? __builtin_fma(0.5 * r, __builtin_fma(-m * r, r, 1.0), r) : r;
     };
     auto put_h = [&](int c, Doubles h) {
         if (h_out && c < n4) ((float4*)h_out)[row4 + c] = make_float4((float)h.v[0], (float)h.v[1], (float)h.v[2], (float)h.v[3]);
@@ -253,6 +249,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rmsnorm_mx_kernel(const
     if constexpr (VPT > 0) {
         auto at = [&](int j) { return min(t + T * j, n4 - 1); };  // chunks past the row repeat its last one
         uint4 xr[VPT], dr[VPT];
+        constexpr bool LATE = T * VPT > 2048;  // weights asked for behind the sum: two workgroups a CU where a row takes most registers
         float4 g[VPT];
         if (xdt == PGMOE_DT_F32) {
 #pragma unroll
@@ -270,21 +267,27 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void add_rmsnorm_mx_kernel(const
                 for (int j = 0; j < VPT; ++j) dr[j] = load(delta, PGMOE_DT_F16, row4 + at(j));
             }
         }
+        if constexpr (!LATE) {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) g[j] = ((const float4*)w)[at(j)];
+            for (int j = 0; j < VPT; ++j) g[j] = ((const float4*)w)[at(j)];
+        }
         __builtin_amdgcn_sched_barrier(0);
+        auto h_of = [&](int j) {
+            const Doubles h = wide(widen4(xr[j], xdt));
+            return delta ? add(h, wide(widen4(dr[j], ddt))) : h;
+        };
         double acc = 0.0;
         Doubles h[VPT];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            h[j] = wide(widen4(xr[j], xdt));
-            if (delta) h[j] = add(h[j], wide(widen4(dr[j], ddt)));
+            h[j] = h_of(j);
             if (t + T * j < n4) acc = squares(acc, h[j]);
         }
         const double r = total(acc);
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int c = t + T * j;
+            if constexpr (LATE) g[j] = ((const float4*)w)[at(j)];
             put_h(c, h[j]);
             put(c, h[j], wide(g[j]), r);
         }
@@ -385,10 +388,11 @@ static int norm_launch(const void* x, int xdt, const void* delta, int ddt, const
         const void* dp = delta ? (const uint8_t*)delta + r * y.cols * (ddt == PGMOE_DT_F32 ? 4 : 2) : nullptr;
         float* hp = h_out ? h_out + r * y.cols : nullptr;
         const dim3 grid(div_up(n, RPB)), block(T * RPB);
+        const double inv = 1.0 / y.cols;
         if (y.e2m1)
-            PG_LAUNCH((add_rmsnorm_mx_kernel<T, VPT, true>), grid, block, 0, st, xp, xdt, dp, ddt, w, eps, hp, z);
+            PG_LAUNCH((add_rmsnorm_mx_kernel<T, VPT, true>), grid, block, 0, st, xp, xdt, dp, ddt, w, eps, inv, hp, z);
         else
-            PG_LAUNCH((add_rmsnorm_mx_kernel<T, VPT, false>), grid, block, 0, st, xp, xdt, dp, ddt, w, eps, hp, z);
+            PG_LAUNCH((add_rmsnorm_mx_kernel<T, VPT, false>), grid, block, 0, st, xp, xdt, dp, ddt, w, eps, inv, hp, z);
         return check_launch("add_rmsnorm_mx");
     });
 }
