@@ -37,7 +37,13 @@ struct MxLinear {
 };
 constexpr int kMxFewRows = 16;  // up to so many rows are read against weights in registers
 // Values of them become blocks inside the product where a workgroup keeps its rows; longer ones would become them again for
-// every 16 outputs (1 x 12288 x 4096 16.1 us; in a launch of their own before, as more rows' are, 11).
+// every 16 outputs (1 x 12288 x 4096 16.1 us; in a launch of their own before, as more rows' are, 11).  Every workgroup makes all the
+// blocks, so more rows gain less; us inside / in a launch before, in a captured graph, fp16 values to 8 bits, K = 4096:
+//   outputs    1 row      8 rows     12 rows    16 rows
+//   4096       4.5/7.0    6.7/7.5    8.1/8.1    9.1/8.5
+//   12288      7.8/9.7    9.3/10.8   11.3/11.4  13.3/12.4
+//   24576      12.1/14.1  13.2/15.2  15.9/16.2  17.5/17.2
+// From 13 rows on the launch before is up to 0.9 us less; outside a graph it costs as much on the host.
 inline bool mx_values_inside(int64_t rows, int64_t cols) { return rows <= kMxFewRows && cols <= 4096; }
 int launch_mx_linear(const MxLinear& L, hipStream_t st);
 // L.x: where the blocks of more rows go.

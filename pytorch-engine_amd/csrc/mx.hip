@@ -401,9 +401,10 @@ int launch_add_rmsnorm_mx(const void* x, int xdt, const void* delta, int ddt, co
                           const MxRows& y, hipStream_t st) {
     const int n4 = y.cols >> 2;
     // 4 threads' work or less each while it fills workgroups of 256, more threads where a row is a CU's only one: 4096 columns,
-    // fp32 and fp32, with 256 / 1024 threads: 1 row 4.3 / 3.4 us, 256 6.4 / 5.2, 700 9.5 / 8.9, 1024 11.5 / 11.7, 4003 41.4
-    // (5.2 TB/s) / 44.3; 2048 columns, 1 row 3.2 / 3.1, 1024 7.4 / 8.4.  8192 columns in two chunks a thread or four of half the
-    // threads: 1 row 4.3 / 5.7, 4003 79.7 (5.4 TB/s) / 85.7; 16384 in registers 152, read twice 203.
+    // fp32 and fp32, with 256 / 1024 threads: 1 row 4.3 / 3.4 us, 256 6.3 / 5.3, 700 10.0 / 9.5, 1024 12.0 / 12.6, 4003 38.0
+    // (5.6 TB/s) / 42.9; 2048 columns, 1 row 3.0 / 3.1, 1024 7.9 / 9.3.  8192 columns in two chunks a thread or four of half the
+    // threads: 1 row 4.5 / 5.0, 4003 both 81.5 (5.2 TB/s); 16384 in registers 156, read twice 205.  In fp32 they took 0.1 to 0.8 us
+    // less up to 1024 rows, 1 to 2 % beyond.
 #define NORM(T, V) return norm_launch<T, V>(x, xdt, delta, ddt, w, eps, h_out, y, st)
     if (n4 <= 64) NORM(64, 1);
     if (n4 <= 128) NORM(64, 2);

@@ -211,11 +211,12 @@ __device__ __forceinline__ void put_pair(const MxLinear& L, int m, int n, int g,
 // ---------------------------------------------------------------- up to 16 rows
 // A workgroup forms NB times 16 outputs of all rows at a time; its W waves take every W-th quad of steps, weights and activations
 // straight to registers, and their sums meet in LDS in wave order.  ONE: a quad is all that a wave has (K <= 512 W): the
-// rows stay in registers, and the workgroup goes on to its next 16 outputs, whose weights are on their way meanwhile.
+// rows stay in registers, and the workgroup goes on to its next 16 outputs, whose weights are asked for during these products
+// (rows kept so: 2048 x 151936 35 for 44 us).  They are waited for at the turn's end, before the sums meet: `w = next` is a copy of
+// registers there.  Other waves of the CU fill that wait, or nothing does.
 // Bound by the weights' arrival and, where they are few, by the latencies of one load, one sum and the launch: us for 1 / 16
-// rows of fp16 values to 8 bits, 4096 x 4096 4.3 / 9.0, 4096 x 24576 12.5 (4.3 TB/s) / 19, 2048 x 151936 31 (5.4) / 39, 12288 x 4096
-// 10.2 / 15.4 (2.6 of it the blocks' own launch).  ONE, the next outputs' weights under way during the sum of these, rows kept:
-// 2048 x 151936 35 for 44 us.
+// rows of fp16 values to 8 bits, inputs x outputs, weights from memory but for the head's: 4096 x 4096 4.4 / 9.1, 4096 x 24576 12.1
+// (4.4 TB/s) / 17.5, 2048 x 151936 27 / 30, 12288 x 4096 10.6 / 15.3 (2.6 of it the blocks' own launch).
 // SRC: the rows come in blocks (-1), or (ONE) as values of a PGMOE_DT_* that become blocks here, in LDS, eight values a lane, a
 // wave its quad of every row: as much work as there are values.
 template <int SRC>
@@ -371,7 +372,9 @@ __global__ __launch_bounds__(64 * W, 4 / NB) void mx_thin_kernel(const MxLinear 
                 w = next;
             } else {
 #pragma unroll 1
-                for (int q = wave; q < Q; q += W) {  // the next quad's weights, or the next outputs' first, on their way
+                // The next quad's weights, or the next outputs' first, are asked for during these products: where NB is 1 behind
+                // most of them, and each step's rows right before their use, so that a quad shows a latency or two.
+                for (int q = wave; q < Q; q += W) {
                     Weights next;
                     Rows then;
                     const bool more = q + W < Q;
@@ -387,7 +390,8 @@ __global__ __launch_bounds__(64 * W, 4 / NB) void mx_thin_kernel(const MxLinear 
             for (int b = 0; b < NB; ++b)
                 part[turn & 1][wave][b][lane] = make_float4(acc[b][0][0], acc[b][0][1], acc[b][0][2], acc[b][0][3]);
         }
-        // (no wait for loads and stores; a buffer is written again behind the next barrier, which its reader passes too)
+        // (not for loads and stores, though the copy above has waited for the loads; a buffer is written again behind the next
+        // barrier, which its reader passes too)
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -429,8 +433,10 @@ static int thin_launch(const MxLinear& L, const MxFloats& F, hipStream_t st) {
 // stages ahead, so that a chain of stages runs at the rate of the products and not at a memory latency each.  At the top of stage
 // s a wave waits until its copies of stage s have landed (EARLY: of s + 1), and the barrier makes all waves' visible; EARLY,
 // the first fragments of s + 1 are then read under the last products of s.  Chunk c (16 bytes) of activation row r lies at
-// c ^ (r / 2 & 7): the 16 rows of a fragment fall on different banks.  Weights lie as they are packed.  Scales of 512 inputs
-// come with the first of their stages: 16 bytes an activation row, which become a word a lane and row, a byte a step.
+// c ^ (r / 2 & 7): the 16 rows of a fragment fall on different banks, but for the bf16 form's, whose chunks 2 g and 2 g + 1 meet
+// (1.05 M conflict cycles at 500 x 4096 x 4096; a turn without them took the same time).  Weights lie as they are packed.
+// Scales of 512 inputs come with the first of their stages: 16 bytes an activation row, which become a word a lane and row, a
+// byte a step.
 //
 // WK parts of a workgroup, WM x WN waves and a ring each, share out the quads of the inputs, and their sums meet in LDS in
 // the parts' order.  They are for few tiles: a CU then has more waves to hide a wait with and more copies under way, and smaller
@@ -761,8 +767,9 @@ static int gemm_launch(const MxLinear& L, hipStream_t st) {
     return check_launch("mx_gemm");
 }
 
-// Which tile: the one whose fit a + b ceil(tiles / CUs) to the times measured is least.  us at K = 4096 (other K change all
-// alike) for n tiles a CU, n = 1 / 2 / 4:
+// Which tile: the one whose fit a + b ceil(tiles / CUs) to the times measured is least.  The rule does not know K: it was fitted at
+// K = 4096 and not measured at others, where a tile whose parts share out the quads gains less (up to 512 inputs one part works).
+// us at K = 4096 for n tiles a CU, n = 1 / 2 / 4:
 //   8 bits  128 x 256 33 / 52 / 100, 128 x 128 22 / 35 / 63, 64 x 128 14 / 22 / 39, 32 x 128 11 / 14 / 26, 32 x 64 8.2 / 11 / 19
 //   4 bits  256 x 256 41 / 77, 128 x 128 17 / 27 / 47, 64 x 64 9.5 / 12.7 / 22, 32 x 128 11.8 / 13 / 24, 32 x 64 7.4 / 13 / 24
 //   fp32    64 x 256 35 / 58 / 115, 64 x 128 21 / 34 / 62, 32 x 128 14 / 22 / 40, 32 x 64 9.8 / 14 / 25
