@@ -63,6 +63,26 @@ def test_norm_of_far_rows(dev, fmt, cols):
             assert torch.equal(H.scales(v), e) and torch.equal(H.unpack(v), codes)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("cols", [96, 4096, 16512])
+def test_norm_of_far_weights(dev, fmt, cols):
+    """Rows that end below fp32's normal range, or beyond it; sums that only h does not hold."""
+    from pgmoe import exec_fused_add_rmsnorm_mx, exec_fused_rmsnorm_mx
+    g = torch.Generator().manual_seed(cols)
+    x, w = torch.randn(5, cols, generator=g), 1 + 0.2 * torch.randn(cols, generator=g)
+    for size in (2.0 ** -120, 2.0 ** -128, 2.0 ** -133, 2.0 ** 120):
+        y = _norm64(x.double(), w * size, float(torch.tensor(1e-6)))
+        # below 2^-126 a value is rounded to 2^-149 first: 2^-14 of the codes' least half step
+        H.check_blocks(exec_fused_rmsnorm_mx(x.to(dev), (w * size).to(dev), 1e-6, fmt), y, 2.0 ** -11)
+    t = exec_fused_rmsnorm_mx(x.to(dev), torch.full((cols,), 3e38, device=dev), 1e-6, fmt)
+    over = _norm64(x.double(), torch.full((cols,), 3e38), 1e-6).abs().ge(2.0 ** 128).reshape(5, -1, 32).any(-1)
+    assert torch.equal(H.scales(t) == 255, over)
+    big = torch.full((5, cols), 3e38).copysign(x)
+    h, t = exec_fused_add_rmsnorm_mx(big.to(dev), big.to(dev), w.to(dev), 1e-6, fmt)
+    codes, e = H.encode(_norm64(2 * big.double(), w, 1e-6), fmt)
+    assert torch.isinf(h).all() and torch.equal(H.scales(t), e) and torch.equal(H.unpack(t), codes)
+
+
 # ---------------------------------------------------------------- activation
 def _act64(act, g, u):
     if act == "silu":
